@@ -58,6 +58,8 @@ extern "C" {
 #define NAIWA_Q8_0 8
 #define NAIWA_Q4_K 12
 #define NAIWA_BF16 30
+#define NAIWA_GGML_MXFP4 39            /* GGUF files only: banks hold the tile order */
+#define NAIWA_MXFP4_T    (0x10000 | 39) /* MXFP4 in tile order (naiwa_mxfp4.h); not a GGML id */
 
 /* ---- activations (src/moe/stages/gpu.rs:15-21) ------------------------------- */
 #define NAIWA_ACT_SILU           0
@@ -174,11 +176,11 @@ typedef struct naiwa_bank {
     int32_t slots;         /* slots in the bank                                */
     int32_t n;             /* output rows                                      */
     int32_t k;             /* input features                                   */
-    int32_t dtype;         /* NAIWA_Q4_K or NAIWA_Q8_0                         */
+    int32_t dtype;         /* NAIWA_Q4_K, NAIWA_Q8_0 or NAIWA_MXFP4_T          */
 } naiwa_bank;
 
 /* Bytes of one [n, k] projection in `dtype` (src/moe/slot.rs:84-95); -1 when
- * k is not a multiple of the block size. */
+ * k is not a multiple of the block size (NAIWA_MXFP4_T: or n not of 16). */
 int64_t naiwa_projection_bytes(int dtype, int64_t n, int64_t k);
 
 /* The replacement of indexed_moe_fused_decode (src/moe/stages/gpu.rs:27-66):
@@ -193,7 +195,13 @@ int64_t naiwa_projection_bytes(int dtype, int64_t n, int64_t k);
  * x 16-byte aligned) take the weights as exact integers with f32 scales, and x
  * and h as f16 times a power of two per row (x) or per 64 features (h): any
  * finite magnitude, within 4e-4 of a 64-bit result.  A NaN or an infinity stays in
- * its row; an infinite activation gives NaN there. */
+ * its row; an infinite activation gives NaN there.
+ * Banks of NAIWA_MXFP4_T (all three, or NAIWA_E_UNSUPPORTED; naiwa_mxfp4.h) take any
+ * number of rows on the matrix cores: H, I multiples of 32, width <= 64, x and out
+ * 16-byte aligned.  Products and sums are f32; an activation is held to 2^-19 of the
+ * largest magnitude of its 32-value block (bf16 x of at least 2^-12 of it exactly):
+ * within 1e-5 of a 64-bit result.  A NaN, an infinity or an h that overflows makes its
+ * pair's dots NaN. */
 int naiwa_moe_decode(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down,
                      const void* x, int x_dtype, const uint32_t* slot_ids, const float* w,
                      int rows, int width, int act, float* out, int64_t stream);
@@ -224,7 +232,7 @@ int naiwa_moe_decode_ex(const naiwa_bank* gate, const naiwa_bank* up, const naiw
  *   T = 4 n I otherwise (h as f32),
  * is at most the array's size; naiwa_moe_decode_scratch_bytes returns S, and
  * the entry point returns NAIWA_E_TOO_LARGE, before any device call, for a
- * larger one.  The 8 MiB array admits 56 pairs (rows <= 28 at top-2) at H 4096,
+ * larger one (MXFP4 banks have a size of their own, the same function's).  The 8 MiB array admits 56 pairs (rows <= 28 at top-2) at H 4096,
  * I 14336, Q4_K; 2712 pairs (rows <= 339 at top-8) at H 2048, I 768.  S is not
  * monotone in n: the staged path's K-part dots cost more per pair than f32 h, so
  * at H 5120, I 1536, top-6, rows 1-55 and 86-227 fit and rows 56-85 do not.
@@ -286,7 +294,10 @@ int naiwa_moe_gather(const uint32_t* ids, int n, int E, uint32_t* perm_out, uint
  * multiplied with v_mfma_f32_32x32x16_bf16 (f32 accumulation); x and h are
  * bf16.  Needs
  * H, I multiples of 128; gate/up Q4_K (H % 256 == 0) or Q8_0, down Q4_K (I %
- * 256 == 0) or Q8_0; T * k <= 65536; slots <= 4096.  Slot ids outside the
+ * 256 == 0) or Q8_0; T * k <= 65536; slots <= 4096.  Banks of NAIWA_MXFP4_T (all
+ * three): H, I multiples of 32, k <= 64, out 16-byte aligned; x held to 2^-14 of the
+ * largest magnitude of its 32-value block (a value of at least 2^-7 of it exactly), h
+ * to 2^-19, products and sums f32.  Slot ids outside the
  * bank contribute nothing.  flags: NAIWA_PREFILL_ACCUMULATE adds to out
  * (e.g. shared experts on top of the routed ones) instead of overwriting. */
 #define NAIWA_PREFILL_ACCUMULATE 1

@@ -22,6 +22,7 @@
 // go to the matrix cores instead, whatever their pair count (decode_mfma.hip).
 #include "decode.h"
 #include "decode_mfma.h"
+#include "mxfp4.h"
 #include "rowdot.h"
 #include "segments.h"
 #include "workspace.h"
@@ -1038,9 +1039,44 @@ int noalloc_scratch(uint8_t** out) {
 
 namespace {
 
+// Whether a call goes to the MXFP4 experts (mxfp4_experts.hip), which refuse mixed formats.
+bool is_mx(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down) {
+    return (gate && gate->dtype == NAIWA_MXFP4_T) || (up && up->dtype == NAIWA_MXFP4_T) ||
+           (down && down->dtype == NAIWA_MXFP4_T);
+}
+
+// A decode call over MXFP4 banks, over the library's buffer or (noalloc) the fixed array.
+int mx_decode(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down, const void* x, int x_dtype,
+              const uint32_t* slot_ids, const float* w, int rows, int width, int act, float* out, int flags,
+              bool noalloc, int64_t stream, uint16_t* res = nullptr, const naiwa_decode_wait* wait = nullptr) {
+    if (flags & ~NAIWA_DECODE_ACCUMULATE) return NAIWA_E_INVALID;
+    if (wait && (!wait->flag || !wait->fail)) return NAIWA_E_INVALID;
+    const NaiwaMxCall c{gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out,
+                        flags & NAIWA_DECODE_ACCUMULATE, 1, res};
+    if (rows > 4096) return NAIWA_E_INVALID;
+    int rc = naiwa_mx_check(c);
+    if (rc || rows == 0) return rc;
+    const size_t bytes = naiwa_mx_scratch_bytes(rows, width, gate->k, gate->n);
+    uint8_t* ws = nullptr;
+    if (noalloc) {
+        if (bytes > kNoAllocScratchBytes) return NAIWA_E_TOO_LARGE;
+        if (bytes && (rc = noalloc_scratch(&ws))) return rc;
+    } else if (bytes && !(ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, bytes, &rc))) {
+        return rc;
+    }
+    if (wait) {
+        decode_wait_kernel<<<1, 64, 0, (hipStream_t)stream>>>(
+            WaitArg{wait->flag, wait->target, wait->limit_ticks, wait->fail});
+        if ((rc = naiwa_hip_rc(hipGetLastError()))) return rc;
+    }
+    return naiwa_mx_run(c, ws, (hipStream_t)stream);
+}
+
 int decode_call(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down, const void* x, int x_dtype,
                 const uint32_t* slot_ids, const float* w, int rows, int width, int act, float* out, int flags,
                 bool chain, int64_t stream) {
+    if (is_mx(gate, up, down))
+        return mx_decode(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, flags, false, stream);
     int rc = check_args(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, flags);
     if (rc || rows == 0) return rc;
     uint8_t* ws = nullptr;
@@ -1070,6 +1106,8 @@ int naiwa_moe_decode_chain(const naiwa_bank* gate, const naiwa_bank* up, const n
 extern "C" int naiwa_moe_decode_noalloc(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down,
                                         const void* x, int x_dtype, const uint32_t* slot_ids, const float* w,
                                         int rows, int width, int act, float* out, int flags, int64_t stream) {
+    if (is_mx(gate, up, down))
+        return mx_decode(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, flags, true, stream);
     int rc = check_args(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, flags);
     if (rc || rows == 0) return rc;
     if (width > 0 && DecodeScratch(rows, width, gate->k, gate->n, down->dtype).total > kNoAllocScratchBytes)
@@ -1086,6 +1124,7 @@ extern "C" int naiwa_moe_decode_noalloc(const naiwa_bank* gate, const naiwa_bank
 
 extern "C" int64_t naiwa_moe_decode_scratch_bytes(int rows, int width, int H, int I, int down_dtype) {
     if (rows < 0 || width < 0 || (int64_t)rows * width > 65536 || H <= 0 || I <= 0 || H % 32 || I % 32) return -1;
+    if (down_dtype == NAIWA_MXFP4_T) return (int64_t)naiwa_mx_scratch_bytes(rows, width, H, I);
     if (down_dtype != NAIWA_Q4_K && down_dtype != NAIWA_Q8_0) return -1;
     if (rows == 0 || width == 0) return 0;
     return (int64_t)DecodeScratch(rows, width, H, I, down_dtype).total;
@@ -1094,6 +1133,12 @@ extern "C" int64_t naiwa_moe_decode_scratch_bytes(int rows, int width, int H, in
 int naiwa_moe_decode_residual(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down, void* x,
                               const uint32_t* slot_ids, const float* w, int rows, int width, int act, float* y,
                               int keep_y, int64_t stream, const naiwa_decode_wait* wait) {
+    if (is_mx(gate, up, down)) {
+        if (rows > 0 && !y) return NAIWA_E_INVALID;
+        if (width == 0) return mx_decode(gate, up, down, x, NAIWA_BF16, slot_ids, w, 0, width, act, y, 0, false, stream);
+        return mx_decode(gate, up, down, x, NAIWA_BF16, slot_ids, w, rows, width, act, keep_y ? y : nullptr, 0, false,
+                         stream, (uint16_t*)x, wait);
+    }
     int rc = check_args(gate, up, down, x, NAIWA_BF16, slot_ids, w, rows, width, act, y, 0);
     if (rc || rows == 0 || width == 0) return rc;
     if (wait && (!wait->flag || !wait->fail)) return NAIWA_E_INVALID;
@@ -1112,6 +1157,8 @@ int naiwa_moe_decode_residual(const naiwa_bank* gate, const naiwa_bank* up, cons
 int naiwa_moe_decode_wait(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down, const void* x,
                           int x_dtype, const uint32_t* slot_ids, const float* w, int rows, int width, int act,
                           float* out, int64_t stream, const naiwa_decode_wait* wait) {
+    if (is_mx(gate, up, down))
+        return mx_decode(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, 0, false, stream, nullptr, wait);
     int rc = check_args(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, 0);
     if (rc || rows == 0) return rc;
     if (wait && (!wait->flag || !wait->fail)) return NAIWA_E_INVALID;

@@ -64,6 +64,7 @@ TypeSize type_size(int t) {
     case 28: return {1, 8};     // F64
     case 29: return {256, 56};  // IQ1_M
     case 30: return {1, 2};     // BF16
+    case 39: return {32, 17};   // MXFP4
     default: return {0, 0};
     }
 }

@@ -38,6 +38,7 @@
 // bf16 operands carry the f32 exponent range: any finite activation goes in
 // without clamping or scaling.
 #include "common.h"
+#include "mxfp4.h"
 #include "unpack_bf16.h"
 #include "workspace.h"
 
@@ -569,6 +570,18 @@ extern "C" int naiwa_moe_prefill(const naiwa_bank* gate, const naiwa_bank* up, c
                                  int flags, int64_t stream) {
     if (!gate || !up || !down || T < 0 || k <= 0 || (flags & ~(NAIWA_PREFILL_ACCUMULATE | NAIWA_PREFILL_RESIDUAL)))
         return NAIWA_E_INVALID;
+    if (gate->dtype == NAIWA_MXFP4_T || up->dtype == NAIWA_MXFP4_T || down->dtype == NAIWA_MXFP4_T) {
+        if (T > 0 && !out) return NAIWA_E_INVALID;
+        if ((int64_t)T * k > 65536) return NAIWA_E_UNSUPPORTED;
+        const NaiwaMxCall c{gate, up, down, x, NAIWA_BF16, slot_ids, w, T, k, act, out,
+                            flags & NAIWA_PREFILL_ACCUMULATE, 0,
+                            (flags & NAIWA_PREFILL_RESIDUAL) ? (uint16_t*)const_cast<void*>(x) : nullptr};
+        int rc = naiwa_mx_check(c);
+        if (rc || T == 0) return rc;
+        const size_t bytes = naiwa_mx_scratch_bytes(T, k, gate->k, gate->n);
+        uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_PREFILL, bytes, &rc);
+        return ws ? naiwa_mx_run(c, ws, (hipStream_t)stream) : rc;
+    }
     if (T == 0) return NAIWA_OK;
     if (!x || !slot_ids || !w || !out) return NAIWA_E_INVALID;
     const int H = gate->k, I = gate->n, slots = gate->slots;

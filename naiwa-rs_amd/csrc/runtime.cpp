@@ -7,6 +7,7 @@
 #include <string.h>
 
 #include "common.h"
+#include "mxfp4.h"
 #include "workspace.h"
 
 namespace {
@@ -211,6 +212,7 @@ int naiwa_device_sync(void) { return naiwa_hip_rc(hipDeviceSynchronize()); }
 int naiwa_last_error(void) { return (int)hipGetLastError(); }
 
 int64_t naiwa_projection_bytes(int dtype, int64_t n, int64_t k) {
+    if (dtype == NAIWA_MXFP4_T) return n < 0 || k < 0 || n % 16 || k % 32 ? -1 : n / 16 * naiwa_mx_strip_bytes(k);
     const int64_t rb = naiwa_row_bytes(dtype, k);
     return rb < 0 || n < 0 ? -1 : rb * n;
 }

@@ -18,6 +18,7 @@ E_INVALID, E_UNSUPPORTED, E_TIMEOUT, E_NOMEM, E_BAD_ID, E_NOT_FOUND, E_DEVICE = 
 E_FORMAT, E_IO, E_TOO_LARGE = -8, -9, -10
 
 F32, F16, Q8_0, Q4_K, BF16 = 0, 1, 8, 12, 30
+GGML_MXFP4, MXFP4_T = 39, 0x10000 | 39   # GGUF blocks; tile order (the banks' form)
 ACT_SILU, ACT_GELU_PYTORCH_TANH = 0, 1
 ROUTE_SOFTMAX_TOPK_RENORM, ROUTE_TOPK_SOFTMAX, ROUTE_SOFTMAX_TOPK = 0, 1, 2
 
@@ -170,6 +171,14 @@ SIGNATURES: dict[str, tuple] = {
     "naiwa_router_topk_biased": (i32, [vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, i64]),
     "naiwa_router_topk_ld": (i32, [vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, i64]),
     "naiwa_moe_prefill": (i32, [_P(Bank), _P(Bank), _P(Bank), vp, vp, vp, i32, i32, i32, vp, i32, i64]),
+    # include/naiwa_mxfp4.h
+    "naiwa_mxfp4_quantize": (i32, [vp, i32, i64, i64, i64, i64, i64, vp, i64, i64]),
+    "naiwa_mxfp4_dequantize": (i32, [vp, i64, i64, i64, i64, vp, i32, i64, i64, i64]),
+    "naiwa_mxfp4_from_ggml": (i32, [vp, i64, i64, vp]),
+    # include/naiwa_balance.h
+    "naiwa_expert_counts": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, i64]),
+    "naiwa_router_balance": (i32, [vp, i32, i32, vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, i64]),
+    "naiwa_router_balance_backward": (i32, [vp, i32, i32, vp, vp, i64, i32, i32, vp, vp, vp, i32, i32, i64]),
     "naiwa_moe_gather": (i32, [vp, i32, i32, vp, vp, vp, i64]),
     "naiwa_synth": (i32, [i32, u64, u64, i64, f32, f32, vp, i64]),
     "naiwa_stack_decode": (i32, [_P(Layer), i32, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, i64]),

@@ -10,8 +10,8 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import check, lib
-from .ops import BLOCK, HostExpertStacks
+from ._lib import GGML_MXFP4, MXFP4_T, check, lib
+from .ops import BLOCK, HostExpertStacks, mxfp4_from_ggml
 
 PROJ_GATE, PROJ_UP, PROJ_DOWN = 0, 1, 2
 
@@ -135,17 +135,23 @@ class GgufFile:
 
     def host_stacks(self, layer: int) -> HostExpertStacks:
         """Pinned host copies of a layer's three projections (gate/up [E, I, H], down
-        [E, H, I]), the sources of expert uploads."""
+        [E, H, I]), the sources of expert uploads; MXFP4 ones in tile order (MXFP4_T)."""
         g, u, d = (self.expert_stack(layer, p) for p in (PROJ_GATE, PROJ_UP, PROJ_DOWN))
         if not (g.experts == u.experts == d.experts and (g.n, g.k) == (u.n, u.k) == (d.k, d.n)):
             raise ValueError(f"layer {layer}: expert stacks disagree: gate [{g.experts},{g.n},{g.k}], "
                              f"up [{u.experts},{u.n},{u.k}], down [{d.experts},{d.n},{d.k}]")
         for p, s in enumerate((g, u, d)):
-            if s.dtype not in BLOCK:
+            if s.dtype not in BLOCK and s.dtype != GGML_MXFP4:
                 raise ValueError(f"layer {layer}: projection {p} is GGML type {s.dtype}, which is not served")
-        stacks = HostExpertStacks(g.experts, g.k, g.n, (g.dtype, u.dtype, d.dtype))
+        held = [MXFP4_T if s.dtype == GGML_MXFP4 else s.dtype for s in (g, u, d)]
+        stacks = HostExpertStacks(g.experts, g.k, g.n, tuple(held))
         for p, s in enumerate((g, u, d)):
+            raw = self.expert_view(layer, p)
+            if held[p] == MXFP4_T:
+                for e, out in enumerate(stacks.view(p)):
+                    mxfp4_from_ggml(raw[e], s.n, s.k, out)
+                continue
             if stacks.expert_bytes[p] != s.expert_bytes:
                 raise ValueError(f"layer {layer}: projection {p} of type {s.dtype} is not served")
-            np.copyto(stacks.view(p), self.expert_view(layer, p))
+            np.copyto(stacks.view(p), raw)
         return stacks

@@ -8,6 +8,10 @@
   same argument meaning (banks, activations, row-major ``[rows, topk]`` local
   slot ids and weights, activation id); the result is ``[rows, hidden]`` f32.
 - ``router_topk`` and ``moe_gather``: routing and grouping on the device.
+- ``mxfp4_quantize`` / ``mxfp4_dequantize`` / ``mxfp4_from_ggml``: MXFP4 projections in
+  the tile order that banks of type ``MXFP4_T`` hold (include/naiwa_mxfp4.h).
+- ``expert_counts``, ``router_balance`` and ``router_balance_backward``: how evenly a
+  router spreads its tokens, and the balance loss's gradient (include/naiwa_balance.h).
 """
 from __future__ import annotations
 
@@ -16,7 +20,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import (ACT_SILU, BF16, E_UNSUPPORTED, F32, Q4_K, Q8_0, ROUTE_SOFTMAX_TOPK_RENORM, STACK_FUSED,
+from ._lib import (ACT_SILU, BF16, E_UNSUPPORTED, F32, MXFP4_T, Q4_K, Q8_0, ROUTE_SOFTMAX_TOPK_RENORM, STACK_FUSED,
                    STACK_LAYERED, Bank, Layer, check, lib)
 from .device import DeviceBuffer, PinnedBuffer
 
@@ -30,26 +34,42 @@ def row_bytes(dtype: int, k: int) -> int:
     return (k // bs) * ts
 
 
+def projection_bytes(dtype: int, n: int, k: int) -> int:
+    """Bytes of one [n, k] projection (src/moe/slot.rs:84-95)."""
+    if dtype != MXFP4_T:
+        return n * row_bytes(dtype, k)
+    if n % 16 or k % 32:
+        raise ValueError(f"[{n}, {k}]: MXFP4 tile order takes rows in sixteens and values in blocks of 32")
+    steps = (k + 127) // 128
+    return n // 16 * (1024 * steps + 256 * ((steps + 3) // 4))
+
+
 def expert_range(dtype: int, n: int, k: int, e: int) -> range:
     """Byte range of expert e in a stacked [E, N, K] tensor (src/moe/expert.rs:123-145)."""
-    stride = n * row_bytes(dtype, k)
+    stride = projection_bytes(dtype, n, k)
     return range(e * stride, (e + 1) * stride)
 
 
 def slot_stride(dtype: int, n: int, k: int) -> int:
     """Bytes between slots: the projection's bytes rounded up to 256."""
-    return (n * row_bytes(dtype, k) + 255) // 256 * 256
+    return (projection_bytes(dtype, n, k) + 255) // 256 * 256
 
 
 class SlotBank:
     """One projection's slot bank on the device."""
 
     def __init__(self, slots: int, n: int, k: int, dtype: int, buffer: DeviceBuffer | None = None,
-                 offset: int = 0, stride: int | None = None):
+                 offset: int = 0, stride: int | None = None, base: int | None = None):
+        """base: device memory that the caller owns (slots * stride bytes), instead of a buffer."""
         self.slots, self.n, self.k, self.dtype = slots, n, k, dtype
         self.stride = slot_stride(dtype, n, k) if stride is None else stride
-        self.expert_bytes = n * row_bytes(dtype, k)
+        self.expert_bytes = projection_bytes(dtype, n, k)
         assert self.stride >= self.expert_bytes
+        if base is not None:
+            if buffer is not None or offset:
+                raise ValueError("a bank over memory of the caller's has no buffer or offset")
+            self.buffer, self.offset, self.base = None, 0, base
+            return
         if buffer is None:
             buffer = DeviceBuffer(self.stride * slots)
             offset = 0
@@ -65,6 +85,11 @@ class SlotBank:
         b = np.ascontiguousarray(expert_bytes, dtype=np.uint8).reshape(-1)
         if b.size != self.expert_bytes:
             raise ValueError(f"expert of {b.size} bytes into a {self.expert_bytes}-byte slot")
+        if self.buffer is None:
+            check(lib().naiwa_memcpy_h2d(self.slot_ptr(slot), b.ctypes.data, b.nbytes, stream), "h2d")
+            if stream == 0:
+                check(lib().naiwa_stream_sync(0), "sync")
+            return
         self.buffer.upload(b, stream, offset=self.offset + slot * self.stride)
 
     def desc(self) -> Bank:
@@ -84,13 +109,24 @@ class LayerBanks:
             self.up = SlotBank(slots, inter, hidden, dtypes[1])
             self.down = SlotBank(slots, hidden, inter, dtypes[2])
             return
-        pb = [inter * row_bytes(dtypes[0], hidden), inter * row_bytes(dtypes[1], hidden),
-              hidden * row_bytes(dtypes[2], inter)]
+        pb = [projection_bytes(dtypes[0], inter, hidden), projection_bytes(dtypes[1], inter, hidden),
+              projection_bytes(dtypes[2], hidden, inter)]
         stride = (sum(pb) + 255) // 256 * 256
         buf = DeviceBuffer(stride * slots)
         self.gate = SlotBank(slots, inter, hidden, dtypes[0], buf, 0, stride)
         self.up = SlotBank(slots, inter, hidden, dtypes[1], buf, pb[0], stride)
         self.down = SlotBank(slots, hidden, inter, dtypes[2], buf, pb[0] + pb[1], stride)
+
+    @classmethod
+    def over(cls, gate: SlotBank, up: SlotBank, down: SlotBank) -> "LayerBanks":
+        """A layer of three banks that exist already."""
+        if (up.n, up.k) != (gate.n, gate.k) or (down.n, down.k) != (gate.k, gate.n) \
+                or not gate.slots == up.slots == down.slots:
+            raise ValueError("the banks' shapes or slots disagree")
+        banks = cls.__new__(cls)
+        banks.hidden, banks.inter, banks.slots = gate.k, gate.n, gate.slots
+        banks.gate, banks.up, banks.down = gate, up, down
+        return banks
 
     def load(self, slot: int, gate: np.ndarray, up: np.ndarray, down: np.ndarray) -> None:
         self.gate.write_slot(slot, gate)
@@ -114,7 +150,7 @@ class HostExpertStacks:
         at e * stride (stride = the expert's bytes), so an expert uploads as one range."""
         self.experts = experts
         shapes = ((inter, hidden, dtypes[0]), (inter, hidden, dtypes[1]), (hidden, inter, dtypes[2]))
-        self.expert_bytes = [n * row_bytes(dt, k) for n, k, dt in shapes]
+        self.expert_bytes = [projection_bytes(dt, n, k) for n, k, dt in shapes]
         if interleaved:
             self.stride = sum(self.expert_bytes)
             self.buffers = [PinnedBuffer(experts * self.stride)]
@@ -218,6 +254,61 @@ def moe_gather(ids, n: int, E: int, perm_out, offsets_out, bad_out=None, stream:
     check(rc, "naiwa_moe_gather")
 
 
+def _opt(a) -> int | None:
+    return None if a is None else _dev(a)
+
+
+def mxfp4_quantize(src, src_dtype: int, n: int, k: int, dst, batch: int = 1, ld: int = 0, src_stride: int = 0,
+                   dst_stride: int = 0, stream: int = 0) -> None:
+    """`batch` [n, k] projections (f32, bf16 or f16; rows ld values apart, projections src_stride values
+    apart) to MXFP4 in tile order, dst_stride bytes apart (0: back to back); device pointers."""
+    check(lib().naiwa_mxfp4_quantize(_dev(src), src_dtype, batch, n, k, ld, src_stride, _dev(dst), dst_stride,
+                                     stream), "naiwa_mxfp4_quantize")
+
+
+def mxfp4_dequantize(src, n: int, k: int, dst, dst_dtype: int, batch: int = 1, ld: int = 0, src_stride: int = 0,
+                     dst_stride: int = 0, stream: int = 0) -> None:
+    """The values of `batch` tile-order projections (src_stride bytes apart) to f32 or bf16 rows."""
+    check(lib().naiwa_mxfp4_dequantize(_dev(src), batch, n, k, src_stride, _dev(dst), dst_dtype, ld, dst_stride,
+                                       stream), "naiwa_mxfp4_dequantize")
+
+
+def mxfp4_from_ggml(blocks: np.ndarray, n: int, k: int, out: np.ndarray | None = None) -> np.ndarray:
+    """Host: one projection's GGML MXFP4 blocks (uint8, n * k / 32 * 17 of them) in tile order."""
+    b = np.ascontiguousarray(blocks, dtype=np.uint8).reshape(-1)
+    size = projection_bytes(MXFP4_T, n, k)
+    if b.size != n * k // 32 * 17:
+        raise ValueError(f"{b.size} bytes are not [{n}, {k}] MXFP4 blocks")
+    if out is None:
+        out = np.empty(size, dtype=np.uint8)
+    if out.dtype != np.uint8 or out.size != size or not out.flags.c_contiguous:
+        raise ValueError(f"out has to be {size} contiguous bytes")
+    check(lib().naiwa_mxfp4_from_ggml(b.ctypes.data, n, k, out.ctypes.data), "naiwa_mxfp4_from_ggml")
+    return out
+
+
+def expert_counts(ids, T: int, k: int, E: int, counts, mask=None, bad=None, ids_ld: int = 0, stream: int = 0) -> None:
+    """counts[E] u32: how often each expert was chosen by the valid tokens (mask u8 [T], None: all)."""
+    check(lib().naiwa_expert_counts(_dev(ids), ids_ld, T, k, E, _opt(mask), _dev(counts), _opt(bad), stream),
+          "naiwa_expert_counts")
+
+
+def router_balance(logits, dtype: int, ids, T: int, E: int, k: int, counts, valid, probs, loss, mask=None, ld: int = 0,
+                   ids_ld: int = 0, stream: int = 0) -> None:
+    """counts[E] u32, valid u32, probs[E] f32 (mean router probabilities) and the balance loss (f32) of a
+    batch; logits [T, E] f32 or bf16."""
+    check(lib().naiwa_router_balance(_dev(logits), dtype, ld, _dev(ids), ids_ld, T, E, k, _opt(mask), _dev(counts),
+                                     _dev(valid), _dev(probs), _dev(loss), stream), "naiwa_router_balance")
+
+
+def router_balance_backward(logits, dtype: int, counts, valid, T: int, E: int, k: int, grad_loss, dlogits, mask=None,
+                            ld: int = 0, dld: int = 0, accumulate: bool = False, stream: int = 0) -> None:
+    """dlogits [T, E] (the logits' type) (+)= grad_loss[0] * dloss/dlogits."""
+    check(lib().naiwa_router_balance_backward(_dev(logits), dtype, ld, _dev(counts), _dev(valid), T, E, k, _opt(mask),
+                                              _dev(grad_loss), _dev(dlogits), dld, 1 if accumulate else 0, stream),
+          "naiwa_router_balance_backward")
+
+
 def layer_desc(router, banks: "LayerBanks", slot_of_expert=None) -> Layer:
     return Layer(_dev(router), banks.gate.desc(), banks.up.desc(), banks.down.desc(),
                  _dev(slot_of_expert) if slot_of_expert is not None else None)
@@ -251,5 +342,6 @@ def synth(dtype: int, seed: int, n: int, out, mean: float = 0.0, std: float = 1.
     check(lib().naiwa_synth(dtype, seed, offset, n, mean, std, _dev(out), stream), "naiwa_synth")
 
 
-__all__ = ["layer_desc", "stack_decode", "stack_status", "synth","SlotBank", "LayerBanks", "indexed_moe_fused_decode", "router_topk", "moe_gather",
-           "row_bytes", "expert_range", "slot_stride", "BF16", "F32", "Q4_K", "Q8_0"]
+__all__ = ["layer_desc", "stack_decode", "stack_status", "synth", "mxfp4_quantize", "mxfp4_dequantize", "mxfp4_from_ggml",
+           "expert_counts", "router_balance", "router_balance_backward", "projection_bytes", "SlotBank", "LayerBanks", "indexed_moe_fused_decode", "router_topk", "moe_gather",
+           "row_bytes", "expert_range", "slot_stride", "BF16", "F32", "MXFP4_T", "Q4_K", "Q8_0"]
