@@ -55,9 +55,11 @@ struct Bank {
     int64_t strip; // bytes of 16 rows
 };
 
-// Rows of activations in P planes of E2M3: row i at base + i * row, block kb at 24 P kb,
-// plane p at 24 p of the block; scales: row i at scales + i * groups * 16, byte
-// 16 (kb / 16) + 4 (kb % 4) + kb / 4 % 4 (a lane's dword holds its block's scale in 4 steps).
+// Rows of activations in P planes of E2M3: row i at base + i * row.  A step of 128 values (4
+// blocks) is 96 P bytes: the first 16 of a block's 24 bytes per plane at head_at, the other 8
+// at tail_at, in the order that the tiles' copies to LDS take (mxfp4_tiles.h).  Scales: row i
+// at scales + i * groups * 16, byte 16 (kb / 16) + 4 (kb % 4) + kb / 4 % 4 for block kb (a
+// lane's dword holds its block's scale in 4 steps).
 struct Planes {
     uint8_t* base;
     uint8_t* scales;
@@ -66,6 +68,10 @@ struct Planes {
 };
 __host__ __device__ inline int64_t plane_row(int planes, int k) { return (int64_t)naiwa_mx_steps(k) * 96 * planes; }
 __device__ __forceinline__ int scale_at(int kb) { return 16 * (kb >> 4) + 4 * (kb & 3) + ((kb >> 2) & 3); }
+
+// Bytes of plane p of block b (of its step's 4).
+__host__ __device__ constexpr int head_at(int P, int b, int p) { return 32 * P * (b & 1) + 16 * ((b >> 1) * P + p); }
+__host__ __device__ constexpr int tail_at(int P, int b, int p) { return 64 * P + 16 * ((b >> 1) * P + p) + 8 * (b & 1); }
 
 // The scale byte of a block whose largest magnitude has the bits m: that magnitude in
 // [2, 4) times 2^(s - 127).  At least 16, so that the planes' scales stay normal.
@@ -115,10 +121,24 @@ segments_kernel(const uint32_t* ids, const float* w, int n, int slots, uint32_t*
     naiwa_segment(sm, ids, w, n, slots, perm, offsets, nullptr, nullptr, nullptr, bad);
 }
 
+__device__ __forceinline__ v8i fp4_operand(v4u v) {
+    v8i o = {};
+    o[0] = (int)v.x, o[1] = (int)v.y, o[2] = (int)v.z, o[3] = (int)v.w;
+    return o;
+}
+
+#include "mxfp4_tiles.h"
+
 // x [rows, H] in P planes, a block of 32 values a thread; the blocks that pad H to whole
-// steps are zeros.  Bound: HBM.
+// steps are zeros.  Bound: HBM.  With tiles, the last block of the launch cuts the sorted pairs
+// into them: the two do not depend on each other.
 template <int P, bool BF16>
-__global__ void __launch_bounds__(kThreads) planes_kernel(const void* x, int64_t rows, int H, Planes out) {
+__global__ void __launch_bounds__(kThreads)
+planes_kernel(const void* x, int64_t rows, int H, Planes out, const uint32_t* offsets, int slots, Tiles tl) {
+    if (tl.n && blockIdx.x == gridDim.x - 1) {
+        tiles_block(offsets, slots, tl);
+        return;
+    }
     const int blocks = 4 * naiwa_mx_steps(H);
     const int64_t b = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (b >= rows * blocks) return;
@@ -150,31 +170,27 @@ __global__ void __launch_bounds__(kThreads) planes_kernel(const void* x, int64_t
     const int s = scale_byte(abs_max(f));
     v6u o[P];
     to_planes<P>(f, s, o);
-    v2u* dst = (v2u*)(out.base + t * out.row + 24 * P * kb);
+    uint8_t* dst = out.base + t * out.row + (int64_t)(kb >> 2) * 96 * P;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) dst[3 * p + i] = v2u{o[p][2 * i], o[p][2 * i + 1]};
+    for (int p = 0; p < P; ++p) {
+        *(v4u*)(dst + head_at(P, kb & 3, p)) = v4u{o[p][0], o[p][1], o[p][2], o[p][3]};
+        *(v2u*)(dst + tail_at(P, kb & 3, p)) = v2u{o[p][4], o[p][5]};
+    }
     out.scales[t * out.groups * 16 + scale_at(kb)] = (uint8_t)s;
 }
 
-__device__ __forceinline__ v8i fp4_operand(v4u v) {
+// The E2M3 operand: plane p of block b of the step at `at`.
+template <int P> __device__ __forceinline__ v8i e2m3_operand(const uint8_t* at, int b, int p) {
+    const v4u h = *(const v4u*)(at + head_at(P, b, p));
+    const v2u t = *(const v2u*)(at + tail_at(P, b, p));
     v8i o = {};
-    o[0] = (int)v.x, o[1] = (int)v.y, o[2] = (int)v.z, o[3] = (int)v.w;
-    return o;
-}
-
-// The E2M3 operand: a block's 24 bytes.
-__device__ __forceinline__ v8i e2m3_operand(const uint8_t* at) {
-    const v2u a = ((const v2u*)at)[0], b = ((const v2u*)at)[1], c = ((const v2u*)at)[2];
-    v8i o = {};
-    o[0] = (int)a.x, o[1] = (int)a.y, o[2] = (int)b.x, o[3] = (int)b.y, o[4] = (int)c.x, o[5] = (int)c.y;
+    o[0] = (int)h.x, o[1] = (int)h.y, o[2] = (int)h.z, o[3] = (int)h.w, o[4] = (int)t.x, o[5] = (int)t.y;
     return o;
 }
 
 // acc += strip rows x planes over steps [t0, t1): S strips of 16 rows, one token row of
-// planes a lane.  wp[i]: strip i's first byte plus 16 lane; xp: the lane's token row plus
-// its block's offset; xs: the row's scales.
+// planes a lane.  wp[i]: strip i's first byte plus 16 lane; xp: the lane's token row;
+// xs: the row's scales.
 template <int S, int P>
 __device__ __forceinline__ void strips_dot(const uint8_t* const (&wp)[S], const uint8_t* xp, const uint8_t* xs, int steps,
                                            int t0, int t1, int lane, v4f (&acc)[S]) {
@@ -185,7 +201,7 @@ __device__ __forceinline__ void strips_dot(const uint8_t* const (&wp)[S], const 
         const int64_t sc = (int64_t)1024 * (4 * g + in_group) + 256 * g - 12 * lane; // 4 lane, from wp's 16 lane
         v8i b[P];
 #pragma unroll
-        for (int p = 0; p < P; ++p) b[p] = e2m3_operand(xp + (int64_t)(96 * P) * t + 24 * p);
+        for (int p = 0; p < P; ++p) b[p] = e2m3_operand<P>(xp + (int64_t)(96 * P) * t, kb, p);
         const uint32_t bs = *(const uint32_t*)(xs + 16 * g + 4 * kb) >> (8 * j) & 255u;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
@@ -225,7 +241,7 @@ gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint3
             const uint8_t* const wp[4] = {gate.base + go, gate.base + go + gate.strip, up.base + uo,
                                           up.base + uo + up.strip};
             const int64_t row = perm[pos] / (uint32_t)width;
-            strips_dot<4, P>(wp, x.base + row * x.row + 24 * P * (lane >> 4), x.scales + row * x.groups * 16, steps, t0,
+            strips_dot<4, P>(wp, x.base + row * x.row, x.scales + row * x.groups * 16, steps, t0,
                              t1, lane, acc);
         }
 #pragma unroll
@@ -261,8 +277,14 @@ gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint3
             if (half == 0 && lane < 16) h.scales[(int64_t)(c0 + lane) * h.groups * 16 + scale_at(fb)] = (uint8_t)sb;
         }
         __syncthreads();
-        for (int i = tid; i < 6 * min(16, e - c0); i += kThreads)
-            *(v4u*)(h.base + (c0 + i / 6) * h.row + 96 * fb + 16 * (i % 6)) = *(const v4u*)(codes[i / 6] + 16 * (i % 6));
+        if (const int tok = tid >> 3, p = (tid >> 1) & 3; c0 + tok < e && tok < 16) {
+            uint8_t* dst = h.base + (int64_t)(c0 + tok) * h.row + (int64_t)(fb >> 2) * 384;
+            const v2u* src = (const v2u*)(codes[tok] + 24 * p);
+            if (tid & 1)
+                *(v2u*)(dst + tail_at(4, fb & 3, p)) = src[2];
+            else
+                *(v4u*)(dst + head_at(4, fb & 3, p)) = v4u{src[0].x, src[0].y, src[1].x, src[1].y};
+        }
     }
 }
 
@@ -287,7 +309,7 @@ down_kernel(Bank down, Planes h, int H, int I, int64_t n, int parts, const uint3
         v4f acc[4] = {};
         const int64_t pos = min(c0 + (lane & 15), e - 1);
         const uint8_t* const wc[4] = {wp[0], wp[1], wp[2], wp[3]};
-        strips_dot<4, 4>(wc, h.base + pos * h.row + 96 * (lane >> 4), h.scales + pos * h.groups * 16, steps, t0, t1,
+        strips_dot<4, 4>(wc, h.base + pos * h.row, h.scales + pos * h.groups * 16, steps, t0, t1,
                          lane, acc);
         __syncthreads();
 #pragma unroll
@@ -366,7 +388,8 @@ int down_parts(int64_t n, int H, int I) {
 }
 
 struct Layout {
-    size_t offsets, perm, bad, x, xs, h, hs, y, total;
+    size_t offsets, perm, bad, tiles, x, xs, h, hs, y, total;
+    int64_t max_tiles;
     int parts;
     Layout(int64_t rows, int width, int H, int I) {
         auto a256 = [](size_t b) { return (b + 255) & ~size_t(255); };
@@ -375,7 +398,9 @@ struct Layout {
         offsets = 0;
         perm = a256(offsets + (size_t)(NAIWA_SEG_MAX_KEYS + 1) * 4);
         bad = a256(perm + n * 4);
-        x = a256(bad + 4);
+        tiles = a256(bad + 4);
+        max_tiles = (int64_t)n / kTile + std::min<int64_t>((int64_t)n, NAIWA_SEG_MAX_KEYS);
+        x = a256(tiles + (size_t)(3 * max_tiles + 1) * 4);
         xs = a256(x + (size_t)rows * plane_row(4, H));
         h = a256(xs + (size_t)rows * naiwa_mx_groups(H) * 16);
         hs = a256(h + n * plane_row(4, I));
@@ -386,6 +411,9 @@ struct Layout {
 
 
 } // namespace
+
+// Whether a call takes tiles of up to 64 pairs (mxfp4_tiles.h) rather than passes of 16.
+extern "C" int naiwa_mx_tiled(int64_t n, int slots) { return n > (int64_t)16 * slots; }
 
 int naiwa_mx_check(const NaiwaMxCall& c) {
     if (!c.gate || !c.up || !c.down) return NAIWA_E_INVALID;
@@ -428,22 +456,49 @@ int naiwa_mx_run(const NaiwaMxCall& c, uint8_t* ws, hipStream_t st) {
     const Bank g{(const uint8_t*)c.gate->base, c.gate->slot_stride, naiwa_mx_strip_bytes(H)};
     const Bank u{(const uint8_t*)c.up->base, c.up->slot_stride, naiwa_mx_strip_bytes(H)};
     const Bank d{(const uint8_t*)c.down->base, c.down->slot_stride, naiwa_mx_strip_bytes(I)};
-    segments_kernel<<<1, NAIWA_SEG_THREADS, 0, st>>>(c.ids, c.skip_zero ? c.w : nullptr, n, slots, perm, offsets,
-                                                     (int*)(ws + L.bad));
     const int64_t xb = (int64_t)c.rows * 4 * naiwa_mx_steps(H);
     const unsigned pb = (unsigned)((xb + kThreads - 1) / kThreads);
-    const dim3 gg(slots, 4 * naiwa_mx_steps(I)), gd(slots, (H + 63) / 64, L.parts);
+    const bool tiled = naiwa_mx_tiled(n, slots) && (uint64_t)c.rows * xp.row <= UINT32_MAX; // the copies' offsets have 32 bits
+    Tiles tl{nullptr, nullptr, nullptr, nullptr};
+    if (tiled) {
+        tl.start = (int*)(ws + L.tiles);
+        tl.count = tl.start + L.max_tiles;
+        tl.slot = tl.count + L.max_tiles;
+        tl.n = tl.slot + L.max_tiles;
+        // pairs of weight 0 are sorted in with the others and left out by the combine
+        if (int rc = naiwa_moe_gather(c.ids, n, slots, perm, offsets, (int*)(ws + L.bad), (int64_t)st)) return rc;
+    } else {
+        segments_kernel<<<1, NAIWA_SEG_THREADS, 0, st>>>(c.ids, c.skip_zero ? c.w : nullptr, n, slots, perm, offsets,
+                                                         (int*)(ws + L.bad));
+    }
+    const unsigned px = pb + (tiled ? 1 : 0);
     if (P == 3)
-        planes_kernel<3, true><<<pb, kThreads, 0, st>>>(c.x, c.rows, H, xp);
+        planes_kernel<3, true><<<px, kThreads, 0, st>>>(c.x, c.rows, H, xp, offsets, slots, tl);
     else if (c.x_dtype == NAIWA_BF16)
-        planes_kernel<4, true><<<pb, kThreads, 0, st>>>(c.x, c.rows, H, xp);
+        planes_kernel<4, true><<<px, kThreads, 0, st>>>(c.x, c.rows, H, xp, offsets, slots, tl);
     else
-        planes_kernel<4, false><<<pb, kThreads, 0, st>>>(c.x, c.rows, H, xp);
-    if (P == 3)
-        gateup_kernel<3><<<gg, kThreads, 0, st>>>(g, u, xp, H, I, c.width, offsets, perm, c.act, hp);
-    else
-        gateup_kernel<4><<<gg, kThreads, 0, st>>>(g, u, xp, H, I, c.width, offsets, perm, c.act, hp);
-    down_kernel<<<gd, kThreads, 0, st>>>(d, hp, H, I, n, L.parts, offsets, perm, y);
+        planes_kernel<4, false><<<px, kThreads, 0, st>>>(c.x, c.rows, H, xp, offsets, slots, tl);
+    if (tiled) {
+        constexpr int NA = 4;
+        const int64_t most = n / kTile + std::min(n, slots);
+        const unsigned t8 = (unsigned)((most + 7) / 8 * 8);
+        const int xcd = n <= (int64_t)128 * slots ? 1 : 0;
+        const unsigned b1 = t8 * ((4 * naiwa_mx_steps(I) + 2 * NA - 1) / (2 * NA)), b2 = t8 * ((H / 32 + 4 * NA - 1) / (4 * NA));
+        if (P == 3)
+            tile_gateup_kernel<NA, 3><<<b1, kThreads, 2 * sizeof(Stage<3>), st>>>(g, u, xp, H, I, c.width, perm, tl, c.act,
+                                                                                  xcd, hp);
+        else
+            tile_gateup_kernel<NA, 4><<<b1, kThreads, 2 * sizeof(Stage<4>), st>>>(g, u, xp, H, I, c.width, perm, tl, c.act,
+                                                                                  xcd, hp);
+        tile_down_kernel<NA><<<b2, kThreads, 2 * sizeof(Stage<4>), st>>>(d, hp, H, I, perm, tl, xcd, y);
+    } else {
+        const dim3 gg(slots, 4 * naiwa_mx_steps(I)), gd(slots, (H + 63) / 64, L.parts);
+        if (P == 3)
+            gateup_kernel<3><<<gg, kThreads, 0, st>>>(g, u, xp, H, I, c.width, offsets, perm, c.act, hp);
+        else
+            gateup_kernel<4><<<gg, kThreads, 0, st>>>(g, u, xp, H, I, c.width, offsets, perm, c.act, hp);
+        down_kernel<<<gd, kThreads, 0, st>>>(d, hp, H, I, n, L.parts, offsets, perm, y);
+    }
     combine_kernel<<<dim3(c.rows, cs), kThreads, 0, st>>>(y, n, L.parts, c.ids, c.w, c.width, slots, H, c.skip_zero,
                                                           c.accumulate, c.out, c.res);
     return naiwa_hip_rc(hipGetLastError());

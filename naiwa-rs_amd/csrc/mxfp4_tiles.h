@@ -1,0 +1,321 @@
+// The MXFP4 experts of many tokens an expert: tiles of up to 64 sorted pairs of one slot
+// against strips of weights, on v_mfma_scale_f32_32x32x64_f8f6f4 (included by
+// mxfp4_experts.hip).
+//
+// A block of 4 waves takes one tile; a wave takes NA tiles of 32 weight rows (half of them
+// gate and half up rows, or down rows) and both halves of the tile's tokens.  A operand:
+// FP4, lane l holds block l / 32 of a 64-value step of row l % 32, 16 bytes straight from the
+// tile order in memory to registers.  B operand: one E2M3 plane, lane l block l / 32 of token
+// l % 32, from LDS.  Accumulator v of lane l is D[8 (v / 4) + 4 (l / 32) + v % 4][l % 32]: row,
+// token.
+//
+// The planes' rows (of x by token, of h by sorted pair) go to LDS by DMA in chunks of 128
+// values, two buffers deep.  A row's chunk is 3 classes of 2 P pieces of 16 bytes: the first 16
+// bytes of every plane of blocks 0 and 2 (class 0) and of blocks 1 and 3 (class 1), step by
+// step; and the last 8 bytes of a plane of both blocks of a step (class 2).  In LDS a class is
+// groups of 4 pieces (and 2 for the rest), [token][piece], the piece number xored with bits of
+// the token so that 16 neighbouring tokens' reads of one piece fall on distinct banks, while
+// 4 neighbouring lanes of a copy read 64 contiguous bytes.
+#pragma once
+
+// lane i of the wave copies 16 bytes from base + off to lds + 16 i.  Issued as inline assembly
+// so that the compiler does not make every later LDS read wait for every copy in flight; each
+// read of copied data follows an explicit vmcnt wait of the issuing wave and a barrier.
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(__attribute__((address_space(3))) const void*)p);
+}
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+// Every copy and load of this wave has landed, and every wave is here.
+__device__ __forceinline__ void landed_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+constexpr int kTile = 64; // pairs a tile
+
+struct Tiles {
+    int* start; // first sorted position
+    int* count; // pairs, at most kTile
+    int* slot;
+    int* n;     // number of tiles
+};
+
+// The sorted pairs cut into tiles of up to 64 pairs of one slot, by one block of kThreads.
+__device__ inline void tiles_block(const uint32_t* offsets, int slots, Tiles t) {
+    __shared__ int part[kThreads];
+    const int tid = threadIdx.x, per = (slots + kThreads - 1) / kThreads;
+    const int s0 = min(slots, tid * per), s1 = min(slots, s0 + per);
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) mine += (int)((offsets[s + 1] - offsets[s] + kTile - 1) / kTile);
+    part[tid] = mine;
+    __syncthreads();
+    for (int m = 1; m < kThreads; m <<= 1) {
+        const int v = tid >= m ? part[tid - m] : 0;
+        __syncthreads();
+        part[tid] += v;
+        __syncthreads();
+    }
+    int at = part[tid] - mine;
+    for (int s = s0; s < s1; ++s) {
+        const int b = (int)offsets[s], n = (int)(offsets[s + 1] - offsets[s]);
+        // the fewest tiles, of about equal numbers of 32-pair halves
+        const int subs = (n + 31) / 32, nt = (n + kTile - 1) / kTile;
+        for (int j = 0; j < nt; ++j, ++at) {
+            const int m0 = 32 * (subs * j / nt), m1 = min(n, 32 * (subs * (j + 1) / nt));
+            t.start[at] = b + m0;
+            t.count[at] = m1 - m0;
+            t.slot[at] = s;
+        }
+    }
+    if (tid == kThreads - 1) *t.n = part[tid];
+}
+
+// The (tile, column) of block b of a grid of ncol * (tiles rounded up to 8) blocks; false for a
+// block with none.  xcd: blocks are dealt to the 8 XCDs round-robin (block b to XCD b % 8), and
+// each XCD takes a run of neighbouring tiles, all columns of one after the other; otherwise
+// column by column within a tile.
+__device__ __forceinline__ bool tile_col(int b, int ntiles, int ncol, int xcd, int* tile, int* col) {
+    if (!xcd) {
+        *tile = b / ncol;
+        *col = b % ncol;
+        return *tile < ntiles;
+    }
+    const int x = b & 7, r = b >> 3;
+    const int t0 = ntiles * x / 8, t1 = ntiles * (x + 1) / 8;
+    if (r >= (t1 - t0) * ncol) return false;
+    *tile = t0 + r / ncol;
+    *col = r % ncol;
+    return true;
+}
+
+// One chunk of 64 rows in P planes.
+template <int P> struct Stage {
+    static constexpr int kFour = 2 * P / 4, kTwo = 2 * P % 4 / 2; // groups of 4 pieces and of 2, per class
+    static constexpr int kClass = 64 * 32 * P;
+    __align__(16) uint8_t v[3 * kClass];
+};
+
+// The wave's copies of chunk t: groups of 4 pieces for tokens 16 wave .. + 15, groups of 2 for
+// tokens 32 (wave & 1) .. + 31 of the classes that fall to waves 0, 1 and to waves 2, 3.
+// off4, off2: the byte offsets of the lane's rows, its piece's included.
+template <int P>
+__device__ __forceinline__ void stage(Stage<P>& st, const uint8_t* base, uint32_t off4, uint32_t off2, int t, int wave) {
+    const uint32_t lds = lds_addr(st.v), at = (uint32_t)t * (96 * P);
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+#pragma unroll
+        for (int g = 0; g < Stage<P>::kFour; ++g)
+            dma16(base, off4 + at + 32 * P * c + 64 * g, lds + Stage<P>::kClass * c + 4096 * g + 1024 * wave);
+        if (Stage<P>::kTwo && (wave >> 1) == (c & 1))
+            dma16(base, off2 + at + 32 * P * c + 64 * Stage<P>::kFour,
+                  lds + Stage<P>::kClass * c + 4096 * Stage<P>::kFour + 1024 * (wave & 1));
+    }
+}
+
+// A lane's places in a Stage: piece i of a class for token `tok`.
+template <int P> __device__ __forceinline__ int piece4(int tok, int i) { return 64 * tok + 16 * (i ^ ((tok >> 2) & 3)); }
+template <int P> __device__ __forceinline__ int piece2(int tok, int i) { return 32 * tok + 16 * (i ^ ((tok >> 3) & 1)); }
+template <int P> __device__ __forceinline__ int piece_at(int tok, int i) {
+    return i < 4 * Stage<P>::kFour ? 4096 * (i / 4) + piece4<P>(tok, i & 3)
+                                   : 4096 * Stage<P>::kFour + piece2<P>(tok, i - 4 * Stage<P>::kFour);
+}
+
+// acc[i][s] += weight tile i x token half s over all of K.  wp[i]: the tile's first strip plus
+// the lane's 16 bytes; its second strip is in the lane's pointer.  half2: the tile has more than
+// 32 pairs.  xs[s]: the lane's token's scales.
+template <int NA, int P>
+__device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base, uint32_t off4, uint32_t off2,
+                                         const uint8_t* const (&wp)[NA], const uint8_t* const (&xs)[2], int steps, bool half2,
+                                         int lane, int wave, v16f (&acc)[NA][2]) {
+    const int par = lane >> 5, tok = lane & 31;
+    stage<P>(st[0], base, off4, off2, 0, wave);
+    v4u a[2][2][NA]; // [buffer][step of the chunk][tile]
+    auto load_a = [&](int t, v4u(&o)[2][NA]) {
+        const int64_t at = (int64_t)1024 * t + 256 * (t >> 2);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < NA; ++i) o[s][i] = *(const v4u*)(wp[i] + at + 512 * s);
+    };
+    load_a(0, a[0]);
+    // the lane's scale bytes of a group of 4 chunks: a byte a chunk, blocks par and 2 + par
+    struct Scales {
+        uint32_t a[NA][2], b[2][2];
+    };
+    auto load_scales = [&](int g) {
+        Scales o;
+        const int64_t sc = (int64_t)1024 * min(4 * g + 4, steps) + 256 * g;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+                o.a[i][s] = *(const uint32_t*)(wp[i] + sc + 128 * s - 12 * (16 * par + (lane & 15)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) o.b[h][s] = *(const uint32_t*)(xs[h] + 16 * g + 4 * (2 * s + par));
+        }
+        return o;
+    };
+    const int groups = (steps + 3) / 4;
+    Scales sc = load_scales(0);
+    for (int g = 0; g < groups; ++g) {
+        const int in_group = min(4, steps - 4 * g);
+        Scales next = sc;
+#define NAIWA_MX_CHUNK(J)                                                                                              \
+    if (J < in_group) {                                                                                                \
+        const int t = 4 * g + J;                                                                                       \
+        landed_barrier();                                                                                              \
+        if (t + 1 < steps) {                                                                                           \
+            stage<P>(st[(J + 1) & 1], base, off4, off2, t + 1, wave);                                                  \
+            load_a(t + 1, a[(J + 1) & 1]);                                                                             \
+        }                                                                                                              \
+        if (J == 0 && g + 1 < groups) next = load_scales(g + 1);                                                       \
+        _Pragma("unroll") for (int s = 0; s < 2; ++s) _Pragma("unroll") for (int h = 0; h < 2; ++h) {                  \
+            if (h && !half2) break;                                                                                    \
+            _Pragma("unroll") for (int p = 0; p < P; ++p) {                                                            \
+                const uint8_t* v = st[J & 1].v;                                                                        \
+                const int k = s * P + p;                                                                               \
+                const v4u head = *(const v4u*)(v + Stage<P>::kClass * par + piece_at<P>(32 * h + tok, k));             \
+                const v2u tail = *(const v2u*)(v + Stage<P>::kClass * 2 + piece_at<P>(32 * h + tok, k) + 8 * par);     \
+                v8i b = {};                                                                                            \
+                b[0] = (int)head.x, b[1] = (int)head.y, b[2] = (int)head.z, b[3] = (int)head.w;                        \
+                b[4] = (int)tail.x, b[5] = (int)tail.y;                                                                \
+                _Pragma("unroll") for (int i = 0; i < NA; ++i)                                                         \
+                    acc[i][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                       \
+                        fp4_operand(a[J & 1][s][i]), b, acc[i][h], 4, 2, J, (int)sc.a[i][s], J,                        \
+                        (int)(sc.b[h][s] - 0x05050505u * p));                                                          \
+            }                                                                                                          \
+        }                                                                                                              \
+    }
+        NAIWA_MX_CHUNK(0)
+        NAIWA_MX_CHUNK(1)
+        NAIWA_MX_CHUNK(2)
+        NAIWA_MX_CHUNK(3)
+#undef NAIWA_MX_CHUNK
+        sc = next;
+    }
+    // the results stay where every lane computes them
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(acc[i][h]));
+}
+
+// The byte offsets of a lane's rows for the copies: row(token) of both groupings.
+template <int P, class F> __device__ __forceinline__ uint32_t copy4(int lane, int wave, F row) {
+    const int tok = 16 * wave + (lane >> 2);
+    return row(tok) + 16 * ((lane & 3) ^ ((tok >> 2) & 3));
+}
+template <int P, class F> __device__ __forceinline__ uint32_t copy2(int lane, int wave, F row) {
+    const int tok = 32 * (wave & 1) + (lane >> 1);
+    return row(tok) + 16 * ((lane & 1) ^ ((tok >> 3) & 1));
+}
+
+// Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in 4 planes.
+template <int NA, int P>
+__global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
+tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,
+                   Planes h) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    Stage<P>(&st)[2] = *reinterpret_cast<Stage<P>(*)[2]>(smem);
+    constexpr int NF = NA / 2; // feature blocks a wave
+    const int blocks = 4 * naiwa_mx_steps(I), ncol = (blocks + 4 * NF - 1) / (4 * NF);
+    int tile, col;
+    if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int start = tl.start[tile], cnt = tl.count[tile], slot = tl.slot[tile];
+    auto row = [&](int tok) -> uint32_t { return perm[start + min(tok, cnt - 1)] / (uint32_t)width; };
+    auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)x.row; };
+    const int fb0 = (4 * col + wave) * NF; // the wave's first feature block
+    const uint8_t* wp[NA];
+    const int64_t lane_at = (int64_t)((lane >> 4) & 1) * gate.strip + 256 * (lane >> 5) + 16 * (lane & 15);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int fb = min(fb0 + f, I / 32 - 1); // blocks past I read the last one again
+        wp[f] = gate.base + (int64_t)slot * gate.stride + 2 * fb * gate.strip + lane_at;
+        wp[NF + f] = up.base + (int64_t)slot * up.stride + 2 * fb * up.strip + lane_at;
+    }
+    const uint8_t* const xs[2] = {x.scales + (int64_t)row(lane & 31) * x.groups * 16,
+                                  x.scales + (int64_t)row(32 + (lane & 31)) * x.groups * 16};
+    v16f acc[NA][2] = {};
+    const uint8_t* wc[NA];
+#pragma unroll
+    for (int i = 0; i < NA; ++i) wc[i] = wp[i];
+    tile_dot<NA, P>(st, x.base, copy4<P>(lane, wave, off), copy2<P>(lane, wave, off),
+                    reinterpret_cast<const uint8_t* const(&)[NA]>(wc), xs, naiwa_mx_steps(H), cnt > 32, lane, wave, acc);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int fb = fb0 + f;
+        if (fb >= blocks) break;
+        // both halves of the tile's tokens: afterwards a lane holds the 32 features of token `lane`
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float a = naiwa_act(act, acc[f][0][i]) * acc[NF + f][0][i];
+            const float b = naiwa_act(act, acc[f][1][i]) * acc[NF + f][1][i];
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+            v[8 * (i / 4) + i % 4] = __uint_as_float(sw[0]);
+            v[8 * (i / 4) + 4 + i % 4] = __uint_as_float(sw[1]);
+        }
+        if (32 * fb >= I)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        const int sb = scale_byte(abs_max(v));
+        v6u o[4];
+        to_planes<4>(v, sb, o);
+        if (lane < cnt) {
+            const int64_t hr = start + lane;
+            uint8_t* dst = h.base + hr * h.row + (int64_t)(fb / 4) * 384;
+            const int s = (fb >> 1) & 1, par = fb & 1;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                *(v4u*)(dst + 128 * par + 16 * (4 * s + p)) = v4u{o[p][0], o[p][1], o[p][2], o[p][3]};
+                *(v2u*)(dst + 256 + 16 * (4 * s + p) + 8 * par) = v2u{o[p][4], o[p][5]};
+            }
+            h.scales[hr * h.groups * 16 + scale_at(fb)] = (uint8_t)sb;
+        }
+    }
+}
+
+// Down of a tile: NA tiles of 32 rows a wave; y[pair][H] unweighted.
+template <int NA>
+__global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
+tile_down_kernel(Bank down, Planes h, int H, int I, const uint32_t* perm, Tiles tl, int xcd, float* y) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    Stage<4>(&st)[2] = *reinterpret_cast<Stage<4>(*)[2]>(smem);
+    const int blocks = H / 32, ncol = (blocks + 4 * NA - 1) / (4 * NA);
+    int tile, col;
+    if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int start = tl.start[tile], cnt = tl.count[tile], slot = tl.slot[tile];
+    auto row = [&](int tok) -> uint32_t { return (uint32_t)min(tok, cnt - 1); };
+    auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)h.row; };
+    const int rb0 = (4 * col + wave) * NA;
+    const uint8_t* wp[NA];
+    const int64_t lane_at = (int64_t)((lane >> 4) & 1) * down.strip + 256 * (lane >> 5) + 16 * (lane & 15);
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+        wp[i] = down.base + (int64_t)slot * down.stride + 2 * min(rb0 + i, blocks - 1) * down.strip + lane_at;
+    const uint8_t* hs = h.scales + (int64_t)start * h.groups * 16;
+    const uint8_t* const xs[2] = {hs + (int64_t)row(lane & 31) * h.groups * 16,
+                                  hs + (int64_t)row(32 + (lane & 31)) * h.groups * 16};
+    v16f acc[NA][2] = {};
+    tile_dot<NA, 4>(st, h.base + (int64_t)start * h.row, copy4<4>(lane, wave, off), copy2<4>(lane, wave, off),
+                    reinterpret_cast<const uint8_t* const(&)[NA]>(wp), xs, naiwa_mx_steps(I), cnt > 32, lane, wave, acc);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const int tok = 32 * s + (lane & 31);
+        if (tok >= cnt) break;
+        float* dst = y + (int64_t)perm[start + tok] * H + 4 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (rb0 + i < blocks)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(v4f*)(dst + 32 * (rb0 + i) + 8 * q) =
+                        v4f{acc[i][s][4 * q], acc[i][s][4 * q + 1], acc[i][s][4 * q + 2], acc[i][s][4 * q + 3]};
+    }
+}
