@@ -13,7 +13,9 @@
  * models and does not train them.
  *
  * Sums are deterministic: counts are integers, and P is added up in f32 over 64 rows
- * at most and beyond that in f64, in an order that depends on the sizes alone.
+ * at most and beyond that in f64, in an order that depends on the sizes alone (and on
+ * whether logits lie so that 4 can be read at once).  The entry points share one
+ * grow-only scratch buffer per device: calls on different streams have to be ordered.
  */
 #ifndef NAIWA_BALANCE_H
 #define NAIWA_BALANCE_H
@@ -33,7 +35,8 @@ int naiwa_expert_counts(const uint32_t* ids, int ids_ld, int64_t T, int k, int E
 /* counts [E], *valid = N, probs [E] = P and *loss of a batch: logits [T, E] f32 or
  * bf16 (dtype), rows ld values apart (0: E); ids as above (ids >= E add to no count).
  * T = 0 gives zeros.  A valid token's row with a NaN or +inf gives NaN in P and the
- * loss; -inf logits have probability 0.  Masked rows are not read.  E <= 1024. */
+ * loss, and so does one of nothing but -inf; other -inf logits have probability 0.  What
+ * masked rows hold does not matter.  E <= 1024. */
 int naiwa_router_balance(const void* logits, int dtype, int ld, const uint32_t* ids, int ids_ld, int64_t T, int E,
                          int k, const uint8_t* mask, uint32_t* counts, uint32_t* valid, float* probs, float* loss,
                          int64_t stream);
