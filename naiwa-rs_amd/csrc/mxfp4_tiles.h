@@ -35,6 +35,16 @@ __device__ __forceinline__ void landed_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// Every LDS access of this wave is done, and every wave is here (loads stay in flight).
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A value that every lane has, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 constexpr int kTile = 64; // pairs a tile
 
 struct Tiles {
@@ -124,14 +134,24 @@ template <int P> __device__ __forceinline__ int piece_at(int tok, int i) {
                                    : 4096 * Stage<P>::kFour + piece2<P>(tok, i - 4 * Stage<P>::kFour);
 }
 
-// acc[i][s] += weight tile i x token half s over all of K.  wp[i]: the tile's first strip plus
-// the lane's 16 bytes; its second strip is in the lane's pointer.  half2: the tile has more than
-// 32 pairs.  xs[s]: the lane's token's scales.
-template <int NA, int P>
+// Plane k % P of the lane's block of step k / P, token `tok`.
+template <int P> __device__ __forceinline__ v6u staged_plane(const uint8_t* v, int par, int tok, int k) {
+    const v4u head = *(const v4u*)(v + Stage<P>::kClass * par + piece_at<P>(tok, k));
+    const v2u tail = *(const v2u*)(v + Stage<P>::kClass * 2 + piece_at<P>(tok, k) + 8 * par);
+    return v6u{head.x, head.y, head.z, head.w, tail.x, tail.y};
+}
+
+// acc[i][s] += weight tile i x token half s < NH over all of K.  wp[i]: the tile's first strip, the
+// same for every lane; strip: bytes to its second.  xs: the scales of row 0, xo[s] the lane's
+// token's offset.  A chunk's operands (step, half, plane) are read from LDS one ahead of the products.
+template <int NA, int P, int NH>
 __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base, uint32_t off4, uint32_t off2,
-                                         const uint8_t* const (&wp)[NA], const uint8_t* const (&xs)[2], int steps, bool half2,
-                                         int lane, int wave, v16f (&acc)[NA][2]) {
+                                         const uint8_t* const (&wp)[NA], uint32_t strip, const uint8_t* xs,
+                                         const uint32_t (&xo)[2], int steps, int lane, int wave, v16f (&acc)[NA][2]) {
     const int par = lane >> 5, tok = lane & 31;
+    // the lane's 16 bytes of weights and 4 of scales: row lane % 16 of a strip, block par
+    const uint32_t lw = ((lane >> 4) & 1) * strip + 256 * par + 16 * (lane & 15);
+    const uint32_t ls = ((lane >> 4) & 1) * strip + 64 * par + 4 * (lane & 15);
     stage<P>(st[0], base, off4, off2, 0, wave);
     v4u a[2][2][NA]; // [buffer][step of the chunk][tile]
     auto load_a = [&](int t, v4u(&o)[2][NA]) {
@@ -139,7 +159,7 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < NA; ++i) o[s][i] = *(const v4u*)(wp[i] + at + 512 * s);
+            for (int i = 0; i < NA; ++i) o[s][i] = *(const v4u*)(wp[i] + at + lw + 512 * s);
     };
     load_a(0, a[0]);
     // the lane's scale bytes of a group of 4 chunks: a byte a chunk, blocks par and 2 + par
@@ -153,9 +173,9 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
             for (int i = 0; i < NA; ++i)
-                o.a[i][s] = *(const uint32_t*)(wp[i] + sc + 128 * s - 12 * (16 * par + (lane & 15)));
+                o.a[i][s] = *(const uint32_t*)(wp[i] + sc + ls + 128 * s);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) o.b[h][s] = *(const uint32_t*)(xs[h] + 16 * g + 4 * (2 * s + par));
+            for (int h = 0; h < NH; ++h) o.b[h][s] = *(const uint32_t*)(xs + 16 * g + (xo[h] + 4 * par) + 8 * s);
         }
         return o;
     };
@@ -173,21 +193,22 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
             load_a(t + 1, a[(J + 1) & 1]);                                                                             \
         }                                                                                                              \
         if (J == 0 && g + 1 < groups) next = load_scales(g + 1);                                                       \
-        _Pragma("unroll") for (int s = 0; s < 2; ++s) _Pragma("unroll") for (int h = 0; h < 2; ++h) {                  \
-            if (h && !half2) break;                                                                                    \
-            _Pragma("unroll") for (int p = 0; p < P; ++p) {                                                            \
-                const uint8_t* v = st[J & 1].v;                                                                        \
-                const int k = s * P + p;                                                                               \
-                const v4u head = *(const v4u*)(v + Stage<P>::kClass * par + piece_at<P>(32 * h + tok, k));             \
-                const v2u tail = *(const v2u*)(v + Stage<P>::kClass * 2 + piece_at<P>(32 * h + tok, k) + 8 * par);     \
-                v8i b = {};                                                                                            \
-                b[0] = (int)head.x, b[1] = (int)head.y, b[2] = (int)head.z, b[3] = (int)head.w;                        \
-                b[4] = (int)tail.x, b[5] = (int)tail.y;                                                                \
-                _Pragma("unroll") for (int i = 0; i < NA; ++i)                                                         \
-                    acc[i][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                       \
-                        fp4_operand(a[J & 1][s][i]), b, acc[i][h], 4, 2, J, (int)sc.a[i][s], J,                        \
-                        (int)(sc.b[h][s] - 0x05050505u * p));                                                          \
+        const uint8_t* v = st[J & 1].v;                                                                                \
+        v6u b[2];                                                                                                      \
+        b[0] = staged_plane<P>(v, par, tok, 0);                                                                             \
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                                             \
+        _Pragma("unroll") for (int o = 0; o < 2 * NH * P; ++o) {                                                       \
+            const int s = o / (NH * P), h = o / P % NH, p = o % P;                                                     \
+            if (o + 1 < 2 * NH * P) {                                                                                  \
+                const int n = o + 1, k = n / (NH * P) * P + n % P;                                                     \
+                b[n & 1] = staged_plane<P>(v, par, 32 * (n / P % NH) + tok, k);                                             \
             }                                                                                                          \
+            _Pragma("unroll") for (int i = 0; i < NA; ++i)                                                             \
+                acc[i][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                           \
+                    fp4_operand(a[J & 1][s][i]), e2m3_operand(b[o & 1]), acc[i][h], 4, 2, J, (int)sc.a[i][s], J,                     \
+                    (int)(sc.b[h][s] - 0x05050505u * p));                                                              \
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                                         \
+            __builtin_amdgcn_sched_group_barrier(0x008, NA, 0);                                                        \
         }                                                                                                              \
     }
         NAIWA_MX_CHUNK(0)
@@ -201,7 +222,7 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
 #pragma unroll
     for (int i = 0; i < NA; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) asm volatile("" : "+v"(acc[i][h]));
+        for (int h = 0; h < NH; ++h) asm volatile("" : "+v"(acc[i][h]));
 }
 
 // The byte offsets of a lane's rows for the copies: row(token) of both groupings.
@@ -214,8 +235,8 @@ template <int P, class F> __device__ __forceinline__ uint32_t copy2(int lane, in
     return row(tok) + 16 * ((lane & 1) ^ ((tok >> 3) & 1));
 }
 
-// Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in 4 planes.
-template <int NA, int P>
+// Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in PH planes.
+template <int NA, int P, int PH>
 __global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
 tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,
                    Planes h) {
@@ -226,26 +247,24 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
     int tile, col;
     if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int start = tl.start[tile], cnt = tl.count[tile], slot = tl.slot[tile];
+    const int start = uniform(tl.start[tile]), cnt = uniform(tl.count[tile]), slot = uniform(tl.slot[tile]);
     auto row = [&](int tok) -> uint32_t { return perm[start + min(tok, cnt - 1)] / (uint32_t)width; };
     auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)x.row; };
     const int fb0 = (4 * col + wave) * NF; // the wave's first feature block
     const uint8_t* wp[NA];
-    const int64_t lane_at = (int64_t)((lane >> 4) & 1) * gate.strip + 256 * (lane >> 5) + 16 * (lane & 15);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const int fb = min(fb0 + f, I / 32 - 1); // blocks past I read the last one again
-        wp[f] = gate.base + (int64_t)slot * gate.stride + 2 * fb * gate.strip + lane_at;
-        wp[NF + f] = up.base + (int64_t)slot * up.stride + 2 * fb * up.strip + lane_at;
+        wp[f] = gate.base + (int64_t)slot * gate.stride + 2 * fb * gate.strip;
+        wp[NF + f] = up.base + (int64_t)slot * up.stride + 2 * fb * up.strip;
     }
-    const uint8_t* const xs[2] = {x.scales + (int64_t)row(lane & 31) * x.groups * 16,
-                                  x.scales + (int64_t)row(32 + (lane & 31)) * x.groups * 16};
+    const uint32_t xo[2] = {row(lane & 31) * (uint32_t)x.groups * 16, row(32 + (lane & 31)) * (uint32_t)x.groups * 16};
     v16f acc[NA][2] = {};
-    const uint8_t* wc[NA];
-#pragma unroll
-    for (int i = 0; i < NA; ++i) wc[i] = wp[i];
-    tile_dot<NA, P>(st, x.base, copy4<P>(lane, wave, off), copy2<P>(lane, wave, off),
-                    reinterpret_cast<const uint8_t* const(&)[NA]>(wc), xs, naiwa_mx_steps(H), cnt > 32, lane, wave, acc);
+    const uint32_t off4 = copy4<P>(lane, wave, off), off2 = copy2<P>(lane, wave, off);
+    if (cnt > 32)
+        tile_dot<NA, P, 2>(st, x.base, off4, off2, wp, (uint32_t)gate.strip, x.scales, xo, naiwa_mx_steps(H), lane, wave, acc);
+    else
+        tile_dot<NA, P, 1>(st, x.base, off4, off2, wp, (uint32_t)gate.strip, x.scales, xo, naiwa_mx_steps(H), lane, wave, acc);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const int fb = fb0 + f;
@@ -264,47 +283,40 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.0f;
         const int sb = scale_byte(abs_max(v));
-        v6u o[4];
-        to_planes<4>(v, sb, o);
-        if (lane < cnt) {
-            const int64_t hr = start + lane;
-            uint8_t* dst = h.base + hr * h.row + (int64_t)(fb / 4) * 384;
-            const int s = (fb >> 1) & 1, par = fb & 1;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                *(v4u*)(dst + 128 * par + 16 * (4 * s + p)) = v4u{o[p][0], o[p][1], o[p][2], o[p][3]};
-                *(v2u*)(dst + 256 + 16 * (4 * s + p) + 8 * par) = v2u{o[p][4], o[p][5]};
-            }
-            h.scales[hr * h.groups * 16 + scale_at(fb)] = (uint8_t)sb;
-        }
+        v6u o[PH];
+        to_planes<PH>(v, sb, o);
+        if (lane < cnt)
+            put_block<PH>(h.base + (int64_t)(start + lane) * h.row, h.scales + (int64_t)(start + lane) * h.groups * 16, fb, o, sb);
     }
 }
 
 // Down of a tile: NA tiles of 32 rows a wave; y[pair][H] unweighted.
-template <int NA>
+template <int NA, int P>
 __global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
 tile_down_kernel(Bank down, Planes h, int H, int I, const uint32_t* perm, Tiles tl, int xcd, float* y) {
     extern __shared__ __align__(16) uint8_t smem[];
-    Stage<4>(&st)[2] = *reinterpret_cast<Stage<4>(*)[2]>(smem);
+    Stage<P>(&st)[2] = *reinterpret_cast<Stage<P>(*)[2]>(smem);
     const int blocks = H / 32, ncol = (blocks + 4 * NA - 1) / (4 * NA);
     int tile, col;
     if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int start = tl.start[tile], cnt = tl.count[tile], slot = tl.slot[tile];
+    const int start = uniform(tl.start[tile]), cnt = uniform(tl.count[tile]), slot = uniform(tl.slot[tile]);
     auto row = [&](int tok) -> uint32_t { return (uint32_t)min(tok, cnt - 1); };
     auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)h.row; };
     const int rb0 = (4 * col + wave) * NA;
     const uint8_t* wp[NA];
-    const int64_t lane_at = (int64_t)((lane >> 4) & 1) * down.strip + 256 * (lane >> 5) + 16 * (lane & 15);
 #pragma unroll
     for (int i = 0; i < NA; ++i)
-        wp[i] = down.base + (int64_t)slot * down.stride + 2 * min(rb0 + i, blocks - 1) * down.strip + lane_at;
+        wp[i] = down.base + (int64_t)slot * down.stride + 2 * min(rb0 + i, blocks - 1) * down.strip;
     const uint8_t* hs = h.scales + (int64_t)start * h.groups * 16;
-    const uint8_t* const xs[2] = {hs + (int64_t)row(lane & 31) * h.groups * 16,
-                                  hs + (int64_t)row(32 + (lane & 31)) * h.groups * 16};
+    const uint32_t xo[2] = {row(lane & 31) * (uint32_t)h.groups * 16, row(32 + (lane & 31)) * (uint32_t)h.groups * 16};
     v16f acc[NA][2] = {};
-    tile_dot<NA, 4>(st, h.base + (int64_t)start * h.row, copy4<4>(lane, wave, off), copy2<4>(lane, wave, off),
-                    reinterpret_cast<const uint8_t* const(&)[NA]>(wp), xs, naiwa_mx_steps(I), cnt > 32, lane, wave, acc);
+    const uint8_t* rows = h.base + (int64_t)start * h.row;
+    const uint32_t off4 = copy4<P>(lane, wave, off), off2 = copy2<P>(lane, wave, off);
+    if (cnt > 32)
+        tile_dot<NA, P, 2>(st, rows, off4, off2, wp, (uint32_t)down.strip, hs, xo, naiwa_mx_steps(I), lane, wave, acc);
+    else
+        tile_dot<NA, P, 1>(st, rows, off4, off2, wp, (uint32_t)down.strip, hs, xo, naiwa_mx_steps(I), lane, wave, acc);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const int tok = 32 * s + (lane & 31);
