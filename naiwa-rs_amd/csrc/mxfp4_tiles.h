@@ -10,7 +10,8 @@
 // token.
 //
 // The planes' rows (of x by token, of h by sorted pair) go to LDS by DMA in chunks of 128
-// values, two buffers deep.  A row's chunk is 3 classes of 2 P pieces of 16 bytes: the first 16
+// values: of 64 rows two chunks deep, of 32 (a tile of at most 32 pairs, which HBM bounds)
+// four.  A row's chunk is 3 classes of 2 P pieces of 16 bytes: the first 16
 // bytes of every plane of blocks 0 and 2 (class 0) and of blocks 1 and 3 (class 1), step by
 // step; and the last 8 bytes of a plane of both blocks of a step (class 2).  In LDS a class is
 // groups of 4 pieces (and 2 for the rest), [token][piece], the piece number xored with bits of
@@ -28,9 +29,9 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :: "v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
-// Every copy and load of this wave has landed, and every wave is here.
-__device__ __forceinline__ void landed_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// All but the last N copies and loads of this wave have landed, and every wave is here.
+template <int N> __device__ __forceinline__ void landed_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -102,58 +103,74 @@ __device__ __forceinline__ bool tile_col(int b, int ntiles, int ncol, int xcd, i
     return true;
 }
 
-// One chunk of 64 rows in P planes.
-template <int P> struct Stage {
+// One chunk of 32 NH rows in P planes.
+template <int P, int NH> struct Stage {
+    static constexpr int kRows = 32 * NH;
     static constexpr int kFour = 2 * P / 4, kTwo = 2 * P % 4 / 2; // groups of 4 pieces and of 2, per class
-    static constexpr int kClass = 64 * 32 * P;
+    static constexpr int kClass = kRows * 32 * P;
     __align__(16) uint8_t v[3 * kClass];
 };
+// LDS of a tile kernel: the same for either.
+template <int P> constexpr size_t kStageBytes = 2 * sizeof(Stage<P, 2>);
+static_assert(2 * sizeof(Stage<3, 2>) == 4 * sizeof(Stage<3, 1>), "two chunks of 64 rows or four of 32");
 
-// The wave's copies of chunk t: groups of 4 pieces for tokens 16 wave .. + 15, groups of 2 for
-// tokens 32 (wave & 1) .. + 31 of the classes that fall to waves 0, 1 and to waves 2, 3.
-// off4, off2: the byte offsets of the lane's rows, its piece's included.
-template <int P>
-__device__ __forceinline__ void stage(Stage<P>& st, const uint8_t* base, uint32_t off4, uint32_t off2, int t, int wave) {
-    const uint32_t lds = lds_addr(st.v), at = (uint32_t)t * (96 * P);
+// The wave's copies of chunk t to `st`.  NH = 2: groups of 4 pieces for tokens 16 wave .. + 15,
+// groups of 2 for tokens 32 (wave & 1) .. + 31 of the classes that fall to waves 0, 1 and to
+// waves 2, 3.  NH = 1: groups of 4 for tokens 16 (wave & 1) .. + 15, every second group to waves 0,
+// 1; groups of 2 to waves 2, 3, 2 (P = 3) or 0, 1, 2.  off4, off2: the byte offsets of the lane's
+// rows, its piece's included.
+template <int P, int NH>
+__device__ __forceinline__ void stage(uint8_t* st, const uint8_t* base, uint32_t off4, uint32_t off2, int t, int wave) {
+    using S = Stage<P, NH>;
+    const uint32_t lds = lds_addr(st), at = (uint32_t)t * (96 * P);
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
 #pragma unroll
-        for (int g = 0; g < Stage<P>::kFour; ++g)
-            dma16(base, off4 + at + 32 * P * c + 64 * g, lds + Stage<P>::kClass * c + 4096 * g + 1024 * wave);
-        if (Stage<P>::kTwo && (wave >> 1) == (c & 1))
-            dma16(base, off2 + at + 32 * P * c + 64 * Stage<P>::kFour,
-                  lds + Stage<P>::kClass * c + 4096 * Stage<P>::kFour + 1024 * (wave & 1));
+        for (int g = 0; g < S::kFour; ++g)
+            if (NH == 2 || (wave >> 1) == ((c * S::kFour + g) & 1))
+                dma16(base, off4 + at + 32 * P * c + 64 * g,
+                      lds + S::kClass * c + 64 * S::kRows * g + 1024 * (NH == 2 ? wave : wave & 1));
+        const bool mine = NH == 2 ? (wave >> 1) == (c & 1) : wave == (P == 3 ? 2 + (c & 1) : c);
+        if (S::kTwo && mine)
+            dma16(base, off2 + at + 32 * P * c + 64 * S::kFour,
+                  lds + S::kClass * c + 64 * S::kRows * S::kFour + (NH == 2 ? 1024 * (wave & 1) : 0));
     }
 }
+// The fewest copies that a wave has in a chunk (NH = 1).
+template <int P> constexpr int kCopies = P == 3 ? 2 : 3;
 
-// A lane's places in a Stage: piece i of a class for token `tok`.
-template <int P> __device__ __forceinline__ int piece4(int tok, int i) { return 64 * tok + 16 * (i ^ ((tok >> 2) & 3)); }
-template <int P> __device__ __forceinline__ int piece2(int tok, int i) { return 32 * tok + 16 * (i ^ ((tok >> 3) & 1)); }
-template <int P> __device__ __forceinline__ int piece_at(int tok, int i) {
-    return i < 4 * Stage<P>::kFour ? 4096 * (i / 4) + piece4<P>(tok, i & 3)
-                                   : 4096 * Stage<P>::kFour + piece2<P>(tok, i - 4 * Stage<P>::kFour);
+// A lane's place in a Stage: piece i of a class for token `tok`.
+template <int P, int NH> __device__ __forceinline__ int piece_at(int tok, int i) {
+    using S = Stage<P, NH>;
+    return i < 4 * S::kFour ? 64 * S::kRows * (i / 4) + 64 * tok + 16 * ((i & 3) ^ ((tok >> 2) & 3))
+                            : 64 * S::kRows * S::kFour + 32 * tok + 16 * ((i - 4 * S::kFour) ^ ((tok >> 3) & 1));
 }
 
 // Plane k % P of the lane's block of step k / P, token `tok`.
-template <int P> __device__ __forceinline__ v6u staged_plane(const uint8_t* v, int par, int tok, int k) {
-    const v4u head = *(const v4u*)(v + Stage<P>::kClass * par + piece_at<P>(tok, k));
-    const v2u tail = *(const v2u*)(v + Stage<P>::kClass * 2 + piece_at<P>(tok, k) + 8 * par);
+template <int P, int NH> __device__ __forceinline__ v6u staged_plane(const uint8_t* v, int par, int tok, int k) {
+    const v4u head = *(const v4u*)(v + Stage<P, NH>::kClass * par + piece_at<P, NH>(tok, k));
+    const v2u tail = *(const v2u*)(v + Stage<P, NH>::kClass * 2 + piece_at<P, NH>(tok, k) + 8 * par);
     return v6u{head.x, head.y, head.z, head.w, tail.x, tail.y};
 }
 
 // acc[i][s] += weight tile i x token half s < NH over all of K.  wp[i]: the tile's first strip, the
 // same for every lane; strip: bytes to its second.  xs: the scales of row 0, xo[s] the lane's
 // token's offset.  A chunk's operands (step, half, plane) are read from LDS one ahead of the products.
+// D chunks deep: before chunk t its copies have to have landed.  After them the wave issued the
+// weights of chunk t (2 NA loads) and, with D = 4, the copies and weights of chunks t + 1 and
+// t + 2 (loads and copies end in the order of their issue), so all but that many may be under
+// way; there are fewer of them for the last chunks, which wait for everything.
 template <int NA, int P, int NH>
-__device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base, uint32_t off4, uint32_t off2,
+__device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint32_t off4, uint32_t off2,
                                          const uint8_t* const (&wp)[NA], uint32_t strip, const uint8_t* xs,
                                          const uint32_t (&xo)[2], int steps, int lane, int wave, v16f (&acc)[NA][2]) {
+    constexpr int D = NH == 1 ? 4 : 2, kUnder = D == 4 ? 2 * NA + 2 * (kCopies<P> + 2 * NA) : 0;
+    constexpr uint32_t kStage = sizeof(Stage<P, NH>);
     const int par = lane >> 5, tok = lane & 31;
     // the lane's 16 bytes of weights and 4 of scales: row lane % 16 of a strip, block par
     const uint32_t lw = ((lane >> 4) & 1) * strip + 256 * par + 16 * (lane & 15);
     const uint32_t ls = ((lane >> 4) & 1) * strip + 64 * par + 4 * (lane & 15);
-    stage<P>(st[0], base, off4, off2, 0, wave);
-    v4u a[2][2][NA]; // [buffer][step of the chunk][tile]
+    v4u a[D][2][NA]; // [buffer][step of the chunk][tile]
     auto load_a = [&](int t, v4u(&o)[2][NA]) {
         const int64_t at = (int64_t)1024 * t + 256 * (t >> 2);
 #pragma unroll
@@ -161,7 +178,12 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
 #pragma unroll
             for (int i = 0; i < NA; ++i) o[s][i] = *(const v4u*)(wp[i] + at + lw + 512 * s);
     };
-    load_a(0, a[0]);
+#pragma unroll
+    for (int t = 0; t < D - 1; ++t)
+        if (t < steps) {
+            stage<P, NH>(st + kStage * t, base, off4, off2, t, wave);
+            load_a(t, a[t]);
+        }
     // the lane's scale bytes of a group of 4 chunks: a byte a chunk, blocks par and 2 + par
     struct Scales {
         uint32_t a[NA][2], b[2][2];
@@ -187,25 +209,28 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
 #define NAIWA_MX_CHUNK(J)                                                                                              \
     if (J < in_group) {                                                                                                \
         const int t = 4 * g + J;                                                                                       \
-        landed_barrier();                                                                                              \
-        if (t + 1 < steps) {                                                                                           \
-            stage<P>(st[(J + 1) & 1], base, off4, off2, t + 1, wave);                                                  \
-            load_a(t + 1, a[(J + 1) & 1]);                                                                             \
+        if (D == 2 || t + 2 >= steps)                                                                                  \
+            landed_barrier<0>();                                                                                       \
+        else                                                                                                           \
+            landed_barrier<kUnder>();                                                                                  \
+        if (t + D - 1 < steps) {                                                                                       \
+            stage<P, NH>(st + kStage * ((J + D - 1) % D), base, off4, off2, t + D - 1, wave);                          \
+            load_a(t + D - 1, a[(J + D - 1) % D]);                                                                     \
         }                                                                                                              \
         if (J == 0 && g + 1 < groups) next = load_scales(g + 1);                                                       \
-        const uint8_t* v = st[J & 1].v;                                                                                \
+        const uint8_t* v = st + kStage * (J % D);                                                                      \
         v6u b[2];                                                                                                      \
-        b[0] = staged_plane<P>(v, par, tok, 0);                                                                             \
+        b[0] = staged_plane<P, NH>(v, par, tok, 0);                                                                             \
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                                             \
         _Pragma("unroll") for (int o = 0; o < 2 * NH * P; ++o) {                                                       \
             const int s = o / (NH * P), h = o / P % NH, p = o % P;                                                     \
             if (o + 1 < 2 * NH * P) {                                                                                  \
                 const int n = o + 1, k = n / (NH * P) * P + n % P;                                                     \
-                b[n & 1] = staged_plane<P>(v, par, 32 * (n / P % NH) + tok, k);                                             \
+                b[n & 1] = staged_plane<P, NH>(v, par, 32 * (n / P % NH) + tok, k);                                             \
             }                                                                                                          \
             _Pragma("unroll") for (int i = 0; i < NA; ++i)                                                             \
                 acc[i][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                           \
-                    fp4_operand(a[J & 1][s][i]), e2m3_operand(b[o & 1]), acc[i][h], 4, 2, J, (int)sc.a[i][s], J,                     \
+                    fp4_operand(a[J % D][s][i]), e2m3_operand(b[o & 1]), acc[i][h], 4, 2, J, (int)sc.a[i][s], J,                     \
                     (int)(sc.b[h][s] - 0x05050505u * p));                                                              \
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                                         \
             __builtin_amdgcn_sched_group_barrier(0x008, NA, 0);                                                        \
@@ -226,12 +251,12 @@ __device__ __forceinline__ void tile_dot(Stage<P> (&st)[2], const uint8_t* base,
 }
 
 // The byte offsets of a lane's rows for the copies: row(token) of both groupings.
-template <int P, class F> __device__ __forceinline__ uint32_t copy4(int lane, int wave, F row) {
-    const int tok = 16 * wave + (lane >> 2);
+template <int NH, class F> __device__ __forceinline__ uint32_t copy4(int lane, int wave, F row) {
+    const int tok = 16 * (NH == 2 ? wave : wave & 1) + (lane >> 2);
     return row(tok) + 16 * ((lane & 3) ^ ((tok >> 2) & 3));
 }
-template <int P, class F> __device__ __forceinline__ uint32_t copy2(int lane, int wave, F row) {
-    const int tok = 32 * (wave & 1) + (lane >> 1);
+template <int NH, class F> __device__ __forceinline__ uint32_t copy2(int lane, int wave, F row) {
+    const int tok = 32 * (NH == 2 ? wave & 1 : 0) + (lane >> 1);
     return row(tok) + 16 * ((lane & 1) ^ ((tok >> 3) & 1));
 }
 
@@ -241,7 +266,6 @@ __global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
 tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,
                    Planes h) {
     extern __shared__ __align__(16) uint8_t smem[];
-    Stage<P>(&st)[2] = *reinterpret_cast<Stage<P>(*)[2]>(smem);
     constexpr int NF = NA / 2; // feature blocks a wave
     const int blocks = 4 * naiwa_mx_steps(I), ncol = (blocks + 4 * NF - 1) / (4 * NF);
     int tile, col;
@@ -260,11 +284,14 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
     }
     const uint32_t xo[2] = {row(lane & 31) * (uint32_t)x.groups * 16, row(32 + (lane & 31)) * (uint32_t)x.groups * 16};
     v16f acc[NA][2] = {};
-    const uint32_t off4 = copy4<P>(lane, wave, off), off2 = copy2<P>(lane, wave, off);
+    const int steps = naiwa_mx_steps(H);
+    const uint32_t strip = (uint32_t)gate.strip;
     if (cnt > 32)
-        tile_dot<NA, P, 2>(st, x.base, off4, off2, wp, (uint32_t)gate.strip, x.scales, xo, naiwa_mx_steps(H), lane, wave, acc);
+        tile_dot<NA, P, 2>(smem, x.base, copy4<2>(lane, wave, off), copy2<2>(lane, wave, off), wp, strip, x.scales, xo, steps,
+                           lane, wave, acc);
     else
-        tile_dot<NA, P, 1>(st, x.base, off4, off2, wp, (uint32_t)gate.strip, x.scales, xo, naiwa_mx_steps(H), lane, wave, acc);
+        tile_dot<NA, P, 1>(smem, x.base, copy4<1>(lane, wave, off), copy2<1>(lane, wave, off), wp, strip, x.scales, xo, steps,
+                           lane, wave, acc);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const int fb = fb0 + f;
@@ -290,12 +317,13 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
     }
 }
 
-// Down of a tile: NA tiles of 32 rows a wave; y[pair][H] unweighted.
+// Down of a tile and a K part of part_groups groups of 4 steps: NA tiles of 32 rows a wave;
+// y[part][pair][H] unweighted.
 template <int NA, int P>
 __global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
-tile_down_kernel(Bank down, Planes h, int H, int I, const uint32_t* perm, Tiles tl, int xcd, float* y) {
+tile_down_kernel(Bank down, Planes h, int H, int I, int64_t n, int part_groups, const uint32_t* perm, Tiles tl, int xcd,
+                 float* y) {
     extern __shared__ __align__(16) uint8_t smem[];
-    Stage<P>(&st)[2] = *reinterpret_cast<Stage<P>(*)[2]>(smem);
     const int blocks = H / 32, ncol = (blocks + 4 * NA - 1) / (4 * NA);
     int tile, col;
     if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
@@ -303,25 +331,28 @@ tile_down_kernel(Bank down, Planes h, int H, int I, const uint32_t* perm, Tiles 
     const int start = uniform(tl.start[tile]), cnt = uniform(tl.count[tile]), slot = uniform(tl.slot[tile]);
     auto row = [&](int tok) -> uint32_t { return (uint32_t)min(tok, cnt - 1); };
     auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)h.row; };
-    const int rb0 = (4 * col + wave) * NA;
+    const int rb0 = (4 * col + wave) * NA, g0 = blockIdx.y * part_groups;
+    const int steps = min(naiwa_mx_steps(I) - 4 * g0, 4 * part_groups);
     const uint8_t* wp[NA];
 #pragma unroll
     for (int i = 0; i < NA; ++i)
-        wp[i] = down.base + (int64_t)slot * down.stride + 2 * min(rb0 + i, blocks - 1) * down.strip;
-    const uint8_t* hs = h.scales + (int64_t)start * h.groups * 16;
+        wp[i] = down.base + (int64_t)slot * down.stride + 2 * min(rb0 + i, blocks - 1) * down.strip + (int64_t)4352 * g0;
+    const uint8_t* hs = h.scales + (int64_t)start * h.groups * 16 + 16 * g0;
     const uint32_t xo[2] = {row(lane & 31) * (uint32_t)h.groups * 16, row(32 + (lane & 31)) * (uint32_t)h.groups * 16};
     v16f acc[NA][2] = {};
-    const uint8_t* rows = h.base + (int64_t)start * h.row;
-    const uint32_t off4 = copy4<P>(lane, wave, off), off2 = copy2<P>(lane, wave, off);
+    const uint8_t* rows = h.base + (int64_t)start * h.row + (int64_t)4 * g0 * 96 * P;
+    const uint32_t strip = (uint32_t)down.strip;
     if (cnt > 32)
-        tile_dot<NA, P, 2>(st, rows, off4, off2, wp, (uint32_t)down.strip, hs, xo, naiwa_mx_steps(I), lane, wave, acc);
+        tile_dot<NA, P, 2>(smem, rows, copy4<2>(lane, wave, off), copy2<2>(lane, wave, off), wp, strip, hs, xo, steps, lane,
+                           wave, acc);
     else
-        tile_dot<NA, P, 1>(st, rows, off4, off2, wp, (uint32_t)down.strip, hs, xo, naiwa_mx_steps(I), lane, wave, acc);
+        tile_dot<NA, P, 1>(smem, rows, copy4<1>(lane, wave, off), copy2<1>(lane, wave, off), wp, strip, hs, xo, steps, lane,
+                           wave, acc);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const int tok = 32 * s + (lane & 31);
         if (tok >= cnt) break;
-        float* dst = y + (int64_t)perm[start + tok] * H + 4 * (lane >> 5);
+        float* dst = y + (blockIdx.y * n + perm[start + tok]) * H + 4 * (lane >> 5);
 #pragma unroll
         for (int i = 0; i < NA; ++i)
             if (rb0 + i < blocks)
