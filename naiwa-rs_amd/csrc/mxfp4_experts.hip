@@ -646,7 +646,7 @@ int run_pass(const NaiwaMxCall& c, uint8_t* ws, hipStream_t st) {
         r.combine(1);
         return naiwa_hip_rc(hipGetLastError());
     }
-    if (!c.skip_zero) return r.go<3, 4, true>(); // a prompt chunk
+    if (!c.skip_zero) return r.go<4, 4, true>(); // a prompt chunk
     return c.x_dtype == NAIWA_BF16 ? r.go<4, 5, true>() : r.go<5, 5, false>();
 }
 

@@ -19,6 +19,8 @@
 // 4 neighbouring lanes of a copy read 64 contiguous bytes.
 #pragma once
 
+#include <type_traits>
+
 // lane i of the wave copies 16 bytes from base + off to lds + 16 i.  Issued as inline assembly
 // so that the compiler does not make every later LDS read wait for every copy in flight; each
 // read of copied data follows an explicit vmcnt wait of the issuing wave and a barrier.
@@ -112,32 +114,36 @@ template <int P, int NH> struct Stage {
 };
 // LDS of a tile kernel: the same for either.
 template <int P> constexpr size_t kStageBytes = 2 * sizeof(Stage<P, 2>);
-static_assert(2 * sizeof(Stage<3, 2>) == 4 * sizeof(Stage<3, 1>), "two chunks of 64 rows or four of 32");
+static_assert(2 * sizeof(Stage<5, 2>) == 4 * sizeof(Stage<5, 1>), "two chunks of 64 rows or four of 32");
 
-// The wave's copies of chunk t to `st`.  NH = 2: groups of 4 pieces for tokens 16 wave .. + 15,
-// groups of 2 for tokens 32 (wave & 1) .. + 31 of the classes that fall to waves 0, 1 and to
-// waves 2, 3.  NH = 1: groups of 4 for tokens 16 (wave & 1) .. + 15, every second group to waves 0,
-// 1; groups of 2 to waves 2, 3, 2 (P = 3) or 0, 1, 2.  off4, off2: the byte offsets of the lane's
-// rows, its piece's included.
+// The wave's copies of chunk t to `st`.  NH = 2: both groups of 4 pieces for tokens 16 wave ..
+// + 15; NH = 1: one of them, for tokens 16 (wave & 1) .. + 15.  Groups of 2 for 32 tokens: NH =
+// 2, of classes 0 and 2 by waves 0 and 1, of class 1 by waves 2 and 3, twice; NH = 1, of class 0,
+// 1, 2, 2 by wave 0 .. 3.  Every wave has as many copies, so that no branch divides them.
+// off4, off2: the byte offsets of the lane's rows, its piece's included.
 template <int P, int NH>
 __device__ __forceinline__ void stage(uint8_t* st, const uint8_t* base, uint32_t off4, uint32_t off2, int t, int wave) {
     using S = Stage<P, NH>;
+    static_assert(S::kFour == 2);
     const uint32_t lds = lds_addr(st), at = (uint32_t)t * (96 * P);
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
 #pragma unroll
-        for (int g = 0; g < S::kFour; ++g)
-            if (NH == 2 || (wave >> 1) == ((c * S::kFour + g) & 1))
-                dma16(base, off4 + at + 32 * P * c + 64 * g,
-                      lds + S::kClass * c + 64 * S::kRows * g + 1024 * (NH == 2 ? wave : wave & 1));
-        const bool mine = NH == 2 ? (wave >> 1) == (c & 1) : wave == (P == 3 ? 2 + (c & 1) : c);
-        if (S::kTwo && mine)
+        for (int i = 0; i < NH; ++i) {
+            const int g = NH == 2 ? i : wave >> 1;
+            dma16(base, off4 + at + 32 * P * c + 64 * g,
+                  lds + S::kClass * c + 64 * S::kRows * g + 1024 * (NH == 2 ? wave : wave & 1));
+        }
+    }
+    if (S::kTwo) {
+#pragma unroll
+        for (int i = 0; i < NH; ++i) {
+            const int c = NH == 1 ? min(wave, 2) : wave < 2 ? 2 * i : 1;
             dma16(base, off2 + at + 32 * P * c + 64 * S::kFour,
                   lds + S::kClass * c + 64 * S::kRows * S::kFour + (NH == 2 ? 1024 * (wave & 1) : 0));
+        }
     }
 }
-// The fewest copies that a wave has in a chunk (NH = 1).
-template <int P> constexpr int kCopies = P == 3 ? 2 : 3;
 
 // A lane's place in a Stage: piece i of a class for token `tok`.
 template <int P, int NH> __device__ __forceinline__ int piece_at(int tok, int i) {
@@ -156,93 +162,110 @@ template <int P, int NH> __device__ __forceinline__ v6u staged_plane(const uint8
 // acc[i][s] += weight tile i x token half s < NH over all of K.  wp[i]: the tile's first strip, the
 // same for every lane; strip: bytes to its second.  xs: the scales of row 0, xo[s] the lane's
 // token's offset.  A chunk's operands (step, half, plane) are read from LDS one ahead of the products.
-// D chunks deep: before chunk t its copies have to have landed.  After them the wave issued the
-// weights of chunk t (2 NA loads) and, with D = 4, the copies and weights of chunks t + 1 and
-// t + 2 (loads and copies end in the order of their issue), so all but that many may be under
-// way; there are fewer of them for the last chunks, which wait for everything.
+// Loads and copies end in the order of their issue.  Before chunk t its copies have to have
+// landed; the wave issued since then at least the weights of chunk t + 1 (NH = 2), or those of
+// chunk t and the copies and weights of chunks t + 1 and t + 2 (NH = 1): kUnder may be under way.
+// Past the end the last chunk is loaded again, into buffers that nothing reads, so that this
+// holds to the end and the loop has no branches (the compiler waits for every load where paths
+// with different loads meet).  The empty asm makes the compiler wait for the weights before the
+// next loads are issued: it does not know of the copies and would count them among the weights.
 template <int NA, int P, int NH>
 __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint32_t off4, uint32_t off2,
                                          const uint8_t* const (&wp)[NA], uint32_t strip, const uint8_t* xs,
                                          const uint32_t (&xo)[2], int steps, int lane, int wave, v16f (&acc)[NA][2]) {
-    constexpr int D = NH == 1 ? 4 : 2, kUnder = D == 4 ? 2 * NA + 2 * (kCopies<P> + 2 * NA) : 0;
+    // D chunks of the rows and DA of the weights are in LDS and registers or on the way
+    constexpr int D = NH == 1 ? 4 : 2, DA = NH == 1 ? 4 : 3, kCopies = P == 5 ? 4 : 3;
+    constexpr int kUnder = NH == 1 ? 2 * NA + 2 * (kCopies + 2 * NA) : 2 * NA;
     constexpr uint32_t kStage = sizeof(Stage<P, NH>);
     const int par = lane >> 5, tok = lane & 31;
     // the lane's 16 bytes of weights and 4 of scales: row lane % 16 of a strip, block par
     const uint32_t lw = ((lane >> 4) & 1) * strip + 256 * par + 16 * (lane & 15);
     const uint32_t ls = ((lane >> 4) & 1) * strip + 64 * par + 4 * (lane & 15);
-    v4u a[D][2][NA]; // [buffer][step of the chunk][tile]
+    v4u a[4][2][NA]; // [chunk mod 4][step of the chunk][tile]
     auto load_a = [&](int t, v4u(&o)[2][NA]) {
+        t = min(t, steps - 1);
         const int64_t at = (int64_t)1024 * t + 256 * (t >> 2);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < NA; ++i) o[s][i] = *(const v4u*)(wp[i] + at + lw + 512 * s);
     };
-#pragma unroll
-    for (int t = 0; t < D - 1; ++t)
-        if (t < steps) {
-            stage<P, NH>(st + kStage * t, base, off4, off2, t, wave);
-            load_a(t, a[t]);
-        }
+    auto copy = [&](int t, int buffer) {
+        stage<P, NH>(st + kStage * buffer, base, off4, off2, min(t, steps - 1), wave);
+    };
     // the lane's scale bytes of a group of 4 chunks: a byte a chunk, blocks par and 2 + par
     struct Scales {
-        uint32_t a[NA][2], b[2][2];
+        uint32_t a[NA][2], b[NH][2];
     };
+    const int groups = (steps + 3) / 4;
     auto load_scales = [&](int g) {
+        g = min(g, groups - 1);
         Scales o;
         const int64_t sc = (int64_t)1024 * min(4 * g + 4, steps) + 256 * g;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int i = 0; i < NA; ++i)
-                o.a[i][s] = *(const uint32_t*)(wp[i] + sc + ls + 128 * s);
+            for (int i = 0; i < NA; ++i) o.a[i][s] = *(const uint32_t*)(wp[i] + sc + ls + 128 * s);
 #pragma unroll
             for (int h = 0; h < NH; ++h) o.b[h][s] = *(const uint32_t*)(xs + 16 * g + (xo[h] + 4 * par) + 8 * s);
         }
         return o;
     };
-    const int groups = (steps + 3) / 4;
-    Scales sc = load_scales(0);
-    for (int g = 0; g < groups; ++g) {
-        const int in_group = min(4, steps - 4 * g);
-        Scales next = sc;
-#define NAIWA_MX_CHUNK(J)                                                                                              \
-    if (J < in_group) {                                                                                                \
-        const int t = 4 * g + J;                                                                                       \
-        if (D == 2 || t + 2 >= steps)                                                                                  \
-            landed_barrier<0>();                                                                                       \
-        else                                                                                                           \
-            landed_barrier<kUnder>();                                                                                  \
-        if (t + D - 1 < steps) {                                                                                       \
-            stage<P, NH>(st + kStage * ((J + D - 1) % D), base, off4, off2, t + D - 1, wave);                          \
-            load_a(t + D - 1, a[(J + D - 1) % D]);                                                                     \
-        }                                                                                                              \
-        if (J == 0 && g + 1 < groups) next = load_scales(g + 1);                                                       \
-        const uint8_t* v = st + kStage * (J % D);                                                                      \
-        v6u b[2];                                                                                                      \
-        b[0] = staged_plane<P, NH>(v, par, tok, 0);                                                                             \
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                                             \
-        _Pragma("unroll") for (int o = 0; o < 2 * NH * P; ++o) {                                                       \
-            const int s = o / (NH * P), h = o / P % NH, p = o % P;                                                     \
-            if (o + 1 < 2 * NH * P) {                                                                                  \
-                const int n = o + 1, k = n / (NH * P) * P + n % P;                                                     \
-                b[n & 1] = staged_plane<P, NH>(v, par, 32 * (n / P % NH) + tok, k);                                             \
-            }                                                                                                          \
-            _Pragma("unroll") for (int i = 0; i < NA; ++i)                                                             \
-                acc[i][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                           \
-                    fp4_operand(a[J % D][s][i]), e2m3_operand(b[o & 1]), acc[i][h], 4, 2, J, (int)sc.a[i][s], J,                     \
-                    (int)(sc.b[h][s] - 0x05050505u * p));                                                              \
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);                                                         \
-            __builtin_amdgcn_sched_group_barrier(0x008, NA, 0);                                                        \
-        }                                                                                                              \
+    Scales sc = load_scales(0), next;
+#pragma unroll
+    for (int t = 0; t < DA - 1; ++t) {
+        if (t < D - 1) copy(t, t);
+        load_a(t, a[t]);
     }
-        NAIWA_MX_CHUNK(0)
-        NAIWA_MX_CHUNK(1)
-        NAIWA_MX_CHUNK(2)
-        NAIWA_MX_CHUNK(3)
-#undef NAIWA_MX_CHUNK
+    auto chunk = [&](auto j, int g) {
+        constexpr int J = decltype(j)::value;
+        const int t = 4 * g + J;
+        landed_barrier<kUnder>();
+#pragma unroll
+        for (int i = 0; i < NA; ++i) asm volatile("" : "+v"(a[J][0][i]), "+v"(a[J][1][i]));
+        if constexpr (J == 0) next = load_scales(g + 1);
+        if constexpr (J == 3) {
+#pragma unroll
+            for (int i = 0; i < NA; ++i) asm volatile("" : "+v"(next.a[i][0]), "+v"(next.a[i][1]));
+#pragma unroll
+            for (int h = 0; h < NH; ++h) asm volatile("" : "+v"(next.b[h][0]), "+v"(next.b[h][1]));
+        }
+        copy(t + D - 1, (J + D - 1) % D);
+        load_a(t + DA - 1, a[(J + DA - 1) % 4]);
+        __builtin_amdgcn_sched_barrier(0); // the loads first
+        const uint8_t* v = st + kStage * (J % D);
+        v6u b[2];
+        b[0] = staged_plane<P, NH>(v, par, tok, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+        for (int o = 0; o < 2 * NH * P; ++o) {
+            const int s = o / (NH * P), h = o / P % NH, p = o % P;
+            if (o + 1 < 2 * NH * P) {
+                const int n = o + 1, k = n / (NH * P) * P + n % P;
+                b[n & 1] = staged_plane<P, NH>(v, par, 32 * (n / P % NH) + tok, k);
+            }
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+                acc[i][h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                    fp4_operand(a[J][s][i]), e2m3_operand(b[o & 1]), acc[i][h], 4, 2, J, (int)sc.a[i][s], J,
+                    (int)(sc.b[h][s] - 0x05050505u * p));
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, NA, 0);
+        }
+    };
+    using std::integral_constant;
+    int g = 0;
+    for (; g < steps / 4; ++g) {
+        chunk(integral_constant<int, 0>{}, g);
+        chunk(integral_constant<int, 1>{}, g);
+        chunk(integral_constant<int, 2>{}, g);
+        chunk(integral_constant<int, 3>{}, g);
         sc = next;
     }
+    const int rest = steps - 4 * g;
+    if (rest > 0) chunk(integral_constant<int, 0>{}, g);
+    if (rest > 1) chunk(integral_constant<int, 1>{}, g);
+    if (rest > 2) chunk(integral_constant<int, 2>{}, g);
     // the results stay where every lane computes them
 #pragma unroll
     for (int i = 0; i < NA; ++i)
@@ -298,10 +321,19 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
         if (fb >= blocks) break;
         // both halves of the tile's tokens: afterwards a lane holds the 32 features of token `lane`
         float v[32];
+        auto fold = [&](auto f_act) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) acc[f][s][i] = f_act(acc[f][s][i]) * acc[NF + f][s][i];
+        };
+        if (act == NAIWA_ACT_GELU_PYTORCH_TANH) // one branch, not one a value
+            fold([](float g) { return naiwa_gelu_tanh(g); });
+        else
+            fold([](float g) { return naiwa_silu(g); });
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float a = naiwa_act(act, acc[f][0][i]) * acc[NF + f][0][i];
-            const float b = naiwa_act(act, acc[f][1][i]) * acc[NF + f][1][i];
+            const float a = acc[f][0][i], b = acc[f][1][i];
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
             v[8 * (i / 4) + i % 4] = __uint_as_float(sw[0]);
             v[8 * (i / 4) + 4 + i % 4] = __uint_as_float(sw[1]);
