@@ -165,10 +165,11 @@ template <int P, int NH> __device__ __forceinline__ v6u staged_plane(const uint8
 // Loads and copies end in the order of their issue.  Before chunk t its copies have to have
 // landed; the wave issued since then at least the weights of chunk t + 1 (NH = 2), or those of
 // chunk t and the copies and weights of chunks t + 1 and t + 2 (NH = 1): kUnder may be under way.
-// Past the end the last chunk is loaded again, into buffers that nothing reads, so that this
-// holds to the end and the loop has no branches (the compiler waits for every load where paths
-// with different loads meet).  The empty asm makes the compiler wait for the weights before the
-// next loads are issued: it does not know of the copies and would count them among the weights.
+// The loop issues them without branches, of the last chunk again where there are no more, since
+// the compiler waits for every load where paths with different loads meet; the last group
+// issues what there is and waits for everything from its second chunk on.  The empty asm makes
+// the compiler wait for the weights before the next loads are issued: it does not know of
+// the copies, and a later wait of its own would count them among the weights.
 template <int NA, int P, int NH>
 __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint32_t off4, uint32_t off2,
                                          const uint8_t* const (&wp)[NA], uint32_t strip, const uint8_t* xs,
@@ -217,21 +218,23 @@ __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint3
         if (t < D - 1) copy(t, t);
         load_a(t, a[t]);
     }
-    auto chunk = [&](auto j, int g) {
+    const int last = (steps - 1) / 4; // the last group, of 1 to 4 chunks
+    auto chunk = [&](auto j, auto in_last, int g) {
         constexpr int J = decltype(j)::value;
+        constexpr bool kLast = decltype(in_last)::value;
         const int t = 4 * g + J;
-        landed_barrier<kUnder>();
+        landed_barrier<kLast && J ? 0 : kUnder>();
 #pragma unroll
         for (int i = 0; i < NA; ++i) asm volatile("" : "+v"(a[J][0][i]), "+v"(a[J][1][i]));
-        if constexpr (J == 0) next = load_scales(g + 1);
-        if constexpr (J == 3) {
+        if constexpr (J == 0 && !kLast) next = load_scales(g + 1);
+        if constexpr (J == 3 && !kLast) {
 #pragma unroll
             for (int i = 0; i < NA; ++i) asm volatile("" : "+v"(next.a[i][0]), "+v"(next.a[i][1]));
 #pragma unroll
             for (int h = 0; h < NH; ++h) asm volatile("" : "+v"(next.b[h][0]), "+v"(next.b[h][1]));
         }
-        copy(t + D - 1, (J + D - 1) % D);
-        load_a(t + DA - 1, a[(J + DA - 1) % 4]);
+        if (!kLast || t + D - 1 < steps) copy(t + D - 1, (J + D - 1) % D);
+        if (!kLast || t + DA - 1 < steps) load_a(t + DA - 1, a[(J + DA - 1) % 4]);
         __builtin_amdgcn_sched_barrier(0); // the loads first
         const uint8_t* v = st + kStage * (J % D);
         v6u b[2];
@@ -253,19 +256,23 @@ __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint3
             __builtin_amdgcn_sched_group_barrier(0x008, NA, 0);
         }
     };
-    using std::integral_constant;
-    int g = 0;
-    for (; g < steps / 4; ++g) {
-        chunk(integral_constant<int, 0>{}, g);
-        chunk(integral_constant<int, 1>{}, g);
-        chunk(integral_constant<int, 2>{}, g);
-        chunk(integral_constant<int, 3>{}, g);
+    const std::integral_constant<int, 0> c0;
+    const std::integral_constant<int, 1> c1;
+    const std::integral_constant<int, 2> c2;
+    const std::integral_constant<int, 3> c3;
+    for (int g = 0; g < last; ++g) {
+        chunk(c0, std::false_type{}, g);
+        chunk(c1, std::false_type{}, g);
+        chunk(c2, std::false_type{}, g);
+        chunk(c3, std::false_type{}, g);
         sc = next;
     }
-    const int rest = steps - 4 * g;
-    if (rest > 0) chunk(integral_constant<int, 0>{}, g);
-    if (rest > 1) chunk(integral_constant<int, 1>{}, g);
-    if (rest > 2) chunk(integral_constant<int, 2>{}, g);
+    const int rest = steps - 4 * last;
+    chunk(c0, std::true_type{}, last);
+    if (rest > 1) chunk(c1, std::true_type{}, last);
+    if (rest > 2) chunk(c2, std::true_type{}, last);
+    if (rest > 3) chunk(c3, std::true_type{}, last);
+    if (rest == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // copies of no use: LDS ends with the block
     // the results stay where every lane computes them
 #pragma unroll
     for (int i = 0; i < NA; ++i)

@@ -1,5 +1,6 @@
-"""The compiled MXFP4 experts (CPU only): M0 belongs to the LDS copies, and the several-pass
-conversions to and from E2M3 never write over their own operands."""
+"""The compiled MXFP4 experts (CPU only): M0 belongs to the LDS copies, the tiles' counted waits
+cover the copies they are for, and the several-pass conversions to and from E2M3 never write
+over their own operands."""
 import os
 import re
 import subprocess
@@ -10,7 +11,7 @@ import test_asm_invariants as inv
 
 
 @pytest.fixture(scope="module")
-def asm(tmp_path_factory):
+def text(tmp_path_factory):
     b = inv._build_module()
     if not os.path.exists(b.HIPCC):
         pytest.skip("hipcc is not installed")
@@ -20,8 +21,12 @@ def asm(tmp_path_factory):
                         os.path.join(b.CSRC, "mxfp4_experts.hip"), "-o", str(out)], capture_output=True, text=True,
                        timeout=900)
     assert r.returncode == 0, r.stderr[-2000:]
-    lines = [l.split(";")[0].strip() for l in out.read_text().splitlines()]
-    return [l for l in lines if l and not l.startswith(".")]
+    return [l.split(";")[0].strip() for l in out.read_text().splitlines()]
+
+
+@pytest.fixture(scope="module")
+def asm(text):
+    return [l for l in text if l and not l.startswith(".")]
 
 
 def test_m0_belongs_to_the_lds_copies(asm):
@@ -56,3 +61,77 @@ def test_conversions_do_not_overwrite_their_operands(asm):
 
 def test_nothing_spills(asm):
     assert not [l for l in asm if l.startswith("scratch_")]
+
+
+def _blocks(text, kernel):
+    """{label: (instructions, successors)} of a kernel's basic blocks, and the first label."""
+    start = next(i for i, l in enumerate(text) if re.match(rf"_Z\w*{kernel}\w*:", l))
+    end = next(i for i in range(start, len(text)) if text[i].startswith(".Lfunc_end"))
+    blocks, order, label, n = {"entry": []}, ["entry"], "entry", 0
+    for l in text[start + 1:end]:
+        m = re.match(r"(\.LBB\w+):", l)
+        if m:
+            label = m.group(1)
+        elif l and not l.startswith("."):
+            blocks.setdefault(label, []).append(l)
+            if re.match(r"s_c?branch", l):     # what follows a branch is a block of its own
+                n += 1
+                label = f"after{n}"
+            else:
+                continue
+        else:
+            continue
+        order.append(label)
+        blocks.setdefault(label, [])
+    out = {}
+    for i, b in enumerate(order):
+        ends = blocks[b][-1] if blocks[b] else ""
+        to = [ends.split()[1]] if re.match(r"s_c?branch", ends) else []
+        if not re.match(r"s_branch|s_endpgm", ends) and i + 1 < len(order):
+            to.append(order[i + 1])
+        out[b] = (blocks[b], to)
+    return out
+
+
+@pytest.mark.parametrize("kernel,copies", [("tile_gateup_kernelILi2ELi4ELi4E", 3), ("tile_gateup_kernelILi2ELi4ELi5E", 3),
+                                           ("tile_gateup_kernelILi2ELi5ELi5E", 4), ("tile_down_kernelILi2ELi4E", 3),
+                                           ("tile_down_kernelILi2ELi5E", 4)])
+def test_counted_waits_cover_their_copies(text, kernel, copies):
+    """Along every path to a barrier behind a wait that lets N loads be under way, at least N loads follow the
+    copies of the chunk that is read next: the newest copies before the barrier where the tile is two
+    chunks deep (2 `copies` a chunk), those of two chunks earlier where it is four deep."""
+    blocks = _blocks(text, kernel)
+    # a path's state: loads issued since the end of each of the last 3 runs of copies, the newest first
+    # ("run": copies with no other load between them); None: not on a path yet
+    state = {b: set() for b in blocks}
+    state["entry"] = {(False, ())}
+    work, waits, seen = ["entry"], {}, 0
+    while work:
+        b = work.pop()
+        cur = set(state[b])
+        body, to = blocks[b]
+        for i, l in enumerate(body):
+            lds, load = l.startswith("global_load_lds"), l.startswith(("global_load", "global_store", "scratch_"))
+            if load:
+                nxt = set()
+                for in_run, runs in cur:
+                    if lds and in_run:
+                        nxt.add((True, ((0, runs[0][1] + 1),) + tuple((n + 1, c) for n, c in runs[1:])))
+                    else:
+                        runs = tuple((n + 1, c) for n, c in runs)
+                        nxt.add((lds, (((0, 1),) + runs)[:3]) if lds else (False, runs))
+                cur = {(r, tuple((min(n, 64), c) for n, c in s)) for r, s in nxt}
+            m = re.match(r"s_waitcnt vmcnt\((\d+)\) lgkmcnt\(0\)$", l)
+            if m and i + 1 < len(body) and body[i + 1] == "s_barrier" and int(m.group(1)):
+                for _, runs in cur:
+                    waits.setdefault(int(m.group(1)), set()).add(runs)
+        for t in to:
+            if not cur <= state[t]:
+                state[t] |= cur
+                work.append(t)
+    assert sorted(waits) == [4, 4 + 2 * (copies + 4)]
+    for n, paths in waits.items():
+        for runs in paths:
+            deep = n != 4
+            need = runs[2] if deep else runs[0]
+            assert need[1] == (copies if deep else 2 * copies) and need[0] >= n, (n, runs)
