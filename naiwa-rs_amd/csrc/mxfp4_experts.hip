@@ -560,6 +560,15 @@ namespace {
 
 constexpr int kNA = 2; // tiles of 32 weight rows a wave of the tile kernels
 
+// Whether tiles of ncol columns of blocks are dealt to the XCDs in runs (tile_col): where an
+// XCD's 64 blocks at a time take several tiles with all their columns, neighbouring tiles of an
+// expert share weights in its L2; with more columns, an XCD's share of every tile's columns
+// does.  In microseconds, runs and not, prompt chunks: gate/up 6 columns (Qwen3-30B, 1999 tokens)
+// 250 and 274, 11 (DeepSeek-V2-Lite, 2048) 289 and 321, 16 (8 experts of 1024 x 2048, 512) 46.9 and
+// 45.8, 112 (Mixtral-8x7B, 4096) 3180 and 2822; down 8 columns (Qwen3) 250 and 255, 16 (Mixtral)
+// 2822 and 2814.
+int xcd_order(int ncol) { return ncol < 16; }
+
 struct Run { // one pass's pieces
     const NaiwaMxCall& c;
     Layout L;
@@ -579,13 +588,14 @@ struct Run { // one pass's pieces
         combine_kernel<<<dim3(c.rows, cs), kThreads, 0, st>>>(y(), n, parts, c.ids, c.w, c.width, slots, H, c.skip_zero,
                                                              c.accumulate, c.out, c.res);
     }
-    // Down of at most `most` tiles, and the combine.
-    template <int PH> void down(int64_t most, int xcd) const {
-        const unsigned blocks = (unsigned)(most * ((H / 32 + 4 * kNA - 1) / (4 * kNA)));
+    // Down of at most `most` tiles (a multiple of 8), and the combine.
+    template <int PH> void down(int64_t most) const {
+        const int ncol = (H / 32 + 4 * kNA - 1) / (4 * kNA);
+        const unsigned blocks = (unsigned)(most * ncol);
         const int groups = naiwa_mx_groups(I), part = (groups + down_parts(n, blocks, H, I) - 1) / down_parts(n, blocks, H, I);
         const int parts = (groups + part - 1) / part;
         tile_down_kernel<kNA, PH><<<dim3(blocks, parts), kThreads, kStageBytes<PH>, st>>>(d, h(PH), H, I, n, part, perm, tl,
-                                                                                          xcd, y());
+                                                                                          xcd_order(ncol), y());
         combine(parts);
     }
 
@@ -593,12 +603,14 @@ struct Run { // one pass's pieces
     template <int PX, int PH, bool BF16> bool one() const {
         const size_t xl = (size_t)plane_row(PX, H) + (size_t)naiwa_mx_groups(H) * 16;
         const size_t hl = ((size_t)plane_row(PH, I) + (size_t)naiwa_mx_groups(I) * 16) * c.width;
-        constexpr size_t kLds = 32 * 1024;
+        // With the kernels' own 17 and 33 KB, what a CU has.  One token of H 16384, 4 experts of 1024
+        // top-2, 31 us here and 74 as a tile; of 8 Mixtral-8x7B experts (h of 2 x 14336) 51 and 63.
+        constexpr size_t kLds = 120 * 1024;
         if (xl > kLds) return false;
         gateup_one_kernel<PX, PH, BF16><<<dim3(c.width, 4 * naiwa_mx_steps(I)), kThreads, xl, st>>>(
             g, u, c.x, H, I, c.ids, c.w, c.width, slots, c.skip_zero, c.act, h(PH), perm, tl);
         if (hl > kLds) {
-            down<PH>((n + 7) / 8 * 8, 0);
+            down<PH>((n + 7) / 8 * 8);
             return true;
         }
         int split = 1;
@@ -610,7 +622,11 @@ struct Run { // one pass's pieces
 
     template <int PX, int PH, bool BF16> int go() const {
         if (c.rows == 1 && one<PX, PH, BF16>()) return naiwa_hip_rc(hipGetLastError());
-        const bool sort = n <= 1024; // in the planes' launch; more pairs take a launch of their own
+        // The pairs are sorted in the planes' launch; many pairs, whose sorting takes its one block
+        // longer than the planes take, in a launch of their own.  A call at Qwen3-30B sizes, in the
+        // launch and apart: 128 pairs 52.5 and 54.1 us, 512 77.0 and 78.2, 768 81.3 and 80.4, 2048 115
+        // and 105.
+        const bool sort = n <= 512;
         const Beside with{c.ids, c.skip_zero ? c.w : nullptr, n, slots, perm, offsets, (int*)(ws + L.bad), tl};
         const unsigned pb = (unsigned)(((int64_t)c.rows * 4 * naiwa_mx_steps(H) + kThreads - 1) / kThreads) + 1;
         if (sort) {
@@ -620,13 +636,12 @@ struct Run { // one pass's pieces
             if (int rc = naiwa_moe_gather(c.ids, n, slots, perm, offsets, (int*)(ws + L.bad), (int64_t)st)) return rc;
             planes_kernel<PX, BF16, false><<<pb, kThreads, 0, st>>>(c.x, c.rows, H, x(PX), with);
         }
-        // XCD order while the experts average at most two tiles (the rule of prefill.hip)
         const int64_t most = (n / kTile + std::min(n, slots) + 7) / 8 * 8;
-        const int xcd = n <= (int64_t)128 * slots ? 1 : 0;
-        const unsigned blocks = (unsigned)(most * ((4 * naiwa_mx_steps(I) + 2 * kNA - 1) / (2 * kNA)));
+        const int ncol = (4 * naiwa_mx_steps(I) + 2 * kNA - 1) / (2 * kNA);
+        const unsigned blocks = (unsigned)(most * ncol);
         tile_gateup_kernel<kNA, PX, PH><<<blocks, kThreads, kStageBytes<PX>, st>>>(g, u, x(PX), H, I, c.width, perm, tl, c.act,
-                                                                                  xcd, h(PH));
-        down<PH>(most, xcd);
+                                                                                  xcd_order(ncol), h(PH));
+        down<PH>(most);
         return naiwa_hip_rc(hipGetLastError());
     }
 };

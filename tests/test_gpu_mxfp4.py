@@ -3,12 +3,13 @@
 Tolerance of the products.  An activation enters in planes of E2M3 whose last rounding has
 steps of at most 2^-2 2^(-5 (P - 1)) where the block's largest magnitude M is at least 2
 (csrc/mxfp4_experts.hip): an error of rms at most 2^-3 2^(-5 (P - 1)) / sqrt(12) M, that is
-1.1e-6 M for 4 planes.  In a block of normal values M is about 2.5 times the rms: 2.8e-6 of
-a value, for h, with its heavier tail, up to 5 times: 5.5e-6; f32 x enters gate and up.
-bf16 x is exact but for values under 2^-12 M (4 planes) or 2^-7 M (3 planes: 1 % of normal
-values, off by rms 2^-14 / sqrt(3) M / 2: 2.8e-6 of the norm).  f32 sums of K products add
-about sqrt(K) 2^-24, 4e-6 at K 4096, and the activation a few 2^-24.  Together, as squares:
-sqrt(2 * 2.8^2 + 5.5^2 + 4^2) 1e-6 = 7.9e-6; 1e-5 holds every case.
+1.1e-6 M for 4 planes (bf16 x, h of a prompt chunk), 3.4e-8 M for 5 (f32 x, h of a decode
+call).  In a block of normal values M is about 2.5 times the rms: 2.8e-6 of a value, for h,
+with its heavier tail, up to 5 times: 5.5e-6.  bf16 x is exact but for values under 2^-12 M.
+f32 sums of K products add about sqrt(K) 2^-24, 4e-6 at K 4096 and 1.1e-5 at 33024 if the
+additions' errors were all of the size of the whole sum; partial sums grow as they are added,
+which halves that: 6e-6.  Together, as squares: sqrt(2 * 2.8^2 + 5.5^2 + 4^2) 1e-6 = 7.9e-6, and
+sqrt(6^2 + 4^2) 1e-6 = 7.2e-6 for the longest rows with 5 planes; 1e-5 holds every case.
 """
 import numpy as np
 import pytest
@@ -173,6 +174,12 @@ def decode(nm, ex, x, ids, w, act="silu", out0=None, f32=False, noalloc=False):
     (1, 1, 32, 32, 1), (1, 8, 1024, 2048, 2), (1, 16, 2048, 768, 8), (2, 4, 160, 96, 3), (3, 8, 672, 1408, 6),
     (5, 8, 2048, 1408, 6), (16, 4, 512, 512, 2), (17, 2, 416, 224, 1), (33, 3, 288, 160, 2), (64, 4, 2880, 736, 2),
     (130, 4, 256, 128, 3), (96, 16, 544, 96, 8), (7, 2, 64, 4096, 2),
+    (9, 2, 4256, 1056, 2),     # 33.25 steps of x: a last group of two
+    (5, 3, 96, 2080, 2),       # h in two unequal K parts
+    (300, 8, 128, 96, 4),      # more pairs than are sorted beside the planes
+    (1, 8, 128, 4096, 8),      # one token whose h fills more than LDS
+    (1, 1, 33024, 32, 1),      # and whose x does
+    (1, 2, 11008, 64, 2), (2, 64, 64, 32, 64),
 ])
 @pytest.mark.parametrize("f32", [False, True])
 def test_decode_against_64_bits(gpu, T, E, H, I, k, f32):
@@ -451,3 +458,136 @@ def test_prefill_stream_over_mxfp4(gpu):
         nm.synchronize()
         got = out.download(np.float32).reshape(T, H)
         assert rel(got, M.experts(x, ids, w, *src[l].w, skip_zero=False)) < REL
+
+
+# ---- as callers use them -----------------------------------------------------------------------
+
+
+def test_quantise_route_and_run(gpu):
+    """A layer from f32 weights to its output: quantised on the device, routed, its routing counted and scored,
+    decoded token by token, as a batch and as a prompt chunk, which agree."""
+    nm = gpu
+    rng = np.random.default_rng(80)
+    T, E, H, I, k = 24, 8, 288, 160, 2
+    banks = nm.LayerBanks(E, H, I, (nm.MXFP4_T,) * 3, contiguous=True)
+    w64 = []
+    for bank, n, kk in ((banks.gate, I, H), (banks.up, I, H), (banks.down, H, I)):
+        raw = bf16(rng.standard_normal((E, n, kk)) * 0.05)
+        nm.mxfp4_quantize(nm.DeviceBuffer.from_array(raw), nm.BF16, n, kk, bank.desc().base, batch=E, dst_stride=bank.stride)
+        back = nm.DeviceBuffer(E * n * kk * 4)
+        nm.mxfp4_dequantize(bank.desc().base, n, kk, back, nm.F32, batch=E, src_stride=bank.stride)
+        v = back.download(np.float32).reshape(E, n, kk).astype(np.float64)
+        for e in range(E):
+            assert np.array_equal(v[e], M.values(*M.quantize(f32_of(raw[e]))))
+        w64.append(list(v))
+    x = f32_of(bf16(rng.standard_normal((T, H))))
+    xd = nm.DeviceBuffer.from_array(bf16(x))
+    router = nm.DeviceBuffer.from_array((rng.standard_normal((E, H)) * 0.1).astype(np.float32))
+    ids, w, logits = nm.DeviceBuffer(T * k * 4), nm.DeviceBuffer(T * k * 4), nm.DeviceBuffer(T * E * 4)
+    nm.router_topk(xd, nm.BF16, router, T, H, E, k, ids, w, logits_out=logits)
+    counts, valid, probs, loss = (nm.DeviceBuffer(n * 4) for n in (E, 1, E, 1))
+    nm.router_balance(logits, nm.F32, ids, T, E, k, counts, valid, probs, loss)
+    idn, wn = ids.download(np.uint32).reshape(T, k), w.download(np.float32).reshape(T, k)
+    lg = logits.download(np.float32).reshape(T, E).astype(np.float64)
+    p = np.exp(lg - lg.max(-1, keepdims=True))
+    p = (p / p.sum(-1, keepdims=True)).mean(0)
+    c = np.bincount(idn.ravel(), minlength=E)
+    assert np.array_equal(counts.download(np.uint32), c) and valid.download(np.uint32)[0] == T
+    assert abs(loss.download(np.float32)[0] - E / (k * T) * (c * p).sum()) < 4e-6 * E
+    want = M.experts(x, idn, wn, *w64, skip_zero=False)
+    out = nm.DeviceBuffer(T * H * 4)
+    nm.moe_prefill(banks, xd, ids, w, T, k, out)
+    chunk = out.download(np.float32).reshape(T, H)
+    nm.indexed_moe_fused_decode(banks, xd, nm.BF16, ids, w, T, k, out)
+    batch = out.download(np.float32).reshape(T, H)
+    one = nm.DeviceBuffer(H * 4)
+    for t in range(T):
+        nm.indexed_moe_fused_decode(banks, xd.ptr + t * H * 2, nm.BF16, ids.ptr + t * k * 4, w.ptr + t * k * 4, 1, k, one)
+        assert rel(one.download(np.float32), want[t]) < REL
+    assert rel(chunk, want) < REL and rel(batch, want) < REL
+
+
+def test_streams_and_calls_of_changing_size(gpu):
+    """Calls of many sizes one after the other on a stream of the caller's, nothing between them: each has the
+    scratch of the one before, larger and smaller, and the bits of a call alone."""
+    nm = gpu
+    rng = np.random.default_rng(81)
+    E, H, I, k = 4, 352, 224, 2
+    ex = Experts(nm, 82, E, H, I)
+    st = nm.Stream()
+    jobs = []
+    for T in (70, 1, 9, 400, 1, 33, 2):
+        ids, w = route(rng, T, E, k)
+        x = f32_of(bf16(rng.standard_normal((T, H))))
+        jobs.append((x, ids, w, decode(nm, ex, x, ids, w), prefill(nm, ex, x, ids, w)[0]))
+    bufs = [(nm.DeviceBuffer.from_array(bf16(x)), nm.DeviceBuffer.from_array(ids), nm.DeviceBuffer.from_array(w),
+             nm.DeviceBuffer(x.size * 4), nm.DeviceBuffer(x.size * 4)) for x, ids, w, _, _ in jobs]
+    nm.synchronize()
+    for (x, ids, w, _, _), (xd, idd, wd, o1, o2) in zip(jobs, bufs):
+        T = len(ids)
+        nm.indexed_moe_fused_decode(ex.banks, xd, nm.BF16, idd, wd, T, k, o1, stream=st.handle)
+        nm.moe_prefill(ex.banks, xd, idd, wd, T, k, o2, stream=st.handle)
+    st.sync()
+    for (x, _, _, d, p), (_, _, _, o1, o2) in zip(jobs, bufs):
+        assert np.array_equal(o1.download(np.float32).reshape(x.shape), d)
+        assert np.array_equal(o2.download(np.float32).reshape(x.shape), p)
+
+
+def test_slots_past_4_gib(gpu):
+    """Banks whose slots lie gigabytes apart, and a quantisation whose projections do."""
+    nm = gpu
+    rng = np.random.default_rng(83)
+    E, H, I, k, gap = 4, 256, 96, 2, 3 << 29      # slot 3 starts at 4.5 GiB
+    near = Experts(nm, 84, E, H, I)
+    arena = nm.DeviceBuffer(3 * gap + (1 << 20))
+    offs = (0, 1 << 18, 1 << 19)
+    far = [nm.SlotBank(E, b.n, b.k, nm.MXFP4_T, base=arena.ptr + o, stride=gap)
+           for b, o in zip((near.banks.gate, near.banks.up, near.banks.down), offs)]
+    for b, o in zip((near.banks.gate, near.banks.up, near.banks.down), offs):
+        for e in range(E):
+            arena.upload(b.buffer.download(np.uint8, b.expert_bytes, e * b.stride), offset=e * gap + o)
+    T = 20
+    ids, w = route(rng, T, E, k)
+    ids[:, 0] = 3
+    ids[:, 1] = np.arange(T) % 3
+    x = f32_of(bf16(rng.standard_normal((T, H))))
+    want = decode(nm, near, x, ids, w), decode(nm, near, x[:1], ids[:1], w[:1]), prefill(nm, near, x, ids, w)[0]
+
+    class Far:
+        banks = nm.LayerBanks.over(*far)
+
+    got = decode(nm, Far, x, ids, w), decode(nm, Far, x[:1], ids[:1], w[:1]), prefill(nm, Far, x, ids, w)[0]
+    for a, b in zip(got, want):
+        assert np.array_equal(a, b)
+    n, kk = 32, 64
+    raw = rng.standard_normal((2, n, kk)).astype(np.float32)
+    arena.upload(raw[0], offset=0)
+    arena.upload(raw[1], offset=3 * gap)
+    out = nm.DeviceBuffer(2 * nm.projection_bytes(nm.MXFP4_T, n, kk))
+    nm.mxfp4_quantize(arena, nm.F32, n, kk, out, batch=2, src_stride=3 * gap // 4)
+    packed = out.download(np.uint8).reshape(2, -1)
+    for b in range(2):
+        assert np.array_equal(packed[b], M.tiled(*M.quantize(raw[b])))
+    nm.mxfp4_quantize(nm.DeviceBuffer.from_array(raw), nm.F32, n, kk, arena, batch=2, dst_stride=3 * gap)
+    assert np.array_equal(arena.download(np.uint8, packed.shape[1], 3 * gap), packed[1])
+
+
+def test_rows_past_the_outputs_stay(gpu):
+    """The bytes behind the last row of out, and x without a residual, are left as they are."""
+    nm = gpu
+    rng = np.random.default_rng(85)
+    E, H, I, k = 3, 160, 96, 2
+    ex = Experts(nm, 86, E, H, I)
+    for T in (1, 5, 40):
+        ids, w = route(rng, T, E, k)
+        raw = bf16(rng.standard_normal((T, H)))
+        xd, idd, wd = (nm.DeviceBuffer.from_array(a) for a in (raw, ids, w))
+        for f in ("decode", "prefill"):
+            out = nm.DeviceBuffer.from_array(np.full((T + 3, H), 9.0, np.float32))
+            if f == "decode":
+                nm.indexed_moe_fused_decode(ex.banks, xd, nm.BF16, idd, wd, T, k, out)
+            else:
+                nm.moe_prefill(ex.banks, xd, idd, wd, T, k, out)
+            o = out.download(np.float32).reshape(T + 3, H)
+            assert (o[T:] == 9.0).all() and (o[:T] != 9.0).all()
+            assert np.array_equal(xd.download(np.uint16).reshape(T, H), raw)
