@@ -198,9 +198,9 @@ int64_t naiwa_projection_bytes(int dtype, int64_t n, int64_t k);
  * its row; an infinite activation gives NaN there.
  * Banks of NAIWA_MXFP4_T (all three, or NAIWA_E_UNSUPPORTED; naiwa_mxfp4.h) take any
  * number of rows on the matrix cores: H, I multiples of 32, width <= 64, x and out
- * 16-byte aligned.  Products and sums are f32; an activation is held to 2^-19 of the
- * largest magnitude of its 32-value block (bf16 x of at least 2^-12 of it exactly):
- * within 1e-5 of a 64-bit result.  A NaN, an infinity or an h that overflows makes its
+ * 16-byte aligned.  Products and sums are f32; f32 x and h are held to 2^-24 of the
+ * largest magnitude of their 32-value block, bf16 x to 2^-19 of it (exactly where it is
+ * at least 2^-12 of it): within 1e-5 of a 64-bit result.  A NaN, an infinity or an h that overflows makes its
  * pair's dots NaN. */
 int naiwa_moe_decode(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down,
                      const void* x, int x_dtype, const uint32_t* slot_ids, const float* w,
@@ -295,9 +295,8 @@ int naiwa_moe_gather(const uint32_t* ids, int n, int E, uint32_t* perm_out, uint
  * bf16.  Needs
  * H, I multiples of 128; gate/up Q4_K (H % 256 == 0) or Q8_0, down Q4_K (I %
  * 256 == 0) or Q8_0; T * k <= 65536; slots <= 4096.  Banks of NAIWA_MXFP4_T (all
- * three): H, I multiples of 32, k <= 64, out 16-byte aligned; x held to 2^-14 of the
- * largest magnitude of its 32-value block (a value of at least 2^-7 of it exactly), h
- * to 2^-19, products and sums f32.  Slot ids outside the
+ * three): H, I multiples of 32, k <= 64, x and out 16-byte aligned; the numerics of
+ * naiwa_moe_decode over such banks.  Slot ids outside the
  * bank contribute nothing.  flags: NAIWA_PREFILL_ACCUMULATE adds to out
  * (e.g. shared experts on top of the routed ones) instead of overwriting. */
 #define NAIWA_PREFILL_ACCUMULATE 1

@@ -12,10 +12,10 @@
 // 1 the rest times 2^5 (at most 4) rounded again, and so on; plane p has the scale
 // 2^(s - 127 - 5 p).  With M the block's largest magnitude, P planes hold a value to within
 // 2^(1 - 5 P) M:
-//   3 planes (x of a prompt chunk, bf16): 2^-14 M; a value of at least 2^-7 M exactly;
-//   4 planes (h of a prompt chunk, bf16 x of a decode step): 2^-19 M; a bf16 value of at least
-//     2^-12 M exactly;
-//   5 planes (h and f32 x of a decode step, which HBM bounds): 2^-24 M, an f32's own rounding.
+//   4 planes (bf16 x): 2^-19 M, a bf16 value of at least 2^-12 M exactly;
+//   5 planes (f32 x, h): 2^-24 M, the rounding of an f32 as large as M.
+// A plane less in each (3 and 4) takes 4096 tokens at Mixtral-8x7B sizes from 3.1 to 2.65 ms, with
+// results off by 6e-6 instead of 4e-7, for which f32 sums have no use.
 // FP4 x E2M3 runs at twice the rate of FP4 x FP8 and of bf16 per step (5.4 against 3.4
 // PFLOP/s measured), and its sums are exact up to the f32 accumulator's rounding; with e4m3
 // the matrix cores drop products under about 2^-15 of a step's largest (5e-5 of a sum of
@@ -31,8 +31,8 @@
 //   4. combine: out[t] = the weighted sum over t's pairs in ascending slot order.
 // (2. and 3.: mxfp4_tiles.h.)  One token takes two launches: gate/up lays x out itself, a block
 // per (pair, 32 features), and down combines (gateup_one_kernel, down_one_kernel).
-// No atomics: every run adds the same terms in the same order, and a pair's terms do not
-// depend on the other pairs of the call.
+// No atomics: every run adds the same terms in the same order, and in calls of as many pairs the
+// order of a pair's terms does not depend on the other pairs.
 #include "mxfp4.h"
 #include "segments.h"
 
@@ -661,7 +661,6 @@ int run_pass(const NaiwaMxCall& c, uint8_t* ws, hipStream_t st) {
         r.combine(1);
         return naiwa_hip_rc(hipGetLastError());
     }
-    if (!c.skip_zero) return r.go<4, 4, true>(); // a prompt chunk
     return c.x_dtype == NAIWA_BF16 ? r.go<4, 5, true>() : r.go<5, 5, false>();
 }
 

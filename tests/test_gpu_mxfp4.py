@@ -3,13 +3,12 @@
 Tolerance of the products.  An activation enters in planes of E2M3 whose last rounding has
 steps of at most 2^-2 2^(-5 (P - 1)) where the block's largest magnitude M is at least 2
 (csrc/mxfp4_experts.hip): an error of rms at most 2^-3 2^(-5 (P - 1)) / sqrt(12) M, that is
-1.1e-6 M for 4 planes (bf16 x, h of a prompt chunk), 3.4e-8 M for 5 (f32 x, h of a decode
-call).  In a block of normal values M is about 2.5 times the rms: 2.8e-6 of a value, for h,
-with its heavier tail, up to 5 times: 5.5e-6.  bf16 x is exact but for values under 2^-12 M.
-f32 sums of K products add about sqrt(K) 2^-24, 4e-6 at K 4096 and 1.1e-5 at 33024 if the
-additions' errors were all of the size of the whole sum; partial sums grow as they are added,
-which halves that: 6e-6.  Together, as squares: sqrt(2 * 2.8^2 + 5.5^2 + 4^2) 1e-6 = 7.9e-6, and
-sqrt(6^2 + 4^2) 1e-6 = 7.2e-6 for the longest rows with 5 planes; 1e-5 holds every case.
+3.4e-8 M for 5 planes (f32 x, h); bf16 x in 4 planes is exact but for values under 2^-12 M.
+In a block of normal values M is about 2.5 times the rms, for h up to 5 times: 2e-7 of a
+value.  f32 sums of K products add about sqrt(K) 2^-24, 4e-6 at K 4096 and 1.1e-5 at 33024 if
+the additions' errors were all of the size of the whole sum; partial sums grow as they are
+added, which halves that: 6e-6.  Gate and up enter as a product, down on top: as squares at
+most sqrt(2 * 6^2 + 4^2) 1e-6 = 9.4e-6; 1e-5 holds every case.
 """
 import numpy as np
 import pytest
