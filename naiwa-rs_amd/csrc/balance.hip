@@ -6,10 +6,13 @@
 // registers (one read of the logits), and the probabilities are added up per expert in
 // registers.  The counts meet in an LDS histogram.  Each block leaves its partial sums in the
 // scratch buffer; a second launch, a block per 16 experts, adds them in a fixed order, and the
-// last of its blocks to end adds up the loss.  With one block the first launch does all that.  Backward: the same row in registers, dlogits from it in the same pass.
+// last of its blocks to end adds up the loss.  With one block the first launch does all that.
+// Backward: the same row in registers, dlogits from it in the same pass.
 //
 // Bound: HBM for long batches (the logits are read once each way and the gradient
-// written once); launches and the latency of a row for short ones.
+// written once); launches and the latency of a row for short ones.  32768 tokens, 128 experts,
+// top-8, f32: forward 7.9 + 5.1 us, backward 11.8 us (33.6 MB: 2.8 TB/s); 61 tokens 3.6 and 2.0 us.
+// 64 lanes a row, and one block that joins all partial sums, took 120 us for all three.
 #include "../../include/naiwa_balance.h"
 #include "common.h"
 #include "workspace.h"

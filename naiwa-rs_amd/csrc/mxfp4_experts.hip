@@ -178,7 +178,8 @@ struct Beside {
 
 // x [rows, H] in P planes, a block of 32 values a thread; the blocks that pad H to whole
 // steps are zeros.  The launch's last block cuts the sorted pairs into tiles, SORT: after it
-// sorted them.  Bound: HBM, and latency where rows are few.
+// sorted them.  Bound: HBM, and latency where rows are few: 4096 rows of H 4096 26 us (34 MB in,
+// 50 MB out), 16 rows and their 32 pairs 5.6 us.
 template <int P, bool BF16, bool SORT>
 __global__ void __launch_bounds__(kThreads) planes_kernel(const void* x, int64_t rows, int H, Planes out, Beside with) {
     if (blockIdx.x == gridDim.x - 1) {
@@ -334,7 +335,9 @@ __device__ __forceinline__ void put_h(const Sums<NW>& sums, int tok, bool pad, i
 // Gate/up of one token: a block per (pair, 32 features); each wave lays out its own steps of x in
 // LDS while its first weights are on the way.  Pair j is row j of h; blocks past I (h padded to
 // whole steps) write zeros.  The first block lists the pairs that count as tiles of one pair, for
-// tile_down_kernel.  Dynamic LDS: the planes of x (96 PX bytes a step), their scales (16 a group).
+// tile_down_kernel.  Dynamic LDS: the planes of x, their scales (16 bytes a group).  Bound: latency
+// (the launch, x to planes behind the first weights' way, four waves' sums): 8 of 128 Qwen3-30B
+// experts 6.6 us (13.4 MB), 2 of 8 of 1024 x 2048 6.3 us (4.5 MB).
 template <int PX, int PH, bool BF16>
 __global__ void __launch_bounds__(kThreads, 2)
 gateup_one_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32_t* ids, const float* w, int width, int slots,
@@ -417,7 +420,8 @@ __device__ __forceinline__ void residual4(uint16_t* x, const v4f& y) {
 // Down and combine of one token: a block of 8 waves per 16 rows.  A pair's steps go to the
 // `split` waves of one of 8 / split groups, the groups take the pairs in turn; the sums meet in
 // LDS and 4 lanes of the first wave add them up, pairs in ascending slot order.  Dynamic LDS:
-// h's planes and scales of every pair, copied by all waves.
+// h's planes and scales of every pair, copied by all waves.  Bound: latency, as gate/up: Qwen3-30B
+// sizes 6.5 us (6.7 MB), 8 experts of 1024 x 2048 4.8 us.
 constexpr int kOneWaves = 8;
 template <int PH>
 __global__ void __launch_bounds__(64 * kOneWaves)
@@ -464,7 +468,8 @@ down_one_kernel(Bank down, Planes h, int H, int I, const uint32_t* ids, const fl
 }
 
 // out[t] (+)= the weighted dots of t's pairs in ascending slot order, a pair's K parts in
-// part order; res: also res = bf16(res + out).
+// part order; res: also res = bf16(res + out).  Bound: HBM (4096 tokens at Mixtral-8x7B sizes 35 us,
+// 201 MB: 5.7 TB/s), and the launch for few rows (4 to 5 us).
 __global__ void __launch_bounds__(kThreads)
 combine_kernel(const float* y, int64_t n, int parts, const uint32_t* ids, const float* w, int width, int slots, int H,
                int skip_zero, int accumulate, float* out, uint16_t* res) {

@@ -1,4 +1,4 @@
-// The MXFP4 experts of many tokens an expert: tiles of up to 64 sorted pairs of one slot
+// The MXFP4 experts of more than one token: tiles of up to 64 sorted pairs of one slot
 // against strips of weights, on v_mfma_scale_f32_32x32x64_f8f6f4 (included by
 // mxfp4_experts.hip).
 //
@@ -17,6 +17,17 @@
 // groups of 4 pieces (and 2 for the rest), [token][piece], the piece number xored with bits of
 // the token so that 16 neighbouring tokens' reads of one piece fall on distinct banks, while
 // 4 neighbouring lanes of a copy read 64 contiguous bytes.
+//
+// Bound.  Few tokens an expert: HBM, the weights are read once (96 tokens at Qwen3-30B sizes 4.9
+// TB/s in gate/up, 16 at Mixtral-8x7B sizes 5.0, where a copy reaches 5.1).  Many: the scaled
+// products and the power they draw; 4096 tokens at Mixtral sizes run 1.9 + 1.3 ms, 4.1 and 3.6
+// PFLOP/s of FP4 x E2M3, and 5.4 is what the same products reach from registers alone.  Without the
+// weights' loads gate/up takes 17 % less, without the copies 14 %, without the LDS reads no less.
+// Between (about 50 tokens of small experts): the memory's and the products' times, which two blocks
+// a CU overlap in part, and 1.7 rounds of blocks with 10 us of first loads and epilogue each.
+// Set aside: 128 weight rows a wave (one block a CU), 18 to 25 % slower; three blocks a CU (the
+// compiler spills), 20 % slower; planes of 24 contiguous bytes, three pieces read for two planes
+// (register moves), 3 to 6 % slower.
 #pragma once
 
 #include <type_traits>
@@ -291,6 +302,7 @@ template <int NH, class F> __device__ __forceinline__ uint32_t copy2(int lane, i
 }
 
 // Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in PH planes.
+// 16 tokens at Mixtral-8x7B sizes 94 us (5.3 TB/s), 4096 1.85 ms (1.04 PFLOP/s in 4 planes).
 template <int NA, int P, int PH>
 __global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
 tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,
@@ -357,7 +369,8 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
 }
 
 // Down of a tile and a K part of part_groups groups of 4 steps: NA tiles of 32 rows a wave;
-// y[part][pair][H] unweighted.
+// y[part][pair][H] unweighted.  16 tokens at Mixtral-8x7B sizes 49 us (5.1 TB/s), 4096 1.27 ms
+// (0.76 PFLOP/s in 5 planes).
 template <int NA, int P>
 __global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
 tile_down_kernel(Bank down, Planes h, int H, int I, int64_t n, int part_groups, const uint32_t* perm, Tiles tl, int xcd,
