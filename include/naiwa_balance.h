@@ -45,7 +45,7 @@ int naiwa_router_balance(const void* logits, int dtype, int ld, const uint32_t* 
  * f32) times dloss/dlogits, from the forward's counts and valid.  flags
  * NAIWA_BALANCE_ACCUMULATE adds to dlogits (in f32, rounded once) instead of
  * overwriting; masked rows are then left as they are, otherwise set to 0.  dlogits may
- * be logits. */
+ * be logits, with rows as far apart (NAIWA_E_INVALID otherwise). */
 #define NAIWA_BALANCE_ACCUMULATE 1
 int naiwa_router_balance_backward(const void* logits, int dtype, int ld, const uint32_t* counts,
                                   const uint32_t* valid, int64_t T, int E, int k, const uint8_t* mask,

@@ -411,6 +411,7 @@ extern "C" int naiwa_router_balance_backward(const void* logits, int dtype, int 
     if (E > kMaxE || T > INT32_MAX / k) return NAIWA_E_UNSUPPORTED;
     if (T == 0) return NAIWA_OK;
     if (!logits || !counts || !valid || !grad_loss || !dlogits) return NAIWA_E_INVALID;
+    if (dlogits == logits && (dld ? dld : E) != (ld ? ld : E)) return NAIWA_E_INVALID; // rows over other rows
     const int at_once = E <= 128 ? kThreads / 16 : kWaves; // rows of a block
     const unsigned blocks = (unsigned)std::min<int64_t>((T + at_once - 1) / at_once, 1024);
     hipStream_t st = (hipStream_t)stream;

@@ -16,8 +16,8 @@
 //   5 planes (f32 x, h): 2^-24 M, the rounding of an f32 as large as M.
 // A plane less in each (3 and 4) takes 4096 tokens at Mixtral-8x7B sizes from 3.1 to 2.65 ms, with
 // results off by 6e-6 instead of 4e-7, for which f32 sums have no use.
-// FP4 x E2M3 runs at twice the rate of FP4 x FP8 and of bf16 per step (5.4 against 3.4
-// PFLOP/s measured), and its sums are exact up to the f32 accumulator's rounding; with e4m3
+// FP4 x E2M3 runs at twice the rate of FP4 x FP8 (6 to 7 against 3.6 to 4.3 PFLOP/s from registers,
+// random codes), and its sums are exact up to the f32 accumulator's rounding; with e4m3
 // the matrix cores drop products under about 2^-15 of a step's largest (5e-5 of a sum of
 // codes of all magnitudes).  A block with a NaN or an infinity gets the scale byte 255,
 // which makes its products NaN.
@@ -559,7 +559,6 @@ int naiwa_mx_check(const NaiwaMxCall& c) {
     if (((uintptr_t)c.x | (uintptr_t)c.out) & 15) return NAIWA_E_INVALID;
     return NAIWA_OK;
 }
-
 
 namespace {
 

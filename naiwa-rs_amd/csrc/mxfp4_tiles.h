@@ -11,8 +11,7 @@
 //
 // The planes' rows (of x by token, of h by sorted pair) go to LDS by DMA in chunks of 128
 // values: of 64 rows two chunks deep, of 32 (a tile of at most 32 pairs, which HBM bounds)
-// four.  A row's chunk is 3 classes of 2 P pieces of 16 bytes: the first 16
-// bytes of every plane of blocks 0 and 2 (class 0) and of blocks 1 and 3 (class 1), step by
+// four.  A row's chunk is 3 classes of 2 P pieces of 16 bytes: the first 16 bytes of every plane of blocks 0 and 2 (class 0) and of blocks 1 and 3 (class 1), step by
 // step; and the last 8 bytes of a plane of both blocks of a step (class 2).  In LDS a class is
 // groups of 4 pieces (and 2 for the rest), [token][piece], the piece number xored with bits of
 // the token so that 16 neighbouring tokens' reads of one piece fall on distinct banks, while
@@ -21,13 +20,14 @@
 // Bound.  Few tokens an expert: HBM, the weights are read once (96 tokens at Qwen3-30B sizes 4.9
 // TB/s in gate/up, 16 at Mixtral-8x7B sizes 5.0, where a copy reaches 5.1).  Many: the scaled
 // products and the power they draw; 4096 tokens at Mixtral sizes run 1.9 + 1.3 ms, 4.1 and 3.6
-// PFLOP/s of FP4 x E2M3, and 5.4 is what the same products reach from registers alone.  Without the
-// weights' loads gate/up takes 17 % less, without the copies 14 %, without the LDS reads no less.
+// PFLOP/s of FP4 x E2M3, where the same products from registers alone reach 6 to 7 with random
+// codes and 9.9 with zeros, the chip's full rate: its power is the limit.  Without the weights'
+// loads gate/up takes 17 % less, without the copies 14 %, without the LDS reads no less.
 // Between (about 50 tokens of small experts): the memory's and the products' times, which two blocks
 // a CU overlap in part, and 1.7 rounds of blocks with 10 us of first loads and epilogue each.
 // Set aside: 128 weight rows a wave (one block a CU), 18 to 25 % slower; three blocks a CU (the
 // compiler spills), 20 % slower; planes of 24 contiguous bytes, three pieces read for two planes
-// (register moves), 3 to 6 % slower.
+// (register moves), 3 to 6 % slower; three chunks of 64 rows in LDS, no faster.
 #pragma once
 
 #include <type_traits>

@@ -41,7 +41,7 @@ def test_forward_refuses():
 
 def test_backward_refuses():
     for bad in (dict(T=-1), dict(k=0), dict(E=0), dict(ld=7), dict(dld=7), dict(dld=-1), dict(flags=2), dict(x=None),
-                dict(counts=None), dict(valid=None), dict(g=None), dict(d=None)):
+                dict(counts=None), dict(valid=None), dict(g=None), dict(d=None), dict(x=1 << 20, d=1 << 20, dld=12)):
         assert _backward(**bad) == E_INVALID, bad
     for bad in (dict(E=1025), dict(dt=nm.F16), dict(T=1 << 31)):
         assert _backward(**bad) == E_UNSUPPORTED, bad

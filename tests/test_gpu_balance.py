@@ -199,3 +199,59 @@ def test_results_repeat(gpu):
     for _ in range(3):
         again = run(gpu, x, ids, 128, mask, 1.0)
         assert all(np.array_equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("T,E,ld", [(300, 8, 8), (77, 128, 132), (50, 60, 61), (70, 500, 500)])
+@pytest.mark.parametrize("bf", [False, True])
+def test_gradient_in_the_logits_place(gpu, T, E, ld, bf):
+    nm = gpu
+    rng = np.random.default_rng(E)
+    x, ids, mask = make(rng, T, E, 4, 0.7)
+    wide = np.zeros((T, ld), np.float32)
+    wide[:, :E] = x
+    raw, dt = (bf16(wide), nm.BF16) if bf else (wide, nm.F32)
+    xd, idd, md = (nm.DeviceBuffer.from_array(a) for a in (raw, ids, mask))
+    counts, valid, probs, loss, dd = (nm.DeviceBuffer.from_array(a) for a in (
+        np.zeros(E, np.uint32), np.zeros(1, np.uint32), np.zeros(E, np.float32), np.zeros(1, np.float32), raw))
+    gd = nm.DeviceBuffer.from_array(np.array([0.5], np.float32))
+    nm.router_balance(xd, dt, idd, T, E, 4, counts, valid, probs, loss, mask=md, ld=ld)
+    nm.router_balance_backward(xd, dt, counts, valid, T, E, 4, gd, dd, mask=md, ld=ld, dld=ld)
+    nm.router_balance_backward(xd, dt, counts, valid, T, E, 4, gd, xd, mask=md, ld=ld, dld=ld)
+    assert np.array_equal(xd.download(raw.dtype), dd.download(raw.dtype))
+
+
+def test_captured_and_replayed(gpu):
+    """Counts, loss and gradient in a graph, replayed on new inputs between eager calls of other sizes."""
+    from test_gpu_mxfp4 import Graph
+
+    nm = gpu
+    rng = np.random.default_rng(9)
+    T, E, k = 5000, 64, 6
+    sets = [make(rng, T, E, k, 1)[:2] for _ in range(3)]
+    big = make(rng, 2 * T, E, k, 1)[:2]
+
+    def call(x, ids, T, stream):
+        nm.router_balance(x, nm.F32, ids, T, E, k, *out[:4], stream=stream)
+        nm.router_balance_backward(x, nm.F32, out[0], out[1], T, E, k, gd, out[4], stream=stream)
+
+    out = [nm.DeviceBuffer(n * 4) for n in (E, 1, E, 1, 2 * T * E)]
+    gd = nm.DeviceBuffer.from_array(np.array([1.0], np.float32))
+    xd, idd = nm.DeviceBuffer.from_array(sets[0][0]), nm.DeviceBuffer.from_array(sets[0][1])
+    bx, bi = nm.DeviceBuffer.from_array(big[0]), nm.DeviceBuffer.from_array(big[1])
+    call(bx, bi, 2 * T, 0)           # the scratch is as large as it will be
+    st = nm.Stream()
+    g = Graph(nm, st, lambda: call(xd, idd, T, st.handle))
+    for x, ids in sets:
+        xd.upload(x)
+        idd.upload(ids)
+        call(xd, idd, T, 0)
+        nm.synchronize()
+        want = [o.download(np.uint32, n) for o, n in zip(out, (E, 1, E, 1, T * E))]
+        call(bx, bi, 2 * T, 0)
+        nm.synchronize()
+        for _ in range(2):
+            g.launch()
+            st.sync()
+            for o, v in zip(out, want):
+                assert np.array_equal(o.download(np.uint32, v.size), v)
+    g.close()

@@ -178,6 +178,7 @@ def decode(nm, ex, x, ids, w, act="silu", out0=None, f32=False, noalloc=False):
     (300, 8, 128, 96, 4),      # more pairs than are sorted beside the planes
     (1, 8, 128, 4096, 8),      # one token whose h fills more than LDS
     (1, 1, 33024, 32, 1),      # and whose x does
+    (1, 2, 64, 12288, 2), (1, 1, 24576, 32, 1),   # one token whose h and whose x take most of it
     (1, 2, 11008, 64, 2), (2, 64, 64, 32, 64),
 ])
 @pytest.mark.parametrize("f32", [False, True])
@@ -590,3 +591,71 @@ def test_rows_past_the_outputs_stay(gpu):
             o = out.download(np.float32).reshape(T + 3, H)
             assert (o[T:] == 9.0).all() and (o[:T] != 9.0).all()
             assert np.array_equal(xd.download(np.uint16).reshape(T, H), raw)
+
+
+class Graph:
+    """What `calls` queue on a stream, captured; the library's calls allocate nothing once their scratch is as large
+    as they need."""
+
+    def __init__(self, nm, stream, calls):
+        import ctypes as C
+        self.hip = C.CDLL("libamdhip64.so.7")      # the runtime that the library has loaded
+        self.nm, self.stream, self.graph, self.exec = nm, stream, C.c_void_p(), C.c_void_p()
+        h = C.c_void_p(stream.handle)
+        nm.synchronize()
+        assert self.hip.hipStreamBeginCapture(h, 2) == 0
+        calls()
+        assert self.hip.hipStreamEndCapture(h, C.byref(self.graph)) == 0
+        assert self.hip.hipGraphInstantiate(C.byref(self.exec), self.graph, None, None, C.c_size_t(0)) == 0
+
+    def launch(self):
+        import ctypes as C
+        assert self.hip.hipGraphLaunch(self.exec, C.c_void_p(self.stream.handle)) == 0
+
+    def close(self):
+        self.stream.sync()
+        assert self.hip.hipGraphExecDestroy(self.exec) == 0 and self.hip.hipGraphDestroy(self.graph) == 0
+
+
+@pytest.mark.parametrize("T", [1, 20, 400])
+def test_captured_and_replayed(gpu, T):
+    """Quantisation, a decode call and a prompt chunk in one graph, replayed on new weights, inputs and routing
+    between eager calls of other sizes over the same scratch."""
+    nm = gpu
+    rng = np.random.default_rng(90 + T)
+    E, H, I, k = 4, 288, 160, 2
+    ex = Experts(nm, 91, E, H, I)
+    other = [f32_of(bf16(rng.standard_normal((500, H)))), *route(rng, 500, E, k)]
+    xd, idd, wd = nm.DeviceBuffer(T * H * 2), nm.DeviceBuffer(T * k * 4), nm.DeviceBuffer(T * k * 4)
+    raw, d, p = nm.DeviceBuffer(I * H * 2), nm.DeviceBuffer(T * H * 4), nm.DeviceBuffer(T * H * 4)
+
+    def call(stream):
+        nm.mxfp4_quantize(raw, nm.BF16, I, H, ex.banks.gate.desc().base, stream=stream)   # slot 0's gate
+        nm.indexed_moe_fused_decode(ex.banks, xd, nm.BF16, idd, wd, T, k, d, stream=stream)
+        nm.moe_prefill(ex.banks, xd, idd, wd, T, k, p, stream=stream)
+
+    def eager_others():
+        decode(nm, ex, *other)
+        prefill(nm, ex, *other)
+
+    def inputs():
+        ids, w = route(rng, T, E, k)
+        ids[0, 0] = 0
+        for b, a in ((xd, bf16(rng.standard_normal((T, H)))), (idd, ids), (wd, w),
+                     (raw, bf16(rng.standard_normal((I, H)) * 0.05))):
+            b.upload(a)
+
+    inputs()
+    eager_others()
+    st = nm.Stream()
+    g = Graph(nm, st, lambda: call(st.handle))
+    for _ in range(3):
+        inputs()
+        call(0)
+        want = d.download(np.uint32), p.download(np.uint32)
+        eager_others()
+        for _ in range(2):
+            g.launch()
+            st.sync()
+            assert np.array_equal(d.download(np.uint32), want[0]) and np.array_equal(p.download(np.uint32), want[1])
+    g.close()
