@@ -351,8 +351,8 @@ gateup_one_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32_
         const bool in = id < (uint32_t)slots && !(skip_zero && w[i] == 0.0f);
         const uint64_t m = __ballot(in);
         const int at = __popcll(m & ((1ull << i) - 1));
-        if (in) perm[i] = (uint32_t)i, tl.start[at] = i, tl.count[at] = 1, tl.slot[at] = (int)id;
-        if (i == 0) *tl.n = __popcll(m);
+        if (in) perm[i] = (uint32_t)i, tl.t[at] = make_int4(i, 1, (int)id, 0);
+        if (i >= __popcll(m) && i < 8 * tl.run) tl.t[i] = make_int4(0, 0, 0, 0);
     }
     const uint32_t s = (uint32_t)uniform((int)ids[j]);
     if (s >= (uint32_t)slots || (skip_zero && w[j] == 0.0f)) return;
@@ -520,6 +520,9 @@ int down_parts(int64_t n, int64_t blocks, int H, int I) {
     return parts;
 }
 
+// The most tiles of n pairs over `slots` slots, a multiple of 8.
+int64_t tiles_most(int64_t n, int slots) { return (n / kTile + std::min<int64_t>(n, slots) + 7) / 8 * 8; }
+
 struct Layout {
     size_t offsets, bad, perm, tiles, x, xs, h, hs, y, total;
     int64_t max_tiles;
@@ -530,8 +533,8 @@ struct Layout {
         bad = a256(offsets + (size_t)(NAIWA_SEG_MAX_KEYS + 1) * 4);
         perm = bad + 256;
         tiles = a256(perm + n * 4);
-        max_tiles = (int64_t)n / kTile + std::min<int64_t>((int64_t)n, NAIWA_SEG_MAX_KEYS);
-        x = a256(tiles + (size_t)(3 * max_tiles + 1) * 4);
+        max_tiles = tiles_most((int64_t)n, NAIWA_SEG_MAX_KEYS);
+        x = a256(tiles + (size_t)max_tiles * sizeof(int4));
         xs = a256(x + (size_t)rows * plane_row(kPlanesMost, H));
         h = a256(xs + (size_t)rows * naiwa_mx_groups(H) * 16);
         hs = a256(h + n * plane_row(kPlanesMost, I));
@@ -592,10 +595,10 @@ struct Run { // one pass's pieces
         combine_kernel<<<dim3(c.rows, cs), kThreads, 0, st>>>(y(), n, parts, c.ids, c.w, c.width, slots, H, c.skip_zero,
                                                              c.accumulate, c.out, c.res);
     }
-    // Down of at most `most` tiles (a multiple of 8), and the combine.
-    template <int PH> void down(int64_t most) const {
+    // Down of the tiles, and the combine.
+    template <int PH> void down() const {
         const int ncol = (H / 32 + 4 * kNA - 1) / (4 * kNA);
-        const unsigned blocks = (unsigned)(most * ncol);
+        const unsigned blocks = (unsigned)(8 * tl.run * ncol);
         const int groups = naiwa_mx_groups(I), part = (groups + down_parts(n, blocks, H, I) - 1) / down_parts(n, blocks, H, I);
         const int parts = (groups + part - 1) / part;
         tile_down_kernel<kNA, PH><<<dim3(blocks, parts), kThreads, kStageBytes<PH>, st>>>(d, h(PH), H, I, n, part, perm, tl,
@@ -614,7 +617,7 @@ struct Run { // one pass's pieces
         gateup_one_kernel<PX, PH, BF16><<<dim3(c.width, 4 * naiwa_mx_steps(I)), kThreads, xl, st>>>(
             g, u, c.x, H, I, c.ids, c.w, c.width, slots, c.skip_zero, c.act, h(PH), perm, tl);
         if (hl > kLds) {
-            down<PH>((n + 7) / 8 * 8);
+            down<PH>();
             return true;
         }
         int split = 1;
@@ -640,12 +643,11 @@ struct Run { // one pass's pieces
             if (int rc = naiwa_moe_gather(c.ids, n, slots, perm, offsets, (int*)(ws + L.bad), (int64_t)st)) return rc;
             planes_kernel<PX, BF16, false><<<pb, kThreads, 0, st>>>(c.x, c.rows, H, x(PX), with);
         }
-        const int64_t most = (n / kTile + std::min(n, slots) + 7) / 8 * 8;
         const int ncol = (4 * naiwa_mx_steps(I) + 2 * kNA - 1) / (2 * kNA);
-        const unsigned blocks = (unsigned)(most * ncol);
+        const unsigned blocks = (unsigned)(8 * tl.run * ncol);
         tile_gateup_kernel<kNA, PX, PH><<<blocks, kThreads, kStageBytes<PX>, st>>>(g, u, x(PX), H, I, c.width, perm, tl, c.act,
                                                                                   xcd_order(ncol), h(PH));
-        down<PH>(most);
+        down<PH>();
         return naiwa_hip_rc(hipGetLastError());
     }
 };
@@ -654,13 +656,13 @@ struct Run { // one pass's pieces
 int run_pass(const NaiwaMxCall& c, uint8_t* ws, hipStream_t st) {
     const int H = c.gate->k, I = c.gate->n, n = c.rows * c.width;
     const Layout L(c.rows, c.width, H, I);
-    int* tiles = (int*)(ws + L.tiles);
     const Run r{c, L, ws, st, H, I, c.gate->slots, n,
                 Bank{(const uint8_t*)c.gate->base, c.gate->slot_stride, naiwa_mx_strip_bytes(H)},
                 Bank{(const uint8_t*)c.up->base, c.up->slot_stride, naiwa_mx_strip_bytes(H)},
                 Bank{(const uint8_t*)c.down->base, c.down->slot_stride, naiwa_mx_strip_bytes(I)},
                 (uint32_t*)(ws + L.offsets), (uint32_t*)(ws + L.perm),
-                Tiles{tiles, tiles + L.max_tiles, tiles + 2 * L.max_tiles, tiles + 3 * L.max_tiles}};
+                // (one token has a tile a pair)
+                Tiles{(int4*)(ws + L.tiles), (int)(tiles_most(n, c.rows == 1 ? n : c.gate->slots) / 8)}};
     if (n == 0) {
         r.combine(1);
         return naiwa_hip_rc(hipGetLastError());

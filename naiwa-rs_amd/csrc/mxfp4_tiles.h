@@ -62,13 +62,12 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 constexpr int kTile = 64; // pairs a tile
 
 struct Tiles {
-    int* start; // first sorted position
-    int* count; // pairs, at most kTile
-    int* slot;
-    int* n;     // number of tiles
+    int4* t; // {first sorted position, pairs (at most kTile, 0: no tile), slot}, 8 runs of `run`
+    int run;
 };
 
-// The sorted pairs cut into tiles of up to 64 pairs of one slot, by one block of kThreads.
+// The sorted pairs cut into tiles of up to 64 pairs of one slot, by one block of kThreads: dealt to
+// the runs in order, as evenly as they go.
 __device__ inline void tiles_block(const uint32_t* offsets, int slots, Tiles t) {
     __shared__ int part[kThreads];
     const int tid = threadIdx.x, per = (slots + kThreads - 1) / kThreads;
@@ -76,6 +75,7 @@ __device__ inline void tiles_block(const uint32_t* offsets, int slots, Tiles t) 
     int mine = 0;
     for (int s = s0; s < s1; ++s) mine += (int)((offsets[s + 1] - offsets[s] + kTile - 1) / kTile);
     part[tid] = mine;
+    for (int i = tid; i < 8 * t.run; i += kThreads) t.t[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
     for (int m = 1; m < kThreads; m <<= 1) {
         const int v = tid >= m ? part[tid - m] : 0;
@@ -84,36 +84,27 @@ __device__ inline void tiles_block(const uint32_t* offsets, int slots, Tiles t) 
         __syncthreads();
     }
     int at = part[tid] - mine;
+    const int all = part[kThreads - 1];
     for (int s = s0; s < s1; ++s) {
         const int b = (int)offsets[s], n = (int)(offsets[s + 1] - offsets[s]);
         // the fewest tiles, of about equal numbers of 32-pair halves
         const int subs = (n + 31) / 32, nt = (n + kTile - 1) / kTile;
         for (int j = 0; j < nt; ++j, ++at) {
             const int m0 = 32 * (subs * j / nt), m1 = min(n, 32 * (subs * (j + 1) / nt));
-            t.start[at] = b + m0;
-            t.count[at] = m1 - m0;
-            t.slot[at] = s;
+            const int x = (8 * (at + 1) - 1) / all; // run x holds tiles all x / 8 .. all (x + 1) / 8 - 1
+            t.t[x * t.run + at - all * x / 8] = make_int4(b + m0, m1 - m0, s, 0);
         }
     }
-    if (tid == kThreads - 1) *t.n = part[tid];
 }
 
-// The (tile, column) of block b of a grid of ncol * (tiles rounded up to 8) blocks; false for a
-// block with none.  xcd: blocks are dealt to the 8 XCDs round-robin (block b to XCD b % 8), and
-// each XCD takes a run of neighbouring tiles, all columns of one after the other; otherwise
-// column by column within a tile.
-__device__ __forceinline__ bool tile_col(int b, int ntiles, int ncol, int xcd, int* tile, int* col) {
-    if (!xcd) {
-        *tile = b / ncol;
-        *col = b % ncol;
-        return *tile < ntiles;
-    }
-    const int x = b & 7, r = b >> 3;
-    const int t0 = ntiles * x / 8, t1 = ntiles * (x + 1) / 8;
-    if (r >= (t1 - t0) * ncol) return false;
-    *tile = t0 + r / ncol;
+// The tile and column of block b of a grid of 8 * run * ncol.  xcd: blocks are dealt to the 8 XCDs
+// round-robin (block b to XCD b % 8), and each XCD takes a run of tiles, all columns of one after
+// the other; otherwise column by column within a tile.
+__device__ __forceinline__ int4 tile_col(int b, Tiles t, int ncol, int xcd, int* col) {
+    const int r = xcd ? b >> 3 : b;
     *col = r % ncol;
-    return true;
+    const int4 v = t.t[(xcd ? (b & 7) * t.run : 0) + r / ncol];
+    return make_int4(uniform(v.x), uniform(v.y), uniform(v.z), 0);
 }
 
 // One chunk of 32 NH rows in P planes.
@@ -171,25 +162,33 @@ template <int P, int NH> __device__ __forceinline__ v6u staged_plane(const uint8
 }
 
 // acc[i][s] += weight tile i x token half s < NH over all of K.  wp[i]: the tile's first strip, the
-// same for every lane; strip: bytes to its second.  xs: the scales of row 0, xo[s] the lane's
-// token's offset.  A chunk's operands (step, half, plane) are read from LDS one ahead of the products.
+// same for every lane; strip: bytes to its second.  to_row(row(token)): the token's row of x (row
+// may load; it is waited for when the first weights are on the way).  A chunk's operands (step,
+// half, plane) are read from LDS one ahead of the products.
 // Loads and copies end in the order of their issue.  Before chunk t its copies have to have
 // landed; the wave issued since then at least the weights of chunk t + 1 (NH = 2), or those of
 // chunk t and the copies and weights of chunks t + 1 and t + 2 (NH = 1): kUnder may be under way.
+// The first weights are issued before the first copies, so fewer follow those: `first` of them.
 // The loop issues them without branches, of the last chunk again where there are no more, since
 // the compiler waits for every load where paths with different loads meet; the last group
-// issues what there is and waits for everything from its second chunk on.  The empty asm makes
+// (which may be the first) issues what there is and waits for everything from its second chunk on.  The empty asm makes
 // the compiler wait for the weights before the next loads are issued: it does not know of
 // the copies, and a later wait of its own would count them among the weights.
-template <int NA, int P, int NH>
-__device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint32_t off4, uint32_t off2,
-                                         const uint8_t* const (&wp)[NA], uint32_t strip, const uint8_t* xs,
-                                         const uint32_t (&xo)[2], int steps, int lane, int wave, v16f (&acc)[NA][2]) {
+template <int NA, int P, int NH, class R, class T>
+__device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, const Planes& x, R row, T to_row,
+                                         const uint8_t* const (&wp)[NA], uint32_t strip, const uint8_t* xs, int steps,
+                                         int lane, int wave, v16f (&acc)[NA][2]) {
     // D chunks of the rows and DA of the weights are in LDS and registers or on the way
     constexpr int D = NH == 1 ? 4 : 2, DA = NH == 1 ? 4 : 3, kCopies = P == 5 ? 4 : 3;
     constexpr int kUnder = NH == 1 ? 2 * NA + 2 * (kCopies + 2 * NA) : 2 * NA;
     constexpr uint32_t kStage = sizeof(Stage<P, NH>);
     const int par = lane >> 5, tok = lane & 31;
+    // the tokens whose rows the lane copies, and those of its scales
+    const int tok4 = 16 * (NH == 2 ? wave : wave & 1) + (lane >> 2), tok2 = 32 * (NH == 2 ? wave & 1 : 0) + (lane >> 1);
+    const uint32_t r4 = row(tok4), r2 = row(tok2);
+    uint32_t rx[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) rx[h] = row(32 * h + tok);
     // the lane's 16 bytes of weights and 4 of scales: row lane % 16 of a strip, block par
     const uint32_t lw = ((lane >> 4) & 1) * strip + 256 * par + 16 * (lane & 15);
     const uint32_t ls = ((lane >> 4) & 1) * strip + 64 * par + 4 * (lane & 15);
@@ -202,42 +201,58 @@ __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint3
 #pragma unroll
             for (int i = 0; i < NA; ++i) o[s][i] = *(const v4u*)(wp[i] + at + lw + 512 * s);
     };
-    auto copy = [&](int t, int buffer) {
-        stage<P, NH>(st + kStage * buffer, base, off4, off2, min(t, steps - 1), wave);
-    };
     // the lane's scale bytes of a group of 4 chunks: a byte a chunk, blocks par and 2 + par
     struct Scales {
         uint32_t a[NA][2], b[NH][2];
     };
     const int groups = (steps + 3) / 4;
-    auto load_scales = [&](int g) {
-        g = min(g, groups - 1);
-        Scales o;
+    auto scales_a = [&](int g, Scales& o) {
         const int64_t sc = (int64_t)1024 * min(4 * g + 4, steps) + 256 * g;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < NA; ++i) o.a[i][s] = *(const uint32_t*)(wp[i] + sc + ls + 128 * s);
-#pragma unroll
-            for (int h = 0; h < NH; ++h) o.b[h][s] = *(const uint32_t*)(xs + 16 * g + (xo[h] + 4 * par) + 8 * s);
-        }
-        return o;
     };
-    Scales sc = load_scales(0), next;
+    Scales sc, next;
 #pragma unroll
-    for (int t = 0; t < DA - 1; ++t) {
-        if (t < D - 1) copy(t, t);
-        load_a(t, a[t]);
-    }
+    for (int t = 0; t < DA - 1; ++t) load_a(t, a[t]);
+    scales_a(0, sc);
+    __builtin_amdgcn_sched_barrier(0); // the weights first, then what waits for the rows' numbers
+    const uint32_t off4 = to_row(r4) * (uint32_t)x.row + 16 * ((lane & 3) ^ ((tok4 >> 2) & 3));
+    const uint32_t off2 = to_row(r2) * (uint32_t)x.row + 16 * ((lane & 1) ^ ((tok2 >> 3) & 1));
+    uint32_t xo[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) xo[h] = to_row(rx[h]) * (uint32_t)x.groups * 16 + 4 * par;
+    auto copy = [&](int t, int buffer) {
+        stage<P, NH>(st + kStage * buffer, base, off4, off2, min(t, steps - 1), wave);
+    };
+    auto scales_b = [&](int g, Scales& o) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int h = 0; h < NH; ++h) o.b[h][s] = *(const uint32_t*)(xs + 16 * g + xo[h] + 8 * s);
+    };
+#pragma unroll
+    for (int t = 0; t < D - 1; ++t) copy(t, t);
+    scales_b(0, sc);
     const int last = (steps - 1) / 4; // the last group, of 1 to 4 chunks
     auto chunk = [&](auto j, auto in_last, int g) {
         constexpr int J = decltype(j)::value;
         constexpr bool kLast = decltype(in_last)::value;
         const int t = 4 * g + J;
-        landed_barrier<kLast && J ? 0 : kUnder>();
+        constexpr int first = NH == 1 ? 2 * kCopies + 2 * NA * J : 0;
+        if (kLast)
+            landed_barrier<J ? 0 : first>();
+        else if (g == 0 && J < (NH == 1 ? 3 : 1))
+            landed_barrier<first>();
+        else
+            landed_barrier<kUnder>();
 #pragma unroll
         for (int i = 0; i < NA; ++i) asm volatile("" : "+v"(a[J][0][i]), "+v"(a[J][1][i]));
-        if constexpr (J == 0 && !kLast) next = load_scales(g + 1);
+        if constexpr (J == 0 && !kLast) {
+            scales_a(min(g + 1, groups - 1), next);
+            scales_b(min(g + 1, groups - 1), next);
+        }
         if constexpr (J == 3 && !kLast) {
 #pragma unroll
             for (int i = 0; i < NA; ++i) asm volatile("" : "+v"(next.a[i][0]), "+v"(next.a[i][1]));
@@ -291,31 +306,22 @@ __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, uint3
         for (int h = 0; h < NH; ++h) asm volatile("" : "+v"(acc[i][h]));
 }
 
-// The byte offsets of a lane's rows for the copies: row(token) of both groupings.
-template <int NH, class F> __device__ __forceinline__ uint32_t copy4(int lane, int wave, F row) {
-    const int tok = 16 * (NH == 2 ? wave : wave & 1) + (lane >> 2);
-    return row(tok) + 16 * ((lane & 3) ^ ((tok >> 2) & 3));
-}
-template <int NH, class F> __device__ __forceinline__ uint32_t copy2(int lane, int wave, F row) {
-    const int tok = 32 * (NH == 2 ? wave & 1 : 0) + (lane >> 1);
-    return row(tok) + 16 * ((lane & 1) ^ ((tok >> 3) & 1));
-}
-
 // Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in PH planes.
 // 16 tokens at Mixtral-8x7B sizes 94 us (5.3 TB/s), 4096 1.85 ms (1.04 PFLOP/s in 4 planes).
 template <int NA, int P, int PH>
-__global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
 tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,
                    Planes h) {
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int NF = NA / 2; // feature blocks a wave
     const int blocks = 4 * naiwa_mx_steps(I), ncol = (blocks + 4 * NF - 1) / (4 * NF);
-    int tile, col;
-    if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
+    int col;
+    const int4 tile = tile_col(blockIdx.x, tl, ncol, xcd, &col);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int start = uniform(tl.start[tile]), cnt = uniform(tl.count[tile]), slot = uniform(tl.slot[tile]);
-    auto row = [&](int tok) -> uint32_t { return perm[start + min(tok, cnt - 1)] / (uint32_t)width; };
-    auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)x.row; };
+    const int start = tile.x, cnt = tile.y, slot = tile.z;
+    if (cnt == 0) return;
+    auto pair = [&](int tok) -> uint32_t { return perm[start + min(tok, cnt - 1)]; };
+    auto token = [&](uint32_t p) -> uint32_t { return p / (uint32_t)width; };
     const int fb0 = (4 * col + wave) * NF; // the wave's first feature block
     const uint8_t* wp[NA];
 #pragma unroll
@@ -324,16 +330,13 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
         wp[f] = gate.base + (int64_t)slot * gate.stride + 2 * fb * gate.strip;
         wp[NF + f] = up.base + (int64_t)slot * up.stride + 2 * fb * up.strip;
     }
-    const uint32_t xo[2] = {row(lane & 31) * (uint32_t)x.groups * 16, row(32 + (lane & 31)) * (uint32_t)x.groups * 16};
     v16f acc[NA][2] = {};
     const int steps = naiwa_mx_steps(H);
     const uint32_t strip = (uint32_t)gate.strip;
     if (cnt > 32)
-        tile_dot<NA, P, 2>(smem, x.base, copy4<2>(lane, wave, off), copy2<2>(lane, wave, off), wp, strip, x.scales, xo, steps,
-                           lane, wave, acc);
+        tile_dot<NA, P, 2>(smem, x.base, x, pair, token, wp, strip, x.scales, steps, lane, wave, acc);
     else
-        tile_dot<NA, P, 1>(smem, x.base, copy4<1>(lane, wave, off), copy2<1>(lane, wave, off), wp, strip, x.scales, xo, steps,
-                           lane, wave, acc);
+        tile_dot<NA, P, 1>(smem, x.base, x, pair, token, wp, strip, x.scales, steps, lane, wave, acc);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
         const int fb = fb0 + f;
@@ -372,17 +375,18 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
 // y[part][pair][H] unweighted.  16 tokens at Mixtral-8x7B sizes 49 us (5.1 TB/s), 4096 1.27 ms
 // (0.76 PFLOP/s in 5 planes).
 template <int NA, int P>
-__global__ void __launch_bounds__(kThreads, NA == 4 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
 tile_down_kernel(Bank down, Planes h, int H, int I, int64_t n, int part_groups, const uint32_t* perm, Tiles tl, int xcd,
                  float* y) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int blocks = H / 32, ncol = (blocks + 4 * NA - 1) / (4 * NA);
-    int tile, col;
-    if (!tile_col(blockIdx.x, *tl.n, ncol, xcd, &tile, &col)) return;
+    int col;
+    const int4 tile = tile_col(blockIdx.x, tl, ncol, xcd, &col);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int start = uniform(tl.start[tile]), cnt = uniform(tl.count[tile]), slot = uniform(tl.slot[tile]);
+    const int start = tile.x, cnt = tile.y, slot = tile.z;
+    if (cnt == 0) return;
     auto row = [&](int tok) -> uint32_t { return (uint32_t)min(tok, cnt - 1); };
-    auto off = [&](int tok) -> uint32_t { return row(tok) * (uint32_t)h.row; };
+    auto same = [](uint32_t r) { return r; };
     const int rb0 = (4 * col + wave) * NA, g0 = blockIdx.y * part_groups;
     const int steps = min(naiwa_mx_steps(I) - 4 * g0, 4 * part_groups);
     const uint8_t* wp[NA];
@@ -390,16 +394,13 @@ tile_down_kernel(Bank down, Planes h, int H, int I, int64_t n, int part_groups, 
     for (int i = 0; i < NA; ++i)
         wp[i] = down.base + (int64_t)slot * down.stride + 2 * min(rb0 + i, blocks - 1) * down.strip + (int64_t)4352 * g0;
     const uint8_t* hs = h.scales + (int64_t)start * h.groups * 16 + 16 * g0;
-    const uint32_t xo[2] = {row(lane & 31) * (uint32_t)h.groups * 16, row(32 + (lane & 31)) * (uint32_t)h.groups * 16};
     v16f acc[NA][2] = {};
     const uint8_t* rows = h.base + (int64_t)start * h.row + (int64_t)4 * g0 * 96 * P;
     const uint32_t strip = (uint32_t)down.strip;
     if (cnt > 32)
-        tile_dot<NA, P, 2>(smem, rows, copy4<2>(lane, wave, off), copy2<2>(lane, wave, off), wp, strip, hs, xo, steps, lane,
-                           wave, acc);
+        tile_dot<NA, P, 2>(smem, rows, h, row, same, wp, strip, hs, steps, lane, wave, acc);
     else
-        tile_dot<NA, P, 1>(smem, rows, copy4<1>(lane, wave, off), copy2<1>(lane, wave, off), wp, strip, hs, xo, steps, lane,
-                           wave, acc);
+        tile_dot<NA, P, 1>(smem, rows, h, row, same, wp, strip, hs, steps, lane, wave, acc);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         const int tok = 32 * s + (lane & 31);

@@ -97,40 +97,32 @@ def _blocks(text, kernel):
                                            ("tile_down_kernelILi2ELi5E", 4)])
 def test_counted_waits_cover_their_copies(text, kernel, copies):
     """Along every path to a barrier behind a wait that lets N loads be under way, at least N loads follow the
-    copies of the chunk that is read next: the newest copies before the barrier where the tile is two
-    chunks deep (2 `copies` a chunk), those of two chunks earlier where it is four deep."""
+    copies of the chunk that is read next: the newest copies in tiles of 64 rows, in those of 32 (`copies` a
+    chunk) the ones before the two newest chunks."""
     blocks = _blocks(text, kernel)
-    # a path's state: loads issued since the end of each of the last 3 runs of copies, the newest first
-    # ("run": copies with no other load between them); None: not on a path yet
+    keep = 64                                   # a path's state: its newest loads, c a copy, l another
     state = {b: set() for b in blocks}
-    state["entry"] = {(False, ())}
-    work, waits, seen = ["entry"], {}, 0
+    state["entry"] = {""}
+    work, waits = ["entry"], {}
     while work:
         b = work.pop()
         cur = set(state[b])
         body, to = blocks[b]
         for i, l in enumerate(body):
-            lds, load = l.startswith("global_load_lds"), l.startswith(("global_load", "global_store", "scratch_"))
-            if load:
-                nxt = set()
-                for in_run, runs in cur:
-                    if lds and in_run:
-                        nxt.add((True, ((0, runs[0][1] + 1),) + tuple((n + 1, c) for n, c in runs[1:])))
-                    else:
-                        runs = tuple((n + 1, c) for n, c in runs)
-                        nxt.add((lds, (((0, 1),) + runs)[:3]) if lds else (False, runs))
-                cur = {(r, tuple((min(n, 64), c) for n, c in s)) for r, s in nxt}
+            if l.startswith(("global_load", "global_store", "scratch_")):
+                op = "c" if l.startswith("global_load_lds") else "l"
+                cur = {(s + op)[-keep:] for s in cur}
             m = re.match(r"s_waitcnt vmcnt\((\d+)\) lgkmcnt\(0\)$", l)
-            if m and i + 1 < len(body) and body[i + 1] == "s_barrier" and int(m.group(1)):
-                for _, runs in cur:
-                    waits.setdefault(int(m.group(1)), set()).add(runs)
+            if m and int(m.group(1)) and body[i + 1:i + 2] == ["s_barrier"]:
+                waits.setdefault(int(m.group(1)), set()).update(cur)
         for t in to:
             if not cur <= state[t]:
                 state[t] |= cur
                 work.append(t)
-    assert sorted(waits) == [4, 4 + 2 * (copies + 4)]
+    steady = 4 + 2 * (copies + 4)
+    assert set(waits) == {4, 2 * copies, 2 * copies + 4, 2 * copies + 8, steady}
     for n, paths in waits.items():
-        for runs in paths:
-            deep = n != 4
-            need = runs[2] if deep else runs[0]
-            assert need[1] == (copies if deep else 2 * copies) and need[0] >= n, (n, runs)
+        newer = 0 if n == 4 else 2 * copies
+        for s in paths:
+            at = [i for i, op in enumerate(s) if op == "c"]
+            assert len(at) > newer and len(s) - 1 - at[-1 - newer] >= n, (n, s)
