@@ -19,7 +19,7 @@
 //
 // Bound.  Few tokens an expert: HBM, the weights are read once (96 tokens at Qwen3-30B sizes 4.9
 // TB/s in gate/up, 16 at Mixtral-8x7B sizes 5.0, where a copy reaches 5.1).  Many: the scaled
-// products and the power they draw; 4096 tokens at Mixtral sizes run 1.9 + 1.3 ms, 4.1 and 3.6
+// products and the power they draw; 4096 tokens at Mixtral sizes run 1.8 + 1.2 ms, 4.3 and 3.9
 // PFLOP/s of FP4 x E2M3, where the same products from registers alone reach 6 to 7 with random
 // codes and 9.9 with zeros, the chip's full rate: its power is the limit.  Without the weights'
 // loads gate/up takes 17 % less, without the copies 14 %, without the LDS reads no less.
@@ -307,7 +307,7 @@ __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, const
 }
 
 // Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in PH planes.
-// 16 tokens at Mixtral-8x7B sizes 94 us (5.3 TB/s), 4096 1.85 ms (1.04 PFLOP/s in 4 planes).
+// 16 tokens at Mixtral-8x7B sizes 94 us (5.3 TB/s), 4096 1.79 ms (1.07 PFLOP/s in 4 planes).
 template <int NA, int P, int PH>
 __global__ void __launch_bounds__(kThreads, 2)
 tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,
@@ -372,8 +372,8 @@ tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const 
 }
 
 // Down of a tile and a K part of part_groups groups of 4 steps: NA tiles of 32 rows a wave;
-// y[part][pair][H] unweighted.  16 tokens at Mixtral-8x7B sizes 49 us (5.1 TB/s), 4096 1.27 ms
-// (0.76 PFLOP/s in 5 planes).
+// y[part][pair][H] unweighted.  16 tokens at Mixtral-8x7B sizes 48 us (5.2 TB/s), 4096 1.23 ms
+// (0.78 PFLOP/s in 5 planes).
 template <int NA, int P>
 __global__ void __launch_bounds__(kThreads, 2)
 tile_down_kernel(Bank down, Planes h, int H, int I, int64_t n, int part_groups, const uint32_t* perm, Tiles tl, int xcd,
