@@ -29,8 +29,9 @@
 //   2. gate/up: a block per (tile, 128 features); h = act(g) u in planes;
 //   3. down: a block per (tile, 256 rows, K part); unweighted dots per pair;
 //   4. combine: out[t] = the weighted sum over t's pairs in ascending slot order.
-// (2. and 3.: mxfp4_tiles.h.)  One token takes two launches: gate/up lays x out itself, a block
-// per (pair, 32 features), and down combines (gateup_one_kernel, down_one_kernel).
+// (2. and 3.: mxfp4_tiles.h.)  One token, and few whose experts are small, take two launches:
+// gate/up lays x out itself, a block per (pair, 32 features), and down combines
+// (gateup_pair_kernel, down_pair_kernel).
 // No atomics: every run adds the same terms in the same order, and in calls of as many pairs the
 // order of a pair's terms does not depend on the other pairs.
 #include "mxfp4.h"
@@ -216,7 +217,7 @@ template <int P> __device__ __forceinline__ v6u load_plane(const uint8_t* at, in
 // byte), of one token whose planes are in LDS (xp, xs: the row, the same for every lane): rounds of
 // U steps, all their weights in flight; `before` runs once the first round's are.
 template <int S, int P, class F>
-__device__ __forceinline__ void strips_dot_one(const uint8_t* const (&wp)[S], const uint8_t* xp, const uint8_t* xs, int steps,
+__device__ __forceinline__ void strips_dot(const uint8_t* const (&wp)[S], const uint8_t* xp, const uint8_t* xs, int steps,
                                                int t0, int t1, int lane, v4f (&acc)[S], F before) {
     constexpr int U = 16 / S < 8 ? 16 / S : 8;
     const int kb = lane >> 4;
@@ -332,20 +333,20 @@ __device__ __forceinline__ void put_h(const Sums<NW>& sums, int tok, bool pad, i
     if (f == 0) h.scales[row * h.groups * 16 + scale_at(fb)] = (uint8_t)s;
 }
 
-// Gate/up of one token: a block per (pair, 32 features); each wave lays out its own steps of x in
-// LDS while its first weights are on the way.  Pair j is row j of h; blocks past I (h padded to
-// whole steps) write zeros.  The first block lists the pairs that count as tiles of one pair, for
-// tile_down_kernel.  Dynamic LDS: the planes of x, their scales (16 bytes a group).  Bound: latency
+// Gate/up by pair, for few tokens: a block per (pair, 32 features); each wave lays out its own
+// steps of the token's x in LDS while its first weights are on the way.  Pair j is row j of h;
+// blocks past I (h padded to whole steps) write zeros.  Of one token, the first block lists the
+// pairs that count as tiles of one pair, for tile_down_kernel.  Dynamic LDS: the planes of x, their scales (16 bytes a group).  Bound: latency
 // (the launch, x to planes behind the first weights' way, four waves' sums): 8 of 128 Qwen3-30B
 // experts 6.6 us (13.4 MB), 2 of 8 of 1024 x 2048 6.3 us (4.5 MB).
 template <int PX, int PH, bool BF16>
 __global__ void __launch_bounds__(kThreads, 2)
-gateup_one_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32_t* ids, const float* w, int width, int slots,
+gateup_pair_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32_t* ids, const float* w, int width, int slots,
                   int skip_zero, int act, Planes h, uint32_t* perm, Tiles tl) {
     extern __shared__ __align__(16) uint8_t xl[];
     __shared__ Sums<kWaves> sums;
     const int j = blockIdx.x, fb = blockIdx.y;
-    if (j == 0 && fb == 0 && threadIdx.x < 64) {
+    if (gridDim.x == (unsigned)width && j == 0 && fb == 0 && threadIdx.x < 64) {
         const int i = threadIdx.x;
         const uint32_t id = i < width ? ids[i] : 0xffffffffu;
         const bool in = id < (uint32_t)slots && !(skip_zero && w[i] == 0.0f);
@@ -369,14 +370,14 @@ gateup_one_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32_
         auto stage = [&] {
             for (int kb = 4 * t0 + lane; kb < 4 * t1; kb += 64) {
                 float f[32];
-                load_block<BF16>(x, 0, H, kb, f);
+                load_block<BF16>(x, (int64_t)(j / width) * H, H, kb, f);
                 const int sb = scale_byte(abs_max(f));
                 v6u o[PX];
                 to_planes<PX>(f, sb, o);
                 put_block<PX>(xl, scales, kb, o, sb);
             }
         };
-        strips_dot_one<4, PX>(wp, xl, scales, steps, t0, t1, lane, acc, stage);
+        strips_dot<4, PX>(wp, xl, scales, steps, t0, t1, lane, acc, stage);
     }
     sums.put(threadIdx.x >> 6, lane, acc);
     __syncthreads();
@@ -417,26 +418,28 @@ __device__ __forceinline__ void residual4(uint16_t* x, const v4f& y) {
     *(uint2*)x = z;
 }
 
-// Down and combine of one token: a block of 8 waves per 16 rows.  A pair's steps go to the
+// Down and combine by pair: a block of 8 waves per 16 rows and token.  A pair's steps go to the
 // `split` waves of one of 8 / split groups, the groups take the pairs in turn; the sums meet in
 // LDS and 4 lanes of the first wave add them up, pairs in ascending slot order.  Dynamic LDS:
-// h's planes and scales of every pair, copied by all waves.  Bound: latency, as gate/up: Qwen3-30B
+// h's planes and scales of the token's pairs, copied by all waves.  Bound: latency, as gate/up: Qwen3-30B
 // sizes 6.5 us (6.7 MB), 8 experts of 1024 x 2048 4.8 us.
-constexpr int kOneWaves = 8;
+constexpr int kPairWaves = 8;
 template <int PH>
-__global__ void __launch_bounds__(64 * kOneWaves)
-down_one_kernel(Bank down, Planes h, int H, int I, const uint32_t* ids, const float* w, int width, int slots, int skip_zero,
+__global__ void __launch_bounds__(64 * kPairWaves)
+down_pair_kernel(Bank down, Planes h, int H, int I, const uint32_t* ids, const float* w, int width, int slots, int skip_zero,
                 int split, int accumulate, float* out, uint16_t* res) {
     extern __shared__ __align__(16) uint8_t hl[];
     __shared__ Order order;
-    __shared__ v4f red[kMaxWidth][kOneWaves][4]; // [pair][wave of the group][row / 4]
+    __shared__ v4f red[kMaxWidth][kPairWaves][4]; // [pair][wave of the group][row / 4]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rb = blockIdx.x, steps = naiwa_mx_steps(I), groups = kOneWaves / split, in = wave % split;
+    const int rb = blockIdx.x, steps = naiwa_mx_steps(I), groups = kPairWaves / split, in = wave % split;
+    const int64_t first = (int64_t)blockIdx.y * width; // the token's first pair
+    ids += first, w += first, h.base += first * h.row, h.scales += first * h.groups * 16;
     int t0, t1;
     deal(steps, in, split, &t0, &t1);
     order.make(ids, w, width, slots, skip_zero);
     const int row16 = (int)(h.row / 16);
-    for (int i = tid; i < width * (row16 + h.groups); i += 64 * kOneWaves) {
+    for (int i = tid; i < width * (row16 + h.groups); i += 64 * kPairWaves) {
         const int j = i / (row16 + h.groups), c = i % (row16 + h.groups);
         // pairs that do not count have rows that nobody wrote: copied, never used
         *(v4u*)(hl + (size_t)16 * i) = c < row16 ? *(const v4u*)(h.base + j * h.row + 16 * c)
@@ -449,12 +452,12 @@ down_one_kernel(Bank down, Planes h, int H, int I, const uint32_t* ids, const fl
         const uint8_t* const wp[1] = {down.base + (int64_t)s * down.stride + rb * down.strip};
         const uint8_t* hr = hl + (size_t)16 * j * (row16 + h.groups);
         v4f acc[1] = {};
-        strips_dot_one<1, PH>(wp, hr, hr + 16 * row16, steps, t0, t1, lane, acc, [] {});
+        strips_dot<1, PH>(wp, hr, hr + 16 * row16, steps, t0, t1, lane, acc, [] {});
         if ((lane & 15) == 0) red[q][in][lane >> 4] = acc[0];
     }
     __syncthreads();
     if (tid >= 4) return;
-    const int64_t o = 16 * rb + 4 * tid;
+    const int64_t o = (int64_t)blockIdx.y * H + 16 * rb + 4 * tid;
     v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
     if (accumulate) y = *(const v4f*)(out + o);
     for (int q = 0; q < count; ++q) {
@@ -606,29 +609,41 @@ struct Run { // one pass's pieces
         combine(parts);
     }
 
-    // One token.  False, with nothing launched, where x does not fit in LDS.
-    template <int PX, int PH, bool BF16> bool one() const {
+    // Whether every pair reads its weights for itself (2 launches) instead of in tiles (4 or 5).  One
+    // token has an expert once, so always; few tokens while reading some twice costs less than the
+    // launches: 112 MB of weights at most, and no expert more than twice on average.  In microseconds a
+    // call, by pair and in tiles: Qwen3-30B 2 tokens (41 MB) 18.7 and 27.5, 4 (82) 27.1 and 30.1, 6 (123)
+    // 37.8 and 35.6; DeepSeek-V2-Lite 4 (112) 34.4 and 37.6, 6 (168) 47.4 and 44.1; 8 experts of H 1024, I
+    // 2048 top-2, 8 (54) 22.5 and 25.1, 16 (107, every expert four times) 36.1 and 25.4; Mixtral-8x7B 2
+    // (374) 88.0 and 86.1, 3 (562) 125 and 103.
+    bool few() const {
+        const int64_t expert = 2 * (I / 16) * naiwa_mx_strip_bytes(H) + (H / 16) * naiwa_mx_strip_bytes(I);
+        return c.rows == 1 || (n <= 2 * slots && n * expert <= 112000000);
+    }
+
+    // By pair.  False, with nothing launched, where x (or h of one of several tokens) does not fit in LDS.
+    template <int PX, int PH, bool BF16> bool pairs() const {
         const size_t xl = (size_t)plane_row(PX, H) + (size_t)naiwa_mx_groups(H) * 16;
         const size_t hl = ((size_t)plane_row(PH, I) + (size_t)naiwa_mx_groups(I) * 16) * c.width;
         // With the kernels' own 17 and 33 KB, what a CU has.  One token of H 16384, 4 experts of 1024
         // top-2, 31 us here and 74 as a tile; of 8 Mixtral-8x7B experts (h of 2 x 14336) 51 and 63.
         constexpr size_t kLds = 120 * 1024;
-        if (xl > kLds) return false;
-        gateup_one_kernel<PX, PH, BF16><<<dim3(c.width, 4 * naiwa_mx_steps(I)), kThreads, xl, st>>>(
+        if (xl > kLds || (c.rows > 1 && hl > kLds)) return false;
+        gateup_pair_kernel<PX, PH, BF16><<<dim3(n, 4 * naiwa_mx_steps(I)), kThreads, xl, st>>>(
             g, u, c.x, H, I, c.ids, c.w, c.width, slots, c.skip_zero, c.act, h(PH), perm, tl);
         if (hl > kLds) {
             down<PH>();
             return true;
         }
         int split = 1;
-        while (2 * split * c.width <= kOneWaves && 8 * split <= naiwa_mx_steps(I)) split *= 2;
-        down_one_kernel<PH><<<H / 16, 64 * kOneWaves, hl, st>>>(d, h(PH), H, I, c.ids, c.w, c.width, slots, c.skip_zero, split,
+        while (2 * split * c.width <= kPairWaves && 8 * split <= naiwa_mx_steps(I)) split *= 2;
+        down_pair_kernel<PH><<<dim3(H / 16, c.rows), 64 * kPairWaves, hl, st>>>(d, h(PH), H, I, c.ids, c.w, c.width, slots, c.skip_zero, split,
                                                                 c.accumulate, c.out, c.res);
         return true;
     }
 
     template <int PX, int PH, bool BF16> int go() const {
-        if (c.rows == 1 && one<PX, PH, BF16>()) return naiwa_hip_rc(hipGetLastError());
+        if (few() && pairs<PX, PH, BF16>()) return naiwa_hip_rc(hipGetLastError());
         // The pairs are sorted in the planes' launch; many pairs, whose sorting takes its one block
         // longer than the planes take, in a launch of their own.  A call at Qwen3-30B sizes, in the
         // launch and apart: 128 pairs 52.5 and 54.1 us, 512 77.0 and 78.2, 768 81.3 and 80.4, 2048 115

@@ -180,6 +180,9 @@ def decode(nm, ex, x, ids, w, act="silu", out0=None, f32=False, noalloc=False):
     (1, 1, 33024, 32, 1),      # and whose x does
     (1, 2, 64, 12288, 2), (1, 1, 24576, 32, 1),   # one token whose h and whose x take most of it
     (1, 2, 11008, 64, 2), (2, 64, 64, 32, 64),
+    (8, 8, 96, 64, 2), (4, 16, 288, 160, 6), (3, 8, 544, 736, 5),   # few tokens by pair
+    (2, 1, 96, 64, 2), (4, 4, 288, 160, 3),    # as few in tiles
+    (2, 8, 64, 4096, 8), (2, 2, 33024, 32, 2),  # by pair but for h and x that fill more than LDS
 ])
 @pytest.mark.parametrize("f32", [False, True])
 def test_decode_against_64_bits(gpu, T, E, H, I, k, f32):
@@ -319,7 +322,7 @@ def prefill(nm, ex, x, ids, w, act="silu", out0=None, residual=False):
 
 
 @pytest.mark.parametrize("T,E,H,I,k,act", [
-    (1, 1, 32, 32, 1, "silu"), (63, 4, 160, 96, 2, "silu"), (64, 1, 128, 128, 1, "gelu"), (65, 2, 288, 224, 1, "silu"),
+    (1, 1, 32, 32, 1, "silu"), (3, 8, 160, 96, 2, "gelu"), (63, 4, 160, 96, 2, "silu"), (64, 1, 128, 128, 1, "gelu"), (65, 2, 288, 224, 1, "silu"),
     (129, 3, 512, 416, 3, "silu"), (300, 8, 672, 160, 6, "gelu"), (512, 4, 256, 1408, 2, "silu"),
     (700, 2, 1056, 96, 2, "silu"), (2048, 16, 96, 64, 8, "silu"), (200, 1, 2048, 768, 1, "silu"),
 ])
