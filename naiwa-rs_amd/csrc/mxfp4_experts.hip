@@ -566,6 +566,18 @@ int naiwa_mx_check(const NaiwaMxCall& c) {
     return NAIWA_OK;
 }
 
+// Whether every pair reads its weights for itself (2 launches) instead of in tiles (4 or 5).  One
+// token has an expert once, so always; few tokens while reading some twice costs less than the
+// launches: 112 MB of weights at most, and no expert more than twice on average.  In microseconds a
+// call, by pair and in tiles: Qwen3-30B 2 tokens (41 MB) 18.7 and 27.5, 4 (82) 27.1 and 30.1, 6 (123)
+// 37.8 and 35.6; DeepSeek-V2-Lite 4 (112) 34.4 and 37.6, 6 (168) 47.4 and 44.1; 8 experts of H 1024, I
+// 2048 top-2, 8 (54) 22.5 and 25.1, 16 (107, every expert four times) 36.1 and 25.4; Mixtral-8x7B 2
+// (374) 88.0 and 86.1, 3 (562) 125 and 103.
+extern "C" bool naiwa_mx_by_pair(int rows, int64_t n, int slots, int H, int I) {
+    const int64_t expert = 2 * (I / 16) * naiwa_mx_strip_bytes(H) + (H / 16) * naiwa_mx_strip_bytes(I);
+    return rows == 1 || (n <= 2 * (int64_t)slots && n * expert <= 112000000);
+}
+
 namespace {
 
 constexpr int kNA = 2; // tiles of 32 weight rows a wave of the tile kernels
@@ -609,18 +621,6 @@ struct Run { // one pass's pieces
         combine(parts);
     }
 
-    // Whether every pair reads its weights for itself (2 launches) instead of in tiles (4 or 5).  One
-    // token has an expert once, so always; few tokens while reading some twice costs less than the
-    // launches: 112 MB of weights at most, and no expert more than twice on average.  In microseconds a
-    // call, by pair and in tiles: Qwen3-30B 2 tokens (41 MB) 18.7 and 27.5, 4 (82) 27.1 and 30.1, 6 (123)
-    // 37.8 and 35.6; DeepSeek-V2-Lite 4 (112) 34.4 and 37.6, 6 (168) 47.4 and 44.1; 8 experts of H 1024, I
-    // 2048 top-2, 8 (54) 22.5 and 25.1, 16 (107, every expert four times) 36.1 and 25.4; Mixtral-8x7B 2
-    // (374) 88.0 and 86.1, 3 (562) 125 and 103.
-    bool few() const {
-        const int64_t expert = 2 * (I / 16) * naiwa_mx_strip_bytes(H) + (H / 16) * naiwa_mx_strip_bytes(I);
-        return c.rows == 1 || (n <= 2 * slots && n * expert <= 112000000);
-    }
-
     // By pair.  False, with nothing launched, where x (or h of one of several tokens) does not fit in LDS.
     template <int PX, int PH, bool BF16> bool pairs() const {
         const size_t xl = (size_t)plane_row(PX, H) + (size_t)naiwa_mx_groups(H) * 16;
@@ -643,7 +643,7 @@ struct Run { // one pass's pieces
     }
 
     template <int PX, int PH, bool BF16> int go() const {
-        if (few() && pairs<PX, PH, BF16>()) return naiwa_hip_rc(hipGetLastError());
+        if (naiwa_mx_by_pair(c.rows, n, slots, H, I) && pairs<PX, PH, BF16>()) return naiwa_hip_rc(hipGetLastError());
         // The pairs are sorted in the planes' launch; many pairs, whose sorting takes its one block
         // longer than the planes take, in a launch of their own.  A call at Qwen3-30B sizes, in the
         // launch and apart: 128 pairs 52.5 and 54.1 us, 512 77.0 and 78.2, 768 81.3 and 80.4, 2048 115

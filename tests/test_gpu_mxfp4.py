@@ -178,7 +178,8 @@ def decode(nm, ex, x, ids, w, act="silu", out0=None, f32=False, noalloc=False):
     (300, 8, 128, 96, 4),      # more pairs than are sorted beside the planes
     (1, 8, 128, 4096, 8),      # one token whose h fills more than LDS
     (1, 1, 33024, 32, 1),      # and whose x does
-    (1, 2, 64, 12288, 2), (1, 1, 24576, 32, 1),   # one token whose h and whose x take most of it
+    (1, 3, 64, 10496, 3), (1, 1, 32256, 32, 1),   # one token whose h and whose x just fit
+    (1, 2, 64, 12288, 2), (1, 1, 24576, 32, 1),
     (1, 2, 11008, 64, 2), (2, 64, 64, 32, 64),
     (8, 8, 96, 64, 2), (4, 16, 288, 160, 6), (3, 8, 544, 736, 5),   # few tokens by pair
     (2, 1, 96, 64, 2), (4, 4, 288, 160, 3),    # as few in tiles

@@ -180,3 +180,16 @@ def test_gguf_mxfp4_stacks_are_laid_out_in_tile_order(tmp_path, monkeypatch):
         for p in range(3):
             for e in range(E):
                 assert np.array_equal(stacks.view(p)[e], want[p][e])
+
+
+@pytest.mark.parametrize("rows,k,slots,H,I,by_pair", [
+    (1, 64, 64, 8192, 28672, True),                                     # one token, whatever the sizes
+    (2, 8, 128, 2048, 768, True), (4, 8, 128, 2048, 768, True), (6, 8, 128, 2048, 768, False),
+    (4, 6, 64, 2048, 1408, True), (5, 6, 64, 2048, 1408, False), (2, 2, 8, 4096, 14336, False),
+    (8, 2, 8, 1024, 2048, True), (9, 2, 8, 1024, 2048, False), (2, 1, 1, 32, 32, True), (3, 1, 1, 32, 32, False),
+])
+def test_few_tokens_by_pair(rows, k, slots, H, I, by_pair):
+    """By the bytes that the pairs read and by how often an expert is read, not by the rows alone."""
+    f = nm.lib().naiwa_mx_by_pair
+    f.restype = C.c_bool
+    assert f(rows, C.c_int64(rows * k), slots, H, I) == by_pair
