@@ -528,7 +528,6 @@ int64_t tiles_most(int64_t n, int slots) { return (n / kTile + std::min<int64_t>
 
 struct Layout {
     size_t offsets, bad, perm, tiles, x, xs, h, hs, y, total;
-    int64_t max_tiles;
     Layout(int64_t rows, int width, int H, int I) {
         auto a256 = [](size_t b) { return (b + 255) & ~size_t(255); };
         const size_t n = (size_t)rows * width;
@@ -536,8 +535,7 @@ struct Layout {
         bad = a256(offsets + (size_t)(NAIWA_SEG_MAX_KEYS + 1) * 4);
         perm = bad + 256;
         tiles = a256(perm + n * 4);
-        max_tiles = tiles_most((int64_t)n, NAIWA_SEG_MAX_KEYS);
-        x = a256(tiles + (size_t)max_tiles * sizeof(int4));
+        x = a256(tiles + (size_t)tiles_most((int64_t)n, NAIWA_SEG_MAX_KEYS) * sizeof(int4));
         xs = a256(x + (size_t)rows * plane_row(kPlanesMost, H));
         h = a256(xs + (size_t)rows * naiwa_mx_groups(H) * 16);
         hs = a256(h + n * plane_row(kPlanesMost, I));

@@ -49,13 +49,6 @@ template <int N> __device__ __forceinline__ void landed_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// Every LDS access of this wave is done, and every wave is here (loads stay in flight).
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 // A value that every lane has, in a scalar register.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
