@@ -336,7 +336,8 @@ __device__ __forceinline__ void put_h(const Sums<NW>& sums, int tok, bool pad, i
 // Gate/up by pair, for few tokens: a block per (pair, 32 features); each wave lays out its own
 // steps of the token's x in LDS while its first weights are on the way.  Pair j is row j of h;
 // blocks past I (h padded to whole steps) write zeros.  Of one token, the first block lists the
-// pairs that count as tiles of one pair, for tile_down_kernel.  Dynamic LDS: the planes of x, their scales (16 bytes a group).  Bound: latency
+// pairs that count as tiles of one pair, for tile_down_kernel, and clears the list's other entries: at
+// most 64 in all (naiwa_mx_tiles).  Dynamic LDS: the planes of x, their scales (16 bytes a group).  Bound: latency
 // (the launch, x to planes behind the first weights' way, four waves' sums): 8 of 128 Qwen3-30B
 // experts 6.6 us (13.4 MB), 2 of 8 of 1024 x 2048 6.3 us (4.5 MB).
 template <int PX, int PH, bool BF16>
@@ -526,6 +527,13 @@ int down_parts(int64_t n, int64_t blocks, int H, int I) {
 // The most tiles of n pairs over `slots` slots, a multiple of 8.
 int64_t tiles_most(int64_t n, int slots) { return (n / kTile + std::min<int64_t>(n, slots) + 7) / 8 * 8; }
 
+// Entries of a call's tile list.  One token's tiles hold a pair each (or, sorted, a slot's pairs, of
+// which there are at most kTile): n of them at most.  gateup_pair_kernel lists them by a lane an entry.
+static_assert(kMaxWidth <= 64 && kMaxWidth % 8 == 0 && kMaxWidth <= kTile, "a lane an entry of one token's tile list");
+extern "C" int naiwa_mx_tiles(int rows, int64_t n, int slots) {
+    return (int)(rows == 1 ? (n + 7) / 8 * 8 : tiles_most(n, slots));
+}
+
 struct Layout {
     size_t offsets, bad, perm, tiles, x, xs, h, hs, y, total;
     Layout(int64_t rows, int width, int H, int I) {
@@ -674,8 +682,7 @@ int run_pass(const NaiwaMxCall& c, uint8_t* ws, hipStream_t st) {
                 Bank{(const uint8_t*)c.up->base, c.up->slot_stride, naiwa_mx_strip_bytes(H)},
                 Bank{(const uint8_t*)c.down->base, c.down->slot_stride, naiwa_mx_strip_bytes(I)},
                 (uint32_t*)(ws + L.offsets), (uint32_t*)(ws + L.perm),
-                // (one token has a tile a pair)
-                Tiles{(int4*)(ws + L.tiles), (int)(tiles_most(n, c.rows == 1 ? n : c.gate->slots) / 8)}};
+                Tiles{(int4*)(ws + L.tiles), naiwa_mx_tiles(c.rows, n, c.gate->slots) / 8}};
     if (n == 0) {
         r.combine(1);
         return naiwa_hip_rc(hipGetLastError());

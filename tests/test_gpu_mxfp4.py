@@ -663,3 +663,31 @@ def test_captured_and_replayed(gpu, T):
             st.sync()
             assert np.array_equal(d.download(np.uint32), want[0]) and np.array_equal(p.download(np.uint32), want[1])
     g.close()
+
+
+@pytest.mark.parametrize("width,E,H,I", [(64, 64, 64, 512), (64, 3, 96, 416), (63, 64, 64, 512), (57, 8, 64, 512),
+                                         (64, 64, 64, 384), (48, 4, 33024, 32)])
+def test_one_token_of_the_widest_rows(gpu, width, E, H, I):
+    """Up to 64 experts a token, whose h fills more than LDS (from I 416 on) and goes down in tiles: all pairs,
+    some of them dropped or of no slot, and nothing, over scratch that a larger call has filled."""
+    nm = gpu
+    rng = np.random.default_rng(width + E + I)
+    print(f"[one token {width} {E} {H} {I}]", flush=True)
+    ex = Experts(nm, 130, E, H, I)
+    before = f32_of(bf16(rng.standard_normal((40, H)))), *route(rng, 40, E, 8)
+    for case in range(3):
+        x = f32_of(bf16(rng.standard_normal((1, H))))
+        ids, w = route(rng, 1, E, width)
+        if case == 1:
+            w[0, ::5], ids[0, 2::7], ids[0, 3::11] = 0, E, 0xFFFFFFFF
+        elif case == 2:
+            ids[:] = E
+        want = M.experts(x, ids, w, *ex.w)
+        decode(nm, ex, *before)
+        assert np.array_equal(got := decode(nm, ex, x, ids, w, noalloc=True), decode(nm, ex, x, ids, w))
+        prefill(nm, ex, *before)
+        chunk = prefill(nm, ex, x, ids, w)[0]
+        if case == 2:
+            assert (got == 0).all() and (chunk == 0).all()
+        else:
+            assert rel(got, want) < REL and rel(chunk, want) < REL

@@ -193,3 +193,17 @@ def test_few_tokens_by_pair(rows, k, slots, H, I, by_pair):
     f = nm.lib().naiwa_mx_by_pair
     f.restype = C.c_bool
     assert f(rows, C.c_int64(rows * k), slots, H, I) == by_pair
+
+
+def test_tile_list_of_one_token_is_written_whole():
+    """A wave lists one token's pairs and clears the other entries, an entry a lane: at every width the list
+    holds every pair and has no entry past the wave's 64 lanes (72 at width 64 were 8 that nobody wrote)."""
+    f = nm.lib().naiwa_mx_tiles
+    f.restype = C.c_int
+    for width in range(1, 65):
+        for slots in (1, 8, 64, 4096):
+            t = f(1, C.c_int64(width), slots)
+            assert width <= t <= 64 and t % 8 == 0, (width, slots)
+    # of more tokens at most a tile a slot and one for every further 64 pairs
+    for n, slots in ((2, 1), (65, 1), (66, 2), (512, 128), (65536, 4096), (8192, 4096)):
+        assert f(2, C.c_int64(n), slots) >= min(n, slots) + (n - min(n, slots)) // 64
