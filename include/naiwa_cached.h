@@ -21,7 +21,9 @@
  * memory, a CPU job on a one-thread executor computes those pairs from the
  * host expert stacks (naiwa_cpu_moe_decode), and its result comes back through
  * a result doorbell that the device waits for on the stream and adds last:
- * resident, then staged, then CPU (src/moe/decode.rs:371-381).
+ * resident, then staged, then CPU (src/moe/decode.rs:371-381).  The CPU path
+ * computes Q4_K and Q8_0: a step of an MXFP4 layer that would leave a miss to it
+ * (more missed experts than ring positions, or pcie_frac under 1) is refused.
  */
 #ifndef NAIWA_CACHED_H
 #define NAIWA_CACHED_H
@@ -175,7 +177,8 @@ int naiwa_cached_layer_set_upload_path(naiwa_cached_layer* L, int path);
 /* Misses the ring does not take go to the CPU (1, the default) or, with 0, a
  * step that would leave any miss unstaged is refused with NAIWA_E_UNSUPPORTED
  * before the policy is touched (naiwa_cache_plan decides; no tick, hit count or
- * ring position moves).  No counterpart in the reference, whose misses always
+ * ring position moves).  Layers of a type that the CPU path does not compute
+ * (MXFP4) refuse such a step with either setting.  No counterpart in the reference, whose misses always
  * may go to the CPU; for hosts that keep every expert computation on the GPU. */
 int naiwa_cached_layer_set_cpu_misses(naiwa_cached_layer* L, int on);
 

@@ -221,6 +221,7 @@ struct naiwa_cached_layer {
     // misses left to the CPU: the host stacks, the activation publish page
     // [seq][pad][rows * H f32] (mapped), its publishes so far, and the CPU sum on the device
     bool cpu_misses = true;
+    bool cpu_types = true;         // the CPU path computes the banks' types (Q4_K and Q8_0)
     naiwa_host_experts hx{};
     uint32_t* xpub_host = nullptr;
     uint32_t* xpub_dev = nullptr;
@@ -466,7 +467,8 @@ int forward_impl(naiwa_cached_layer* L, naiwa_cached_layer* next, int swaps_per_
     // a CPU job of an earlier step that failed (its result was not computed): report it
     // before this step touches anything
     int rc = NAIWA_OK;
-    naiwa_executor* ex = L->cpu_misses ? cpu_executor(&rc) : nullptr;
+    const bool cpu_misses = L->cpu_misses && L->cpu_types;
+    naiwa_executor* ex = cpu_misses ? cpu_executor(&rc) : nullptr;
     if (rc) return rc;
     if (ex && (rc = naiwa_executor_take_error(ex, nullptr, 0))) return rc;
     rc = L->ensure_rows(rows);
@@ -526,7 +528,7 @@ int forward_impl(naiwa_cached_layer* L, naiwa_cached_layer* next, int swaps_per_
     }
     // without the CPU path, a step that would leave a miss unstaged is refused before
     // the policy is touched (no tick, hit count or ring position moves)
-    if (!L->cpu_misses) {
+    if (!cpu_misses) {
         naiwa_step_plan plan{};
         if ((rc = naiwa_cache_plan(L->cache, L->ring_len, L->ids_h, L->w_h, rows, k, pcie_frac, &plan))) return rc;
         if (plan.cpu > 0) return NAIWA_E_UNSUPPORTED;
@@ -779,6 +781,8 @@ int naiwa_cached_layer_create(const naiwa_cached_layer_desc* d, naiwa_ring* ring
     L->ring = ring;
     L->ring_len = ring_len;
     L->copy = (hipStream_t)copy_stream;
+    for (int dt : {d->gate.dtype, d->up.dtype, d->down.dtype})
+        if (dt != NAIWA_Q4_K && dt != NAIWA_Q8_0) L->cpu_types = false;
     L->bytes[0] = (size_t)naiwa_projection_bytes(d->gate.dtype, d->inter, d->hidden);
     L->bytes[1] = (size_t)naiwa_projection_bytes(d->up.dtype, d->inter, d->hidden);
     L->bytes[2] = (size_t)naiwa_projection_bytes(d->down.dtype, d->hidden, d->inter);

@@ -273,7 +273,8 @@ class CachedLayer:
         check(lib().naiwa_cached_layer_set_upload_path(self._h, path), "cached_layer_set_upload_path")
 
     def set_cpu_misses(self, on: bool) -> None:
-        """Misses the ring does not take run on the CPU (default), or such a step is refused."""
+        """Misses the ring does not take run on the CPU (default), or such a step is refused (of an
+        MXFP4 layer always)."""
         check(lib().naiwa_cached_layer_set_cpu_misses(self._h, 1 if on else 0), "cached_layer_set_cpu_misses")
 
     def upload_timeouts(self) -> int:

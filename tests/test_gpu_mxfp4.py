@@ -691,3 +691,57 @@ def test_one_token_of_the_widest_rows(gpu, width, E, H, I):
             assert (got == 0).all() and (chunk == 0).all()
         else:
             assert rel(got, want) < REL and rel(chunk, want) < REL
+
+
+class Cached:
+    """A partial-cache layer over MXFP4, its misses staged from pinned host stacks of tile order."""
+
+    def __init__(self, nm, seed, E, H, I, k, usable):
+        rng = np.random.default_rng(seed)
+        self.src = Experts(nm, seed + 1, E, H, I)
+        self.stacks = nm.HostExpertStacks(E, H, I, (nm.MXFP4_T,) * 3, interleaved=True)
+        for p, bank in enumerate((self.src.banks.gate, self.src.banks.up, self.src.banks.down)):
+            for e in range(E):
+                self.stacks.view(p)[e] = bank.buffer.download(np.uint8, bank.expert_bytes, e * bank.stride)
+        self.router = nm.DeviceBuffer.from_array((rng.standard_normal((E, H)) * 0.05).astype(np.float32))
+        self.ring, self.copy = nm.policy.StagingRing(), nm.Stream()
+        self.banks = nm.LayerBanks(usable + self.ring.length, H, I, (nm.MXFP4_T,) * 3, contiguous=True)
+        self.layer = nm.policy.CachedLayer(self.router.ptr, self.banks, self.stacks, E, k, usable, self.ring,
+                                           self.copy.handle)
+
+    def state(self):
+        c = self.layer.cache
+        return (c.tick, c.hit_counts().tolist(), [c.slot_state(s) for s in range(c.slots)], self.ring.acquire(0))
+
+
+def test_partial_cache_refuses_misses_that_it_cannot_stage(gpu):
+    """The CPU path does not compute MXFP4: a step with more missed experts than ring positions, or with fewer of
+    them streamed, is refused as a whole, whatever set_cpu_misses says; the policy stays and the next step is right."""
+    nm = gpu
+    rng = np.random.default_rng(140)
+    E, H, I, k, usable, rows = 64, 128, 64, 8, 4, 6
+    c = Cached(nm, 141, E, H, I, k, usable)
+    x = bf16(rng.standard_normal((rows, H)))
+    xd = nm.DeviceBuffer.from_array(x)
+    ids, w, out = nm.DeviceBuffer(rows * k * 4), nm.DeviceBuffer(rows * k * 4), nm.DeviceBuffer(rows * H * 4)
+    nm.router_topk(xd, nm.BF16, c.router, rows, H, E, k, ids, w)
+    idn, wn = ids.download(np.uint32).reshape(rows, k), w.download(np.float32).reshape(rows, k)
+    assert len(np.unique(idn)) > c.ring.length + usable
+    for on in (True, False):
+        c.layer.set_cpu_misses(on)
+        for n, frac in ((rows, 1.0), (rows, 0.5), (1, 0.5), (1, 0.0)):
+            before = c.state()
+            with pytest.raises(nm.NaiwaError) as e:
+                c.layer.forward(xd, n, out, pcie_frac=frac)
+            assert e.value.rc == nm.E_UNSUPPORTED and c.state() == before, (on, n, frac)
+            x2 = nm.DeviceBuffer.from_array(x)
+            with pytest.raises(nm.NaiwaError) as e:
+                nm.policy.CachedLayer.stack_forward([c.layer], x2.ptr, n, out.ptr, pcie_frac=frac)
+            assert e.value.rc == nm.E_UNSUPPORTED and c.state() == before, (on, n, frac)
+            assert np.array_equal(x2.download(np.uint16).reshape(rows, H), x)
+        for t in range(2):
+            info = c.layer.forward(xd.ptr + t * H * 2, 1, out)
+            nm.synchronize()
+            assert info["cpu"] == 0 and info["hits"] + info["staged"] == k
+            got = out.download(np.float32, H)
+            assert rel(got, M.experts(f32_of(x[t:t + 1]), idn[t:t + 1], wn[t:t + 1], *c.src.w)[0]) < REL
