@@ -7,11 +7,12 @@
 // registers.  The counts meet in an LDS histogram.  Each block leaves its partial sums in the
 // scratch buffer; a second launch, a block per 16 experts, adds them in a fixed order, and the
 // last of its blocks to end adds up the loss.  With one block the first launch does all that.
-// Backward: the same row in registers, dlogits from it in the same pass.
+// Backward: the same row in registers, dlogits from it in the same pass: p (c - sum p c), with the row's
+// mean count taken off the counts first as an integer, so that nearly even counts lose nothing.
 //
 // Bound: HBM for long batches (the logits are read once each way and the gradient
 // written once); launches and the latency of a row for short ones.  32768 tokens, 128 experts,
-// top-8, f32: forward 7.9 + 5.1 us, backward 11.8 us (33.6 MB: 2.8 TB/s); 61 tokens 3.6 and 2.0 us.
+// top-8, f32: forward 7.9 + 5.1 us, backward 10.0 us (33.6 MB: 3.4 TB/s); 61 tokens 3.6 and 1.8 us.
 // 64 lanes a row, and one block that joins all partial sums, took 120 us for all three.
 #include "../../include/naiwa_balance.h"
 #include "common.h"
@@ -284,18 +285,26 @@ backward_kernel(const void* logits, int64_t ld, const uint32_t* counts, const ui
     const int tid = threadIdx.x, l = tid % L;
     const double N = (double)max(1u, *valid);
     const float coef = (float)((double)*grad_loss * (double)E / ((double)k * N * N));
-    float c[V];
+    int c[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) c[i] = R::expert(l, i) < E ? (float)counts[R::expert(l, i)] : 0.0f;
+    for (int i = 0; i < V; ++i) c[i] = R::expert(l, i) < E ? (int)counts[R::expert(l, i)] : 0;
     for (int64_t t0 = (int64_t)blockIdx.x * G; t0 < T; t0 += (int64_t)gridDim.x * G) {
         const int64_t t = t0 + tid / L;
         const bool in = t < T;
-        float e[V], s = 0.0f;
+        float e[V], d[V], mean = 0.0f, s = 0.0f;
         row_load<R, BF16>(logits, t * ld, in, E, l, e);
         const bool live = in && (!mask || mask[t]);
         const float inv = row_exp<R>(live, E, l, e);
+        // The row's mean count, rounded to an integer, comes off the counts as an integer first (the
+        // gradient does not change when all counts do): what follows errs relative to the counts' spread
+        // about it, not to the counts, which in a well balanced batch are a thousand times that.  Counts
+        // are under 2^31 (T k is).
 #pragma unroll
-        for (int i = 0; i < V; ++i) s = __builtin_fmaf(e[i] * inv, c[i], s);
+        for (int i = 0; i < V; ++i) e[i] *= inv, mean = __builtin_fmaf(e[i], (float)c[i], mean);
+        mean = lanes_all<L>(mean, [](float a, float b) { return a + b; });
+        const int m = (int)rintf(fminf(mean, 2147483520.0f)); // (a NaN stays in e)
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] = (float)(c[i] - m), s = __builtin_fmaf(e[i], d[i], s);
         s = lanes_all<L>(s, [](float a, float b) { return a + b; });
         if (!in || (!live && accumulate)) continue;
         constexpr int S = R::X4 ? 4 : 1;
@@ -303,7 +312,7 @@ backward_kernel(const void* logits, int64_t ld, const uint32_t* counts, const ui
         for (int i = 0; i < V; i += S) {
             if (R::expert(l, i) >= E) break;
             const int64_t at = t * dld + R::expert(l, i);
-            float d[S], old[S] = {};
+            float g[S], old[S] = {};
             if (accumulate) {
                 if constexpr (R::X4)
                     load4<BF16>(dlogits, at, old);
@@ -311,16 +320,16 @@ backward_kernel(const void* logits, int64_t ld, const uint32_t* counts, const ui
                     old[0] = load<BF16>(dlogits, at);
             }
 #pragma unroll
-            for (int j = 0; j < S; ++j) d[j] = old[j] + (live ? coef * (e[i + j] * inv) * (c[i + j] - s) : 0.0f);
+            for (int j = 0; j < S; ++j) g[j] = old[j] + (live ? coef * e[i + j] * (d[i + j] - s) : 0.0f);
             if constexpr (R::X4 && BF16)
-                *(uint2*)((uint16_t*)dlogits + at) = make_uint2(naiwa_f32_to_bf16(d[0]) | naiwa_f32_to_bf16(d[1]) << 16,
-                                                                naiwa_f32_to_bf16(d[2]) | naiwa_f32_to_bf16(d[3]) << 16);
+                *(uint2*)((uint16_t*)dlogits + at) = make_uint2(naiwa_f32_to_bf16(g[0]) | naiwa_f32_to_bf16(g[1]) << 16,
+                                                                naiwa_f32_to_bf16(g[2]) | naiwa_f32_to_bf16(g[3]) << 16);
             else if constexpr (R::X4)
-                *(float4*)((float*)dlogits + at) = make_float4(d[0], d[1], d[2], d[3]);
+                *(float4*)((float*)dlogits + at) = make_float4(g[0], g[1], g[2], g[3]);
             else if (BF16)
-                ((uint16_t*)dlogits)[at] = (uint16_t)naiwa_f32_to_bf16(d[0]);
+                ((uint16_t*)dlogits)[at] = (uint16_t)naiwa_f32_to_bf16(g[0]);
             else
-                ((float*)dlogits)[at] = d[0];
+                ((float*)dlogits)[at] = g[0];
         }
     }
 }

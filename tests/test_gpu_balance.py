@@ -255,3 +255,56 @@ def test_captured_and_replayed(gpu):
             for o, v in zip(out, want):
                 assert np.array_equal(o.download(np.uint32, v.size), v)
     g.close()
+
+
+def backward(nm, x, counts, valid, k, g=1.0, bf=False, ld=0):
+    """dlogits of counts and a number of tokens that the caller has, of a longer batch say."""
+    T, E = x.shape
+    wide = np.zeros((T, ld or E), np.float32)
+    wide[:, :E] = x
+    raw = bf16(wide) if bf else wide
+    xd, dd = nm.DeviceBuffer.from_array(raw), nm.DeviceBuffer.from_array(np.zeros_like(raw))
+    cd, vd = nm.DeviceBuffer.from_array(counts.astype(np.uint32)), nm.DeviceBuffer.from_array(np.array([valid], np.uint32))
+    gd = nm.DeviceBuffer.from_array(np.array([g], np.float32))
+    nm.router_balance_backward(xd, nm.BF16 if bf else nm.F32, cd, vd, T, E, k, gd, dd, ld=ld, dld=ld)
+    d = dd.download(np.uint16 if bf else np.float32, raw.size).reshape(raw.shape)[:, :E]
+    return f32_of(d) if bf else d
+
+
+@pytest.mark.parametrize("kind,E,k,N,spread", [
+    ("even", 128, 8, 32768, 2), ("even", 128, 8, 1 << 18, 2), ("even", 60, 4, 1 << 22, 50), ("even", 1000, 8, 1 << 20, 3),
+    ("even", 8, 2, (1 << 30) - 1, 5),      # counts past 2^24
+    ("even", 16, 2, 1 << 20, 0),           # all alike: no gradient
+    ("closed", 128, 8, 32768, 2),          # a quarter of the experts closed: -inf, and chosen by nobody
+    ("sure", 128, 8, 32768, 300),          # rows that are almost sure of their expert
+    ("one", 64, 2, 1 << 20, 0),            # all choices of one expert
+])
+@pytest.mark.parametrize("bf,ld", [(False, 0), (False, 1), (True, 0)])
+def test_gradient_of_nearly_even_counts(gpu, kind, E, k, N, spread, bf, ld):
+    """Counts that differ by much less than they are large, as the loss makes them.
+
+    The gradient p_j (c_j - s), s = sum p c, does not change when all counts do by an integer m.  With m next
+    to s, c_j - m is exact up to 2^24 and s - m errs by a few 2^-24 of sum p |c - m|, which is of the size of the
+    gradient's own c_j - s: with a probability's few 2^-24 (and |logit| 2^-24) under 1e-5 of the norm."""
+    rng = np.random.default_rng(E + N % 1000 + spread)
+    T = 200
+    x = (rng.standard_normal((T, E)) * (8.0 if kind == "sure" else 1.0)).astype(np.float32)
+    live = E - E // 4 if kind == "closed" else E
+    counts = N * k // live + np.rint(rng.standard_normal(E) * spread).astype(np.int64)
+    if kind == "closed":
+        x[:, live:] = -np.inf
+        counts[live:] = 0
+    if kind == "one":
+        counts[:] = 0
+        counts[3] = N * k
+    if bf:
+        x = f32_of(bf16(x))
+    z = np.exp(x.astype(np.float64) - x.max(-1, keepdims=True))
+    z /= z.sum(-1, keepdims=True)
+    want = E / (k * float(N) ** 2) * z * (counts - (z * counts).sum(-1, keepdims=True))
+    print(f"[backward {kind} {E} {N} {bf} {ld}]", flush=True)
+    d = backward(gpu, x, counts, N, k, bf=bf, ld=E + 1 if ld else 0)
+    if spread == 0 and kind == "even":
+        assert (d == 0).all()
+    else:
+        assert rel(d, want) < (2.0 ** -8 if bf else 1e-5)
