@@ -99,7 +99,7 @@ struct Part {         // the blocks' partial sums
     double* loss;     // [blocks of the second launch]
     uint32_t* counts; // [blocks][E]
     uint32_t* valid;  // [blocks]
-    uint32_t* ended;  // blocks of the second launch that have ended; 0 between calls
+    uint32_t* ended;  // blocks of the second launch that have ended, cleared by the first launch
 };
 
 // The results of experts e0 .. e0 + kFinishE - 1 from `blocks` (at most kMaxBlocks) partial
@@ -248,6 +248,8 @@ forward_kernel(const void* logits, int64_t ld, const uint32_t* ids, int64_t ids_
         }
     }
     if (tid == 0) part.valid[blk] = nvalid;
+    // (no call relies on what an earlier one left: the first one may be captured and run later)
+    if (blk == 0 && tid == 0) *part.ended = 0;
     if (gridDim.x == 1) {
         double sum = 0.0;
         uint32_t N = 0;
@@ -274,7 +276,6 @@ finish_kernel(Part part, int blocks, int E, int k, uint32_t* counts, uint32_t* v
         sum += __hip_atomic_load(part.loss + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     *valid = N;
     *loss = (float)(sum * ((double)E / (double)k));
-    __hip_atomic_store(part.ended, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 template <class R, bool BF16>
@@ -345,16 +346,14 @@ int ids_ok(const uint32_t* ids, int ids_ld, int64_t T, int k, int E) {
 
 __global__ void zero_kernel(uint32_t* p) { *p = 0; }
 
-// The scratch of a call; its word that has to be 0 between calls is cleared when it is new.
-int part_of(int blocks, int E, hipStream_t st, Part* p) {
+// The scratch of a call; nothing in it outlives the call.
+int part_of(int blocks, int E, Part* p) {
     const size_t n = (size_t)blocks * E;
     int rc = 0;
-    bool fresh = false;
-    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_BALANCE, 1024 + n * 12 + (size_t)blocks * 4, &rc, &fresh);
+    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_BALANCE, 1024 + n * 12 + (size_t)blocks * 4, &rc);
     if (!ws) return rc;
     *p = Part{(double*)(ws + 1024), (double*)ws, (uint32_t*)(ws + 1024 + 8 * n), (uint32_t*)(ws + 1024 + 12 * n),
               (uint32_t*)(ws + 1020)};
-    if (fresh) zero_kernel<<<1, 1, 0, st>>>(p->ended);
     return NAIWA_OK;
 }
 
@@ -379,7 +378,7 @@ extern "C" int naiwa_expert_counts(const uint32_t* ids, int ids_ld, int64_t T, i
     const int blocks = blocks_of(T);
     hipStream_t st = (hipStream_t)stream;
     Part part;
-    if (int rc = part_of(blocks, E, st, &part)) return rc;
+    if (int rc = part_of(blocks, E, &part)) return rc;
     if (bad) zero_kernel<<<1, 1, 0, st>>>(bad);
     forward_kernel<Row<64, 0, false>, false><<<blocks, kThreads, 0, st>>>(nullptr, 0, ids, ids_ld ? ids_ld : k, T,
                                                           (int)((T + blocks - 1) / blocks), E, k, mask, part, counts, nullptr,
@@ -397,7 +396,7 @@ extern "C" int naiwa_router_balance(const void* logits, int dtype, int ld, const
     const int blocks = blocks_of(T);
     hipStream_t st = (hipStream_t)stream;
     Part part;
-    if (int rc = part_of(blocks, E, st, &part)) return rc;
+    if (int rc = part_of(blocks, E, &part)) return rc;
     auto go = [&](auto* kernel) {
         kernel<<<blocks, kThreads, 0, st>>>(logits, ld ? ld : E, ids, ids_ld ? ids_ld : k, T,
                                             (int)((T + blocks - 1) / blocks), E, k, mask, part, counts, valid, probs, loss, nullptr);

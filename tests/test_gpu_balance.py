@@ -308,3 +308,47 @@ def test_gradient_of_nearly_even_counts(gpu, kind, E, k, N, spread, bf, ld):
         assert (d == 0).all()
     else:
         assert rel(d, want) < (2.0 ** -8 if bf else 1e-5)
+
+
+FIRST_CALL_CAPTURED = """
+import numpy as np
+import naiwa_moe as nm
+from test_gpu_balance import make, reference
+from test_gpu_mxfp4 import Graph
+
+rng = np.random.default_rng(1)
+T, E, k = 5000, 64, 6
+x, ids, _ = make(rng, T, E, k, 1)
+xd, idd = nm.DeviceBuffer.from_array(x), nm.DeviceBuffer.from_array(ids)
+out = [nm.DeviceBuffer.from_array(np.full(n, 7, np.uint32)) for n in (E, 1, E, 1)]
+dirty = [nm.DeviceBuffer.from_array(np.full(1 << 16, 0xFF, np.uint8)) for _ in range(64)]
+nm.synchronize()
+del dirty
+call = lambda s: nm.router_balance(xd, nm.F32, idd, T, E, k, *out, stream=s)
+st = nm.Stream()
+g = Graph(nm, st, lambda: call(st.handle))
+loss = reference(x, ids, E, None, 1.0)[3]
+for launch in (lambda: call(0), g.launch, lambda: call(0), g.launch, g.launch):
+    out[3].upload(np.zeros(1, np.float32))
+    nm.synchronize()
+    launch()
+    nm.synchronize()
+    assert abs(out[3].download(np.float32, 1)[0] - loss) <= 2e-6 * loss, out[3].download(np.float32, 1)
+    assert out[1].download(np.uint32, 1)[0] == T
+g.close()
+print("done", flush=True)
+"""
+
+
+def test_first_call_of_a_process_captured(gpu):
+    """What a call keeps in its scratch needs no earlier call: the first one of a process is captured, into memory
+    that held other things, and an eager call follows before the graph has run."""
+    import os
+    import subprocess
+    import sys
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    path = [here, os.path.join(os.path.dirname(here), "naiwa-rs_amd")]
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], capture_output=True, text=True, timeout=100,
+                       env={**os.environ, "PYTHONPATH": os.pathsep.join(path)})
+    assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
