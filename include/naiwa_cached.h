@@ -100,7 +100,10 @@ typedef struct naiwa_lookahead_step {
 typedef struct naiwa_cached_layer naiwa_cached_layer;
 
 /* The layer keeps a pointer to `ring` (shared by layers of one shape, as the
- * reference shares its ring) and owns a naiwa_cache of `usable` slots. */
+ * reference shares its ring) and owns a naiwa_cache of `usable` slots.  MXFP4
+ * banks are checked here as naiwa_moe_decode checks them (all three of the type,
+ * at most 4096 slots, top_k <= 64, the activation); their steps need x and out
+ * 16-byte aligned. */
 int naiwa_cached_layer_create(const naiwa_cached_layer_desc* d, naiwa_ring* ring, int ring_len,
                               int64_t copy_stream, naiwa_cached_layer** out);
 int naiwa_cached_layer_destroy(naiwa_cached_layer* L);

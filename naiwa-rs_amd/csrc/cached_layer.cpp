@@ -23,6 +23,7 @@
 #include "../../include/naiwa_doorbell.h"
 #include "common.h"
 #include "decode.h"
+#include "mxfp4.h"
 #include "router.h"
 #include "upload.h"
 
@@ -222,6 +223,7 @@ struct naiwa_cached_layer {
     // [seq][pad][rows * H f32] (mapped), its publishes so far, and the CPU sum on the device
     bool cpu_misses = true;
     bool cpu_types = true;         // the CPU path computes the banks' types (Q4_K and Q8_0)
+    bool mx = false;               // MXFP4 banks
     naiwa_host_experts hx{};
     uint32_t* xpub_host = nullptr;
     uint32_t* xpub_dev = nullptr;
@@ -462,6 +464,9 @@ int forward_impl(naiwa_cached_layer* L, naiwa_cached_layer* next, int swaps_per_
     // doorbell, sized for this layer's top_k
     if (next && (next == L || next->d.hidden != L->d.hidden || next->d.top_k != L->d.top_k)) return NAIWA_E_INVALID;
     const naiwa_cached_layer_desc& d = L->d;
+    // what the MXFP4 experts refuse about x and out, before the policy is touched
+    if (L->mx && (rows > 4096 || (int64_t)rows * d.top_k > 65536 || (((uintptr_t)x | (uintptr_t)out) & 15)))
+        return NAIWA_E_INVALID;
     const int k = d.top_k, n = rows * k;
     hipStream_t st = (hipStream_t)stream;
     // a CPU job of an earlier step that failed (its result was not computed): report it
@@ -775,8 +780,16 @@ int naiwa_cached_layer_create(const naiwa_cached_layer_desc* d, naiwa_ring* ring
     if (!bank_ok(d->gate, d->inter, d->hidden, need) || !bank_ok(d->up, d->inter, d->hidden, need) ||
         !bank_ok(d->down, d->hidden, d->inter, need))
         return NAIWA_E_INVALID;
+    bool mx = false;
+    for (int dt : {d->gate.dtype, d->up.dtype, d->down.dtype}) mx |= dt == NAIWA_MXFP4_T;
+    if (mx) { // what the experts refuse about banks, width and activation, a step could only report late
+        const NaiwaMxCall c{&d->gate, &d->up, &d->down, nullptr, NAIWA_BF16, nullptr, nullptr,
+                            0, d->top_k, d->act, nullptr, 0, 1, nullptr};
+        if (int rc = naiwa_mx_check(c)) return rc;
+    }
     naiwa_cached_layer* L = new (std::nothrow) naiwa_cached_layer;
     if (!L) return NAIWA_E_NOMEM;
+    L->mx = mx;
     L->d = *d;
     L->ring = ring;
     L->ring_len = ring_len;

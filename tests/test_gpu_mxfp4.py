@@ -745,3 +745,19 @@ def test_partial_cache_refuses_misses_that_it_cannot_stage(gpu):
             assert info["cpu"] == 0 and info["hits"] + info["staged"] == k
             got = out.download(np.float32, H)
             assert rel(got, M.experts(f32_of(x[t:t + 1]), idn[t:t + 1], wn[t:t + 1], *c.src.w)[0]) < REL
+
+
+def test_partial_cache_refuses_a_call_before_the_policy_moves(gpu):
+    """x or out that the experts do not take, and more rows than a call's."""
+    nm = gpu
+    E, H, I, k = 8, 128, 64, 2
+    c = Cached(nm, 150, E, H, I, k, 4)
+    xd, out = nm.DeviceBuffer.from_array(np.zeros(2 * H, np.uint16)), nm.DeviceBuffer(2 * H * 4)
+    before = c.state()
+    for x, rows, o in ((xd.ptr + 8, 1, out.ptr), (xd.ptr, 1, out.ptr + 4), (xd.ptr, 4097, out.ptr)):
+        with pytest.raises(nm.NaiwaError) as e:
+            c.layer.forward(x, rows, o)
+        assert e.value.rc == nm.E_INVALID and c.state() == before
+    assert c.layer.forward(xd, 2, out)["cpu"] == 0
+    nm.synchronize()
+    assert (out.download(np.float32) == 0).all() and c.state() != before

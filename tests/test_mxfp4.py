@@ -207,3 +207,27 @@ def test_tile_list_of_one_token_is_written_whole():
     # of more tokens at most a tile a slot and one for every further 64 pairs
     for n, slots in ((2, 1), (65, 1), (66, 2), (512, 128), (65536, 4096), (8192, 4096)):
         assert f(2, C.c_int64(n), slots) >= min(n, slots) + (n - min(n, slots)) // 64
+
+
+def _cached(g, u, d, H, I, top_k=2, act=0, usable=2, ring=2):
+    """naiwa_cached_layer_create over made-up addresses, refused before any of them is used."""
+    r = nm.policy.StagingRing()
+    desc = _lib.CachedLayerDesc(4096, None, g, u, d, 1 << 20, 1 << 20, 1 << 20, 8, top_k, H, I, usable, 0, act, 0)
+    h = C.c_void_p()
+    rc = nm.lib().naiwa_cached_layer_create(C.byref(desc), r._h, ring, 0, C.byref(h))
+    assert h.value is None
+    return rc
+
+
+def test_cached_layer_refuses_banks_that_its_steps_could_not_run():
+    H, I = 256, 96
+    ok = _bank(I, H), _bank(I, H), _bank(H, I)
+    q = lambda n, k: Bank(1 << 20, 1 << 20, 4, n, k, nm.Q8_0)  # noqa: E731
+    for mixed in ((ok[0], ok[1], q(H, I)), (q(I, H), ok[1], ok[2]), (q(I, H), q(I, H), ok[2]), (ok[0], q(I, H), q(H, I))):
+        assert _cached(*mixed, H, I) == E_UNSUPPORTED
+    assert _cached(*ok, H, I, top_k=65) == E_UNSUPPORTED and _cached(*ok, H, I, act=2) == E_UNSUPPORTED
+    many = _bank(I, H, slots=5000), _bank(I, H, slots=5000), _bank(H, I, slots=5000)
+    assert _cached(*many, H, I) == E_UNSUPPORTED
+    assert _cached(_bank(I, H, slots=5), ok[1], ok[2], H, I) == E_INVALID
+    assert _cached(_bank(I, H, base=(1 << 20) + 8), ok[1], ok[2], H, I) == E_INVALID
+    assert _cached(_bank(80, H), _bank(80, H), Bank(1 << 20, 1 << 20, 4, H, 80, nm.MXFP4_T), H, 80) == E_INVALID
