@@ -17,6 +17,8 @@
 namespace {
 
 constexpr int kThreads = 256;
+// Blocks of a launch: HIP takes fewer than 2^32 threads along a dimension.
+constexpr int64_t kLaunch = 1 << 23;
 
 // 8 values of a row from p as f32; T: float, or uint16_t holding bf16 (DT NAIWA_BF16) or f16.
 template <int DT>
@@ -35,10 +37,11 @@ __device__ __forceinline__ void load8(const void* p, float (&f)[8]) {
     }
 }
 
-// Group number b of the call: projection, strip, group of steps.
+// Group number b of a launch: projection, strip, group of steps.
 struct Where {
-    int64_t strips, groups;
+    int64_t strips, groups, first;
     __device__ __forceinline__ void split(int64_t b, int64_t& proj, int64_t& strip, int& group) const {
+        b += first;
         group = (int)(b % groups);
         strip = b / groups % strips;
         proj = b / groups / strips;
@@ -165,6 +168,14 @@ int check(const void* rows, int64_t batch, int64_t n, int64_t k, int64_t& ld, in
     return NAIWA_OK;
 }
 
+// f(blocks, where) for the groups of a call, at most kLaunch of them at a time.
+template <class F> int launches(int64_t batch, int64_t n, int64_t k, F f) {
+    Where wh{n / 16, naiwa_mx_groups(k), 0};
+    const int64_t all = batch * wh.strips * wh.groups;
+    for (; wh.first < all; wh.first += kLaunch) f((unsigned)(all - wh.first < kLaunch ? all - wh.first : kLaunch), wh);
+    return naiwa_hip_rc(hipGetLastError());
+}
+
 } // namespace
 
 extern "C" int naiwa_mxfp4_quantize(const void* src, int src_dtype, int64_t batch, int64_t n, int64_t k, int64_t ld,
@@ -172,18 +183,17 @@ extern "C" int naiwa_mxfp4_quantize(const void* src, int src_dtype, int64_t batc
     if (src_dtype != NAIWA_F32 && src_dtype != NAIWA_BF16 && src_dtype != NAIWA_F16) return NAIWA_E_UNSUPPORTED;
     if (int rc = check(src, batch, n, k, ld, src_stride, dst, dst_stride)) return rc;
     if (batch == 0 || n == 0 || k == 0) return NAIWA_OK;
-    const Where wh{n / 16, naiwa_mx_groups(k)};
-    const unsigned blocks = (unsigned)(batch * wh.strips * wh.groups);
-    hipStream_t st = (hipStream_t)stream;
-    const uint8_t* s = (const uint8_t*)src;
-    uint8_t* d = (uint8_t*)dst;
-    if (src_dtype == NAIWA_F32)
-        quantize_kernel<NAIWA_F32><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, ld, src_stride, d, dst_stride);
-    else if (src_dtype == NAIWA_BF16)
-        quantize_kernel<NAIWA_BF16><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, ld, src_stride, d, dst_stride);
-    else
-        quantize_kernel<NAIWA_F16><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, ld, src_stride, d, dst_stride);
-    return naiwa_hip_rc(hipGetLastError());
+    return launches(batch, n, k, [&](unsigned blocks, const Where& wh) {
+        hipStream_t st = (hipStream_t)stream;
+        const uint8_t* s = (const uint8_t*)src;
+        uint8_t* d = (uint8_t*)dst;
+        if (src_dtype == NAIWA_F32)
+            quantize_kernel<NAIWA_F32><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, ld, src_stride, d, dst_stride);
+        else if (src_dtype == NAIWA_BF16)
+            quantize_kernel<NAIWA_BF16><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, ld, src_stride, d, dst_stride);
+        else
+            quantize_kernel<NAIWA_F16><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, ld, src_stride, d, dst_stride);
+    });
 }
 
 extern "C" int naiwa_mxfp4_dequantize(const void* src, int64_t batch, int64_t n, int64_t k, int64_t src_stride,
@@ -191,16 +201,15 @@ extern "C" int naiwa_mxfp4_dequantize(const void* src, int64_t batch, int64_t n,
     if (dst_dtype != NAIWA_F32 && dst_dtype != NAIWA_BF16) return NAIWA_E_UNSUPPORTED;
     if (int rc = check(dst, batch, n, k, ld, dst_stride, src, src_stride)) return rc;
     if (batch == 0 || n == 0 || k == 0) return NAIWA_OK;
-    const Where wh{n / 16, naiwa_mx_groups(k)};
-    const unsigned blocks = (unsigned)(batch * wh.strips * wh.groups);
-    hipStream_t st = (hipStream_t)stream;
-    const uint8_t* s = (const uint8_t*)src;
-    uint8_t* d = (uint8_t*)dst;
-    if (dst_dtype == NAIWA_F32)
-        dequantize_kernel<NAIWA_F32><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, src_stride, d, ld, dst_stride);
-    else
-        dequantize_kernel<NAIWA_BF16><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, src_stride, d, ld, dst_stride);
-    return naiwa_hip_rc(hipGetLastError());
+    return launches(batch, n, k, [&](unsigned blocks, const Where& wh) {
+        hipStream_t st = (hipStream_t)stream;
+        const uint8_t* s = (const uint8_t*)src;
+        uint8_t* d = (uint8_t*)dst;
+        if (dst_dtype == NAIWA_F32)
+            dequantize_kernel<NAIWA_F32><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, src_stride, d, ld, dst_stride);
+        else
+            dequantize_kernel<NAIWA_BF16><<<blocks, kThreads, 0, st>>>(s, wh, (int)k, src_stride, d, ld, dst_stride);
+    });
 }
 
 extern "C" int naiwa_mxfp4_from_ggml(const void* src, int64_t n, int64_t k, void* dst) {

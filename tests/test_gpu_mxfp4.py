@@ -761,3 +761,28 @@ def test_partial_cache_refuses_a_call_before_the_policy_moves(gpu):
     assert c.layer.forward(xd, 2, out)["cpu"] == 0
     nm.synchronize()
     assert (out.download(np.float32) == 0).all() and c.state() != before
+
+
+def test_quantize_past_the_threads_of_a_launch(gpu):
+    """2^24 + 3 groups of 16 rows, 256 threads each: more threads than one launch takes.  Rows at both ends and
+    about the groups where launches may meet, there and back."""
+    nm = gpu
+    n, k = 16 * ((1 << 24) + 3), 32
+    size = nm.projection_bytes(nm.MXFP4_T, 16, k)
+    if nm.mem_info()[0] < 3 * n * k * 2:
+        pytest.skip("not enough free memory")
+    src, dst, back = nm.DeviceBuffer(n * k * 2), nm.DeviceBuffer(n // 16 * size), nm.DeviceBuffer(n * k * 2)
+    rng = np.random.default_rng(160)
+    rows = {at: bf16(rng.standard_normal((16, k))) for at in (0, (1 << 23) - 1, 1 << 23, (1 << 24) - 1, 1 << 24,
+                                                              (1 << 24) + 2)}
+    src.zero()
+    for at, r in rows.items():
+        src.upload(r, offset=at * 16 * k * 2)
+    nm.mxfp4_quantize(src, nm.BF16, n, k, dst)
+    nm.mxfp4_dequantize(dst, n, k, back, nm.BF16)
+    nm.synchronize()
+    for at, r in rows.items():
+        code, s = M.quantize(f32_of(r))
+        assert np.array_equal(dst.download(np.uint8, size, at * size), M.tiled(code, s)), at
+        got = f32_of(back.download(np.uint16, 16 * k, at * 16 * k * 2)).reshape(16, k)
+        assert np.array_equal(got, M.values(code, s).astype(np.float32)), at
