@@ -198,7 +198,8 @@ int64_t naiwa_projection_bytes(int dtype, int64_t n, int64_t k);
  * its row; an infinite activation gives NaN there.
  * Banks of NAIWA_MXFP4_T (all three, or NAIWA_E_UNSUPPORTED; naiwa_mxfp4.h) take any
  * number of rows on the matrix cores: H, I multiples of 32, width <= 64, x and out
- * 16-byte aligned.  Products and sums are f32; f32 x and h are held to 2^-24 of the
+ * 16-byte aligned; NAIWA_E_UNSUPPORTED past what a launch takes (I over 2^21, or 2^24 tiles
+ * of up to 64 pairs of a slot times 128 features or 256 rows).  Products and sums are f32; f32 x and h are held to 2^-24 of the
  * largest magnitude of their 32-value block, bf16 x to 2^-19 of it (exactly where it is
  * at least 2^-12 of it): within 1e-5 of a 64-bit result.  A NaN, an infinity or an h that overflows makes its
  * pair's dots NaN. */

@@ -515,6 +515,11 @@ bool bank_ok(const naiwa_bank* b) {
 
 constexpr int kPlanesMost = 5;
 
+constexpr int kNA = 2; // tiles of 32 weight rows a wave of the tile kernels
+// Columns of blocks of a tile: 4 waves of kNA / 2 features blocks (gate and up) or kNA row blocks.
+int gateup_cols(int I) { return (4 * naiwa_mx_steps(I) + 2 * kNA - 1) / (2 * kNA); }
+int down_cols(int H) { return (H / 32 + 4 * kNA - 1) / (4 * kNA); }
+
 // K parts of a down projection of `blocks` blocks, in groups of 4 steps: blocks for two a CU as
 // long as a part has two groups, and 64 MB of dots at most, which stay in the caches.  16 rows of
 // 8 experts top-2, H 4096, I 14336 (128 blocks) 4 parts and 1: 170 and 215 us a call.
@@ -552,6 +557,11 @@ struct Layout {
     }
 };
 
+// Rows of a pass: the copies of x to LDS have 32-bit offsets.
+int rows_per_pass(int rows, int H) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(rows, UINT32_MAX / plane_row(kPlanesMost, H)));
+}
+
 } // namespace
 
 int naiwa_mx_check(const NaiwaMxCall& c) {
@@ -569,6 +579,11 @@ int naiwa_mx_check(const NaiwaMxCall& c) {
     if (c.act != NAIWA_ACT_SILU && c.act != NAIWA_ACT_GELU_PYTORCH_TANH) return NAIWA_E_UNSUPPORTED;
     if (c.rows > 0 && (!c.x || !(c.out || c.res) || (c.width > 0 && (!c.ids || !c.w)))) return NAIWA_E_INVALID;
     if (((uintptr_t)c.x | (uintptr_t)c.out) & 15) return NAIWA_E_INVALID;
+    // A grid of 2^32 threads along x wraps without an error; along y 65536 blocks are HIP's limit.
+    const int rows = rows_per_pass(c.rows, H);
+    const int64_t tiles = naiwa_mx_tiles(rows, (int64_t)rows * c.width, c.gate->slots);
+    if (tiles * std::max(gateup_cols(I), down_cols(H)) * kThreads > UINT32_MAX) return NAIWA_E_UNSUPPORTED;
+    if (4 * (int64_t)naiwa_mx_steps(I) > 65536) return NAIWA_E_UNSUPPORTED;
     return NAIWA_OK;
 }
 
@@ -585,8 +600,6 @@ extern "C" bool naiwa_mx_by_pair(int rows, int64_t n, int slots, int H, int I) {
 }
 
 namespace {
-
-constexpr int kNA = 2; // tiles of 32 weight rows a wave of the tile kernels
 
 // Whether tiles of ncol columns of blocks are dealt to the XCDs in runs (tile_col): where an
 // XCD's 64 blocks at a time take several tiles with all their columns, neighbouring tiles of an
@@ -618,7 +631,7 @@ struct Run { // one pass's pieces
     }
     // Down of the tiles, and the combine.
     template <int PH> void down() const {
-        const int ncol = (H / 32 + 4 * kNA - 1) / (4 * kNA);
+        const int ncol = down_cols(H);
         const unsigned blocks = (unsigned)(8 * tl.run * ncol);
         const int groups = naiwa_mx_groups(I), part = (groups + down_parts(n, blocks, H, I) - 1) / down_parts(n, blocks, H, I);
         const int parts = (groups + part - 1) / part;
@@ -664,7 +677,7 @@ struct Run { // one pass's pieces
             if (int rc = naiwa_moe_gather(c.ids, n, slots, perm, offsets, (int*)(ws + L.bad), (int64_t)st)) return rc;
             planes_kernel<PX, BF16, false><<<pb, kThreads, 0, st>>>(c.x, c.rows, H, x(PX), with);
         }
-        const int ncol = (4 * naiwa_mx_steps(I) + 2 * kNA - 1) / (2 * kNA);
+        const int ncol = gateup_cols(I);
         const unsigned blocks = (unsigned)(8 * tl.run * ncol);
         tile_gateup_kernel<kNA, PX, PH><<<blocks, kThreads, kStageBytes<PX>, st>>>(g, u, x(PX), H, I, c.width, perm, tl, c.act,
                                                                                   xcd_order(ncol), h(PH));
@@ -688,11 +701,6 @@ int run_pass(const NaiwaMxCall& c, uint8_t* ws, hipStream_t st) {
         return naiwa_hip_rc(hipGetLastError());
     }
     return c.x_dtype == NAIWA_BF16 ? r.go<4, 5, true>() : r.go<5, 5, false>();
-}
-
-// Rows of a pass: the copies of x to LDS have 32-bit offsets.
-int rows_per_pass(int rows, int H) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(rows, UINT32_MAX / plane_row(kPlanesMost, H)));
 }
 
 } // namespace

@@ -231,3 +231,15 @@ def test_cached_layer_refuses_banks_that_its_steps_could_not_run():
     assert _cached(_bank(I, H, slots=5), ok[1], ok[2], H, I) == E_INVALID
     assert _cached(_bank(I, H, base=(1 << 20) + 8), ok[1], ok[2], H, I) == E_INVALID
     assert _cached(_bank(80, H), _bank(80, H), Bank(1 << 20, 1 << 20, 4, H, 80, nm.MXFP4_T), H, 80) == E_INVALID
+
+
+def test_expert_products_past_a_launch_are_refused():
+    """More blocks than a launch's 2^32 threads: 4096 slots of 2^20 features, a pair each; and more blocks of
+    features than a grid has along y."""
+    H, I = 32, 1 << 20
+    b = [_bank(n, k, slots=4096, base=1 << 40) for n, k in ((I, H), (I, H), (H, I))]
+    for call in (_decode, _prefill):
+        assert call(*b, rows=512, width=8) == E_UNSUPPORTED
+    wide = [_bank(n, k, base=1 << 40) for n, k in (((1 << 21) + 128, H), ((1 << 21) + 128, H), (H, (1 << 21) + 128))]
+    for call in (_decode, _prefill):
+        assert call(*wide) == E_UNSUPPORTED
