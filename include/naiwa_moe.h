@@ -199,10 +199,13 @@ int64_t naiwa_projection_bytes(int dtype, int64_t n, int64_t k);
  * Banks of NAIWA_MXFP4_T (all three, or NAIWA_E_UNSUPPORTED; naiwa_mxfp4.h) take any
  * number of rows on the matrix cores: H, I multiples of 32, width <= 64, x and out
  * 16-byte aligned; NAIWA_E_UNSUPPORTED past what a launch takes (I over 2^21, or 2^24 tiles
- * of up to 64 pairs of a slot times 128 features or 256 rows).  Products and sums are f32; f32 x and h are held to 2^-24 of the
- * largest magnitude of their 32-value block, bf16 x to 2^-19 of it (exactly where it is
- * at least 2^-12 of it): within 1e-5 of a 64-bit result.  A NaN, an infinity or an h that overflows makes its
- * pair's dots NaN. */
+ * of up to 64 pairs of a slot times 128 features or 256 rows).  Products and sums are f32.
+ * f32 x and h are held to 2^-24 of the largest magnitude of their 32-value block (or 2^-126),
+ * bf16 x to 2^-19 of it (or 2^-121; exactly where it is at least 2^-12 of it): a dot errs by at
+ * most that share of sum |w| max |x| over its blocks, beside its sum's rounding.  Without
+ * outliers in x that is within 1e-5 of a 64-bit result (4e-7 for normally distributed x); rows
+ * of weights that do not see an outlier of 2^8 times the rest lose up to 2^-19 2^8 = 5e-4 with
+ * bf16 x.  A NaN, an infinity or an h that overflows makes its pair's dots NaN. */
 int naiwa_moe_decode(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* down,
                      const void* x, int x_dtype, const uint32_t* slot_ids, const float* w,
                      int rows, int width, int act, float* out, int64_t stream);
