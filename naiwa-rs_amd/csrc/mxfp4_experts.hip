@@ -14,6 +14,8 @@
 // 2^(1 - 5 P) M:
 //   4 planes (bf16 x): 2^-19 M, a bf16 value of at least 2^-12 M exactly;
 //   5 planes (f32 x, h): 2^-24 M, the rounding of an f32 as large as M.
+// (Under M of 2^-102 the planes' scales stop: 2^-121 and 2^-126.)  What an outlier hides in its block is
+// lost to rows of weights that do not see the outlier: 2^-19 2^8 of the rest at one of 2^8 times it.
 // A plane less in each (3 and 4) takes 4096 tokens at Mixtral-8x7B sizes from 3.1 to 2.65 ms, with
 // results off by 6e-6 instead of 4e-7, for which f32 sums have no use.
 // FP4 x E2M3 runs at twice the rate of FP4 x FP8 (6 to 7 against 3.6 to 4.3 PFLOP/s from registers,
@@ -99,7 +101,9 @@ template <int P, int N> __device__ __forceinline__ void to_planes(const float (&
         v6u c = __builtin_bit_cast(v6u, __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale));
         // The conversions run in several passes, and the compiler may give the result registers
         // of an operand, which then are overwritten before they are read (seen: the codes of the
-        // last plane, off by whole binades).  The operands stay in use past the result.
+        // last plane, off by whole binades).  The operands' use past the result keeps them in place
+        // with this compiler, which it need not (it may copy them): test_asm_mxfp4.py looks for
+        // shared registers in what is compiled.
         asm volatile("" : "+v"(c) : "v"(even), "v"(odd), "v"(scale));
         o[p] = c;
         if (p + 1 < P) {
