@@ -271,31 +271,31 @@ __device__ __forceinline__ void deal(int steps, int mine, int all, int* t0, int*
     *t1 = (int)((int64_t)steps * (mine + 1) / all);
 }
 
-// The sums of a block's NW waves over 4 strips of 16 rows and 16 tokens.  Lane l of a wave holds
-// D[4 (l / 16) + i][l % 16]: row 4 (l / 16) + i of a strip, token l % 16; a group of 4 rows is
-// padded by a token, so that reads down the rows of a token spread over the banks.
+// The sums of a block's NW waves over 4 strips of 16 rows, of one token: the columns of D are alike,
+// and lane 16 q holds rows 4 q .. 4 q + 3 of column 0.
 template <int NW> struct Sums {
-    v4f v[NW][4][4][17];
+    v4f v[NW][4][4];
     __device__ __forceinline__ void put(int wave, int lane, const v4f (&acc)[4]) {
+        if (lane & 15) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[wave][i][lane >> 4][lane & 15] = acc[i];
+        for (int i = 0; i < 4; ++i) v[wave][i][lane >> 4] = acc[i];
     }
-    __device__ __forceinline__ float row(int strip, int r, int tok) const {
+    __device__ __forceinline__ float row(int strip, int r) const {
         float o = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) o += v[w][strip][r >> 2][tok][r & 3];
+        for (int w = 0; w < NW; ++w) o += v[w][strip][r >> 2][r & 3];
         return o;
     }
 };
 
-// h of 32 features (strips 0, 1 of the sums: gate, 2, 3: up) and one token, a feature a lane of
-// 32, to row `row` of the planes as block fb.  Bits of E2M3 by hand: |y| <= 4 is a multiple of 1/8
-// under 2 and of 1/4 from there on, so adding 1.5 2^20 or 1.5 2^21 rounds it to nearest even, and
-// the low bits of that sum are the code (less 8 in the upper binade).
+// h of 32 features (strips 0, 1 of the sums: gate, 2, 3: up), a feature a lane of 32, to row `row`
+// of the planes as block fb.  Bits of E2M3 by hand: |y| <= 4 is a multiple of 1/8 under 2 and of 1/4
+// from there on, so adding 1.5 2^20 or 1.5 2^21 rounds it to nearest even, and the low bits of that
+// sum are the code (less 8 in the upper binade).
 template <int PH, int NW>
-__device__ __forceinline__ void put_h(const Sums<NW>& sums, int tok, bool pad, int act, int fb, int64_t row, const Planes& h) {
+__device__ __forceinline__ void put_h(const Sums<NW>& sums, bool pad, int act, int fb, int64_t row, const Planes& h) {
     const int f = threadIdx.x & 31;
-    const float g = sums.row(f >> 4, f & 15, tok), u = sums.row(2 + (f >> 4), f & 15, tok);
+    const float g = sums.row(f >> 4, f & 15), u = sums.row(2 + (f >> 4), f & 15);
     const float v = pad ? 0.0f : naiwa_act(act, g) * u;
     uint32_t m = __float_as_uint(v) & 0x7fffffffu;
     m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));
@@ -341,9 +341,9 @@ __device__ __forceinline__ void put_h(const Sums<NW>& sums, int tok, bool pad, i
 // steps of the token's x in LDS while its first weights are on the way.  Pair j is row j of h;
 // blocks past I (h padded to whole steps) write zeros.  Of one token, the first block lists the
 // pairs that count as tiles of one pair, for tile_down_kernel, and clears the list's other entries: at
-// most 64 in all (naiwa_mx_tiles).  Dynamic LDS: the planes of x, their scales (16 bytes a group).  Bound: latency
-// (the launch, x to planes behind the first weights' way, four waves' sums): 8 of 128 Qwen3-30B
-// experts 6.6 us (13.4 MB), 2 of 8 of 1024 x 2048 6.3 us (4.5 MB).
+// most 64 in all (naiwa_mx_tiles).  Dynamic LDS: the planes of x, their scales (16 bytes a group).
+// Bound: latency (the launch, x to planes behind the first weights' way, four waves' sums): 8 of 128
+// Qwen3-30B experts 6.6 us (13.4 MB), 2 of 8 of 1024 x 2048 6.3 us (4.5 MB).
 template <int PX, int PH, bool BF16>
 __global__ void __launch_bounds__(kThreads, 2)
 gateup_pair_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32_t* ids, const float* w, int width, int slots,
@@ -386,7 +386,7 @@ gateup_pair_kernel(Bank gate, Bank up, const void* x, int H, int I, const uint32
     }
     sums.put(threadIdx.x >> 6, lane, acc);
     __syncthreads();
-    if (threadIdx.x < 32) put_h<PH>(sums, 0, pad, act, fb, j, h);
+    if (threadIdx.x < 32) put_h<PH>(sums, pad, act, fb, j, h);
 }
 
 // A token's pairs that count, in ascending slot order (pair j before j' of the same slot, j < j').
@@ -648,8 +648,8 @@ struct Run { // one pass's pieces
     template <int PX, int PH, bool BF16> bool pairs() const {
         const size_t xl = (size_t)plane_row(PX, H) + (size_t)naiwa_mx_groups(H) * 16;
         const size_t hl = ((size_t)plane_row(PH, I) + (size_t)naiwa_mx_groups(I) * 16) * c.width;
-        // With the kernels' own 17 and 33 KB, what a CU has.  One token of H 16384, 4 experts of 1024
-        // top-2, 31 us here and 74 as a tile; of 8 Mixtral-8x7B experts (h of 2 x 14336) 51 and 63.
+        // With down's own 33 KB, what a CU has.  One token of H 16384, 4 experts of 1024 top-2, 31 us here
+        // and 74 as a tile; of 8 Mixtral-8x7B experts (h of 2 x 14336) 51 and 63.
         constexpr size_t kLds = 120 * 1024;
         if (xl > kLds || (c.rows > 1 && hl > kLds)) return false;
         gateup_pair_kernel<PX, PH, BF16><<<dim3(n, 4 * naiwa_mx_steps(I)), kThreads, xl, st>>>(
