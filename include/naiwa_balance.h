@@ -15,7 +15,8 @@
  * Sums are deterministic: counts are integers, and P is added up in f32 over 64 rows
  * at most and beyond that in f64, in an order that depends on the sizes alone (and on
  * whether logits lie so that 4 can be read at once).  The entry points share one
- * grow-only scratch buffer per device: calls on different streams have to be ordered.
+ * grow-only scratch buffer per device: calls on different streams have to be ordered, and
+ * a graph's replays and other calls.  Captured calls keep the buffer that they were given.
  */
 #ifndef NAIWA_BALANCE_H
 #define NAIWA_BALANCE_H

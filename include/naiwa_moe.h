@@ -11,7 +11,8 @@
  * (when it keeps its logits internally) and layered-stack entry points reuse
  * one grow-only scratch buffer per device and entry point from call to call:
  * two such calls on different streams must be ordered by the caller (an event
- * between them).  The fused stack orders its launches itself, whatever their
+ * between them), and so must a graph's replays and other such calls.  A buffer that a
+ * captured call was given stays allocated when a later call needs a larger one.  The fused stack orders its launches itself, whatever their
  * streams.
  *
  * Reference interfaces each group replaces (naiwa-rs paths):

@@ -347,10 +347,10 @@ int ids_ok(const uint32_t* ids, int ids_ld, int64_t T, int k, int E) {
 __global__ void zero_kernel(uint32_t* p) { *p = 0; }
 
 // The scratch of a call; nothing in it outlives the call.
-int part_of(int blocks, int E, Part* p) {
+int part_of(int blocks, int E, hipStream_t st, Part* p) {
     const size_t n = (size_t)blocks * E;
     int rc = 0;
-    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_BALANCE, 1024 + n * 12 + (size_t)blocks * 4, &rc);
+    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_BALANCE, 1024 + n * 12 + (size_t)blocks * 4, &rc, st);
     if (!ws) return rc;
     *p = Part{(double*)(ws + 1024), (double*)ws, (uint32_t*)(ws + 1024 + 8 * n), (uint32_t*)(ws + 1024 + 12 * n),
               (uint32_t*)(ws + 1020)};
@@ -378,7 +378,7 @@ extern "C" int naiwa_expert_counts(const uint32_t* ids, int ids_ld, int64_t T, i
     const int blocks = blocks_of(T);
     hipStream_t st = (hipStream_t)stream;
     Part part;
-    if (int rc = part_of(blocks, E, &part)) return rc;
+    if (int rc = part_of(blocks, E, st, &part)) return rc;
     if (bad) zero_kernel<<<1, 1, 0, st>>>(bad);
     forward_kernel<Row<64, 0, false>, false><<<blocks, kThreads, 0, st>>>(nullptr, 0, ids, ids_ld ? ids_ld : k, T,
                                                           (int)((T + blocks - 1) / blocks), E, k, mask, part, counts, nullptr,
@@ -396,7 +396,7 @@ extern "C" int naiwa_router_balance(const void* logits, int dtype, int ld, const
     const int blocks = blocks_of(T);
     hipStream_t st = (hipStream_t)stream;
     Part part;
-    if (int rc = part_of(blocks, E, &part)) return rc;
+    if (int rc = part_of(blocks, E, st, &part)) return rc;
     auto go = [&](auto* kernel) {
         kernel<<<blocks, kThreads, 0, st>>>(logits, ld ? ld : E, ids, ids_ld ? ids_ld : k, T,
                                             (int)((T + blocks - 1) / blocks), E, k, mask, part, counts, valid, probs, loss, nullptr);

@@ -1061,7 +1061,7 @@ int mx_decode(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* do
     if (noalloc) {
         if (bytes > kNoAllocScratchBytes) return NAIWA_E_TOO_LARGE;
         if (bytes && (rc = noalloc_scratch(&ws))) return rc;
-    } else if (bytes && !(ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, bytes, &rc))) {
+    } else if (bytes && !(ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, bytes, &rc, (hipStream_t)stream))) {
         return rc;
     }
     if (wait) {
@@ -1082,7 +1082,8 @@ int decode_call(const naiwa_bank* gate, const naiwa_bank* up, const naiwa_bank* 
     uint8_t* ws = nullptr;
     const MfmaPlan mfma = mfma_plan(gate, up, down, x, rows, width, kMfmaScratchMax, chain);
     if (width > 0) {
-        ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, call_bytes(mfma, gate, down, rows, width), &rc);
+        ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, call_bytes(mfma, gate, down, rows, width), &rc,
+                                     (hipStream_t)stream);
         if (!ws) return rc;
     }
     return decode_launch(gate, up, down, x, x_dtype, slot_ids, w, rows, width, act, out, flags, mfma, ws,
@@ -1143,7 +1144,8 @@ int naiwa_moe_decode_residual(const naiwa_bank* gate, const naiwa_bank* up, cons
     if (rc || rows == 0 || width == 0) return rc;
     if (wait && (!wait->flag || !wait->fail)) return NAIWA_E_INVALID;
     const MfmaPlan mfma = mfma_plan(gate, up, down, x, rows, width, kMfmaScratchMax, true);
-    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, call_bytes(mfma, gate, down, rows, width), &rc);
+    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, call_bytes(mfma, gate, down, rows, width), &rc,
+                                     (hipStream_t)stream);
     if (!ws) return rc;
     if (mfma.on || split_path(rows * width, width))
         return decode_launch(gate, up, down, x, NAIWA_BF16, slot_ids, w, rows, width, act, keep_y ? y : nullptr, 0,
@@ -1165,7 +1167,8 @@ int naiwa_moe_decode_wait(const naiwa_bank* gate, const naiwa_bank* up, const na
     uint8_t* ws = nullptr;
     const MfmaPlan mfma = mfma_plan(gate, up, down, x, rows, width, kMfmaScratchMax, true);
     if (width > 0) {
-        ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, call_bytes(mfma, gate, down, rows, width), &rc);
+        ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_DECODE, call_bytes(mfma, gate, down, rows, width), &rc,
+                                     (hipStream_t)stream);
         if (!ws) return rc;
     } else if (wait) {
         // nothing to compute: the wait still orders the stream

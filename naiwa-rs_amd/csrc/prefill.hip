@@ -579,7 +579,7 @@ extern "C" int naiwa_moe_prefill(const naiwa_bank* gate, const naiwa_bank* up, c
         int rc = naiwa_mx_check(c);
         if (rc || T == 0) return rc;
         const size_t bytes = naiwa_mx_scratch_bytes(T, k, gate->k, gate->n);
-        uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_PREFILL, bytes, &rc);
+        uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_PREFILL, bytes, &rc, (hipStream_t)stream);
         return ws ? naiwa_mx_run(c, ws, (hipStream_t)stream) : rc;
     }
     if (T == 0) return NAIWA_OK;
@@ -614,7 +614,7 @@ extern "C" int naiwa_moe_prefill(const naiwa_bank* gate, const naiwa_bank* up, c
     const size_t o_h = a256(o_x + (size_t)T * H * 2), o_y = a256(o_h + (size_t)n * I * 2);
     const size_t total = a256(o_y + (size_t)n * H * 4);
     int rc = 0;
-    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_PREFILL, total, &rc);
+    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_PREFILL, total, &rc, (hipStream_t)stream);
     if (!ws) return rc;
     uint32_t* perm = (uint32_t*)(ws + o_perm);
     uint32_t* offsets = (uint32_t*)(ws + o_off);

@@ -434,7 +434,7 @@ extern "C" int naiwa_router_topk_ld(const void* x, int x_dtype, const float* W, 
     float* logits = logits_out;
     if (!logits) {
         int rc = 0;
-        logits = (float*)naiwa_scratch(NAIWA_SCRATCH_ROUTER, (size_t)rows * E * 4, &rc);
+        logits = (float*)naiwa_scratch(NAIWA_SCRATCH_ROUTER, (size_t)rows * E * 4, &rc, st);
         if (!logits) return rc;
     }
     // One block per (expert, row) for few rows, and whenever the 16-row blocks would not

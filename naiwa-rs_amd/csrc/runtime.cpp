@@ -16,9 +16,7 @@ std::mutex g_scratch_mu;
 NaiwaScratch g_scratch[kMaxDevices][NAIWA_SCRATCH_TAGS];
 } // namespace
 
-void* naiwa_scratch(int tag, size_t bytes, int* rc) { return naiwa_scratch(tag, bytes, rc, nullptr); }
-
-void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh) {
+static void* scratch(int tag, size_t bytes, int* rc, bool* fresh, bool capturing) {
     if (fresh) *fresh = false;
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -31,25 +29,34 @@ void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh) {
     if (s.bytes < bytes) {
         size_t want = bytes < 4096 ? 4096 : bytes;
         want = (want + 255) & ~size_t(255);
-        if (s.ptr) {
+        void* p = nullptr;
+        // The old buffer goes first, except one that a graph holds, and under capture, where
+        // no synchronisation is allowed.
+        if (s.ptr && !s.captured && !capturing) {
             // A queued kernel may still read the old buffer.
             e = hipDeviceSynchronize();
             if (e != hipSuccess) { *rc = (int)e; return nullptr; }
             (void)hipFree(s.ptr);
-            s.ptr = nullptr;
-            s.bytes = 0;
+            s = NaiwaScratch{};
         }
-        e = hipMalloc(&s.ptr, want);
-        if (e != hipSuccess) {
-            s.ptr = nullptr;
+        if (hipMalloc(&p, want) != hipSuccess) {
             *rc = NAIWA_E_NOMEM;
             return nullptr;
         }
-        s.bytes = want;
+        s = NaiwaScratch{p, want, false};
         if (fresh) *fresh = true;
     }
+    s.captured |= capturing;
     *rc = NAIWA_OK;
     return s.ptr;
+}
+
+void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh) { return scratch(tag, bytes, rc, fresh, false); }
+
+void* naiwa_scratch(int tag, size_t bytes, int* rc, hipStream_t stream) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone; // (the null stream cannot be captured)
+    if (stream && hipStreamIsCapturing(stream, &st) != hipSuccess) st = hipStreamCaptureStatusNone;
+    return scratch(tag, bytes, rc, nullptr, st != hipStreamCaptureStatusNone);
 }
 
 extern "C" {

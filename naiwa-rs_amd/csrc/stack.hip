@@ -61,7 +61,7 @@ extern "C" int naiwa_stack_decode_y(const naiwa_layer* layers, int n_layers, voi
     // scratch: ids, w, slots, w_mapped (n each) | y [rows * H] f32
     const size_t seg = ((size_t)n * 4 + 255) & ~size_t(255);
     int rc = 0;
-    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_STACK, 4 * seg + (size_t)rows * H * 4, &rc);
+    uint8_t* ws = (uint8_t*)naiwa_scratch(NAIWA_SCRATCH_STACK, 4 * seg + (size_t)rows * H * 4, &rc, st);
     if (!ws) return rc;
     uint32_t* ids_tmp = (uint32_t*)ws;
     float* w_tmp = (float*)(ws + seg);

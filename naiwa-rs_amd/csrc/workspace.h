@@ -15,14 +15,17 @@
 struct NaiwaScratch {
     void* ptr = nullptr;
     size_t bytes = 0;
+    bool captured = false; // a call under stream capture was given it
 };
 
 // Returns a device pointer of at least `bytes` for (device, tag), growing the
-// buffer (with a device sync, since a kernel may still read the old one).
-void* naiwa_scratch(int tag, size_t bytes, int* rc);
-// As above; *fresh tells whether this call (re)allocated the buffer, whose
-// contents are then undefined.
-void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh);
+// buffer (with a device sync, since a kernel may still read the old one).  A buffer
+// that a call under capture on `stream` was given is never freed, since the graph holds
+// its address: a larger call leaves it and allocates another.
+void* naiwa_scratch(int tag, size_t bytes, int* rc, hipStream_t stream);
+// For calls that are not captured; *fresh tells whether this call (re)allocated the
+// buffer, whose contents are then undefined.
+void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh = nullptr);
 
 // One buffer per user: a buffer shared by two entry points would let one overwrite what
 // the other keeps there between calls (the fused kernel's tagged exchange words are only
