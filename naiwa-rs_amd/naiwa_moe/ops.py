@@ -281,8 +281,10 @@ def mxfp4_from_ggml(blocks: np.ndarray, n: int, k: int, out: np.ndarray | None =
         raise ValueError(f"{b.size} bytes are not [{n}, {k}] MXFP4 blocks")
     if out is None:
         out = np.empty(size, dtype=np.uint8)
-    if out.dtype != np.uint8 or out.size != size or not out.flags.c_contiguous:
-        raise ValueError(f"out has to be {size} contiguous bytes")
+    if out.dtype != np.uint8 or out.size != size or not (out.flags.c_contiguous and out.flags.writeable):
+        raise ValueError(f"out has to be {size} contiguous bytes that can be written")
+    if np.may_share_memory(b, out):
+        raise ValueError("blocks and out overlap")
     check(lib().naiwa_mxfp4_from_ggml(b.ctypes.data, n, k, out.ctypes.data), "naiwa_mxfp4_from_ggml")
     return out
 

@@ -243,3 +243,17 @@ def test_expert_products_past_a_launch_are_refused():
     wide = [_bank(n, k, base=1 << 40) for n, k in (((1 << 21) + 128, H), ((1 << 21) + 128, H), (H, (1 << 21) + 128))]
     for call in (_decode, _prefill):
         assert call(*wide) == E_UNSUPPORTED
+
+
+def test_from_ggml_refuses_outputs_that_it_may_not_write():
+    """A read-only array (a view of a mapped file, say), one of another size or type, one over the blocks."""
+    size = nm.projection_bytes(nm.MXFP4_T, 16, 32)
+    mem = np.zeros(4096, np.uint8)
+    blocks = mem[:16 * 17]
+    fixed = np.zeros(size, np.uint8)
+    fixed.flags.writeable = False
+    for out in (fixed, np.zeros(size + 1, np.uint8), np.zeros(size, np.int8), np.zeros(2 * size, np.uint8)[::2],
+                mem[16:16 + size]):
+        with pytest.raises(ValueError):
+            nm.mxfp4_from_ggml(blocks, 16, 32, out)
+    assert nm.mxfp4_from_ggml(blocks, 16, 32, mem[1024:1024 + size]).size == size
