@@ -17,12 +17,12 @@
 // the token so that 16 neighbouring tokens' reads of one piece fall on distinct banks, while
 // 4 neighbouring lanes of a copy read 64 contiguous bytes.
 //
-// Bound.  Few tokens an expert: HBM, the weights are read once (96 tokens at Qwen3-30B sizes 4.9
-// TB/s in gate/up, 16 at Mixtral-8x7B sizes 5.0, where a copy reaches 5.1).  Many: the scaled
-// products and the power they draw; 4096 tokens at Mixtral sizes run 1.8 + 1.2 ms, 4.3 and 3.9
-// PFLOP/s of FP4 x E2M3, where the same products from registers alone reach 6 to 7 with random
-// codes and 9.9 with zeros, the chip's full rate: its power is the limit.  Without the weights'
-// loads gate/up takes 17 % less, without the copies 14 %, without the LDS reads no less.
+// Bound.  Few tokens an expert: HBM, the weights are read once, at the rates that stand at the
+// kernels (reads alone are not held to a copy's 5.1 TB/s).  Many: the scaled products and the
+// power they draw; 4096 tokens at Mixtral sizes run 1.8 + 1.2 ms, 4.3 and 3.9 PFLOP/s of FP4 x
+// E2M3, where the same products from registers alone reach 6 to 7 with random codes and 9.9 with
+// zeros, the chip's full rate: its power is the limit.  Without the weights' loads gate/up takes
+// 17 % less, without the copies 14 %, without the LDS reads no less.
 // Between (about 50 tokens of small experts): the memory's and the products' times, which two blocks
 // a CU overlap in part, and 1.7 rounds of blocks with 10 us of first loads and epilogue each.
 // Set aside: 128 weight rows a wave (one block a CU), 18 to 25 % slower; three blocks a CU (the
@@ -300,7 +300,8 @@ __device__ __forceinline__ void tile_dot(uint8_t* st, const uint8_t* base, const
 }
 
 // Gate/up of a tile: a wave's NA / 2 blocks of 32 features, gate and up; h in PH planes.
-// 16 tokens at Mixtral-8x7B sizes 94 us (5.3 TB/s), 4096 1.79 ms (1.07 PFLOP/s in 4 planes).
+// 16 tokens at Mixtral-8x7B sizes 94 us (5.3 TB/s), 96 at Qwen3-30B sizes 40 us (5.3 TB/s), 4096 at
+// Mixtral sizes 1.79 ms (1.07 PFLOP/s in 4 planes).
 template <int NA, int P, int PH>
 __global__ void __launch_bounds__(kThreads, 2)
 tile_gateup_kernel(Bank gate, Bank up, Planes x, int H, int I, int width, const uint32_t* perm, Tiles tl, int act, int xcd,

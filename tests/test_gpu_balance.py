@@ -2,9 +2,9 @@
 
 Tolerances: a probability errs by a few 2^-24 (its exponential, the sum, the division) and
 by |logit| 2^-24 through the difference to the row's largest; sums of them are f64 past 64
-rows: 2e-6 relative for logits of a few units.  The gradient p (c - sum c p) loses what
-c and the sum share: at most E 2^-24 sum(c p) / |c - sum c p|, far under 1e-5 of the norm
-for counts that differ at all.  bf16 gradients are rounded once: 2^-8 of a value each, at
+rows: 2e-6 relative for logits of a few units.  The gradient p (c - sum c p) is
+formed from counts less an integer m next to the sum, so it errs by a few 2^-24 of p (|c - m| +
+sum p |c - m|), which is of its own size: under 1e-5 of the norm.  bf16 gradients are rounded once: 2^-8 of a value each, at
 most 2^-8 of the norm.
 """
 import numpy as np
