@@ -1,0 +1,207 @@
+// naiwa_linear_input_grad and naiwa_linear_weight_grad (include/naiwa_linear.h) on linear_tiles.h's tiles.
+//
+// Input: dx[m][k] = sum_n dy[m][n] W[n][k]; J is dy, I the weights with the contraction as row index.  Two
+// matrices (a gate and its up) are one contraction of twice the length.
+// Weights: dw[n][k] = sum_m dy[m][n] x[m][k]; the contraction is the row index of both operands, and a block's
+// sum runs over its expert's rows.  The bias gradient is one more product per fragment of dy, with ones.
+#include "linear_tiles.h"
+
+#include <algorithm>
+
+namespace {
+
+struct InputArgs {
+    const uint16_t *w, *u, *dy, *dy_up;
+    int64_t w_ld, w_stride, u_ld, u_stride, dy_ld;
+    const uint32_t* offsets;
+    uint32_t rows;
+    int experts, n, k, act;
+    const uint16_t *pre, *pre_up;
+    void *dx, *dx_up;
+    int64_t pre_ld, dx_ld;
+    bool dx_f32, accumulate;
+};
+
+template <bool F16> __device__ __forceinline__ void input_store(const InputArgs& a, uint32_t m, int k, lin_f32x4 g) {
+    const int left = a.k - k;
+    if (a.pre) {
+        const lin_f32x4 p = load_4<F16>(a.pre, m * a.pre_ld + k, left, false);
+        lin_f32x4 q = {1.0f, 1.0f, 1.0f, 1.0f}, up;
+        if (a.pre_up) q = load_4<F16>(a.pre_up, m * a.pre_ld + k, left, false);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v, slope;
+            lin_act_slope(a.act, p[i], &v, &slope);
+            up[i] = g[i] * v;
+            g[i] = g[i] * slope * q[i];
+        }
+        if (a.pre_up) store_4<F16>(a.dx_up, m * a.dx_ld + k, left, a.dx_f32, up);
+    } else if (a.accumulate) {
+        g += load_4<F16>(a.dx, m * a.dx_ld + k, left, a.dx_f32);
+    }
+    store_4<F16>(a.dx, m * a.dx_ld + k, left, a.dx_f32, g);
+}
+
+template <class S>
+__global__ void __launch_bounds__(S::TH, 2)
+input_grad_kernel(InputArgs a, uint32_t nI) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
+    const Segments seg(a.offsets, a.rows, a.experts, S::TJ);
+    uint32_t it, jt, m0;
+    if (!tile_of_block(blockIdx.x, nI, seg.tiles, &it, &jt)) return;
+    int e, nj;
+    seg.find(jt, S::TJ, &e, &m0, &nj);
+    const int k0 = it * S::TI, ni = min(S::TI, a.k - k0);
+    const TileView iv[2] = {{a.w + e * a.w_stride + k0, a.w_ld, ni}, {a.u + e * a.u_stride + k0, a.u_ld, ni}};
+    const TileView jv[2] = {{a.dy + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}, {a.dy_up + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}};
+    lin_f32x4 acc[S::FI][S::FJ] = {};
+    tile_product<S>(iv, jv, a.u ? 2 : 1, a.n, lds, acc, [](auto&) {});
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int fj = 0; fj < S::FJ; ++fj) {
+        const int j = S::j_first(wave) + 16 * fj + (lane & 15);
+        if (j >= nj) continue;
+#pragma unroll
+        for (int fi = 0; fi < S::FI; ++fi) {
+            const int i = S::i_first(wave) + 16 * fi + 4 * (lane >> 4);
+            if (i < ni) input_store<S::F16>(a, m0 + j, k0 + i, acc[fi][fj]);
+        }
+    }
+}
+
+struct WeightArgs {
+    const uint16_t *dy, *x;
+    int64_t dy_ld, x_ld;
+    const uint32_t* offsets;
+    uint32_t rows;
+    int n, k;
+    void* dw;
+    int64_t ld, stride;
+    float* dbias;
+    bool dw_f32, accumulate;
+};
+
+template <class S>
+__global__ void __launch_bounds__(S::TH, 2)
+weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
+    const int e = blockIdx.y;
+    uint32_t it, jt;
+    if (!tile_of_block(blockIdx.x, nI, nJ, &it, &jt)) return;
+    uint32_t m0 = 0, m1 = a.rows;
+    if (a.offsets) m0 = offset_at(a.offsets, e, a.rows), m1 = max(m0, offset_at(a.offsets, e + 1, a.rows));
+    const int k0 = it * S::TI, ni = min(S::TI, a.k - k0), n0 = jt * S::TJ, nj = min(S::TJ, a.n - n0);
+    const TileView iv[1] = {{a.x + m0 * a.x_ld + k0, a.x_ld, ni}}, jv[1] = {{a.dy + m0 * a.dy_ld + n0, a.dy_ld, nj}};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    lin_f32x4 acc[S::FI][S::FJ] = {}, sum[S::FJ] = {};
+    const bool bias = a.dbias && it == 0 && S::i_first(wave) == 0; // whose share the bias gradient is
+    const short one = S::F16 ? (short)0x3c00 : (short)0x3f80;
+    const lin_s16x8 ones = {one, one, one, one, one, one, one, one};
+    tile_product<S>(iv, jv, 1, m1 - m0, lds, acc, [&](auto& b) {
+        if (bias)
+#pragma unroll
+            for (int f = 0; f < S::FJ; ++f) sum[f] = lin_mfma<S::F16>(ones, b[f], sum[f]);
+    });
+    if (a.accumulate && m0 == m1) return;
+#pragma unroll
+    for (int fj = 0; fj < S::FJ; ++fj) {
+        const int j = S::j_first(wave) + 16 * fj + (lane & 15);
+        if (j >= nj) continue;
+        if (bias && lane < 16) {
+            float* to = a.dbias + (int64_t)e * a.n + n0 + j;
+            *to = sum[fj][0] + (a.accumulate ? *to : 0.0f);
+        }
+#pragma unroll
+        for (int fi = 0; fi < S::FI; ++fi) {
+            const int i = S::i_first(wave) + 16 * fi + 4 * (lane >> 4), left = ni - i;
+            if (left <= 0) continue;
+            const int64_t at = e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i;
+            lin_f32x4 v = acc[fi][fj];
+            if (a.accumulate) v += load_4<S::F16>(a.dw, at, left, a.dw_f32);
+            store_4<S::F16>(a.dw, at, left, a.dw_f32, v);
+        }
+    }
+}
+
+template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
+    const int64_t nI = (a.k + S::TI - 1) / S::TI;
+    const int64_t nJ = (int64_t)a.rows / S::TJ + (a.offsets ? std::min<int64_t>(a.experts, a.rows) : a.rows % S::TJ != 0);
+    const int64_t blocks = (nI * nJ + 7) / 8 * 8;
+    if (blocks * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED; // a launch's threads
+    input_grad_kernel<S><<<(unsigned)blocks, S::TH, 0, st>>>(a, (uint32_t)nI);
+    return naiwa_hip_rc(hipGetLastError());
+}
+template <bool F16> int input_grad(const InputArgs& a, bool direct, hipStream_t st) {
+    return direct ? launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, true>>(a, st)
+                  : launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, false>>(a, st);
+}
+
+template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream_t st) {
+    const int64_t nI = (a.k + S::TI - 1) / S::TI, nJ = (a.n + S::TJ - 1) / S::TJ, blocks = (nI * nJ + 7) / 8 * 8;
+    if (blocks * experts * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED;
+    weight_grad_kernel<S><<<dim3((unsigned)blocks, experts), S::TH, 0, st>>>(a, (uint32_t)nI, (uint32_t)nJ);
+    return naiwa_hip_rc(hipGetLastError());
+}
+template <bool F16> int weight_grad(const WeightArgs& a, int experts, bool direct, hipStream_t st) {
+    return direct ? launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, true>>(a, experts, st)
+                  : launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, false>>(a, experts, st);
+}
+
+} // namespace
+
+extern "C" int naiwa_linear_input_grad(const naiwa_weights* w, const naiwa_weights* up, const void* dy, const void* dy_up,
+                                       int64_t dy_ld, const uint32_t* offsets, int64_t rows, int act, const void* pre,
+                                       const void* pre_up, int64_t pre_ld, void* dx, void* dx_up, int dx_dtype,
+                                       int64_t dx_ld, int flags, int64_t stream) {
+    if (int rc = lin_pair_ok(w, up)) return rc;
+    const int n = w->n, k = w->k;
+    if (rows < 0 || dy_ld < 0 || pre_ld < 0 || dx_ld < 0 || (dy_ld && dy_ld < n) || (pre_ld && pre_ld < k) ||
+        (dx_ld && dx_ld < k) || (!offsets && w->experts != 1) || (flags & ~NAIWA_LINEAR_ACCUMULATE) || !up != !dy_up ||
+        (pre_up && !pre) || !pre_up != !dx_up || (pre && flags))
+        return NAIWA_E_INVALID;
+    dy_ld = dy_ld ? dy_ld : n, pre_ld = pre_ld ? pre_ld : k, dx_ld = dx_ld ? dx_ld : k;
+    if (!lin_act_ok(act)) return NAIWA_E_UNSUPPORTED;
+    if (dx_dtype != NAIWA_F32 && dx_dtype != w->dtype) return NAIWA_E_UNSUPPORTED;
+    if (rows > INT32_MAX || dy_ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
+    if (rows == 0) return NAIWA_OK;
+    if (!dy || !dx) return NAIWA_E_INVALID;
+    const InputArgs a{(const uint16_t*)w->w, up ? (const uint16_t*)up->w : nullptr, (const uint16_t*)dy, (const uint16_t*)dy_up,
+                      lin_ld(w), lin_stride(w), up ? lin_ld(up) : 0, up ? lin_stride(up) : 0, dy_ld, offsets, (uint32_t)rows,
+                      w->experts, n, k, act, (const uint16_t*)pre, (const uint16_t*)pre_up, dx, dx_up, pre_ld, dx_ld,
+                      dx_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0};
+    const int64_t w_bytes = lin_bytes(w), u_bytes = up ? lin_bytes(up) : 0;
+    const int64_t o_bytes = lin_span(rows, dx_ld, k, lin_size(dx_dtype)), p_bytes = lin_span(rows, pre_ld, k, 2);
+    for (const void* o : {(const void*)dx, (const void*)dx_up})
+        if (lin_overlap(o, o_bytes, dy, lin_span(rows, dy_ld, n, 2)) || lin_overlap(o, o_bytes, dy_up, lin_span(rows, dy_ld, n, 2)) ||
+            lin_overlap(o, o_bytes, a.w, w_bytes) || lin_overlap(o, o_bytes, a.u, u_bytes) ||
+            lin_overlap(o, o_bytes, pre, p_bytes) || lin_overlap(o, o_bytes, pre_up, p_bytes))
+            return NAIWA_E_INVALID;
+    if (lin_overlap(dx, o_bytes, dx_up, o_bytes)) return NAIWA_E_INVALID;
+    const bool direct = !((n | k) & 7) && lin_aligned(a.w, a.w_ld, a.w_stride) && lin_aligned(dy, dy_ld, 0) &&
+                        (!up || (lin_aligned(a.u, a.u_ld, a.u_stride) && lin_aligned(dy_up, dy_ld, 0)));
+    hipStream_t st = (hipStream_t)stream;
+    return w->dtype == NAIWA_BF16 ? input_grad<false>(a, direct, st) : input_grad<true>(a, direct, st);
+}
+
+extern "C" int naiwa_linear_weight_grad(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype,
+                                        const uint32_t* offsets, int experts, int64_t rows, int n, int k, void* dw,
+                                        int dw_dtype, int64_t ld, int64_t stride, float* dbias, int flags, int64_t stream) {
+    if (int rc = lin_sizes_ok(experts, n, k, ld, stride)) return rc;
+    if (rows < 0 || dy_ld < 0 || x_ld < 0 || (dy_ld && dy_ld < n) || (x_ld && x_ld < k) || (!offsets && experts != 1) ||
+        (flags & ~NAIWA_LINEAR_ACCUMULATE) || !dw)
+        return NAIWA_E_INVALID;
+    dy_ld = dy_ld ? dy_ld : n, x_ld = x_ld ? x_ld : k, ld = ld ? ld : k, stride = stride ? stride : n * ld;
+    if ((dtype != NAIWA_BF16 && dtype != NAIWA_F16) || (dw_dtype != NAIWA_F32 && dw_dtype != dtype)) return NAIWA_E_UNSUPPORTED;
+    if (rows > INT32_MAX || dy_ld > kMaxLd || x_ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
+    if (rows && (!dy || !x)) return NAIWA_E_INVALID;
+    const WeightArgs a{(const uint16_t*)dy, (const uint16_t*)x, dy_ld, x_ld, offsets, (uint32_t)rows, n, k, dw, ld, stride, dbias,
+                       dw_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0};
+    const int64_t dy_bytes = lin_span(rows, dy_ld, n, 2), x_bytes = lin_span(rows, x_ld, k, 2);
+    const int64_t w_bytes = ((experts - 1) * stride + (n - 1) * ld + k) * lin_size(dw_dtype), b_bytes = (int64_t)experts * n * 4;
+    if (lin_overlap(dw, w_bytes, dy, dy_bytes) || lin_overlap(dw, w_bytes, x, x_bytes) || lin_overlap(dbias, b_bytes, dy, dy_bytes) ||
+        lin_overlap(dbias, b_bytes, x, x_bytes) || lin_overlap(dw, w_bytes, dbias, b_bytes))
+        return NAIWA_E_INVALID;
+    const bool direct = !((n | k) & 7) && lin_aligned(dy, dy_ld, 0) && lin_aligned(x, x_ld, 0);
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == NAIWA_BF16 ? weight_grad<false>(a, experts, direct, st) : weight_grad<true>(a, experts, direct, st);
+}

@@ -40,5 +40,6 @@ enum {
     NAIWA_SCRATCH_FUSED_TOKENS = 6, // fused stack: per-launch outputs of two-launch steps
     NAIWA_SCRATCH_PREFILL = 7,
     NAIWA_SCRATCH_BALANCE = 8, // partial sums of the balance loss
-    NAIWA_SCRATCH_TAGS = 9
+    NAIWA_SCRATCH_SORT = 9,    // counts of longer sorts by expert
+    NAIWA_SCRATCH_TAGS = 10
 };

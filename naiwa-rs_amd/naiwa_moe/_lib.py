@@ -20,6 +20,8 @@ E_FORMAT, E_IO, E_TOO_LARGE = -8, -9, -10
 F32, F16, Q8_0, Q4_K, BF16 = 0, 1, 8, 12, 30
 GGML_MXFP4, MXFP4_T = 39, 0x10000 | 39   # GGUF blocks; tile order (the banks' form)
 ACT_SILU, ACT_GELU_PYTORCH_TANH = 0, 1
+ACT_NONE = -1                            # products over 16-bit weights only (include/naiwa_linear.h)
+NO_ROW = 0xFFFFFFFF                      # inv of a pair that is in no segment (include/naiwa_tokens.h)
 ROUTE_SOFTMAX_TOPK_RENORM, ROUTE_TOPK_SOFTMAX, ROUTE_SOFTMAX_TOPK = 0, 1, 2
 
 
@@ -40,6 +42,12 @@ class Layer(C.Structure):
     """naiwa_layer: router + the three banks + the expert->slot table of one layer."""
     _fields_ = [("router", C.c_void_p), ("gate", Bank), ("up", Bank), ("down", Bank),
                 ("slot_of_expert", C.c_void_p)]
+
+
+class LinearWeights(C.Structure):
+    """naiwa_weights: 16-bit weights [experts, n, k] with a bias (include/naiwa_linear.h)."""
+    _fields_ = [("w", C.c_void_p), ("bias", C.c_void_p), ("ld", C.c_int64), ("stride", C.c_int64),
+                ("experts", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("dtype", C.c_int32)]
 
 
 STACK_LAYERED, STACK_FUSED = 0, 1
@@ -179,6 +187,20 @@ SIGNATURES: dict[str, tuple] = {
     "naiwa_expert_counts": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, i64]),
     "naiwa_router_balance": (i32, [vp, i32, i32, vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, i64]),
     "naiwa_router_balance_backward": (i32, [vp, i32, i32, vp, vp, i64, i32, i32, vp, vp, vp, i32, i32, i64]),
+    # include/naiwa_tokens.h
+    "naiwa_expert_sort": (i32, [vp, i32, i64, i32, i32, vp, vp, vp, vp, vp, i64]),
+    "naiwa_tokens_to_experts": (i32, [vp, i32, i64, vp, i64, i32, i32, vp, i64, i64]),
+    "naiwa_tokens_from_experts": (i32, [vp, i32, i64, vp, vp, i32, i64, i32, i32, vp, i32, i64, i32, i64]),
+    "naiwa_tokens_from_experts_backward": (i32, [vp, i32, i64, vp, i32, i64, vp, vp, i32, i64, i32, i32, vp, i64, vp, i32,
+                                                 i64]),
+    "naiwa_router_topk_backward": (i32, [vp, i32, i32, vp, i32, vp, i32, i64, i32, i32, i32, vp, vp, i32, i32, i64]),
+    # include/naiwa_linear.h
+    "naiwa_linear": (i32, [_P(LinearWeights), _P(LinearWeights), vp, i64, vp, i64, i32, vp, i64, vp, i32, i64, vp, vp, i64,
+                           i64]),
+    "naiwa_linear_input_grad": (i32, [_P(LinearWeights), _P(LinearWeights), vp, vp, i64, vp, i64, i32, vp, vp, i64, vp, vp,
+                                      i32, i64, i32, i64]),
+    "naiwa_linear_weight_grad": (i32, [vp, i64, vp, i64, i32, vp, i32, i64, i32, i32, vp, i32, i64, i64, vp, i32, i64]),
+    "naiwa_act_backward": (i32, [vp, vp, vp, i32, i64, i32, i64, i32, vp, vp, i64]),
     "naiwa_moe_gather": (i32, [vp, i32, i32, vp, vp, vp, i64]),
     "naiwa_synth": (i32, [i32, u64, u64, i64, f32, f32, vp, i64]),
     "naiwa_stack_decode": (i32, [_P(Layer), i32, vp, i32, i32, i32, i32, i32, i32, vp, vp, i32, i64]),
