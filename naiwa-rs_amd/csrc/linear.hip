@@ -39,7 +39,7 @@ template <bool F16> __device__ __forceinline__ void forward_store(const ForwardA
 }
 
 template <class S>
-__global__ void __launch_bounds__(S::TH, 2)
+__global__ void __launch_bounds__(S::TH, S::kWavesEU)
 linear_kernel(ForwardArgs a, uint32_t nI) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
     constexpr int kN = S::PAIR ? S::TI / 2 : S::TI; // features of a tile
@@ -53,19 +53,10 @@ linear_kernel(ForwardArgs a, uint32_t nI) {
                             {a.u + e * a.u_stride + (int64_t)n0 * a.u_ld, a.u_ld, ni}};
     const TileView jv[1] = {{a.x + (int64_t)m0 * a.x_ld, a.x_ld, nj}};
     lin_f32x4 acc[S::FI][S::FJ] = {};
-    tile_product<S>(iv, jv, 1, a.k, lds, acc, [](auto&) {});
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int F = S::PAIR ? S::FI / 2 : S::FI;
-#pragma unroll
-    for (int fj = 0; fj < S::FJ; ++fj) {
-        const int j = S::j_first(wave) + 16 * fj + (lane & 15);
-        if (j >= nj) continue;
-#pragma unroll
-        for (int fi = 0; fi < F; ++fi) {
-            const int i = S::i_first(wave) + 16 * fi + 4 * (lane >> 4);
-            if (i < ni) forward_store<S::F16>(a, e, m0 + j, n0 + i, acc[fi][fj], acc[S::PAIR ? fi + F : fi][fj]);
-        }
-    }
+    tile_product<S>(iv, jv, a.k, 0, (a.k + kStep - 1) / kStep, lds, acc, [](auto&) {});
+    each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 p, lin_f32x4 q) {
+        if (j < nj && i < ni) forward_store<S::F16>(a, e, m0 + j, n0 + i, p, q);
+    });
 }
 
 template <class S> int launch(const ForwardArgs& a, hipStream_t st) {
@@ -79,7 +70,7 @@ template <class S> int launch(const ForwardArgs& a, hipStream_t st) {
 }
 
 template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hipStream_t st) {
-    return direct ? launch<Shape<128, 128, 2, 2, kRows, kRows, F16, true, PAIR>>(a, st)
+    return direct ? launch<Shape<256, 256, 2, 4, kRows, kRows, F16, true, PAIR>>(a, st)
                   : launch<Shape<128, 128, 2, 2, kRows, kRows, F16, false, PAIR>>(a, st);
 }
 

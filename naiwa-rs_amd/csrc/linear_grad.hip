@@ -43,7 +43,7 @@ template <bool F16> __device__ __forceinline__ void input_store(const InputArgs&
 }
 
 template <class S>
-__global__ void __launch_bounds__(S::TH, 2)
+__global__ void __launch_bounds__(S::TH, S::kWavesEU)
 input_grad_kernel(InputArgs a, uint32_t nI) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
     const Segments seg(a.offsets, a.rows, a.experts, S::TJ);
@@ -55,18 +55,10 @@ input_grad_kernel(InputArgs a, uint32_t nI) {
     const TileView iv[2] = {{a.w + e * a.w_stride + k0, a.w_ld, ni}, {a.u + e * a.u_stride + k0, a.u_ld, ni}};
     const TileView jv[2] = {{a.dy + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}, {a.dy_up + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}};
     lin_f32x4 acc[S::FI][S::FJ] = {};
-    tile_product<S>(iv, jv, a.u ? 2 : 1, a.n, lds, acc, [](auto&) {});
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int fj = 0; fj < S::FJ; ++fj) {
-        const int j = S::j_first(wave) + 16 * fj + (lane & 15);
-        if (j >= nj) continue;
-#pragma unroll
-        for (int fi = 0; fi < S::FI; ++fi) {
-            const int i = S::i_first(wave) + 16 * fi + 4 * (lane >> 4);
-            if (i < ni) input_store<S::F16>(a, m0 + j, k0 + i, acc[fi][fj]);
-        }
-    }
+    tile_product<S>(iv, jv, a.n, 0, (a.n + kStep - 1) / kStep * (a.u ? 2 : 1), lds, acc, [](auto&) {});
+    each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 g, lin_f32x4) {
+        if (j < nj && i < ni) input_store<S::F16>(a, m0 + j, k0 + i, g);
+    });
 }
 
 struct WeightArgs {
@@ -82,7 +74,7 @@ struct WeightArgs {
 };
 
 template <class S>
-__global__ void __launch_bounds__(S::TH, 2)
+__global__ void __launch_bounds__(S::TH, S::kWavesEU)
 weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
     const int e = blockIdx.y;
@@ -97,30 +89,26 @@ weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ) {
     const bool bias = a.dbias && it == 0 && S::i_first(wave) == 0; // whose share the bias gradient is
     const short one = S::F16 ? (short)0x3c00 : (short)0x3f80;
     const lin_s16x8 ones = {one, one, one, one, one, one, one, one};
-    tile_product<S>(iv, jv, 1, m1 - m0, lds, acc, [&](auto& b) {
+    tile_product<S>(iv, jv, m1 - m0, 0, (int)((m1 - m0 + kStep - 1) / kStep), lds, acc, [&](auto& b) {
         if (bias)
 #pragma unroll
             for (int f = 0; f < S::FJ; ++f) sum[f] = lin_mfma<S::F16>(ones, b[f], sum[f]);
     });
     if (a.accumulate && m0 == m1) return;
+    if (bias && lane < 16) {
 #pragma unroll
-    for (int fj = 0; fj < S::FJ; ++fj) {
-        const int j = S::j_first(wave) + 16 * fj + (lane & 15);
-        if (j >= nj) continue;
-        if (bias && lane < 16) {
+        for (int fj = 0; fj < S::FJ; ++fj) {
+            const int j = S::j_first(wave) + 16 * fj + lane;
             float* to = a.dbias + (int64_t)e * a.n + n0 + j;
-            *to = sum[fj][0] + (a.accumulate ? *to : 0.0f);
-        }
-#pragma unroll
-        for (int fi = 0; fi < S::FI; ++fi) {
-            const int i = S::i_first(wave) + 16 * fi + 4 * (lane >> 4), left = ni - i;
-            if (left <= 0) continue;
-            const int64_t at = e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i;
-            lin_f32x4 v = acc[fi][fj];
-            if (a.accumulate) v += load_4<S::F16>(a.dw, at, left, a.dw_f32);
-            store_4<S::F16>(a.dw, at, left, a.dw_f32, v);
+            if (j < nj) *to = sum[fj][0] + (a.accumulate ? *to : 0.0f);
         }
     }
+    each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 v, lin_f32x4) {
+        if (j >= nj || i >= ni) return;
+        const int64_t at = e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i;
+        if (a.accumulate) v += load_4<S::F16>(a.dw, at, ni - i, a.dw_f32);
+        store_4<S::F16>(a.dw, at, ni - i, a.dw_f32, v);
+    });
 }
 
 template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
@@ -132,7 +120,7 @@ template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
     return naiwa_hip_rc(hipGetLastError());
 }
 template <bool F16> int input_grad(const InputArgs& a, bool direct, hipStream_t st) {
-    return direct ? launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, true>>(a, st)
+    return direct ? launch_input<Shape<256, 256, 2, 4, kCols, kRows, F16, true>>(a, st)
                   : launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, false>>(a, st);
 }
 
@@ -143,7 +131,7 @@ template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream
     return naiwa_hip_rc(hipGetLastError());
 }
 template <bool F16> int weight_grad(const WeightArgs& a, int experts, bool direct, hipStream_t st) {
-    return direct ? launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, true>>(a, experts, st)
+    return direct ? launch_weight<Shape<256, 256, 2, 4, kCols, kCols, F16, true>>(a, experts, st)
                   : launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, false>>(a, experts, st);
 }
 

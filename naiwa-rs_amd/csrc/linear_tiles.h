@@ -6,14 +6,19 @@
 // holds 4 consecutive i of one j, so i is the index that is contiguous in the output: the
 // weights' features forward, the input's in both gradients.
 //
-// Tiles of 64 contraction steps lie in LDS twice over: one is read while the next lands in the
-// other, copied from memory without passing registers (16 bytes a lane).  Buffer ranges make what lies behind a
-// segment's last row zero, lanes behind the last of c ask for an address out of range.  Both layouts keep
-// 16-byte pieces whole and permute them so that no two lanes of a read share a bank:
-//   contiguous: row r of 64 values, piece q at r * 128 + 16 (q ^ (r & 7)); 16-byte reads;
+// Steps of 32 contraction values lie in a ring of 4 LDS buffers, copied from memory without passing
+// registers (16 bytes a lane).  In step t a wave multiplies what it read of step t, reads step t + 1 and starts the
+// copies of step t + 4 into the buffer that step t left, all three interleaved; one barrier a step says
+// that step t + 1 has landed and step t's buffer is free.  Buffer ranges make what lies behind a segment's last
+// row zero, lanes behind the last of c ask for an address out of range, and so do steps behind the last
+// (the ring's counted waits stay the same to the end).  Both layouts keep 16-byte pieces whole and
+// permute them so that no two lanes of a read share a bank:
+//   contiguous: row r of 32 values, piece q at r * 64 + 16 (q ^ (r >> 2 & 3)); 16-byte reads;
 //   row index:  row c of T values, the pair of pieces f (16 values) at 32 (f ^ s(c)), s(c) = c & 3 | (c >> 3 & 1)
 //               << 2, read by the transposing LDS read (4 rows x 16 values a group of 16 lanes).
-// Operands that are not multiples of 16 bytes pass through registers, value by value at their ends.
+// Operands that are not multiples of 16 bytes pass through registers two steps ahead, value by value at their ends.
+// At the end the accumulators go through LDS once more, so that what follows the product works on rows:
+// whole lines of memory, and code that is there once.
 #pragma once
 
 #include "../../include/naiwa_linear.h"
@@ -30,7 +35,8 @@ typedef _Float16 lin_f16x8 __attribute__((ext_vector_type(8)));
 typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
 typedef short lin_s16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kStep = 64;           // contraction steps of a tile in LDS
+constexpr int kStep = 32;           // contraction values of a step
+constexpr int kRing = 4;            // steps in LDS
 constexpr uint32_t kFar = 1u << 31; // an offset past every range
 
 enum { kRows = 0, kCols = 1 }; // the contraction index is contiguous, or the row index
@@ -69,42 +75,56 @@ template <int N> __device__ __forceinline__ void copies_landed() {
 template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
     static_assert(!PAIR || (LAYOUT == kRows && NW % 2 == 0), "whole waves a half");
     static constexpr int kBytes = T * kStep * 2;
-    static constexpr int kCopies = kBytes / 1024 / NW; // a wave's, 1 KB each
-    static constexpr int kPieces = kBytes / 16 / (NW * 64);
-    static constexpr int kRowPieces = LAYOUT == kRows ? kStep / 8 : T / 8; // pieces of a row in LDS
-    static_assert(kCopies * 1024 * NW == kBytes, "whole copies");
+    static constexpr int kLanes = kBytes / NW / 16 < 64 ? kBytes / NW / 16 : 64; // that take part in a copy
+    static constexpr int kCopies = kBytes / NW / 16 / kLanes;                    // a wave's
+    static constexpr int kPieces = (kBytes / 16 + NW * 64 - 1) / (NW * 64);      // a thread's, through registers
+    static constexpr int kRowPieces = LAYOUT == kRows ? kStep / 8 : T / 8;       // pieces of a row in LDS
+    static constexpr int kPer = kLanes / kRowPieces;                             // rows of a copy
+    static_assert(kCopies * kLanes * 16 * NW == kBytes && kPer > 0, "whole copies of whole rows");
 
     static __device__ __forceinline__ int swizzle(int row) { // of a piece's place in its row
-        if (LAYOUT == kRows) return row & 7;
+        if (LAYOUT == kRows) return (row >> 2) & 3;
         return ((row & 3) | ((row >> 1) & 4)) << 1 & (kRowPieces - 1);
     }
 
-    // ---- by copies
-    // The copies of contraction steps c0 .. c0 + 63 of C.
-    static __device__ __forceinline__ void copy(const TileView* views, int64_t c0, int64_t C, uint32_t lds, int wave, int lane) {
-        TileView v = PAIR && wave >= NW / 2 ? views[1] : views[0];
-        if (PAIR && wave >= NW / 2) v.base -= T / 2 * v.ld, v.valid += T / 2; // (rows from T / 2 on)
-        const uint32_t ld2 = (uint32_t)v.ld * 2;
-        if constexpr (LAYOUT == kRows) {
-            const lin_u32x4 r = range_of(v.base + c0, ((v.valid - 1) * v.ld + (C - c0)) * 2);
-            const int piece = (lane & 7) ^ (lane >> 3);
-            const uint32_t off = 8 * piece < C - c0 ? (uint32_t)(lane >> 3) * ld2 + 16 * piece : kFar;
+    // ---- by copies: begin(), then one(i) for a wave's copies
+    struct Copier {
+        uint32_t off[kCopies]; // of the lane's pieces, from the step's first value
+        uint32_t lds;          // of the wave's part of the first buffer
+        int piece;             // of its row (kRows; the same in all of a wave's copies, 16 rows or one apart)
+        bool in;
+        __device__ __forceinline__ Copier(uint32_t at, int wave, int lane) : in(lane < kLanes) {
+            lds = __builtin_amdgcn_readfirstlane(at + wave * (kBytes / NW));
+        }
+        // At views with rows so far apart.
+        __device__ __forceinline__ void aim(const TileView* views, int wave, int lane) {
+            const bool second = PAIR && wave >= NW / 2;
+            const uint32_t ld2 = (uint32_t)(second ? views[1].ld : views[0].ld) * 2;
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
-                const int row = 8 * (wave * kCopies + i);
-                copy16(r, off + (uint32_t)row * ld2, lds + (wave * kCopies + i) * 1024);
-            }
-        } else {
-            const lin_u32x4 r = range_of(v.base + c0 * v.ld, ((C - c0 - 1) * v.ld + v.valid) * 2);
-            constexpr int kPer = 64 / kRowPieces; // rows of a copy
-#pragma unroll
-            for (int i = 0; i < kCopies; ++i) {
-                const int row = (wave * kCopies + i) * kPer + lane / kRowPieces;
-                const int piece = (lane % kRowPieces) ^ swizzle(row);
-                copy16(r, (uint32_t)row * ld2 + 16 * piece, lds + (wave * kCopies + i) * 1024);
+                const int r = (wave * kCopies + i) * kPer + lane / kRowPieces; // (rows of a PAIR's second half from its view's own first)
+                piece = (lane % kRowPieces) ^ swizzle(r);
+                off[i] = (uint32_t)(second ? r - T / 2 : r) * ld2 + 16 * piece;
             }
         }
-    }
+        lin_u32x4 range;
+        bool far;
+        // The step of contraction values c0 .. c0 + 31 of C (none if c0 >= C).
+        __device__ __forceinline__ void begin(const TileView* views, int64_t c0, int64_t C, int wave, int lane) {
+            const TileView v = PAIR && wave >= NW / 2 ? views[1] : views[0];
+            const int64_t left = C - c0;
+            if constexpr (LAYOUT == kRows) {
+                range = range_of(v.base + c0, left > 0 && v.valid > 0 ? ((v.valid - 1) * v.ld + left) * 2 : 0);
+                far = 8 * piece >= left;
+            } else {
+                range = range_of(v.base + c0 * v.ld, left > 0 ? ((left - 1) * v.ld + v.valid) * 2 : 0);
+                far = false;
+            }
+        }
+        __device__ __forceinline__ void one(int i, uint32_t buffer) const {
+            if (kLanes == 64 || in) copy16(range, LAYOUT == kRows && far ? kFar : off[i], lds + buffer + i * (kLanes * 16));
+        }
+    };
 
     // ---- through registers
     struct Held {
@@ -118,9 +138,9 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
             const bool second = PAIR && row >= T / 2;
             const TileView v = second ? views[1] : views[0];
             if (second) row -= T / 2;
-            // LDS row `row`, values at .. at + 7 of it, of which `n` exist
+            // LDS row `row`, values at .. at + 7 of it, of which `left` exist
             const int64_t left = LAYOUT == kRows ? C - c0 - at : v.valid - at;
-            const bool in = LAYOUT == kRows ? row < v.valid : row < C - c0;
+            const bool in = LAYOUT == kRows ? row < v.valid : row < C - c0 && row < kStep;
             const uint16_t* s = LAYOUT == kRows ? v.base + row * v.ld + c0 + at : v.base + (c0 + row) * v.ld + at;
             lin_u32x4 w = {};
             if (in && left >= 8) {
@@ -137,19 +157,17 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int p = tid + i * NW * 64, row = p / kRowPieces, piece = (p % kRowPieces) ^ swizzle(row);
-            *(lin_u32x4*)(lds + row * (kRowPieces * 16) + piece * 16) = h.v[i];
+            if (kBytes % (NW * 1024) == 0 || p < kBytes / 16) *(lin_u32x4*)(lds + row * (kRowPieces * 16) + piece * 16) = h.v[i];
         }
     }
 
-    // ---- fragments: F of 16 rows (columns) from the wave's first, `first`, of 32 contraction steps (half kk)
+    // ---- fragments: F of 16 rows (columns) from `first` on
     template <int F> struct Reader {
-        uint32_t at[LAYOUT == kRows ? 2 : F];
-        // frag f is rows first + 16 f + lane % 16, c = 32 kk + 8 (lane / 16) + 0 .. 7
+        uint32_t at[LAYOUT == kRows ? 1 : F];
+        // frag f is rows first + 16 f + lane % 16, c = 8 (lane / 16) + 0 .. 7
         __device__ __forceinline__ Reader(int first, int lane) {
             if constexpr (LAYOUT == kRows) {
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk)
-                    at[kk] = (uint32_t)(first + (lane & 15)) * 128 + ((((lane >> 4) + 4 * kk) ^ (lane & 7)) << 4);
+                at[0] = (uint32_t)(first + (lane & 15)) * 64 + (((lane >> 4) ^ swizzle(lane & 15)) << 4);
             } else {
                 const int row = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
@@ -157,16 +175,16 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
                     at[f] = (uint32_t)row * (T * 2) + (((first / 16 + f) * 2 ^ swizzle(row)) << 4) + 8 * (lane & 3);
             }
         }
-        // buf: the tile's LDS address
-        __device__ __forceinline__ lin_s16x8 get(uint32_t buf, int f, int kk) const {
+        // buf: the step's LDS address
+        __device__ __forceinline__ lin_s16x8 get(uint32_t buf, int f) const {
             typedef __attribute__((address_space(3))) const lin_s16x8* P8;
             typedef __attribute__((address_space(3))) lin_s16x4* P4;
             if constexpr (LAYOUT == kRows) {
-                return *(P8)(buf + at[kk] + f * 2048);
+                return *(P8)(uintptr_t)(buf + at[0] + f * 1024);
             } else {
-                const uint32_t a = buf + at[f] + kk * (32 * T * 2);
-                const lin_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)a);
-                const lin_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(a + 4 * T * 2));
+                const uint32_t a = buf + at[f];
+                const lin_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)a);
+                const lin_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(a + 4 * T * 2));
                 return lin_s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             }
         }
@@ -186,77 +204,155 @@ template <int TI_, int TJ_, int NWI_, int NWJ_, int LI_, int LJ_, bool F16_, boo
     static constexpr int TI = TI_, TJ = TJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, TH = NW * 64;
     static constexpr int FI = TI / NWI / 16, FJ = TJ / NWJ / 16;
     static constexpr bool F16 = F16_, DIRECT = DIRECT_, PAIR = PAIR_;
+    static constexpr int kWavesEU = FI * FJ > 32 ? 1 : 2; // waves of a SIMD, by their accumulators
     typedef Tile<TI, LI_, NW, PAIR_> I;
     typedef Tile<TJ, LJ_, NW, false> J;
     static constexpr int kBuf = I::kBytes + J::kBytes;
-    static constexpr int kLds = 2 * kBuf;
+    static constexpr int kLds = kRing * kBuf;
+    static constexpr int kWaveI = TI / NWI, kWaveJ = TJ / NWJ;
     // The wave's first I row (fragments of a PAIR: f < FI / 2 from here, the others TI / 2 on).
-    static __device__ __forceinline__ int i_first(int wave) { return wave % NWI * (TI / NWI) / (PAIR ? 2 : 1); }
-    static __device__ __forceinline__ int j_first(int wave) { return wave / NWI * (TJ / NWJ); }
+    static __device__ __forceinline__ int i_first(int wave) { return wave % NWI * kWaveI / (PAIR ? 2 : 1); }
+    static __device__ __forceinline__ int j_first(int wave) { return wave / NWI * kWaveJ; }
 };
 
-// acc[fi][fj] += the tile's product over `sources` contraction ranges of C each: iv[0] and jv[0], then iv[1] and
-// jv[1].  (A PAIR has one range, and iv[0], iv[1] are the matrices of its halves.)  each(b) is called with every
-// half step's J fragments.
+// acc[fi][fj] += the tile's product over steps s0 .. s1 - 1 of `sources` contraction ranges of C each: iv[0] and jv[0],
+// then iv[1] and jv[1].  (A PAIR has one range, and iv[0], iv[1] are the matrices of its halves.)  each(b) is
+// called with every step's J fragments.
 template <class S, class Each>
-__device__ __forceinline__ void tile_product(const TileView* iv, const TileView* jv, int sources, int64_t C, uint8_t* lds,
+__device__ __forceinline__ void tile_product(const TileView* iv, const TileView* jv, int64_t C, int s0, int s1, uint8_t* lds,
                                              lin_f32x4 (&acc)[S::FI][S::FJ], Each each) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int per = (int)((C + kStep - 1) / kStep), steps = per * sources;
+    const int per = (int)((C + kStep - 1) / kStep);
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(lds));
     typedef typename S::I I;
     typedef typename S::J J;
+    constexpr int kCopies = I::kCopies + J::kCopies;
     const typename I::template Reader<S::PAIR ? S::FI / 2 : S::FI> ri(S::i_first(wave), lane);
     const typename J::template Reader<S::FJ> rj(S::j_first(wave), lane);
-    typename I::Held hi;
-    typename J::Held hj;
-    auto fetch = [&](int step, int buf) {
-        const int s = step >= per ? 1 : 0; // (of a PAIR always 0)
-        const int64_t c0 = (int64_t)(step - s * per) * kStep;
+    typename I::Copier ci(at, wave, lane);
+    typename J::Copier cj(at + I::kBytes, wave, lane);
+    typename I::Held hi[2];
+    typename J::Held hj[2];
+    auto source = [&](int step, int64_t* c0) { // (of a PAIR always 0)
+        const int s = step >= per && !S::PAIR ? 1 : 0;
+        *c0 = step < s1 ? (int64_t)(step - s * per) * kStep : C;
+        return s;
+    };
+    auto begin = [&](int step) {
+        int64_t c0;
+        const int s = source(step, &c0);
+        if (step == s0 || (step == per && step < s1 && !S::PAIR)) {
+            ci.aim(S::PAIR || !s ? iv : iv + 1, wave, lane);
+            cj.aim(s ? jv + 1 : jv, wave, lane);
+        }
+        ci.begin(S::PAIR || !s ? iv : iv + 1, c0, C, wave, lane);
+        cj.begin(s ? jv + 1 : jv, c0, C, wave, lane);
+    };
+    auto copy = [&](int i, uint32_t buffer) { i < I::kCopies ? ci.one(i, buffer) : cj.one(i - I::kCopies, buffer); };
+    auto load = [&](int step, int p) {
+        int64_t c0;
+        const int s = source(step, &c0);
+        I::load(S::PAIR || !s ? iv : iv + 1, c0, C, tid, hi[p]);
+        J::load(s ? jv + 1 : jv, c0, C, tid, hj[p]);
+    };
+    auto store = [&](uint32_t buffer, int p) {
+        I::store(hi[p], lds + buffer, tid);
+        J::store(hj[p], lds + buffer + I::kBytes, tid);
+    };
+    auto read_i = [&](uint32_t buffer, int f) {
+        if (S::PAIR && f >= S::FI / 2) return ri.get(at + buffer + S::TI / 2 * (kStep * 2), f - S::FI / 2); // (a PAIR's I is kRows)
+        return ri.get(at + buffer, f);
+    };
+    auto read_j = [&](uint32_t buffer, int f) { return rj.get(at + buffer + I::kBytes, f); };
+
+    lin_s16x8 a[2][S::FI], b[2][S::FJ];
+    if constexpr (S::DIRECT) {
+#pragma unroll
+        for (int i = 0; i < kRing; ++i) {
+            begin(s0 + i);
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) copy(c, i * S::kBuf);
+        }
+        copies_landed<(kRing - 1) * kCopies>();
+    } else {
+        load(s0, 0), load(s0 + 1, 1);
+        store(0, 0), store(S::kBuf, 1);
+        load(s0 + 2, 0), load(s0 + 3, 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int f = 0; f < S::FI; ++f) a[0][f] = read_i(0, f);
+#pragma unroll
+    for (int f = 0; f < S::FJ; ++f) b[0][f] = read_j(0, f);
+    uint32_t mine = 0; // the buffer of step t
+    auto step = [&](int t, auto parity) {
+        constexpr int p = decltype(parity)::value;
+        const uint32_t next = mine + S::kBuf == S::kLds ? 0 : mine + S::kBuf;
         if constexpr (S::DIRECT) {
-            I::copy(S::PAIR || !s ? iv : iv + 1, c0, C, at + buf * S::kBuf, wave, lane);
-            J::copy(s ? jv + 1 : jv, c0, C, at + buf * S::kBuf + I::kBytes, wave, lane);
+            copies_landed<(kRing - 2) * kCopies>();
+            begin(t + kRing);
         } else {
-            I::load(S::PAIR || !s ? iv : iv + 1, c0, C, tid, hi);
-            J::load(s ? jv + 1 : jv, c0, C, tid, hj);
+            __syncthreads();
+            const uint32_t then = mine + 2 * S::kBuf >= S::kLds ? mine + 2 * S::kBuf - S::kLds : mine + 2 * S::kBuf;
+            store(then, p);
+            load(t + kRing, p);
         }
+        each(b[p]);
+        // Parts of the step in order: some reads of the next, some copies, a row of products.
+        constexpr int kReads = S::FI + S::FJ, kParts = S::FI;
+#pragma unroll
+        for (int fi = 0; fi < kParts; ++fi) {
+#pragma unroll
+            for (int r = 0; r < kReads; ++r)
+                if (r * kParts / kReads == fi) {
+                    if (r < S::FI) a[p ^ 1][r] = read_i(next, r);
+                    else b[p ^ 1][r - S::FI] = read_j(next, r - S::FI);
+                }
+            if constexpr (S::DIRECT)
+#pragma unroll
+                for (int c = 0; c < kCopies; ++c)
+                    if (c * kParts / kCopies == fi) copy(c, mine);
+#pragma unroll
+            for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[p][fi], b[p][fj], acc[fi][fj]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        mine = next;
     };
-    auto keep = [&](int buf) {
-        if constexpr (!S::DIRECT) {
-            I::store(hi, lds + buf * S::kBuf, tid);
-            J::store(hj, lds + buf * S::kBuf + I::kBytes, tid);
+    for (int t = s0; t < s1; t += 2) { // (an odd number's last step multiplies zeros)
+        step(t, std::integral_constant<int, 0>());
+        step(t + 1, std::integral_constant<int, 1>());
+    }
+}
+
+// f(j, i, v, q) for 4 values v at a time, i .. i + 3 of row j of the wave's part of the tile: of a PAIR v is of the first
+// matrix, q of the second, and i runs over one.  Every wave of the block calls it.
+template <class S, class F>
+__device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[S::FI][S::FJ], F f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kPieces = S::kWaveI / 4;                               // of a row in LDS
+    constexpr int kFit = S::kLds / S::NW / (S::kWaveI * 16 * 4);         // J fragments at a time
+    constexpr int kAt = kFit < S::FJ ? kFit : S::FJ;
+    static_assert(kAt > 0 && S::FJ % kAt == 0, "whole fragments");
+    constexpr int kTake = S::PAIR ? kPieces / 2 : kPieces;               // lanes of a row
+    static_assert(64 % kTake == 0, "whole rows");
+    constexpr int kRowsAt = 64 / kTake;
+    uint8_t* mine = lds + wave * (kAt * 16 * S::kWaveI * 4);
+    auto at = [&](int row, int piece) { return (lin_f32x4*)(mine + row * (kPieces * 16) + ((piece ^ (row & 15 & (kPieces - 1))) << 4)); };
+    copies_landed<0>(); // of steps behind the last too
+#pragma unroll
+    for (int h = 0; h < S::FJ; h += kAt) {
+#pragma unroll
+        for (int fj = 0; fj < kAt; ++fj)
+#pragma unroll
+            for (int fi = 0; fi < S::FI; ++fi) *at(16 * fj + (lane & 15), 4 * fi + (lane >> 4)) = acc[fi][h + fj];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int r = 0; r < kAt * 16; r += kRowsAt) {
+            const int row = r + lane / kTake, piece = lane % kTake;
+            const lin_f32x4 v = *at(row, piece), q = S::PAIR ? *at(row, piece + kTake) : v;
+            f(S::j_first(wave) + 16 * h + row, S::i_first(wave) + 4 * piece, v, q);
         }
-    };
-    if (steps == 0) return;
-    fetch(0, 0);
-    keep(0);
-    copies_landed<0>();
-    for (int step = 0; step < steps; ++step) {
-        const int buf = step & 1;
-        if (step + 1 < steps) fetch(step + 1, buf ^ 1);
-        const uint32_t ib = at + buf * S::kBuf, jb = ib + I::kBytes;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            lin_s16x8 a[S::FI], b[S::FJ];
-#pragma unroll
-            for (int f = 0; f < S::FI; ++f) {
-                if (S::PAIR && f >= S::FI / 2)
-                    a[f] = ri.get(ib + S::TI / 2 * 128, f - S::FI / 2, kk); // (a PAIR's I is kRows)
-                else
-                    a[f] = ri.get(ib, f, kk);
-            }
-#pragma unroll
-            for (int f = 0; f < S::FJ; ++f) b[f] = rj.get(jb, f, kk);
-            each(b);
-#pragma unroll
-            for (int fi = 0; fi < S::FI; ++fi)
-#pragma unroll
-                for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[fi], b[fj], acc[fi][fj]);
-        }
-        if (step + 1 < steps) {
-            keep(buf ^ 1);
-            copies_landed<0>();
-        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
