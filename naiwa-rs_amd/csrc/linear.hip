@@ -70,8 +70,8 @@ template <class S> int launch(const ForwardArgs& a, hipStream_t st) {
 }
 
 template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hipStream_t st) {
-    return direct ? launch<Shape<256, 256, 2, 4, kRows, kRows, F16, true, PAIR>>(a, st)
-                  : launch<Shape<128, 128, 2, 2, kRows, kRows, F16, false, PAIR>>(a, st);
+    return direct ? launch<Shape<256, 256, 2, 4, 4, kRows, kRows, F16, true, PAIR>>(a, st)
+                  : launch<Shape<128, 128, 2, 2, 4, kRows, kRows, F16, false, PAIR>>(a, st);
 }
 
 // ---- the activation's gradient alone

@@ -13,7 +13,8 @@
 // row zero, lanes behind the last of c ask for an address out of range, and so do steps behind the last
 // (the ring's counted waits stay the same to the end).  Both layouts keep 16-byte pieces whole and
 // permute them so that no two lanes of a read share a bank:
-//   contiguous: row r of 32 values, piece q at r * 64 + 16 (q ^ (r >> 2 & 3)); 16-byte reads;
+//   contiguous: row r of 32 values, piece q at r * 64 + 16 (q ^ g), g = 0, 2, 3, 1 for rows in fours; 16-byte reads, of
+//               which the LDS takes lanes 0-3, 12-15, 20-27 at a time, then 4-11, 16-19, 28-31, and so on;
 //   row index:  row c of T values, the pair of pieces f (16 values) at 32 (f ^ s(c)), s(c) = c & 3 | (c >> 3 & 1)
 //               << 2, read by the transposing LDS read (4 rows x 16 values a group of 16 lanes).
 // Operands that are not multiples of 16 bytes pass through registers two steps ahead, value by value at their ends.
@@ -36,7 +37,6 @@ typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
 typedef short lin_s16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 32;           // contraction values of a step
-constexpr int kRing = 4;            // steps in LDS
 constexpr uint32_t kFar = 1u << 31; // an offset past every range
 
 enum { kRows = 0, kCols = 1 }; // the contraction index is contiguous, or the row index
@@ -83,7 +83,7 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
     static_assert(kCopies * kLanes * 16 * NW == kBytes && kPer > 0, "whole copies of whole rows");
 
     static __device__ __forceinline__ int swizzle(int row) { // of a piece's place in its row
-        if (LAYOUT == kRows) return (row >> 2) & 3;
+        if (LAYOUT == kRows) return ((row >> 1) & 2) ^ ((row >> 3) & 1) * 3;
         return ((row & 3) | ((row >> 1) & 4)) << 1 & (kRowPieces - 1);
     }
 
@@ -200,7 +200,8 @@ template <bool F16> __device__ __forceinline__ lin_f32x4 lin_mfma(lin_s16x8 a, l
 
 // A block's shape.  PAIR: the I tile's halves are two matrices' rows of the same features (a gate
 // and its up), and a wave's first and second half of fragments belong to them.
-template <int TI_, int TJ_, int NWI_, int NWJ_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false> struct Shape {
+template <int TI_, int TJ_, int NWI_, int NWJ_, int RING_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false> struct Shape {
+    static constexpr int kRing = RING_; // steps in LDS
     static constexpr int TI = TI_, TJ = TJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, TH = NW * 64;
     static constexpr int FI = TI / NWI / 16, FJ = TJ / NWJ / 16;
     static constexpr bool F16 = F16_, DIRECT = DIRECT_, PAIR = PAIR_;
@@ -265,16 +266,60 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
     };
     auto read_j = [&](uint32_t buffer, int f) { return rj.get(at + buffer + I::kBytes, f); };
 
-    lin_s16x8 a[2][S::FI], b[2][S::FJ];
-    if constexpr (S::DIRECT) {
+    if constexpr (S::NW == 8) {
+        static_assert(S::DIRECT && S::kRing == 4, "");
+        // Two groups of 4 waves, one of each on a SIMD, half a step apart: while one multiplies, the other reads its
+        // next fragments and starts copies.
+        const bool second = wave >= 4;
+        constexpr int kAhead = 3;
 #pragma unroll
-        for (int i = 0; i < kRing; ++i) {
+        for (int i = 0; i < kAhead; ++i) {
             begin(s0 + i);
 #pragma unroll
             for (int c = 0; c < kCopies; ++c) copy(c, i * S::kBuf);
         }
-        copies_landed<(kRing - 1) * kCopies>();
+        copies_landed<2 * kCopies>();
+        if (second) asm volatile("s_barrier" ::: "memory");
+        uint32_t mine = 0, then = kAhead * S::kBuf;
+        lin_s16x8 a[S::FI], b[S::FJ];
+        for (int t = s0; t < s1; ++t) {
+            begin(t + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < S::FJ; ++f) b[f] = read_j(mine, f);
+#pragma unroll
+            for (int f = 0; f < S::FI; ++f) a[f] = read_i(mine, f);
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) copy(c, then);
+            mine = mine + S::kBuf == S::kLds ? 0 : mine + S::kBuf;
+            then = then + S::kBuf == S::kLds ? 0 : then + S::kBuf;
+            if (second) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * kCopies) : "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            each(b);
+#pragma unroll
+            for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+                for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[fi], b[fj], acc[fi][fj]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            copies_landed<2 * kCopies>();
+        }
+        if (!second) asm volatile("s_barrier" ::: "memory");
+        return;
+    }
+    lin_s16x8 a[2][S::FI], b[2][S::FJ];
+    if constexpr (S::DIRECT) {
+#pragma unroll
+        for (int i = 0; i < S::kRing; ++i) {
+            begin(s0 + i);
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) copy(c, i * S::kBuf);
+        }
+        copies_landed<(S::kRing - 1) * kCopies>();
     } else {
+        static_assert(S::kRing == 4, "what is loaded two steps ahead of its place");
         load(s0, 0), load(s0 + 1, 1);
         store(0, 0), store(S::kBuf, 1);
         load(s0 + 2, 0), load(s0 + 3, 1);
@@ -289,13 +334,13 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
         constexpr int p = decltype(parity)::value;
         const uint32_t next = mine + S::kBuf == S::kLds ? 0 : mine + S::kBuf;
         if constexpr (S::DIRECT) {
-            copies_landed<(kRing - 2) * kCopies>();
-            begin(t + kRing);
+            copies_landed<(S::kRing - 2) * kCopies>();
+            begin(t + S::kRing);
         } else {
             __syncthreads();
             const uint32_t then = mine + 2 * S::kBuf >= S::kLds ? mine + 2 * S::kBuf - S::kLds : mine + 2 * S::kBuf;
             store(then, p);
-            load(t + kRing, p);
+            load(t + 4, p);
         }
         each(b[p]);
         // Parts of the step in order: some reads of the next, some copies, a row of products.
