@@ -3,7 +3,7 @@
 // a tile of each matrix), J the rows, so that a lane ends with 4 consecutive features of a row.
 #include "linear_tiles.h"
 
-#include <algorithm>
+
 
 namespace {
 
@@ -39,8 +39,8 @@ template <bool F16> __device__ __forceinline__ void forward_store(const ForwardA
 }
 
 template <class S>
-__global__ void __launch_bounds__(S::TH, S::kWavesEU)
-linear_kernel(ForwardArgs a, uint32_t nI) {
+__global__ void __launch_bounds__(S::TH, 2)
+linear_kernel(ForwardArgs a, uint32_t nI, Parts parts) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
     constexpr int kN = S::PAIR ? S::TI / 2 : S::TI; // features of a tile
     const Segments seg(a.offsets, a.rows, a.experts, S::TJ);
@@ -48,30 +48,180 @@ linear_kernel(ForwardArgs a, uint32_t nI) {
     if (!tile_of_block(blockIdx.x, nI, seg.tiles, &it, &jt)) return;
     int e, nj;
     seg.find(jt, S::TJ, &e, &m0, &nj);
-    const int n0 = it * kN, ni = min(kN, a.n - n0);
+    const int n0 = it * kN, ni = min(kN, a.n - n0), z = blockIdx.y;
     const TileView iv[2] = {{a.w + e * a.w_stride + (int64_t)n0 * a.w_ld, a.w_ld, ni},
                             {a.u + e * a.u_stride + (int64_t)n0 * a.u_ld, a.u_ld, ni}};
     const TileView jv[1] = {{a.x + (int64_t)m0 * a.x_ld, a.x_ld, nj}};
     lin_f32x4 acc[S::FI][S::FJ] = {};
-    tile_product<S>(iv, jv, a.k, 0, (a.k + kStep - 1) / kStep, lds, acc, [](auto&) {});
+    const int64_t steps = (a.k + S::kStep - 1) / S::kStep;
+    const int s0 = (int)(steps * z / parts.splits), s1 = (int)(steps * (z + 1) / parts.splits);
+    tile_product<S, false>(iv, jv, a.k, s0, s1, turn_of_block(blockIdx.x, s1 - s0, false), lds, acc, [](auto&) {});
     each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 p, lin_f32x4 q) {
-        if (j < nj && i < ni) forward_store<S::F16>(a, e, m0 + j, n0 + i, p, q);
+        if (j >= nj || i >= ni) return;
+        if (parts.splits == 1) {
+            forward_store<S::F16>(a, e, m0 + j, n0 + i, p, q);
+        } else {
+            const int64_t at = (int64_t)(m0 + j) * a.n + n0 + i;
+            store_4<false>(parts.at(z, 0), at, ni - i, true, p);
+            if (S::PAIR) store_4<false>(parts.at(z, 1), at, ni - i, true, q);
+        }
     });
 }
 
+// Behind linear_kernel's parts: a thread takes 4 features of a row.
+template <bool F16>
+__global__ void __launch_bounds__(256)
+linear_finish_kernel(ForwardArgs a, Parts parts) {
+    const uint32_t quads = (a.n + 3) / 4;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)quads * a.rows; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t m = (uint32_t)(i / quads), n = (uint32_t)(i - (uint64_t)m * quads) * 4;
+        const int e = expert_of_row(a.offsets, a.experts, a.rows, m);
+        if (e < 0) continue;
+        const int64_t at = (int64_t)m * a.n + n;
+        const lin_f32x4 p = parts.sum(0, at, a.n - n), q = a.u ? parts.sum(1, at, a.n - n) : p;
+        forward_store<F16>(a, e, m, n, p, q);
+    }
+}
+
+// Few rows an expert: every block takes 32 features (16 of each matrix of a PAIR) and up to 16 FJ rows, its 8 waves every
+// eighth 64 values of the contraction, straight from memory into the MFMA operands, at any address: a lane takes 16
+// contiguous values as two products' (8 lanes x 16 bytes side by side, 64 bytes a row, fetched half lines).  The waves' sums meet in LDS.
+constexpr int kFewWaves = 8, kFewAhead = 2;
+template <bool F16, bool PAIR, int FJ>
+__global__ void __launch_bounds__(64 * kFewWaves)
+linear_few_kernel(ForwardArgs a, uint32_t nI) {
+    __shared__ lin_f32x4 sums[kFewWaves][2 * FJ][64];
+    constexpr int kN = PAIR ? 16 : 32;
+    const Segments seg(a.offsets, a.rows, a.experts, 16 * FJ);
+    // (the row tiles of a weight strip one after the other, on one XCD)
+    const uint64_t total = (uint64_t)nI * seg.tiles, per = (total + 7) / 8, t = blockIdx.x % 8 * per + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= per || t >= total) return;
+    int e, nj;
+    uint32_t m0;
+    seg.find((uint32_t)(t / nI), 16 * FJ, &e, &m0, &nj);
+    const int n0 = (int)(t % nI) * kN, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c0 = 16 * (lane >> 4);
+    // rows that do not exist are read as the last one that does; their products are not stored
+    const uint16_t* wp[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+        const int n = min(n0 + (PAIR ? 0 : 16 * f) + r, a.n - 1);
+        wp[f] = PAIR && f ? a.u + e * a.u_stride + n * a.u_ld + c0 : a.w + e * a.w_stride + n * a.w_ld + c0;
+    }
+    const uint16_t* xp[FJ];
+#pragma unroll
+    for (int f = 0; f < FJ; ++f) xp[f] = a.x + (m0 + min(16 * f + r, nj - 1)) * a.x_ld + c0;
+    lin_f32x4 acc[2][FJ] = {};
+    auto get = [&](const uint16_t* p, int c) {
+        lin_s16x8 v = {};
+        if (c + c0 + 8 <= a.k) {
+            __builtin_memcpy(&v, p + c, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + c0 + j < a.k) v[j] = (short)p[c + j];
+        }
+        return v;
+    };
+    auto product = [&](const lin_s16x8 (&w)[2], const lin_s16x8 (&x)[FJ]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) acc[i][j] = lin_mfma<F16>(w[i], x[j], acc[i][j]);
+    };
+    constexpr int kStride = 64 * kFewWaves;
+    int c = 64 * wave;
+    for (; c + kStride * (kFewAhead - 1) + 64 <= a.k; c += kStride * kFewAhead) {
+        lin_s16x8 w[2 * kFewAhead][2], x[2 * kFewAhead][FJ];
+#pragma unroll
+        for (int u = 0; u < 2 * kFewAhead; ++u) {
+            const int at = c + u / 2 * kStride + u % 2 * 8;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) __builtin_memcpy(&w[u][i], wp[i] + at, 16);
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) __builtin_memcpy(&x[u][j], xp[j] + at, 16);
+        }
+#pragma unroll
+        for (int u = 0; u < 2 * kFewAhead; ++u) product(w[u], x[u]);
+    }
+    for (; c < a.k; c += kStride) {
+        lin_s16x8 w[2][2], x[2][FJ];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[u][i] = get(wp[i], c + 8 * u);
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) x[u][j] = get(xp[j], c + 8 * u);
+        }
+        product(w[0], x[0]), product(w[1], x[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) sums[wave][i * FJ + j][lane] = acc[i][j];
+    __syncthreads();
+    // a wave a fragment of rows, and of features where they are one matrix's
+    constexpr int kParts = PAIR ? FJ : 2 * FJ;
+    for (int f = wave; f < kParts; f += kFewWaves) {
+        lin_f32x4 p = {}, q = {};
+        for (int w = 0; w < kFewWaves; ++w) {
+            p += sums[w][f][lane];
+            if (PAIR) q += sums[w][FJ + f][lane];
+        }
+        const int j = 16 * (f % FJ) + r, n = n0 + 16 * (f / FJ) + 4 * (lane >> 4);
+        if (j < nj && n < a.n) forward_store<F16>(a, e, m0 + j, n, p, q);
+    }
+}
+
 template <class S> int launch(const ForwardArgs& a, hipStream_t st) {
-    constexpr int kN = S::PAIR ? S::TI / 2 : S::TI;
-    const int64_t nI = (a.n + kN - 1) / kN;
-    const int64_t nJ = (int64_t)a.rows / S::TJ + (a.offsets ? std::min<int64_t>(a.experts, a.rows) : a.rows % S::TJ != 0);
+    constexpr int kN = S::PAIR ? S::TI / 2 : S::TI, kPlanes = S::PAIR ? 2 : 1;
+    const int64_t nI = (a.n + kN - 1) / kN, nJ = lin_j_tiles(a.rows, a.experts, a.offsets, S::TJ);
+    const int64_t plane = (int64_t)a.rows * a.n;
+    const int splits = lin_splits(nI * nJ, (a.k + S::kStep - 1) / S::kStep, plane * kPlanes);
     const int64_t blocks = (nI * nJ + 7) / 8 * 8;
-    if (blocks * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED; // a launch's threads
-    linear_kernel<S><<<(unsigned)blocks, S::TH, 0, st>>>(a, (uint32_t)nI);
+    if (blocks * splits * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED; // a launch's threads
+    Parts parts;
+    if (int rc = lin_parts(splits, kPlanes, plane, st, &parts)) return rc;
+    linear_kernel<S><<<dim3((unsigned)blocks, splits), S::TH, 0, st>>>(a, (uint32_t)nI, parts);
+    if (splits > 1) {
+        const unsigned finish = (unsigned)std::min<int64_t>((plane / 4 + a.rows + 255) / 256, 1 << 16);
+        linear_finish_kernel<S::F16><<<finish, 256, 0, st>>>(a, parts);
+    }
+    return naiwa_hip_rc(hipGetLastError());
+}
+template <bool F16, bool PAIR, int FJ> int launch_few(const ForwardArgs& a, hipStream_t st) {
+    constexpr int kN = PAIR ? 16 : 32;
+    const int64_t nI = (a.n + kN - 1) / kN, nJ = lin_j_tiles(a.rows, a.experts, a.offsets, 16 * FJ);
+    const int64_t blocks = (nI * nJ + 7) / 8 * 8;
+    if (blocks * 64 * kFewWaves >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED;
+    linear_few_kernel<F16, PAIR, FJ><<<(unsigned)blocks, 64 * kFewWaves, 0, st>>>(a, (uint32_t)nI);
     return naiwa_hip_rc(hipGetLastError());
 }
 
+// Which kernel a call takes (experts 0: dense).
+enum { kFew16, kFew32, kFew64, kMid, kBig };
+int lin_forward_kind(int64_t rows, int experts, int64_t n, int64_t k, bool pair) {
+    const bool grouped = experts > 0;
+    const int64_t avg = grouped ? rows / experts : rows, bytes = 2 * std::max(experts, 1) * n * k * (pair ? 2 : 1);
+    const int64_t strips = (n + (pair ? 15 : 31)) / (pair ? 16 : 32);
+    // Straight from memory while a strip's rows are one tile's or what more read again is in the caches, and a block a CU takes it.
+    if (bytes <= (16 << 20)) {
+        for (int f = 0; f < 3; ++f)
+            if (strips * lin_j_alike(rows, experts, grouped, 16 << f) <= 256) return kFew16 + f;
+    } else if (avg <= 2 && strips * std::min<int64_t>(std::max(experts, 1), rows) >= 256) {
+        return kFew16;
+    }
+    const int64_t tiles = (n * (pair ? 2 : 1) + 255) / 256 * lin_j_alike(rows, experts, grouped, 256);
+    return lin_big(tiles, (k + 63) / 64, avg) ? kBig : kMid;
+}
+
 template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hipStream_t st) {
-    return direct ? launch<Shape<256, 256, 2, 4, 4, kRows, kRows, F16, true, PAIR>>(a, st)
-                  : launch<Shape<128, 128, 2, 2, 4, kRows, kRows, F16, false, PAIR>>(a, st);
+    const int kind = lin_forward_kind(a.rows, a.offsets ? a.experts : 0, a.n, a.k, PAIR);
+    if (kind == kFew16) return launch_few<F16, PAIR, 1>(a, st);
+    if (kind == kFew32) return launch_few<F16, PAIR, 2>(a, st);
+    if (kind == kFew64) return launch_few<F16, PAIR, 4>(a, st);
+    if (!direct) return launch<Shape<128, 128, 2, 2, kRows, kRows, F16, false, PAIR>>(a, st);
+    return kind == kBig ? launch<Shape<256, 256, 2, 4, kRows, kRows, F16, true, PAIR>>(a, st)
+                     : launch<Shape<128, 128, 2, 2, kRows, kRows, F16, true, PAIR>>(a, st);
 }
 
 // ---- the activation's gradient alone

@@ -6,7 +6,7 @@
 // sum runs over its expert's rows.  The bias gradient is one more product per fragment of dy, with ones.
 #include "linear_tiles.h"
 
-#include <algorithm>
+
 
 namespace {
 
@@ -42,23 +42,39 @@ template <bool F16> __device__ __forceinline__ void input_store(const InputArgs&
     store_4<F16>(a.dx, m * a.dx_ld + k, left, a.dx_f32, g);
 }
 
-template <class S>
-__global__ void __launch_bounds__(S::TH, S::kWavesEU)
-input_grad_kernel(InputArgs a, uint32_t nI) {
+template <class S, bool DUAL>
+__global__ void __launch_bounds__(S::TH, 2)
+input_grad_kernel(InputArgs a, uint32_t nI, Parts parts) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
     const Segments seg(a.offsets, a.rows, a.experts, S::TJ);
     uint32_t it, jt, m0;
     if (!tile_of_block(blockIdx.x, nI, seg.tiles, &it, &jt)) return;
     int e, nj;
     seg.find(jt, S::TJ, &e, &m0, &nj);
-    const int k0 = it * S::TI, ni = min(S::TI, a.k - k0);
+    const int k0 = it * S::TI, ni = min(S::TI, a.k - k0), z = blockIdx.y;
     const TileView iv[2] = {{a.w + e * a.w_stride + k0, a.w_ld, ni}, {a.u + e * a.u_stride + k0, a.u_ld, ni}};
     const TileView jv[2] = {{a.dy + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}, {a.dy_up + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}};
     lin_f32x4 acc[S::FI][S::FJ] = {};
-    tile_product<S>(iv, jv, a.n, 0, (a.n + kStep - 1) / kStep * (a.u ? 2 : 1), lds, acc, [](auto&) {});
+    const int64_t steps = (int64_t)((a.n + S::kStep - 1) / S::kStep) * (DUAL ? 2 : 1);
+    const int s0 = (int)(steps * z / parts.splits), s1 = (int)(steps * (z + 1) / parts.splits);
+    tile_product<S, DUAL>(iv, jv, a.n, s0, s1, turn_of_block(blockIdx.x, s1 - s0, false), lds, acc, [](auto&) {});
     each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 g, lin_f32x4) {
-        if (j < nj && i < ni) input_store<S::F16>(a, m0 + j, k0 + i, g);
+        if (j >= nj || i >= ni) return;
+        if (parts.splits == 1) input_store<S::F16>(a, m0 + j, k0 + i, g);
+        else store_4<false>(parts.at(z, 0), (int64_t)(m0 + j) * a.k + k0 + i, ni - i, true, g);
     });
+}
+
+// Behind its parts: a thread takes 4 values of a row.
+template <bool F16>
+__global__ void __launch_bounds__(256)
+input_finish_kernel(InputArgs a, Parts parts) {
+    const uint32_t quads = (a.k + 3) / 4;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)quads * a.rows; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t m = (uint32_t)(i / quads), k = (uint32_t)(i - (uint64_t)m * quads) * 4;
+        if (expert_of_row(a.offsets, a.experts, a.rows, m) >= 0)
+            input_store<F16>(a, m, k, parts.sum(0, (int64_t)m * a.k + k, a.k - k));
+    }
 }
 
 struct WeightArgs {
@@ -73,23 +89,40 @@ struct WeightArgs {
     bool dw_f32, accumulate;
 };
 
+// 4 values of a weight's row, `left` of them, behind the sum.
+template <bool F16> __device__ __forceinline__ void weight_store(const WeightArgs& a, int e, int n, int k, int left, lin_f32x4 v) {
+    const int64_t at = e * a.stride + n * a.ld + k;
+    if (a.accumulate) v += load_4<F16>(a.dw, at, left, a.dw_f32);
+    store_4<F16>(a.dw, at, left, a.dw_f32, v);
+}
+__device__ __forceinline__ void bias_store(const WeightArgs& a, int e, int n, float v) {
+    float* to = a.dbias + (int64_t)e * a.n + n;
+    *to = v + (a.accumulate ? *to : 0.0f);
+}
+__device__ __forceinline__ void segment_of(const WeightArgs& a, int e, uint32_t* m0, uint32_t* m1) {
+    *m0 = a.offsets ? offset_at(a.offsets, e, a.rows) : 0;
+    *m1 = a.offsets ? max(*m0, offset_at(a.offsets, e + 1, a.rows)) : a.rows;
+}
+
+// parts: plane 0 [experts][n][k]; the bias's parts lie behind all planes, [splits][experts][n].
 template <class S>
-__global__ void __launch_bounds__(S::TH, S::kWavesEU)
-weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ) {
+__global__ void __launch_bounds__(S::TH, 2)
+weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ, Parts parts) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::kLds];
-    uint32_t it, jt;
+    uint32_t it, jt, m0, m1;
     if (!tile_of_block(blockIdx.x, nI, nJ, &it, &jt)) return;
-    const int e = blockIdx.y; // (all XCDs share an expert: with an expert each the calls of uneven ones took 1.4 times as long)
-    uint32_t m0 = 0, m1 = a.rows;
-    if (a.offsets) m0 = offset_at(a.offsets, e, a.rows), m1 = max(m0, offset_at(a.offsets, e + 1, a.rows));
+    const int e = blockIdx.y, z = blockIdx.z; // (all XCDs share an expert: with an expert each, uneven ones took 1.4 times as long)
+    segment_of(a, e, &m0, &m1);
     const int k0 = it * S::TI, ni = min(S::TI, a.k - k0), n0 = jt * S::TJ, nj = min(S::TJ, a.n - n0);
-    const TileView iv[1] = {{a.x + m0 * a.x_ld + k0, a.x_ld, ni}}, jv[1] = {{a.dy + m0 * a.dy_ld + n0, a.dy_ld, nj}};
+    const TileView iv[2] = {{a.x + m0 * a.x_ld + k0, a.x_ld, ni}, {}}, jv[1] = {{a.dy + m0 * a.dy_ld + n0, a.dy_ld, nj}};
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     lin_f32x4 acc[S::FI][S::FJ] = {}, sum[S::FJ] = {};
     const bool bias = a.dbias && it == 0 && S::i_first(wave) == 0; // whose share the bias gradient is
     const short one = S::F16 ? (short)0x3c00 : (short)0x3f80;
     const lin_s16x8 ones = {one, one, one, one, one, one, one, one};
-    tile_product<S>(iv, jv, m1 - m0, 0, (int)((m1 - m0 + kStep - 1) / kStep), lds, acc, [&](auto& b) {
+    const int64_t steps = (m1 - m0 + S::kStep - 1) / S::kStep;
+    const int s0 = (int)(steps * z / parts.splits), s1 = (int)(steps * (z + 1) / parts.splits);
+    tile_product<S, false>(iv, jv, m1 - m0, s0, s1, turn_of_block(blockIdx.x, s1 - s0, true), lds, acc, [&](auto& b) {
         if (bias)
 #pragma unroll
             for (int f = 0; f < S::FJ; ++f) sum[f] = lin_mfma<S::F16>(ones, b[f], sum[f]);
@@ -99,40 +132,86 @@ weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ) {
 #pragma unroll
         for (int fj = 0; fj < S::FJ; ++fj) {
             const int j = S::j_first(wave) + 16 * fj + lane;
-            float* to = a.dbias + (int64_t)e * a.n + n0 + j;
-            if (j < nj) *to = sum[fj][0] + (a.accumulate ? *to : 0.0f);
+            if (j >= nj) continue;
+            if (parts.splits == 1) bias_store(a, e, n0 + j, sum[fj][0]);
+            else parts.at(parts.splits, 0)[((int64_t)z * gridDim.y + e) * a.n + n0 + j] = sum[fj][0];
         }
     }
     each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 v, lin_f32x4) {
         if (j >= nj || i >= ni) return;
-        const int64_t at = e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i;
-        if (a.accumulate) v += load_4<S::F16>(a.dw, at, ni - i, a.dw_f32);
-        store_4<S::F16>(a.dw, at, ni - i, a.dw_f32, v);
+        if (parts.splits == 1) weight_store<S::F16>(a, e, n0 + j, k0 + i, ni - i, v);
+        else store_4<false>(parts.at(z, 0), ((int64_t)e * a.n + n0 + j) * a.k + k0 + i, ni - i, true, v);
     });
 }
 
+// Behind its parts: a thread takes 4 values of a weight's row.
+template <bool F16>
+__global__ void __launch_bounds__(256)
+weight_finish_kernel(WeightArgs a, int experts, Parts parts) {
+    const uint32_t quads = (a.k + 3) / 4;
+    const uint64_t all = (uint64_t)quads * a.n * experts;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+        const uint64_t row = i / quads;
+        const uint32_t k = (uint32_t)(i - row * quads) * 4, e = (uint32_t)(row / a.n), n = (uint32_t)(row - (uint64_t)e * a.n);
+        uint32_t m0, m1;
+        segment_of(a, e, &m0, &m1);
+        if (a.accumulate && m0 == m1) continue;
+        weight_store<F16>(a, e, n, k, a.k - k, parts.sum(0, (int64_t)row * a.k + k, a.k - k));
+        if (a.dbias && k == 0) {
+            float v = 0.0f;
+            for (int z = 0; z < parts.splits; ++z) v += parts.at(parts.splits, 0)[((int64_t)z * experts + e) * a.n + n];
+            bias_store(a, e, n, v);
+        }
+    }
+}
+
 template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
-    const int64_t nI = (a.k + S::TI - 1) / S::TI;
-    const int64_t nJ = (int64_t)a.rows / S::TJ + (a.offsets ? std::min<int64_t>(a.experts, a.rows) : a.rows % S::TJ != 0);
+    const int64_t nI = (a.k + S::TI - 1) / S::TI, nJ = lin_j_tiles(a.rows, a.experts, a.offsets, S::TJ);
+    const int64_t plane = (int64_t)a.rows * a.k;
+    const int splits = lin_splits(nI * nJ, (int64_t)(a.n + S::kStep - 1) / S::kStep * (a.u ? 2 : 1), plane);
     const int64_t blocks = (nI * nJ + 7) / 8 * 8;
-    if (blocks * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED; // a launch's threads
-    input_grad_kernel<S><<<(unsigned)blocks, S::TH, 0, st>>>(a, (uint32_t)nI);
+    if (blocks * splits * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED; // a launch's threads
+    Parts parts;
+    if (int rc = lin_parts(splits, 1, plane, st, &parts)) return rc;
+    const dim3 grid((unsigned)blocks, splits);
+    if (a.u) input_grad_kernel<S, true><<<grid, S::TH, 0, st>>>(a, (uint32_t)nI, parts);
+    else input_grad_kernel<S, false><<<grid, S::TH, 0, st>>>(a, (uint32_t)nI, parts);
+    if (splits > 1) {
+        const unsigned finish = (unsigned)std::min<int64_t>((plane / 4 + a.rows + 255) / 256, 1 << 16);
+        input_finish_kernel<S::F16><<<finish, 256, 0, st>>>(a, parts);
+    }
     return naiwa_hip_rc(hipGetLastError());
 }
 template <bool F16> int input_grad(const InputArgs& a, bool direct, hipStream_t st) {
-    return direct ? launch_input<Shape<256, 256, 2, 4, 4, kCols, kRows, F16, true>>(a, st)
-                  : launch_input<Shape<128, 128, 2, 2, 4, kCols, kRows, F16, false>>(a, st);
+    const int64_t tiles = (int64_t)((a.k + 255) / 256) * lin_j_alike(a.rows, a.experts, a.offsets, 256);
+    const bool big = lin_big(tiles, (int64_t)(a.n + 63) / 64 * (a.u ? 2 : 1), a.rows / (a.offsets ? a.experts : 1));
+    if (!direct) return launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, false>>(a, st);
+    return big ? launch_input<Shape<256, 256, 2, 4, kCols, kRows, F16, true>>(a, st)
+                     : launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, true>>(a, st);
 }
 
 template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream_t st) {
-    const int64_t nI = (a.k + S::TI - 1) / S::TI, nJ = (a.n + S::TJ - 1) / S::TJ, blocks = (nI * nJ + 7) / 8 * 8;
-    if (blocks * experts * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED;
-    weight_grad_kernel<S><<<dim3((unsigned)blocks, experts), S::TH, 0, st>>>(a, (uint32_t)nI, (uint32_t)nJ);
+    const int64_t nI = (a.k + S::TI - 1) / S::TI, nJ = (a.n + S::TJ - 1) / S::TJ;
+    const int64_t plane = (int64_t)experts * a.n * a.k, bias = a.dbias ? (int64_t)experts * a.n : 0;
+    const int splits = lin_splits(nI * nJ * experts, a.rows / experts / S::kStep, plane + bias);
+    const int64_t blocks = (nI * nJ + 7) / 8 * 8;
+    if (blocks * experts * splits * S::TH >= (int64_t)1 << 32) return NAIWA_E_UNSUPPORTED;
+    Parts parts;
+    if (int rc = lin_parts(splits, 1, plane + bias, st, &parts)) return rc;
+    parts.plane = plane; // (the bias's parts behind the planes)
+    weight_grad_kernel<S><<<dim3((unsigned)blocks, experts, splits), S::TH, 0, st>>>(a, (uint32_t)nI, (uint32_t)nJ, parts);
+    if (splits > 1) {
+        const int64_t quads = (int64_t)(a.k + 3) / 4 * a.n * experts;
+        weight_finish_kernel<S::F16><<<(unsigned)std::min<int64_t>((quads + 255) / 256, 1 << 16), 256, 0, st>>>(a, experts, parts);
+    }
     return naiwa_hip_rc(hipGetLastError());
 }
 template <bool F16> int weight_grad(const WeightArgs& a, int experts, bool direct, hipStream_t st) {
-    return direct ? launch_weight<Shape<256, 256, 2, 4, 4, kCols, kCols, F16, true>>(a, experts, st)
-                  : launch_weight<Shape<128, 128, 2, 2, 4, kCols, kCols, F16, false>>(a, experts, st);
+    const int64_t tiles = (int64_t)experts * ((a.k + 255) / 256) * ((a.n + 255) / 256);
+    const bool big = lin_big(tiles, a.rows / experts / 64 + 1, 64);
+    if (!direct) return launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, false>>(a, experts, st);
+    return big ? launch_weight<Shape<256, 256, 2, 4, kCols, kCols, F16, true>>(a, experts, st)
+                     : launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, true>>(a, experts, st);
 }
 
 } // namespace

@@ -6,17 +6,24 @@
 // holds 4 consecutive i of one j, so i is the index that is contiguous in the output: the
 // weights' features forward, the input's in both gradients.
 //
-// Steps of 32 contraction values lie in a ring of 4 LDS buffers, copied from memory without passing
-// registers (16 bytes a lane).  In step t a wave multiplies what it read of step t, reads step t + 1 and starts the
-// copies of step t + 4 into the buffer that step t left, all three interleaved; one barrier a step says
-// that step t + 1 has landed and step t's buffer is free.  Buffer ranges make what lies behind a segment's last
-// row zero, lanes behind the last of c ask for an address out of range, and so do steps behind the last
-// (the ring's counted waits stay the same to the end).  Both layouts keep 16-byte pieces whole and
-// permute them so that no two lanes of a read share a bank:
-//   contiguous: row r of 32 values, piece q at r * 64 + 16 (q ^ g), g = 0, 2, 3, 1 for rows in fours; 16-byte reads, of
-//               which the LDS takes lanes 0-3, 12-15, 20-27 at a time, then 4-11, 16-19, 28-31, and so on;
-//   row index:  row c of T values, the pair of pieces f (16 values) at 32 (f ^ s(c)), s(c) = c & 3 | (c >> 3 & 1)
-//               << 2, read by the transposing LDS read (4 rows x 16 values a group of 16 lanes).
+// Steps of the contraction lie in LDS several times over: while one is read, others land, copied from memory
+// without passing registers (16 bytes a lane).  Buffer ranges make what lies behind a segment's last row zero, lanes
+// behind the last of c ask for an address out of range, and so do steps behind the last (the counted
+// waits stay the same to the end).  Two kinds of block:
+//   8 waves, 256 x 256, steps of 64, all of a CU's LDS.  The waves are two groups, one wave of each on a SIMD, that
+//     take turns in reading and multiplying (setprio and a barrier a phase).  What bounds it is how fast rows come out of
+//     L2 (with the copies left out 4096 x 4096 x 14336 takes 233 us, without the products 377): hence whole 128-byte
+//     lines, three buffers of I and two of J, and copies spread over the phases.
+//   4 waves, 128 x 128, steps of 32 in a ring of 4, two blocks a CU: in step t a wave multiplies what it read of
+//     step t, reads step t + 1 and starts the copies of step t + 4, interleaved; one barrier a step.
+// The XCDs begin at different steps and go round (turn_of_block): reading the same columns at a time they meet at
+// the same memory channels (4096 x 4096 x 14336 403 -> 389 us, the weights' gradient of 64 experts 332 -> 286).
+// Both layouts keep 16-byte pieces whole and permute them so that no two lanes of a read share a bank (the LDS takes
+// lanes 0-3, 12-15, 20-27 of a 16-byte read at a time, then 4-11, 16-19, 28-31, and so on):
+//   contiguous: row r, piece q at place q ^ (r & 6) of its row of 64 values, of one of 32 at q ^ g with g = 0, 2, 3, 1 for
+//     rows in fours;
+//   row index: row c of T values, the pair of pieces f (16 values) at 32 (f ^ s(c)), s(c) = c & 3 | (c >> 3 & 1)
+//     << 2, read by the transposing LDS read (4 rows x 16 values a group of 16 lanes).
 // Operands that are not multiples of 16 bytes pass through registers two steps ahead, value by value at their ends.
 // At the end the accumulators go through LDS once more, so that what follows the product works on rows:
 // whole lines of memory, and code that is there once.
@@ -24,7 +31,9 @@
 
 #include "../../include/naiwa_linear.h"
 #include "common.h"
+#include "workspace.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -36,8 +45,9 @@ typedef _Float16 lin_f16x8 __attribute__((ext_vector_type(8)));
 typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
 typedef short lin_s16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kStep = 32;           // contraction values of a step
 constexpr uint32_t kFar = 1u << 31; // an offset past every range
+
+constexpr int kRing = 4; // steps in LDS of the 4-wave shapes
 
 enum { kRows = 0, kCols = 1 }; // the contraction index is contiguous, or the row index
 
@@ -47,6 +57,9 @@ struct TileView {
     int64_t ld;           // values between rows
     int valid;            // the tile's rows (kRows) or columns (kCols) that exist
 };
+__device__ __forceinline__ TileView pick(bool second, const TileView& a, const TileView& b) {
+    return {second ? b.base : a.base, second ? b.ld : a.ld, second ? b.valid : a.valid};
+}
 
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
@@ -72,18 +85,18 @@ template <int N> __device__ __forceinline__ void copies_landed() {
 
 // One operand of T rows (or columns), loaded by NW waves.  PAIR (kRows): the second half of its rows are
 // those of a second view.
-template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
+template <int T, int LAYOUT, int NW, bool PAIR, int STEP> struct Tile {
     static_assert(!PAIR || (LAYOUT == kRows && NW % 2 == 0), "whole waves a half");
-    static constexpr int kBytes = T * kStep * 2;
+    static constexpr int kBytes = T * STEP * 2;
     static constexpr int kLanes = kBytes / NW / 16 < 64 ? kBytes / NW / 16 : 64; // that take part in a copy
     static constexpr int kCopies = kBytes / NW / 16 / kLanes;                    // a wave's
     static constexpr int kPieces = (kBytes / 16 + NW * 64 - 1) / (NW * 64);      // a thread's, through registers
-    static constexpr int kRowPieces = LAYOUT == kRows ? kStep / 8 : T / 8;       // pieces of a row in LDS
+    static constexpr int kRowPieces = LAYOUT == kRows ? STEP / 8 : T / 8;       // pieces of a row in LDS
     static constexpr int kPer = kLanes / kRowPieces;                             // rows of a copy
     static_assert(kCopies * kLanes * 16 * NW == kBytes && kPer > 0, "whole copies of whole rows");
 
     static __device__ __forceinline__ int swizzle(int row) { // of a piece's place in its row
-        if (LAYOUT == kRows) return ((row >> 1) & 2) ^ ((row >> 3) & 1) * 3;
+        if (LAYOUT == kRows) return STEP == 64 ? row & 6 : ((row >> 1) & 2) ^ ((row >> 3) & 1) * 3;
         return ((row & 3) | ((row >> 1) & 4)) << 1 & (kRowPieces - 1);
     }
 
@@ -91,15 +104,15 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
     struct Copier {
         uint32_t off[kCopies]; // of the lane's pieces, from the step's first value
         uint32_t lds;          // of the wave's part of the first buffer
-        int piece;             // of its row (kRows; the same in all of a wave's copies, 16 rows or one apart)
+        int piece;             // of its row (kRows: the same in all of a wave's copies)
         bool in;
         __device__ __forceinline__ Copier(uint32_t at, int wave, int lane) : in(lane < kLanes) {
             lds = __builtin_amdgcn_readfirstlane(at + wave * (kBytes / NW));
         }
-        // At views with rows so far apart.
-        __device__ __forceinline__ void aim(const TileView* views, int wave, int lane) {
+        // At the wave's view: rows so far apart.
+        __device__ __forceinline__ void aim(const TileView& v, int wave, int lane) {
             const bool second = PAIR && wave >= NW / 2;
-            const uint32_t ld2 = (uint32_t)(second ? views[1].ld : views[0].ld) * 2;
+            const uint32_t ld2 = (uint32_t)v.ld * 2;
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
                 const int r = (wave * kCopies + i) * kPer + lane / kRowPieces; // (rows of a PAIR's second half from its view's own first)
@@ -110,8 +123,7 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
         lin_u32x4 range;
         bool far;
         // The step of contraction values c0 .. c0 + 31 of C (none if c0 >= C).
-        __device__ __forceinline__ void begin(const TileView* views, int64_t c0, int64_t C, int wave, int lane) {
-            const TileView v = PAIR && wave >= NW / 2 ? views[1] : views[0];
+        __device__ __forceinline__ void begin(const TileView& v, int64_t c0, int64_t C) {
             const int64_t left = C - c0;
             if constexpr (LAYOUT == kRows) {
                 range = range_of(v.base + c0, left > 0 && v.valid > 0 ? ((v.valid - 1) * v.ld + left) * 2 : 0);
@@ -130,17 +142,21 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
     struct Held {
         lin_u32x4 v[kPieces];
     };
+    static __device__ __forceinline__ void load(const TileView& one, int64_t c0, int64_t C, int tid, Held& h) {
+        const TileView both[2] = {one, one};
+        load(both, c0, C, tid, h);
+    }
     static __device__ __forceinline__ void load(const TileView* views, int64_t c0, int64_t C, int tid, Held& h) {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int p = tid + i * NW * 64, at = p % kRowPieces * 8;
             int row = p / kRowPieces;
             const bool second = PAIR && row >= T / 2;
-            const TileView v = second ? views[1] : views[0];
+            const TileView v = pick(second, views[0], views[1]);
             if (second) row -= T / 2;
             // LDS row `row`, values at .. at + 7 of it, of which `left` exist
             const int64_t left = LAYOUT == kRows ? C - c0 - at : v.valid - at;
-            const bool in = LAYOUT == kRows ? row < v.valid : row < C - c0 && row < kStep;
+            const bool in = LAYOUT == kRows ? row < v.valid : row < C - c0 && row < STEP;
             const uint16_t* s = LAYOUT == kRows ? v.base + row * v.ld + c0 + at : v.base + (c0 + row) * v.ld + at;
             lin_u32x4 w = {};
             if (in && left >= 8) {
@@ -163,11 +179,13 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
 
     // ---- fragments: F of 16 rows (columns) from `first` on
     template <int F> struct Reader {
-        uint32_t at[LAYOUT == kRows ? 1 : F];
-        // frag f is rows first + 16 f + lane % 16, c = 8 (lane / 16) + 0 .. 7
+        uint32_t at[LAYOUT == kRows ? STEP / 32 : F];
+        // frag f is rows first + 16 f + lane % 16, c = 32 h + 8 (lane / 16) + 0 .. 7
         __device__ __forceinline__ Reader(int first, int lane) {
             if constexpr (LAYOUT == kRows) {
-                at[0] = (uint32_t)(first + (lane & 15)) * 64 + (((lane >> 4) ^ swizzle(lane & 15)) << 4);
+#pragma unroll
+                for (int h = 0; h < STEP / 32; ++h)
+                    at[h] = (uint32_t)(first + (lane & 15)) * (STEP * 2) + ((((lane >> 4) + 4 * h) ^ swizzle(lane & 15)) << 4);
             } else {
                 const int row = 8 * (lane >> 4) + ((lane & 15) >> 2);
 #pragma unroll
@@ -176,13 +194,13 @@ template <int T, int LAYOUT, int NW, bool PAIR> struct Tile {
             }
         }
         // buf: the step's LDS address
-        __device__ __forceinline__ lin_s16x8 get(uint32_t buf, int f) const {
+        __device__ __forceinline__ lin_s16x8 get(uint32_t buf, int f, int h) const {
             typedef __attribute__((address_space(3))) const lin_s16x8* P8;
             typedef __attribute__((address_space(3))) lin_s16x4* P4;
             if constexpr (LAYOUT == kRows) {
-                return *(P8)(uintptr_t)(buf + at[0] + f * 1024);
+                return *(P8)(uintptr_t)(buf + at[h] + f * (STEP * 32));
             } else {
-                const uint32_t a = buf + at[f];
+                const uint32_t a = buf + at[f] + h * (32 * T * 2);
                 const lin_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)a);
                 const lin_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P4)(uintptr_t)(a + 4 * T * 2));
                 return lin_s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -198,31 +216,31 @@ template <bool F16> __device__ __forceinline__ lin_f32x4 lin_mfma(lin_s16x8 a, l
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8, a), __builtin_bit_cast(lin_bf16x8, b), c, 0, 0, 0);
 }
 
-// A block's shape.  PAIR: the I tile's halves are two matrices' rows of the same features (a gate
+// A block's shape: 8 waves and a tile that fills a CU's LDS, or 4 waves and half as much.  PAIR: the I tile's halves are two matrices' rows of the same features (a gate
 // and its up), and a wave's first and second half of fragments belong to them.
-template <int TI_, int TJ_, int NWI_, int NWJ_, int RING_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false> struct Shape {
-    static constexpr int kRing = RING_; // steps in LDS
+template <int TI_, int TJ_, int NWI_, int NWJ_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false> struct Shape {
     static constexpr int TI = TI_, TJ = TJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, TH = NW * 64;
     static constexpr int FI = TI / NWI / 16, FJ = TJ / NWJ / 16;
     static constexpr bool F16 = F16_, DIRECT = DIRECT_, PAIR = PAIR_;
-    static constexpr int kWavesEU = FI * FJ > 32 ? 1 : 2; // waves of a SIMD, by their accumulators
-    typedef Tile<TI, LI_, NW, PAIR_> I;
-    typedef Tile<TJ, LJ_, NW, false> J;
+    static constexpr int kStep = NW == 8 ? 64 : 32; // contraction values of a step
+    typedef Tile<TI, LI_, NW, PAIR_, kStep> I;
+    typedef Tile<TJ, LJ_, NW, false, kStep> J;
     static constexpr int kBuf = I::kBytes + J::kBytes;
-    static constexpr int kLds = kRing * kBuf;
+    static constexpr int kLds = NW == 8 ? 3 * I::kBytes + 2 * J::kBytes : kRing * kBuf;
     static constexpr int kWaveI = TI / NWI, kWaveJ = TJ / NWJ;
     // The wave's first I row (fragments of a PAIR: f < FI / 2 from here, the others TI / 2 on).
     static __device__ __forceinline__ int i_first(int wave) { return wave % NWI * kWaveI / (PAIR ? 2 : 1); }
     static __device__ __forceinline__ int j_first(int wave) { return wave / NWI * kWaveJ; }
 };
 
-// acc[fi][fj] += the tile's product over steps s0 .. s1 - 1 of `sources` contraction ranges of C each: iv[0] and jv[0],
-// then iv[1] and jv[1].  (A PAIR has one range, and iv[0], iv[1] are the matrices of its halves.)  each(b) is
+// acc[fi][fj] += the tile's product over steps s0 .. s1 - 1 of one contraction range of C, or two (DUAL): iv[0] and jv[0],
+// then iv[1] and jv[1], beginning `turn` steps behind s0 and going round.  (A PAIR has one range, and iv[0], iv[1] are the matrices of its halves.)  each(b) is
 // called with every step's J fragments.
-template <class S, class Each>
-__device__ __forceinline__ void tile_product(const TileView* iv, const TileView* jv, int64_t C, int s0, int s1, uint8_t* lds,
+template <class S, bool DUAL, class Each>
+__device__ __forceinline__ void tile_product(const TileView* iv, const TileView* jv, int64_t C, int s0, int s1, int turn, uint8_t* lds,
                                              lin_f32x4 (&acc)[S::FI][S::FJ], Each each) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int kStep = S::kStep;
     const int per = (int)((C + kStep - 1) / kStep);
     const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(lds));
     typedef typename S::I I;
@@ -231,80 +249,101 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
     const typename I::template Reader<S::PAIR ? S::FI / 2 : S::FI> ri(S::i_first(wave), lane);
     const typename J::template Reader<S::FJ> rj(S::j_first(wave), lane);
     typename I::Copier ci(at, wave, lane);
-    typename J::Copier cj(at + I::kBytes, wave, lane);
+    typename J::Copier cj(at + (S::NW == 8 ? 3 : 1) * I::kBytes, wave, lane);
     typename I::Held hi[2];
     typename J::Held hj[2];
-    auto source = [&](int step, int64_t* c0) { // (of a PAIR always 0)
-        const int s = step >= per && !S::PAIR ? 1 : 0;
-        *c0 = step < s1 ? (int64_t)(step - s * per) * kStep : C;
-        return s;
+    if (s1 > s0) turn %= s1 - s0;
+    // Step `step`'s first contraction value (C behind the last), and whether it is of the second range.
+    auto source = [&](int step, int64_t* c0) {
+        const int u = step + turn < s1 ? step + turn : step + turn - (s1 - s0);
+        const bool second = DUAL && u >= per;
+        *c0 = step < s1 ? (int64_t)(second ? u - per : u) * kStep : C;
+        return second;
     };
-    auto begin = [&](int step) {
+    bool at_i = false, at_j = false; // which range the copies are aimed at
+    auto begin_i = [&](int step) {
         int64_t c0;
-        const int s = source(step, &c0);
-        if (step == s0 || (step == per && step < s1 && !S::PAIR)) {
-            ci.aim(S::PAIR || !s ? iv : iv + 1, wave, lane);
-            cj.aim(s ? jv + 1 : jv, wave, lane);
-        }
-        ci.begin(S::PAIR || !s ? iv : iv + 1, c0, C, wave, lane);
-        cj.begin(s ? jv + 1 : jv, c0, C, wave, lane);
+        const bool second = source(step, &c0);
+        const TileView v = pick(S::PAIR ? wave >= S::NW / 2 : second, iv[0], iv[1]);
+        if (step == s0 || (DUAL && second != at_i)) ci.aim(v, wave, lane), at_i = second;
+        ci.begin(v, c0, C);
     };
+    auto begin_j = [&](int step) {
+        int64_t c0;
+        const bool second = source(step, &c0);
+        const TileView v = DUAL ? pick(second, jv[0], jv[1]) : jv[0];
+        if (step == s0 || (DUAL && second != at_j)) cj.aim(v, wave, lane), at_j = second;
+        cj.begin(v, c0, C);
+    };
+    auto begin = [&](int step) { begin_i(step), begin_j(step); };
     auto copy = [&](int i, uint32_t buffer) { i < I::kCopies ? ci.one(i, buffer) : cj.one(i - I::kCopies, buffer); };
     auto load = [&](int step, int p) {
         int64_t c0;
-        const int s = source(step, &c0);
-        I::load(S::PAIR || !s ? iv : iv + 1, c0, C, tid, hi[p]);
-        J::load(s ? jv + 1 : jv, c0, C, tid, hj[p]);
+        const bool second = source(step, &c0);
+        const TileView i[2] = {pick(second, iv[0], iv[1]), iv[1]};
+        I::load(S::PAIR ? iv : i, c0, C, tid, hi[p]);
+        J::load(DUAL ? pick(second, jv[0], jv[1]) : jv[0], c0, C, tid, hj[p]);
     };
     auto store = [&](uint32_t buffer, int p) {
         I::store(hi[p], lds + buffer, tid);
         J::store(hj[p], lds + buffer + I::kBytes, tid);
     };
-    auto read_i = [&](uint32_t buffer, int f) {
-        if (S::PAIR && f >= S::FI / 2) return ri.get(at + buffer + S::TI / 2 * (kStep * 2), f - S::FI / 2); // (a PAIR's I is kRows)
-        return ri.get(at + buffer, f);
+    auto read_i = [&](uint32_t buffer, int f, int h = 0) {
+        if (S::PAIR && f >= S::FI / 2) return ri.get(at + buffer + S::TI / 2 * (kStep * 2), f - S::FI / 2, h); // (a PAIR's I is kRows)
+        return ri.get(at + buffer, f, h);
     };
-    auto read_j = [&](uint32_t buffer, int f) { return rj.get(at + buffer + I::kBytes, f); };
+    auto read_j = [&](uint32_t buffer, int f, int h = 0) { return rj.get(at + buffer + I::kBytes, f, h); };
 
     if constexpr (S::NW == 8) {
-        static_assert(S::DIRECT && S::kRing == 4, "");
-        // Two groups of 4 waves, one of each on a SIMD, half a step apart: while one multiplies, the other reads its
-        // next fragments and starts copies.
+        static_assert(S::DIRECT, "");
+        // Two groups of 4 waves, one wave of each on a SIMD, a phase apart: while one reads half a step, the other
+        // multiplies one.  A step's copies begin when both groups have read what lies there: J's a step ahead (three
+        // phases to land), I's two steps ahead, as far as LDS reaches.
         const bool second = wave >= 4;
-        constexpr int kAhead = 3;
+        begin_i(s0), begin_j(s0);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            begin(s0 + i);
+        for (int c = 0; c < J::kCopies; ++c) cj.one(c, 0);
 #pragma unroll
-            for (int c = 0; c < kCopies; ++c) copy(c, i * S::kBuf);
-        }
-        copies_landed<2 * kCopies>();
+        for (int c = 0; c < I::kCopies; ++c) ci.one(c, 0);
+        begin_i(s0 + 1);
+#pragma unroll
+        for (int c = 0; c < I::kCopies; ++c) ci.one(c, I::kBytes);
+        copies_landed<I::kCopies>();
         if (second) asm volatile("s_barrier" ::: "memory");
-        uint32_t mine = 0, then = kAhead * S::kBuf;
+        uint32_t mi = 0, mj = 0, then = 2 * I::kBytes;
         lin_s16x8 a[S::FI], b[S::FJ];
         for (int t = s0; t < s1; ++t) {
-            begin(t + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
+            begin_j(t + 1);
+            begin_i(t + 2);
 #pragma unroll
-            for (int f = 0; f < S::FJ; ++f) b[f] = read_j(mine, f);
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int f = 0; f < S::FI; ++f) a[f] = read_i(mine, f);
+                for (int f = 0; f < S::FJ; ++f) b[f] = rj.get(at + 3 * I::kBytes + mj, f, h);
 #pragma unroll
-            for (int c = 0; c < kCopies; ++c) copy(c, then);
-            mine = mine + S::kBuf == S::kLds ? 0 : mine + S::kBuf;
-            then = then + S::kBuf == S::kLds ? 0 : then + S::kBuf;
-            if (second) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * kCopies) : "memory");
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_setprio(1);
-            each(b);
+                for (int f = 0; f < S::FI; ++f) a[f] = read_i(mi, f, h);
+                if (h == 0) {
 #pragma unroll
-            for (int fi = 0; fi < S::FI; ++fi)
+                    for (int c = 0; c < J::kCopies; ++c) cj.one(c, J::kBytes - mj);
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                } else {
 #pragma unroll
-                for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[fi], b[fj], acc[fi][fj]);
-            __builtin_amdgcn_s_setprio(0);
-            __builtin_amdgcn_sched_barrier(0);
-            copies_landed<2 * kCopies>();
+                    for (int c = 0; c < I::kCopies; ++c) ci.one(c, then);
+                    copies_landed<I::kCopies>(); // (of the next step)
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                each(b);
+#pragma unroll
+                for (int fi = 0; fi < S::FI; ++fi)
+#pragma unroll
+                    for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[fi], b[fj], acc[fi][fj]);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("s_barrier" ::: "memory");
+            }
+            mi = mi == 2 * I::kBytes ? 0 : mi + I::kBytes;
+            then = then == 2 * I::kBytes ? 0 : then + I::kBytes;
+            mj = J::kBytes - mj;
         }
         if (!second) asm volatile("s_barrier" ::: "memory");
         return;
@@ -312,14 +351,13 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
     lin_s16x8 a[2][S::FI], b[2][S::FJ];
     if constexpr (S::DIRECT) {
 #pragma unroll
-        for (int i = 0; i < S::kRing; ++i) {
+        for (int i = 0; i < kRing; ++i) {
             begin(s0 + i);
 #pragma unroll
             for (int c = 0; c < kCopies; ++c) copy(c, i * S::kBuf);
         }
-        copies_landed<(S::kRing - 1) * kCopies>();
+        copies_landed<(kRing - 1) * kCopies>();
     } else {
-        static_assert(S::kRing == 4, "what is loaded two steps ahead of its place");
         load(s0, 0), load(s0 + 1, 1);
         store(0, 0), store(S::kBuf, 1);
         load(s0 + 2, 0), load(s0 + 3, 1);
@@ -334,13 +372,13 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
         constexpr int p = decltype(parity)::value;
         const uint32_t next = mine + S::kBuf == S::kLds ? 0 : mine + S::kBuf;
         if constexpr (S::DIRECT) {
-            copies_landed<(S::kRing - 2) * kCopies>();
-            begin(t + S::kRing);
+            copies_landed<(kRing - 2) * kCopies>();
+            begin(t + kRing);
         } else {
             __syncthreads();
             const uint32_t then = mine + 2 * S::kBuf >= S::kLds ? mine + 2 * S::kBuf - S::kLds : mine + 2 * S::kBuf;
             store(then, p);
-            load(t + 4, p);
+            load(t + kRing, p);
         }
         each(b[p]);
         // Parts of the step in order: some reads of the next, some copies, a row of products.
@@ -473,6 +511,11 @@ __device__ __forceinline__ bool tile_of_block(uint32_t b, uint32_t nI, uint32_t 
     return true;
 }
 
+// Where a block begins a contraction of so many steps, its XCD's blocks alike or each a step on.
+__device__ __forceinline__ int turn_of_block(uint32_t b, int steps, bool apart) {
+    return (int)((b % 8) * (uint32_t)steps / 8 + (apart ? b / 8 % 8 : 0));
+}
+
 // ---- values -----------------------------------------------------------------------------
 
 template <bool F16> __device__ __forceinline__ float lin_get(uint16_t v) { return F16 ? naiwa_f16_to_f32(v) : naiwa_bf16_to_f32(v); }
@@ -547,6 +590,34 @@ __device__ __forceinline__ void lin_act_slope(int act, float v, float* a, float*
     }
 }
 
+// ---- sums in parts ----------------------------------------------------------------------
+
+// Where a call has few tiles and long sums, `splits` blocks take a tile, each a part of its steps, and leave f32 sums in
+// scratch: part z's of plane p (a PAIR has two) [rows][width].  A second launch adds the parts up in their order.
+struct Parts {
+    float* p;
+    int splits, planes;
+    int64_t plane; // values of one
+    __device__ __forceinline__ float* at(int z, int q) const { return p + ((int64_t)z * planes + q) * plane; }
+    __device__ __forceinline__ lin_f32x4 sum(int q, int64_t i, int n) const {
+        lin_f32x4 v = {};
+        for (int z = 0; z < splits; ++z) v += load_4<false>(at(z, q), i, n, true);
+        return v;
+    }
+};
+
+// The expert whose rows hold m (at most `rows` rows): -1 if none.
+__device__ __forceinline__ int expert_of_row(const uint32_t* offsets, int experts, uint32_t rows, uint32_t m) {
+    if (!offsets) return 0;
+    int lo = 0, hi = experts; // the last e with offsets[e] <= m
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (offset_at(offsets, mid, rows) <= m) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo < experts && offset_at(offsets, lo, rows) <= m && m < offset_at(offsets, lo + 1, rows) ? lo : -1;
+}
+
 // ---- host -------------------------------------------------------------------------------
 
 constexpr int64_t kMaxLd = 1 << 21;
@@ -561,6 +632,34 @@ static inline bool lin_overlap(const void* a, int64_t a_bytes, const void* b, in
 }
 static inline int64_t lin_span(int64_t rows, int64_t ld, int64_t n, int size) { return rows > 0 ? ((rows - 1) * ld + n) * size : 0; }
 static inline int lin_size(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
+// How many blocks take a tile of `steps` steps in a call of `tiles` tiles whose sums are `values` f32 values: a block a CU, 8
+// steps at least each, and at most 64 MB of sums.  (One block a tile, 16 rows x 88 x 728 and 1 x 128 x 3424 took 28 and 38 us, a
+// step's latency each.  Two blocks a CU or 4 steps were as fast or up to 20 % slower, but for long contractions of few rows:
+// 25 against 32 us for the input gradient of 16 rows x 4096 x 14336.)
+static inline int lin_splits(int64_t tiles, int64_t steps, int64_t values) {
+    const int64_t s = std::min<int64_t>({256 / std::max<int64_t>(tiles, 1), steps / 8, 64, (16 << 20) / std::max<int64_t>(values, 1)});
+    return s < 2 ? 1 : (int)s;
+}
+static inline int lin_parts(int splits, int planes, int64_t plane, hipStream_t st, Parts* p) {
+    *p = Parts{nullptr, splits, planes, plane};
+    if (splits == 1) return NAIWA_OK;
+    int rc = 0;
+    p->p = (float*)naiwa_scratch(NAIWA_SCRATCH_LINEAR, (size_t)splits * planes * plane * 4, &rc, st);
+    return p->p ? NAIWA_OK : rc;
+}
+// Whether a call takes 256 x 256 tiles: `tiles` of them of `steps` 64-value steps, `rows` a segment on average (few leave
+// most of a tile empty).  128 and 256 wide, us: 1024 rows x 2048 x 2048 25 and 31, 4096 48 and 52, 512 rows x 4096 x 14336 91 and
+// 70, 2048 277 and 188; gated, 64 experts of 1408 x 2048 with 64 rows each 179 and 181, 96 201 and 189, 512 590 and 444; weight
+// gradients of 2048 x 2048 from 2048 rows 35 and 42, 4096 62 and 55.
+static inline bool lin_big(int64_t tiles, int64_t steps, int64_t rows) { return tiles * steps >= 3500 && rows >= 64; }
+// J tiles of `tile` rows that segments of `rows` rows have in all, if they are alike.
+static inline int64_t lin_j_alike(int64_t rows, int experts, bool grouped, int tile) {
+    return grouped ? std::max<int64_t>(std::min<int64_t>(experts, rows), rows / tile) : (rows + tile - 1) / tile;
+}
+// J tiles of `tile` rows that segments of `rows` rows may have.
+static inline int64_t lin_j_tiles(int64_t rows, int experts, bool grouped, int tile) {
+    return grouped ? rows / tile + std::min<int64_t>(experts, rows) : (rows + tile - 1) / tile;
+}
 static inline bool lin_act_ok(int act) {
     return act == NAIWA_ACT_NONE || act == NAIWA_ACT_SILU || act == NAIWA_ACT_GELU_PYTORCH_TANH;
 }

@@ -41,5 +41,6 @@ enum {
     NAIWA_SCRATCH_PREFILL = 7,
     NAIWA_SCRATCH_BALANCE = 8, // partial sums of the balance loss
     NAIWA_SCRATCH_SORT = 9,    // counts of longer sorts by expert
-    NAIWA_SCRATCH_TAGS = 10
+    NAIWA_SCRATCH_LINEAR = 10, // partial sums of products with few tiles
+    NAIWA_SCRATCH_TAGS = 11
 };
