@@ -21,22 +21,46 @@ struct ForwardArgs {
     bool out_f32;
 };
 
-// 4 features of a row, n .. n + 3 (`left` of them exist), behind the product.
-template <bool F16> __device__ __forceinline__ void forward_store(const ForwardArgs& a, int e, uint32_t m, int n, lin_f32x4 p, lin_f32x4 q) {
-    const int left = a.n - n;
-    if (a.b) p += load_4<F16>(a.b, (int64_t)e * a.n + n, left, true);
-    if (a.pre) store_4<F16>(a.pre, m * a.pre_ld + n, left, false, p);
-    lin_f32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = lin_act(a.act, p[i]);
-    if (a.u) {
-        if (a.c) q += load_4<F16>(a.c, (int64_t)e * a.n + n, left, true);
-        if (a.pre_up) store_4<F16>(a.pre_up, m * a.pre_ld + n, left, false, q);
-        v *= q;
+// What follows the product, for features n0 + i .. n0 + i + 3 of row m0 + j.
+template <bool F16> struct ForwardOut {
+    struct More {
+        lin_f32x4 residual;
+    };
+    const ForwardArgs& a;
+    int e, n0;
+    int64_t m0;
+    lin_f32x4 b, c;
+    __device__ __forceinline__ void column(int i) {
+        const int n = n0 + i, left = a.n - n;
+        b = a.b ? load_4<F16>(a.b, (int64_t)e * a.n + n, left, true) : lin_f32x4{};
+        c = a.u && a.c ? load_4<F16>(a.c, (int64_t)e * a.n + n, left, true) : lin_f32x4{};
     }
-    if (a.residual) v += load_4<F16>(a.residual, m * a.residual_ld + n, left, a.out_f32);
-    store_4<F16>(a.out, m * a.out_ld + n, left, a.out_f32, v);
-}
+    __device__ __forceinline__ More more(int j, int i) const {
+        const int n = n0 + i;
+        return {a.residual ? load_4<F16>(a.residual, (m0 + j) * a.residual_ld + n, a.n - n, a.out_f32) : lin_f32x4{}};
+    }
+    __device__ __forceinline__ void store(int j, int i, lin_f32x4 p, lin_f32x4 q, const More& more) const {
+        const int n = n0 + i, left = a.n - n;
+        const int64_t m = m0 + j;
+        p += b;
+        if (a.pre) store_4<F16>(a.pre, m * a.pre_ld + n, left, false, p);
+        lin_f32x4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = lin_act(a.act, p[x]);
+        if (a.u) {
+            q += c;
+            if (a.pre_up) store_4<F16>(a.pre_up, m * a.pre_ld + n, left, false, q);
+            v *= q;
+        }
+        if (a.residual) v += more.residual;
+        store_4<F16>(a.out, m * a.out_ld + n, left, a.out_f32, v);
+    }
+    // One piece alone.
+    __device__ __forceinline__ void one(int j, int i, lin_f32x4 p, lin_f32x4 q) {
+        column(i);
+        store(j, i, p, q, more(j, i));
+    }
+};
 
 template <class S>
 __global__ void __launch_bounds__(S::TH, 2)
@@ -56,31 +80,26 @@ linear_kernel(ForwardArgs a, uint32_t nI, Parts parts) {
     const int64_t steps = (a.k + S::kStep - 1) / S::kStep;
     const int s0 = (int)(steps * z / parts.splits), s1 = (int)(steps * (z + 1) / parts.splits);
     tile_product<S, false>(iv, jv, a.k, s0, s1, turn_of_block(blockIdx.x, s1 - s0, false), lds, acc, [](auto&) {});
-    each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 p, lin_f32x4 q) {
-        if (j >= nj || i >= ni) return;
-        if (parts.splits == 1) {
-            forward_store<S::F16>(a, e, m0 + j, n0 + i, p, q);
-        } else {
-            const int64_t at = (int64_t)(m0 + j) * a.n + n0 + i;
-            store_4<false>(parts.at(z, 0), at, ni - i, true, p);
-            if (S::PAIR) store_4<false>(parts.at(z, 1), at, ni - i, true, q);
-        }
-    });
+    if (parts.splits == 1) {
+        each_piece<S>(lds, acc, ni, nj, ForwardOut<S::F16>{a, e, n0, m0});
+    } else {
+        const int64_t at = (int64_t)m0 * a.n + n0;
+        each_piece<S>(lds, acc, ni, nj, PartOut<S::PAIR>{parts.at(z, 0) + at, S::PAIR ? parts.at(z, 1) + at : nullptr, a.n, ni});
+    }
 }
 
-// Behind linear_kernel's parts: a thread takes 4 features of a row.
-template <bool F16>
+// Behind linear_kernel's parts: 4 features of a row at a time.
+template <bool F16, int G>
 __global__ void __launch_bounds__(256)
 linear_finish_kernel(ForwardArgs a, Parts parts) {
     const uint32_t quads = (a.n + 3) / 4;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)quads * a.rows; i += (uint64_t)gridDim.x * 256) {
+    each_sum<G>(parts, (uint64_t)quads * a.rows, [&](uint64_t i, bool in, bool first, auto sum) {
         const uint32_t m = (uint32_t)(i / quads), n = (uint32_t)(i - (uint64_t)m * quads) * 4;
-        const int e = expert_of_row(a.offsets, a.experts, a.rows, m);
-        if (e < 0) continue;
+        const int e = in ? expert_of_row(a.offsets, a.experts, a.rows, m) : -1;
         const int64_t at = (int64_t)m * a.n + n;
-        const lin_f32x4 p = parts.sum(0, at, a.n - n), q = a.u ? parts.sum(1, at, a.n - n) : p;
-        forward_store<F16>(a, e, m, n, p, q);
-    }
+        const lin_f32x4 p = sum(0, at, a.n - n, e >= 0), q = a.u ? sum(1, at, a.n - n, e >= 0) : p;
+        if (first && e >= 0) ForwardOut<F16>{a, e, (int)n, m}.one(0, 0, p, q);
+    });
 }
 
 // Few rows an expert: every block takes 32 features (16 of each matrix of a PAIR) and up to 16 FJ rows, its 8 waves every
@@ -168,7 +187,7 @@ linear_few_kernel(ForwardArgs a, uint32_t nI) {
             if (PAIR) q += sums[w][FJ + f][lane];
         }
         const int j = 16 * (f % FJ) + r, n = n0 + 16 * (f / FJ) + 4 * (lane >> 4);
-        if (j < nj && n < a.n) forward_store<F16>(a, e, m0 + j, n, p, q);
+        if (j < nj && n < a.n) ForwardOut<F16>{a, e, n, m0}.one(j, 0, p, q);
     }
 }
 
@@ -183,8 +202,9 @@ template <class S> int launch(const ForwardArgs& a, hipStream_t st) {
     if (int rc = lin_parts(splits, kPlanes, plane, st, &parts)) return rc;
     linear_kernel<S><<<dim3((unsigned)blocks, splits), S::TH, 0, st>>>(a, (uint32_t)nI, parts);
     if (splits > 1) {
-        const unsigned finish = (unsigned)std::min<int64_t>((plane / 4 + a.rows + 255) / 256, 1 << 16);
-        linear_finish_kernel<S::F16><<<finish, 256, 0, st>>>(a, parts);
+        const int64_t quads = (int64_t)(a.n + 3) / 4 * a.rows;
+        if (splits <= 8) linear_finish_kernel<S::F16, 1><<<lin_finish_blocks(quads, 1), 256, 0, st>>>(a, parts);
+        else linear_finish_kernel<S::F16, 16><<<lin_finish_blocks(quads, 16), 256, 0, st>>>(a, parts);
     }
     return naiwa_hip_rc(hipGetLastError());
 }

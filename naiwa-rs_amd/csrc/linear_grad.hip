@@ -22,25 +22,45 @@ struct InputArgs {
     bool dx_f32, accumulate;
 };
 
-template <bool F16> __device__ __forceinline__ void input_store(const InputArgs& a, uint32_t m, int k, lin_f32x4 g) {
-    const int left = a.k - k;
-    if (a.pre) {
-        const lin_f32x4 p = load_4<F16>(a.pre, m * a.pre_ld + k, left, false);
-        lin_f32x4 q = {1.0f, 1.0f, 1.0f, 1.0f}, up;
-        if (a.pre_up) q = load_4<F16>(a.pre_up, m * a.pre_ld + k, left, false);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v, slope;
-            lin_act_slope(a.act, p[i], &v, &slope);
-            up[i] = g[i] * v;
-            g[i] = g[i] * slope * q[i];
+// What follows the product, for values k0 + i .. k0 + i + 3 of row m0 + j.
+template <bool F16> struct InputOut {
+    struct More {
+        lin_f32x4 p, q; // pre and pre_up, or dx's old values in p
+    };
+    const InputArgs& a;
+    int k0;
+    int64_t m0;
+    __device__ __forceinline__ void column(int) {}
+    __device__ __forceinline__ More more(int j, int i) const {
+        const int k = k0 + i, left = a.k - k;
+        More m = {{}, {1.0f, 1.0f, 1.0f, 1.0f}};
+        if (a.pre) {
+            m.p = load_4<F16>(a.pre, (m0 + j) * a.pre_ld + k, left, false);
+            if (a.pre_up) m.q = load_4<F16>(a.pre_up, (m0 + j) * a.pre_ld + k, left, false);
+        } else if (a.accumulate) {
+            m.p = load_4<F16>(a.dx, (m0 + j) * a.dx_ld + k, left, a.dx_f32);
         }
-        if (a.pre_up) store_4<F16>(a.dx_up, m * a.dx_ld + k, left, a.dx_f32, up);
-    } else if (a.accumulate) {
-        g += load_4<F16>(a.dx, m * a.dx_ld + k, left, a.dx_f32);
+        return m;
     }
-    store_4<F16>(a.dx, m * a.dx_ld + k, left, a.dx_f32, g);
-}
+    __device__ __forceinline__ void store(int j, int i, lin_f32x4 g, lin_f32x4, const More& m) const {
+        const int k = k0 + i, left = a.k - k;
+        const int64_t at = (m0 + j) * a.dx_ld + k;
+        if (a.pre) {
+            lin_f32x4 up;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                float v, slope;
+                lin_act_slope(a.act, m.p[x], &v, &slope);
+                up[x] = g[x] * v;
+                g[x] = g[x] * slope * m.q[x];
+            }
+            if (a.pre_up) store_4<F16>(a.dx_up, at, left, a.dx_f32, up);
+        } else if (a.accumulate) {
+            g += m.p;
+        }
+        store_4<F16>(a.dx, at, left, a.dx_f32, g);
+    }
+};
 
 template <class S, bool DUAL>
 __global__ void __launch_bounds__(S::TH, 2)
@@ -52,29 +72,28 @@ input_grad_kernel(InputArgs a, uint32_t nI, Parts parts) {
     int e, nj;
     seg.find(jt, S::TJ, &e, &m0, &nj);
     const int k0 = it * S::TI, ni = min(S::TI, a.k - k0), z = blockIdx.y;
-    const TileView iv[2] = {{a.w + e * a.w_stride + k0, a.w_ld, ni}, {a.u + e * a.u_stride + k0, a.u_ld, ni}};
+    const TileView iv[2] = {{a.w + e * a.w_stride + k0, a.w_ld, ni, k0}, {a.u + e * a.u_stride + k0, a.u_ld, ni, k0}};
     const TileView jv[2] = {{a.dy + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}, {a.dy_up + (int64_t)m0 * a.dy_ld, a.dy_ld, nj}};
     lin_f32x4 acc[S::FI][S::FJ] = {};
     const int64_t steps = (int64_t)((a.n + S::kStep - 1) / S::kStep) * (DUAL ? 2 : 1);
     const int s0 = (int)(steps * z / parts.splits), s1 = (int)(steps * (z + 1) / parts.splits);
     tile_product<S, DUAL>(iv, jv, a.n, s0, s1, turn_of_block(blockIdx.x, s1 - s0, false), lds, acc, [](auto&) {});
-    each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 g, lin_f32x4) {
-        if (j >= nj || i >= ni) return;
-        if (parts.splits == 1) input_store<S::F16>(a, m0 + j, k0 + i, g);
-        else store_4<false>(parts.at(z, 0), (int64_t)(m0 + j) * a.k + k0 + i, ni - i, true, g);
-    });
+    if (parts.splits == 1) each_piece<S>(lds, acc, ni, nj, InputOut<S::F16>{a, k0, m0});
+    else each_piece<S>(lds, acc, ni, nj, PartOut<false>{parts.at(z, 0) + (int64_t)m0 * a.k + k0, nullptr, a.k, ni});
 }
 
-// Behind its parts: a thread takes 4 values of a row.
-template <bool F16>
+// Behind its parts: 4 values of a row at a time.
+template <bool F16, int G>
 __global__ void __launch_bounds__(256)
 input_finish_kernel(InputArgs a, Parts parts) {
     const uint32_t quads = (a.k + 3) / 4;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)quads * a.rows; i += (uint64_t)gridDim.x * 256) {
+    each_sum<G>(parts, (uint64_t)quads * a.rows, [&](uint64_t i, bool in, bool first, auto sum) {
         const uint32_t m = (uint32_t)(i / quads), k = (uint32_t)(i - (uint64_t)m * quads) * 4;
-        if (expert_of_row(a.offsets, a.experts, a.rows, m) >= 0)
-            input_store<F16>(a, m, k, parts.sum(0, (int64_t)m * a.k + k, a.k - k));
-    }
+        in = in && expert_of_row(a.offsets, a.experts, a.rows, m) >= 0;
+        const lin_f32x4 g = sum(0, (int64_t)m * a.k + k, a.k - k, in);
+        const InputOut<F16> out{a, (int)k, m};
+        if (first && in) out.store(0, 0, g, {}, out.more(0, 0));
+    });
 }
 
 struct WeightArgs {
@@ -89,12 +108,23 @@ struct WeightArgs {
     bool dw_f32, accumulate;
 };
 
-// 4 values of a weight's row, `left` of them, behind the sum.
-template <bool F16> __device__ __forceinline__ void weight_store(const WeightArgs& a, int e, int n, int k, int left, lin_f32x4 v) {
-    const int64_t at = e * a.stride + n * a.ld + k;
-    if (a.accumulate) v += load_4<F16>(a.dw, at, left, a.dw_f32);
-    store_4<F16>(a.dw, at, left, a.dw_f32, v);
-}
+// What follows the sum, for values k0 + i .. k0 + i + 3 of weight row n0 + j.
+template <bool F16> struct WeightOut {
+    struct More {
+        lin_f32x4 old;
+    };
+    const WeightArgs& a;
+    int e, n0, k0;
+    __device__ __forceinline__ int64_t at(int j, int i) const { return e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i; }
+    __device__ __forceinline__ void column(int) {}
+    __device__ __forceinline__ More more(int j, int i) const {
+        return {a.accumulate ? load_4<F16>(a.dw, at(j, i), a.k - k0 - i, a.dw_f32) : lin_f32x4{}};
+    }
+    __device__ __forceinline__ void store(int j, int i, lin_f32x4 v, lin_f32x4, const More& m) const {
+        if (a.accumulate) v += m.old;
+        store_4<F16>(a.dw, at(j, i), a.k - k0 - i, a.dw_f32, v);
+    }
+};
 __device__ __forceinline__ void bias_store(const WeightArgs& a, int e, int n, float v) {
     float* to = a.dbias + (int64_t)e * a.n + n;
     *to = v + (a.accumulate ? *to : 0.0f);
@@ -114,7 +144,7 @@ weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ, Parts parts) {
     const int e = blockIdx.y, z = blockIdx.z; // (all XCDs share an expert: with an expert each, uneven ones took 1.4 times as long)
     segment_of(a, e, &m0, &m1);
     const int k0 = it * S::TI, ni = min(S::TI, a.k - k0), n0 = jt * S::TJ, nj = min(S::TJ, a.n - n0);
-    const TileView iv[2] = {{a.x + m0 * a.x_ld + k0, a.x_ld, ni}, {}}, jv[1] = {{a.dy + m0 * a.dy_ld + n0, a.dy_ld, nj}};
+    const TileView iv[2] = {{a.x + m0 * a.x_ld + k0, a.x_ld, ni, k0}, {}}, jv[1] = {{a.dy + m0 * a.dy_ld + n0, a.dy_ld, nj, n0}};
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     lin_f32x4 acc[S::FI][S::FJ] = {}, sum[S::FJ] = {};
     const bool bias = a.dbias && it == 0 && S::i_first(wave) == 0; // whose share the bias gradient is
@@ -137,31 +167,38 @@ weight_grad_kernel(WeightArgs a, uint32_t nI, uint32_t nJ, Parts parts) {
             else parts.at(parts.splits, 0)[((int64_t)z * gridDim.y + e) * a.n + n0 + j] = sum[fj][0];
         }
     }
-    each_piece<S>(lds, acc, [&](int j, int i, lin_f32x4 v, lin_f32x4) {
-        if (j >= nj || i >= ni) return;
-        if (parts.splits == 1) weight_store<S::F16>(a, e, n0 + j, k0 + i, ni - i, v);
-        else store_4<false>(parts.at(z, 0), ((int64_t)e * a.n + n0 + j) * a.k + k0 + i, ni - i, true, v);
-    });
+    if (parts.splits == 1) {
+        each_piece<S>(lds, acc, ni, nj, WeightOut<S::F16>{a, e, n0, k0});
+    } else {
+        each_piece<S>(lds, acc, ni, nj, PartOut<false>{parts.at(z, 0) + ((int64_t)e * a.n + n0) * a.k + k0, nullptr, a.k, ni});
+    }
 }
 
-// Behind its parts: a thread takes 4 values of a weight's row.
-template <bool F16>
+// Behind its parts: 4 values of a weight's row at a time, and a block's share of the biases behind them.
+template <bool F16, int G>
 __global__ void __launch_bounds__(256)
 weight_finish_kernel(WeightArgs a, int experts, Parts parts) {
     const uint32_t quads = (a.k + 3) / 4;
-    const uint64_t all = (uint64_t)quads * a.n * experts;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t row = i / quads;
-        const uint32_t k = (uint32_t)(i - row * quads) * 4, e = (uint32_t)(row / a.n), n = (uint32_t)(row - (uint64_t)e * a.n);
+    auto live = [&](uint32_t e) { // an accumulating call leaves experts without rows alone
         uint32_t m0, m1;
         segment_of(a, e, &m0, &m1);
-        if (a.accumulate && m0 == m1) continue;
-        weight_store<F16>(a, e, n, k, a.k - k, parts.sum(0, (int64_t)row * a.k + k, a.k - k));
-        if (a.dbias && k == 0) {
-            float v = 0.0f;
-            for (int z = 0; z < parts.splits; ++z) v += parts.at(parts.splits, 0)[((int64_t)z * experts + e) * a.n + n];
-            bias_store(a, e, n, v);
-        }
+        return !(a.accumulate && m0 == m1);
+    };
+    each_sum<G>(parts, (uint64_t)quads * a.n * experts, [&](uint64_t i, bool in, bool first, auto sum) {
+        const uint64_t row = i / quads;
+        const uint32_t k = (uint32_t)(i - row * quads) * 4, e = (uint32_t)(row / a.n), n = (uint32_t)(row - (uint64_t)e * a.n);
+        in = in && live(e);
+        const lin_f32x4 v = sum(0, (int64_t)row * a.k + k, a.k - k, in);
+        const WeightOut<F16> out{a, (int)e, (int)n, (int)k};
+        if (first && in) out.store(0, 0, v, {}, out.more(0, 0));
+    });
+    if (!a.dbias) return;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)a.n * experts; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t e = (uint32_t)(i / a.n), n = (uint32_t)(i - (uint64_t)e * a.n);
+        if (!live(e)) continue;
+        float v = 0.0f;
+        for (int z = 0; z < parts.splits; ++z) v += parts.at(parts.splits, 0)[((int64_t)z * experts + e) * a.n + n];
+        bias_store(a, e, n, v);
     }
 }
 
@@ -177,8 +214,9 @@ template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
     if (a.u) input_grad_kernel<S, true><<<grid, S::TH, 0, st>>>(a, (uint32_t)nI, parts);
     else input_grad_kernel<S, false><<<grid, S::TH, 0, st>>>(a, (uint32_t)nI, parts);
     if (splits > 1) {
-        const unsigned finish = (unsigned)std::min<int64_t>((plane / 4 + a.rows + 255) / 256, 1 << 16);
-        input_finish_kernel<S::F16><<<finish, 256, 0, st>>>(a, parts);
+        const int64_t quads = (int64_t)(a.k + 3) / 4 * a.rows;
+        if (splits <= 8) input_finish_kernel<S::F16, 1><<<lin_finish_blocks(quads, 1), 256, 0, st>>>(a, parts);
+        else input_finish_kernel<S::F16, 16><<<lin_finish_blocks(quads, 16), 256, 0, st>>>(a, parts);
     }
     return naiwa_hip_rc(hipGetLastError());
 }
@@ -202,7 +240,8 @@ template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream
     weight_grad_kernel<S><<<dim3((unsigned)blocks, experts, splits), S::TH, 0, st>>>(a, (uint32_t)nI, (uint32_t)nJ, parts);
     if (splits > 1) {
         const int64_t quads = (int64_t)(a.k + 3) / 4 * a.n * experts;
-        weight_finish_kernel<S::F16><<<(unsigned)std::min<int64_t>((quads + 255) / 256, 1 << 16), 256, 0, st>>>(a, experts, parts);
+        if (splits <= 8) weight_finish_kernel<S::F16, 1><<<lin_finish_blocks(quads, 1), 256, 0, st>>>(a, experts, parts);
+        else weight_finish_kernel<S::F16, 16><<<lin_finish_blocks(quads, 16), 256, 0, st>>>(a, experts, parts);
     }
     return naiwa_hip_rc(hipGetLastError());
 }

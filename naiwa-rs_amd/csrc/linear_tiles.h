@@ -56,9 +56,10 @@ struct TileView {
     const uint16_t* base; // the tile's first value at contraction index 0
     int64_t ld;           // values between rows
     int valid;            // the tile's rows (kRows) or columns (kCols) that exist
+    int first;            // columns that lie before them (kCols)
 };
 __device__ __forceinline__ TileView pick(bool second, const TileView& a, const TileView& b) {
-    return {second ? b.base : a.base, second ? b.ld : a.ld, second ? b.valid : a.valid};
+    return {second ? b.base : a.base, second ? b.ld : a.ld, second ? b.valid : a.valid, second ? b.first : a.first};
 }
 
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
@@ -90,7 +91,7 @@ template <int T, int LAYOUT, int NW, bool PAIR, int STEP> struct Tile {
     static constexpr int kBytes = T * STEP * 2;
     static constexpr int kLanes = kBytes / NW / 16 < 64 ? kBytes / NW / 16 : 64; // that take part in a copy
     static constexpr int kCopies = kBytes / NW / 16 / kLanes;                    // a wave's
-    static constexpr int kPieces = (kBytes / 16 + NW * 64 - 1) / (NW * 64);      // a thread's, through registers
+    static constexpr int kPieces = kBytes / 16 / (NW * 64);                      // a thread's, through registers
     static constexpr int kRowPieces = LAYOUT == kRows ? STEP / 8 : T / 8;       // pieces of a row in LDS
     static constexpr int kPer = kLanes / kRowPieces;                             // rows of a copy
     static_assert(kCopies * kLanes * 16 * NW == kBytes && kPer > 0, "whole copies of whole rows");
@@ -138,44 +139,81 @@ template <int T, int LAYOUT, int NW, bool PAIR, int STEP> struct Tile {
         }
     };
 
-    // ---- through registers
+    // ---- through registers: aim() at a view, then load() a step's pieces and store() them
     struct Held {
         lin_u32x4 v[kPieces];
     };
-    static __device__ __forceinline__ void load(const TileView& one, int64_t c0, int64_t C, int tid, Held& h) {
-        const TileView both[2] = {one, one};
-        load(both, c0, C, tid, h);
-    }
-    static __device__ __forceinline__ void load(const TileView* views, int64_t c0, int64_t C, int tid, Held& h) {
+    struct Loader {
+        int off[kPieces];   // bytes from the step's first value to the lane's piece, moved back into its row where it passes the end
+        int moved[kPieces]; // by so many values
+        int tid;
+        __device__ __forceinline__ Loader(int t) : tid(t) {}
+        static __device__ __forceinline__ bool second(int i) { return PAIR && i * (NW * 64) / kRowPieces >= T / 2; } // (uniform)
+        __device__ __forceinline__ int row_of(int i) const { return (tid + i * (NW * 64)) / kRowPieces - (second(i) ? T / 2 : 0); }
+        __device__ __forceinline__ int at_of(int i) const { return (tid + i * (NW * 64)) % kRowPieces * 8; }
+        __device__ __forceinline__ void aim(const TileView* views) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int p = tid + i * NW * 64, at = p % kRowPieces * 8;
-            int row = p / kRowPieces;
-            const bool second = PAIR && row >= T / 2;
-            const TileView v = pick(second, views[0], views[1]);
-            if (second) row -= T / 2;
-            // LDS row `row`, values at .. at + 7 of it, of which `left` exist
-            const int64_t left = LAYOUT == kRows ? C - c0 - at : v.valid - at;
-            const bool in = LAYOUT == kRows ? row < v.valid : row < C - c0 && row < STEP;
-            const uint16_t* s = LAYOUT == kRows ? v.base + row * v.ld + c0 + at : v.base + (c0 + row) * v.ld + at;
-            lin_u32x4 w = {};
-            if (in && left >= 8) {
-                __builtin_memcpy(&w, s, 16);
-            } else if (in) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < left) w[j / 2] |= (uint32_t)s[j] << (16 * (j % 2));
+            for (int i = 0; i < kPieces; ++i) {
+                const TileView v = second(i) ? views[1] : views[0];
+                const int at = at_of(i), to = LAYOUT == kRows || v.first + v.valid < 8 ? at : min(at, v.valid - 8);
+                // (rows that do not exist are read as the last that does: what comes of them is not stored)
+                const int row = LAYOUT == kRows ? min(row_of(i), v.valid - 1) : row_of(i);
+                off[i] = row * ((int)v.ld * 2) + to * 2;
+                moved[i] = at - to;
             }
-            h.v[i] = w;
         }
-    }
-    static __device__ __forceinline__ void store(const Held& h, uint8_t* lds, int tid) {
+        // v's values from `by` on, zeros behind.
+        static __device__ __forceinline__ lin_u32x4 from(lin_u32x4 v, int by) {
+            if (by & 4) v = lin_u32x4{v[2], v[3], 0, 0};
+            if (by & 2) v = lin_u32x4{v[1], v[2], v[3], 0};
+            if (by & 1) v = lin_u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+            return by < 8 ? v : lin_u32x4{};
+        }
+        // The step of contraction values c0 .. of C (none if c0 >= C).
+        __device__ __forceinline__ void load(const TileView* views, int64_t c0, int64_t C, Held& h) const {
+            const int64_t left = C - c0;
+            // a row of fewer than 8 values holds no piece to move: value by value
+            const bool tiny = LAYOUT == kRows ? C < 8 : views[0].first + views[0].valid < 8;
+            if (left >= STEP && !tiny) { // (uniform)
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int p = tid + i * NW * 64, row = p / kRowPieces, piece = (p % kRowPieces) ^ swizzle(row);
-            if (kBytes % (NW * 1024) == 0 || p < kBytes / 16) *(lin_u32x4*)(lds + row * (kRowPieces * 16) + piece * 16) = h.v[i];
+                for (int i = 0; i < kPieces; ++i) {
+                    const TileView& v = second(i) ? views[1] : views[0];
+                    const uint8_t* s = (const uint8_t*)(LAYOUT == kRows ? v.base + c0 : v.base + c0 * v.ld);
+                    __builtin_memcpy(&h.v[i], s + off[i], 16);
+                }
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const TileView& v = second(i) ? views[1] : views[0];
+                const int row = row_of(i), at = at_of(i);
+                const bool in = LAYOUT == kRows ? row < v.valid && at < left : row < left && at < v.valid;
+                lin_u32x4 w = {};
+                if (in && tiny) {
+                    const uint16_t* s = LAYOUT == kRows ? v.base + row * v.ld + c0 + at : v.base + (c0 + row) * v.ld + at;
+                    const int n = (int)min((int64_t)8, LAYOUT == kRows ? left - at : (int64_t)v.valid - at);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < n) w[j / 2] |= (uint32_t)s[j] << (16 * (j % 2));
+                } else if (in) {
+                    const uint8_t* s = (const uint8_t*)(LAYOUT == kRows ? v.base + c0 : v.base + c0 * v.ld);
+                    const int back = LAYOUT == kRows ? max(0, at + 8 - (int)left) : 0;
+                    __builtin_memcpy(&w, s + off[i] - 2 * back, 16);
+                    w = from(w, back);
+                }
+                h.v[i] = w;
+            }
         }
-    }
+        __device__ __forceinline__ void store(const Held& h, uint8_t* lds) const {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int p = tid + i * (NW * 64), row = p / kRowPieces, piece = (p % kRowPieces) ^ swizzle(row);
+                lin_u32x4 w = h.v[i];
+                if (LAYOUT == kCols && moved[i]) w = from(w, moved[i]);
+                *(lin_u32x4*)(lds + row * (kRowPieces * 16) + piece * 16) = w;
+            }
+        }
+    };
 
     // ---- fragments: F of 16 rows (columns) from `first` on
     template <int F> struct Reader {
@@ -277,16 +315,19 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
     };
     auto begin = [&](int step) { begin_i(step), begin_j(step); };
     auto copy = [&](int i, uint32_t buffer) { i < I::kCopies ? ci.one(i, buffer) : cj.one(i - I::kCopies, buffer); };
+    typename I::Loader li(tid);
+    typename J::Loader lj(tid);
     auto load = [&](int step, int p) {
         int64_t c0;
         const bool second = source(step, &c0);
-        const TileView i[2] = {pick(second, iv[0], iv[1]), iv[1]};
-        I::load(S::PAIR ? iv : i, c0, C, tid, hi[p]);
-        J::load(DUAL ? pick(second, jv[0], jv[1]) : jv[0], c0, C, tid, hj[p]);
+        const TileView i[2] = {S::PAIR ? iv[0] : pick(second, iv[0], iv[1]), iv[1]}, j = DUAL ? pick(second, jv[0], jv[1]) : jv[0];
+        if (step == s0 || (DUAL && second != at_i)) li.aim(i), lj.aim(&j), at_i = second;
+        li.load(i, c0, C, hi[p]);
+        lj.load(&j, c0, C, hj[p]);
     };
     auto store = [&](uint32_t buffer, int p) {
-        I::store(hi[p], lds + buffer, tid);
-        J::store(hj[p], lds + buffer + I::kBytes, tid);
+        li.store(hi[p], lds + buffer);
+        lj.store(hj[p], lds + buffer + I::kBytes);
     };
     auto read_i = [&](uint32_t buffer, int f, int h = 0) {
         if (S::PAIR && f >= S::FI / 2) return ri.get(at + buffer + S::TI / 2 * (kStep * 2), f - S::FI / 2, h); // (a PAIR's I is kRows)
@@ -407,37 +448,64 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
     }
 }
 
-// f(j, i, v, q) for 4 values v at a time, i .. i + 3 of row j of the wave's part of the tile: of a PAIR v is of the first
-// matrix, q of the second, and i runs over one.  Every wave of the block calls it.
-template <class S, class F>
-__device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[S::FI][S::FJ], F f) {
+// What follows the product, for 4 values at a time: i .. i + 3 of row j of the tile (of a PAIR i runs over one matrix's).  An
+// Out has
+//   column(i): what is the same for all rows of a lane;
+//   More, more(j, i): what is read for 4 values of a row;
+//   store(j, i, v, q, more): v, and of a PAIR the second matrix's q.
+// Several rows' reads go out before the first is stored: their latency passes once.  Every wave of the block calls it.
+template <class S, class Out>
+__device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[S::FI][S::FJ], int ni, int nj, Out out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     constexpr int kPieces = S::kWaveI / 4;                               // of a row in LDS
     constexpr int kFit = S::kLds / S::NW / (S::kWaveI * 16 * 4);         // J fragments at a time
-    constexpr int kAt = kFit < S::FJ ? kFit : S::FJ;
-    static_assert(kAt > 0 && S::FJ % kAt == 0, "whole fragments");
+    constexpr int kAt = kFit >= S::FJ ? S::FJ : kFit >= 2 ? 2 : 1;
+    static_assert(kFit > 0 && S::FJ % kAt == 0, "whole fragments");
     constexpr int kTake = S::PAIR ? kPieces / 2 : kPieces;               // lanes of a row
     static_assert(64 % kTake == 0, "whole rows");
-    constexpr int kRowsAt = 64 / kTake;
+    constexpr int kRowsAt = 64 / kTake, kAhead = 4;
+    static_assert(kAt * 16 % (kRowsAt * kAhead) == 0, "whole turns");
     uint8_t* mine = lds + wave * (kAt * 16 * S::kWaveI * 4);
     auto at = [&](int row, int piece) { return (lin_f32x4*)(mine + row * (kPieces * 16) + ((piece ^ (row & 15 & (kPieces - 1))) << 4)); };
+    const int piece = lane % kTake, i = S::i_first(wave) + 4 * piece;
+    if (i < ni) out.column(i);
     copies_landed<0>(); // of steps behind the last too
 #pragma unroll
     for (int h = 0; h < S::FJ; h += kAt) {
+        if (S::j_first(wave) + 16 * h >= nj) break; // (the wave's other rows lie behind)
 #pragma unroll
         for (int fj = 0; fj < kAt; ++fj)
 #pragma unroll
             for (int fi = 0; fi < S::FI; ++fi) *at(16 * fj + (lane & 15), 4 * fi + (lane >> 4)) = acc[fi][h + fj];
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-        for (int r = 0; r < kAt * 16; r += kRowsAt) {
-            const int row = r + lane / kTake, piece = lane % kTake;
-            const lin_f32x4 v = *at(row, piece), q = S::PAIR ? *at(row, piece + kTake) : v;
-            f(S::j_first(wave) + 16 * h + row, S::i_first(wave) + 4 * piece, v, q);
+        for (int r = 0; r < kAt * 16; r += kRowsAt * kAhead) {
+            const int row = r + lane / kTake, j = S::j_first(wave) + 16 * h + row;
+            lin_f32x4 v[kAhead], q[kAhead];
+            typename Out::More m[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                v[u] = *at(row + u * kRowsAt, piece), q[u] = S::PAIR ? *at(row + u * kRowsAt, piece + kTake) : v[u];
+                if (j + u * kRowsAt < nj && i < ni) m[u] = out.more(j + u * kRowsAt, i);
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (j + u * kRowsAt < nj && i < ni) out.store(j + u * kRowsAt, i, v[u], q[u], m[u]);
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
+struct NoMore {};
+// f32 sums of a tile, to a part.
+template <bool PAIR> struct PartOut {
+    typedef NoMore More;
+    float *p, *q;   // at the tile's first value
+    int64_t width;  // of a row
+    int ni;
+    __device__ __forceinline__ void column(int) {}
+    __device__ __forceinline__ More more(int, int) const { return {}; }
+    __device__ __forceinline__ void store(int j, int i, lin_f32x4 v, lin_f32x4 u, More) const;
+};
 
 // ---- segments ---------------------------------------------------------------------------
 
@@ -574,6 +642,11 @@ template <bool F16> __device__ __forceinline__ void store_4(void* p, int64_t at,
     }
 }
 
+template <bool PAIR> __device__ __forceinline__ void PartOut<PAIR>::store(int j, int i, lin_f32x4 v, lin_f32x4 u, More) const {
+    store_4<false>(p, j * width + i, ni - i, true, v);
+    if (PAIR) store_4<false>(q, j * width + i, ni - i, true, u);
+}
+
 __device__ __forceinline__ float lin_act(int act, float v) { return act == NAIWA_ACT_NONE ? v : naiwa_act(act, v); }
 // act and its slope.
 __device__ __forceinline__ void lin_act_slope(int act, float v, float* a, float* slope) {
@@ -599,12 +672,32 @@ struct Parts {
     int splits, planes;
     int64_t plane; // values of one
     __device__ __forceinline__ float* at(int z, int q) const { return p + ((int64_t)z * planes + q) * plane; }
-    __device__ __forceinline__ lin_f32x4 sum(int q, int64_t i, int n) const {
-        lin_f32x4 v = {};
-        for (int z = 0; z < splits; ++z) v += load_4<false>(at(z, q), i, n, true);
-        return v;
-    }
 };
+
+// Blocks of 256 threads that add up the parts of 4 values at a time: f(index, sum) for every index < all, sum(q, i, n) being the
+// sum over the parts of plane q's values i .. i + 3 (n of them exist).  G threads share an index, each every G-th part.
+template <int G, class F> __device__ __forceinline__ void each_sum(const Parts& parts, uint64_t all, F f) {
+    constexpr int Q = 256 / G;
+    __shared__ lin_f32x4 sums[G == 1 ? 1 : G][G == 1 ? 1 : Q];
+    const int t = threadIdx.x % Q, g = threadIdx.x / Q;
+    for (uint64_t b = (uint64_t)blockIdx.x * Q; b < all; b += (uint64_t)gridDim.x * Q) {
+        // (with G > 1 all threads come to every sum, and the first of an index goes on with it)
+        f(b + t, b + t < all, g == 0, [&](int q, int64_t i, int n, bool in) {
+            lin_f32x4 v = {};
+            if (in)
+                for (int z = g; z < parts.splits; z += G) v += load_4<false>(parts.at(z, q), i, n, true);
+            if constexpr (G > 1) {
+                __syncthreads();
+                sums[g][t] = v;
+                __syncthreads();
+                v = {};
+                if (g == 0)
+                    for (int x = 0; x < G; ++x) v += sums[x][t];
+            }
+            return v;
+        });
+    }
+}
 
 // The expert whose rows hold m (at most `rows` rows): -1 if none.
 __device__ __forceinline__ int expert_of_row(const uint32_t* offsets, int experts, uint32_t rows, uint32_t m) {
@@ -637,7 +730,7 @@ static inline int lin_size(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
 // step's latency each.  Two blocks a CU or 4 steps were as fast or up to 20 % slower, but for long contractions of few rows:
 // 25 against 32 us for the input gradient of 16 rows x 4096 x 14336.)
 static inline int lin_splits(int64_t tiles, int64_t steps, int64_t values) {
-    const int64_t s = std::min<int64_t>({256 / std::max<int64_t>(tiles, 1), steps / 8, 64, (16 << 20) / std::max<int64_t>(values, 1)});
+    const int64_t s = std::min<int64_t>({256 / std::max<int64_t>(tiles, 1), steps / 8, 256, (16 << 20) / std::max<int64_t>(values, 1)});
     return s < 2 ? 1 : (int)s;
 }
 static inline int lin_parts(int splits, int planes, int64_t plane, hipStream_t st, Parts* p) {
@@ -646,6 +739,10 @@ static inline int lin_parts(int splits, int planes, int64_t plane, hipStream_t s
     int rc = 0;
     p->p = (float*)naiwa_scratch(NAIWA_SCRATCH_LINEAR, (size_t)splits * planes * plane * 4, &rc, st);
     return p->p ? NAIWA_OK : rc;
+}
+// Blocks of 256 threads that finish so many quads of sums, `group` threads each.
+static inline unsigned lin_finish_blocks(int64_t quads, int group) {
+    return (unsigned)std::min<int64_t>((quads * group + 255) / 256, 1 << 16);
 }
 // Whether a call takes 256 x 256 tiles: `tiles` of them of `steps` 64-value steps, `rows` a segment on average (few leave
 // most of a tile empty).  128 and 256 wide, us: 1024 rows x 2048 x 2048 25 and 31, 4096 48 and 52, 512 rows x 4096 x 14336 91 and
