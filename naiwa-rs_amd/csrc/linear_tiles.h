@@ -725,12 +725,14 @@ static inline bool lin_overlap(const void* a, int64_t a_bytes, const void* b, in
 }
 static inline int64_t lin_span(int64_t rows, int64_t ld, int64_t n, int size) { return rows > 0 ? ((rows - 1) * ld + n) * size : 0; }
 static inline int lin_size(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
-// How many blocks take a tile of `steps` steps in a call of `tiles` tiles whose sums are `values` f32 values: a block a CU, 8
-// steps at least each, and at most 64 MB of sums.  (One block a tile, 16 rows x 88 x 728 and 1 x 128 x 3424 took 28 and 38 us, a
-// step's latency each.  Two blocks a CU or 4 steps were as fast or up to 20 % slower, but for long contractions of few rows:
-// 25 against 32 us for the input gradient of 16 rows x 4096 x 14336.)
+// How many blocks take a tile of `steps` steps in a call of `tiles` tiles whose sums are `values` f32 values: a block a CU, of 8
+// steps at least, or of long sums two, and at most 64 MB of parts.  (One block a tile, 16 rows x 88 x 728 and 1 x 128 x 3424
+// took 28 and 38 us, a step's latency each.  Two blocks a CU instead of one: the input gradient of 16 rows x 4096 x 14336 33 and
+// 27 us, 1024 rows x 2048 x 2048, of 64 steps in all, 25 and 28.)
 static inline int lin_splits(int64_t tiles, int64_t steps, int64_t values) {
-    const int64_t s = std::min<int64_t>({256 / std::max<int64_t>(tiles, 1), steps / 8, 256, (16 << 20) / std::max<int64_t>(values, 1)});
+    tiles = std::max<int64_t>(tiles, 1);
+    const int64_t one = std::min(256 / tiles, steps / 8), two = std::min(512 / tiles, steps / 24);
+    const int64_t s = std::min<int64_t>({std::max(one, two), 256, (16 << 20) / std::max<int64_t>(values, 1)});
     return s < 2 ? 1 : (int)s;
 }
 static inline int lin_parts(int splits, int planes, int64_t plane, hipStream_t st, Parts* p) {

@@ -23,7 +23,7 @@ namespace {
 constexpr int kSortE = 4096;
 constexpr int kOne = 4096;        // pairs that one block sorts in one launch
 constexpr int kSortBlocks = 512;  // most blocks of the three launches
-constexpr int kRunLeast = 2048;   // fewest pairs of their blocks
+constexpr int kRunLeast = 512;    // fewest pairs of their blocks (131,072 pairs of 128 experts: 18.8 us with 2048, 12.6 with 512)
 
 struct Pairs {
     const uint32_t* ids;
@@ -248,6 +248,20 @@ struct F16 {
     static __device__ __forceinline__ float get(T v) { return naiwa_f16_to_f32(v); }
     static __device__ __forceinline__ T put(float v) { return (uint16_t)naiwa_f32_to_f16(v); }
 };
+// 16 bytes of an expert's row, which a launch reads or writes once.  PAST: past the caches, for calls whose rows they would not
+// hold (kPast): 16384 tokens of top-8, 2048 bf16 each, 537 MB, take 107 and 95 us to the experts, 140 and 126 back, 214 and
+// 200 for the gradient; 2048 tokens, 67 MB, 18 and 27 us back, 23 and 29 for the gradient.
+constexpr int64_t kPast = (int64_t)256 << 20;
+typedef uint32_t piece16 __attribute__((ext_vector_type(4), aligned(2)));
+template <bool PAST> __device__ __forceinline__ void put16(void* p, uint4 v) {
+    const piece16 w = __builtin_bit_cast(piece16, v);
+    if (PAST) __builtin_nontemporal_store(w, (piece16*)p);
+    else *(piece16*)p = w;
+}
+template <bool PAST> __device__ __forceinline__ uint4 get16(const void* p) {
+    return __builtin_bit_cast(uint4, PAST ? __builtin_nontemporal_load((const piece16*)p) : *(const piece16*)p);
+}
+
 template <class D, int N> __device__ __forceinline__ void loads(const typename D::T* p, float (&o)[N]) {
     typename D::T v[N];
     __builtin_memcpy(v, p, sizeof(v));
@@ -261,83 +275,117 @@ template <class D, int N> __device__ __forceinline__ void stores(typename D::T* 
     __builtin_memcpy(p, v, sizeof(v));
 }
 
-// L lanes take an item (a token or a pair): f(item, lane of L) for every item of the grid's share.
-template <class F> __device__ __forceinline__ void by_item(int64_t items, int L, F f) {
-    const int G = kThreads / L, l = threadIdx.x & (L - 1);
-    for (int64_t i0 = (int64_t)blockIdx.x * G; i0 < items; i0 += (int64_t)gridDim.x * G) {
-        const int64_t i = i0 + threadIdx.x / L;
-        if (i < items) f(i, l);
-    }
+// L lanes take an item (a token or a pair): f(item, lane of L) for every item of the grid's share.  With a wave an item, the
+// item is a scalar, and so is what is read of its pairs.
+template <bool WAVE, class F> __device__ __forceinline__ void by_item(int64_t items, int L, F f) {
+    const int G = WAVE ? kThreads / 64 : kThreads / L, l = WAVE ? threadIdx.x & 63 : threadIdx.x & (L - 1);
+    const int mine = WAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / L;
+    for (int64_t i0 = (int64_t)blockIdx.x * G; i0 < items; i0 += (int64_t)gridDim.x * G)
+        if (i0 + mine < items) f(i0 + mine, l);
+}
+// A row's pieces of N values, kAhead a lane at a time: f(c0, whole) takes those at c0, c0 + L N, .. (whole: all of them lie in
+// the row).
+constexpr int kAhead = 4;
+template <int N, class F> __device__ __forceinline__ void by_pieces(int H, int L, int l, F f) {
+    for (int c = l * N; c < H; c += kAhead * L * N) f(c, c + (kAhead - 1) * L * N + N <= H);
 }
 
+constexpr int kMaxH = 1 << 24;
+
 // U: a value of the rows' size (its bits are what moves).
-template <class U>
+template <class U, bool WAVE, bool PAST>
 __global__ void __launch_bounds__(kThreads)
 to_experts_kernel(const U* x, int64_t ld, const uint32_t* inv, int64_t T, int k, int H, U* rows, int64_t rows_ld, int L) {
     constexpr int N = 16 / sizeof(U);
+    if (WAVE) L = 64;
     const uint32_t n = (uint32_t)(T * k);
-    by_item(T, L, [&](int64_t t, int l) {
+    by_item<WAVE>(T, L, [&](int64_t t, int l) {
         const U* from = x + t * ld;
-        for (int c = l * N; c < H; c += L * N) {
-            const bool whole = c + N <= H;
-            uint4 v = {};
-            if (whole) __builtin_memcpy(&v, from + c, 16);
+        by_pieces<N>(H, L, l, [&](int c0, bool all) {
+            uint4 v[kAhead] = {};
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (all || c0 + u * L * N + N <= H) __builtin_memcpy(&v[u], from + c0 + u * L * N, 16);
             for (int j = 0; j < k; ++j) {
                 const uint32_t r = inv[t * k + j];
                 if (r >= n) continue;
                 U* to = rows + (int64_t)r * rows_ld;
-                if (whole)
-                    __builtin_memcpy(to + c, &v, 16);
-                else
-                    for (int i = c; i < H; ++i) to[i] = from[i];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int c = c0 + u * L * N;
+                    if (all || c + N <= H)
+                        put16<PAST>(to + c, v[u]);
+                    else
+                        for (int i = c; i < H; ++i) to[i] = from[i];
+                }
             }
-        }
+        });
     });
 }
 
-// Y: the rows' type, O: out's.
-template <class Y, class O>
+// Y: the rows' type, O: out's.  A lane takes one piece of a token's row (`parts` waves a row); eight rows' pieces are read before
+// the first is added.
+template <class Y, class O, bool WAVE, bool PAST>
 __global__ void __launch_bounds__(kThreads)
 from_experts_kernel(const typename Y::T* y, int64_t ld, const uint32_t* inv, const float* w, int64_t w_ld, int64_t T, int k,
-                    int H, typename O::T* out, int64_t out_ld, int accumulate, int L) {
-    constexpr int N = 16 / sizeof(typename Y::T);
+                    int H, typename O::T* out, int64_t out_ld, int accumulate, int L, uint32_t parts) {
+    constexpr int N = 16 / sizeof(typename Y::T), kRows = 8;
+    if (WAVE) L = 64;
     const uint32_t n = (uint32_t)(T * k);
-    by_item(T, L, [&](int64_t t, int l) {
+    by_item<WAVE>(T * parts, L, [&](int64_t item, int l) {
+        const int64_t t = WAVE ? item / parts : item;
         typename O::T* to = out + t * out_ld;
-        int c = l * N;
-        for (; c + N <= H; c += L * N) {
-            float s[N] = {};
-            if (accumulate) loads<O, N>(to + c, s);
-            for (int j = 0; j < k; ++j) {
-                const uint32_t r = inv[t * k + j];
-                if (r >= n) continue;
-                const float f = w ? w[t * w_ld + j] : 1.0f;
-                float v[N];
-                loads<Y, N>(y + (int64_t)r * ld + c, v);
+        const int c = ((WAVE ? (int)(item - t * parts) * 64 : 0) + l) * N;
+        if (c < H) {
+            if (c + N <= H) {
+                float s[N] = {};
+                if (accumulate) loads<O, N>(to + c, s);
+                for (int j0 = 0; j0 < k; j0 += kRows) {
+                    float f[kRows];
+                    typename Y::T v[kRows][N];
 #pragma unroll
-                for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(f, v[i], s[i]);
+                    for (int u = 0; u < kRows; ++u) {
+                        const int j = min(j0 + u, k - 1);
+                        const uint32_t r = inv[t * k + j];
+                        const bool in = j0 + u < k && r < n;
+                        f[u] = !in ? 0.0f : w ? w[t * w_ld + j] : 1.0f;
+                        if (in) {
+                            const uint4 z = get16<PAST>(y + (int64_t)r * ld + c);
+                            __builtin_memcpy(v[u], &z, 16);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < N; ++i) v[u][i] = 0;
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kRows; ++u)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(f[u], Y::get(v[u][i]), s[i]);
+                }
+                stores<O, N>(to + c, s);
+                return;
             }
-            stores<O, N>(to + c, s);
-        }
-        for (; c < H; ++c) { // the one lane whose piece passes the end
-            float s = accumulate ? O::get(to[c]) : 0.0f;
-            for (int j = 0; j < k; ++j) {
-                const uint32_t r = inv[t * k + j];
-                if (r < n) s = __builtin_fmaf(w ? w[t * w_ld + j] : 1.0f, Y::get(y[(int64_t)r * ld + c]), s);
+            for (int x = c; x < H; ++x) { // the one lane whose piece passes the end
+                float s = accumulate ? O::get(to[x]) : 0.0f;
+                for (int j = 0; j < k; ++j) {
+                    const uint32_t r = inv[t * k + j];
+                    if (r < n) s = __builtin_fmaf(w ? w[t * w_ld + j] : 1.0f, Y::get(y[(int64_t)r * ld + x]), s);
+                }
+                to[x] = O::put(s);
             }
-            to[c] = O::put(s);
         }
     });
 }
 
-template <class Y, class O>
+template <class Y, class O, bool WAVE, bool PAST>
 __global__ void __launch_bounds__(kThreads)
 from_experts_backward_kernel(const typename O::T* dout, int64_t dout_ld, const typename Y::T* y, int64_t ld,
                              const uint32_t* inv, const float* w, int64_t w_ld, int64_t T, int k, int H,
                              typename Y::T* dy, int64_t dy_ld, float* dw, int64_t dw_ld, int L) {
     constexpr int N = 16 / sizeof(typename Y::T);
+    if (WAVE) L = 64;
     const uint32_t n = (uint32_t)(T * k);
-    by_item(T * k, L, [&](int64_t p, int l) {
+    by_item<WAVE>(T * k, L, [&](int64_t p, int l) {
         const uint32_t t = (uint32_t)p / (uint32_t)k, j = (uint32_t)p - t * (uint32_t)k, r = inv[p];
         float dot = 0.0f;
         if (r < n) {
@@ -345,26 +393,42 @@ from_experts_backward_kernel(const typename O::T* dout, int64_t dout_ld, const t
             const typename O::T* from = dout + t * dout_ld;
             const typename Y::T* row = y + (int64_t)r * ld;
             typename Y::T* to = dy + (int64_t)r * dy_ld;
-            int c = l * N;
-            for (; c + N <= H; c += L * N) {
-                float d[N], v[N];
-                loads<O, N>(from + c, d);
-                if (dw) {
-                    loads<Y, N>(row + c, v);
+            by_pieces<N>(H, L, l, [&](int c0, bool all) {
+                float d[kAhead][N];
+                typename Y::T v[kAhead][N];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) dot = __builtin_fmaf(d[i], v[i], dot);
+                for (int u = 0; u < kAhead; ++u) {
+                    const int c = c0 + u * L * N;
+                    if (!all && c + N > H) continue;
+                    loads<O, N>(from + c, d[u]);
+                    if (dw) {
+                        const uint4 z = get16<PAST>(row + c);
+                        __builtin_memcpy(v[u], &z, 16);
+                    }
                 }
-                if (dy) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) d[i] *= f;
-                    stores<Y, N>(to + c, d);
+                for (int u = 0; u < kAhead; ++u) {
+                    const int c = c0 + u * L * N;
+                    if (all || c + N <= H) {
+                        if (dw)
+#pragma unroll
+                            for (int i = 0; i < N; ++i) dot = __builtin_fmaf(d[u][i], Y::get(v[u][i]), dot);
+                        if (dy) {
+#pragma unroll
+                            for (int i = 0; i < N; ++i) v[u][i] = Y::put(d[u][i] * f);
+                            uint4 z;
+                            __builtin_memcpy(&z, v[u], 16);
+                            put16<PAST>(to + c, z);
+                        }
+                    } else {
+                        for (int x = c; x < H; ++x) {
+                            const float d1 = O::get(from[x]);
+                            if (dw) dot = __builtin_fmaf(d1, Y::get(row[x]), dot);
+                            if (dy) to[x] = Y::put(d1 * f);
+                        }
+                    }
                 }
-            }
-            for (; c < H; ++c) {
-                const float d = O::get(from[c]);
-                if (dw) dot = __builtin_fmaf(d, Y::get(row[c]), dot);
-                if (dy) to[c] = Y::put(d * f);
-            }
+            });
         }
         if (dw) { // (all lanes of the item are here: its bounds are the same for them)
             for (int m = 1; m < L; m <<= 1) dot += __shfl_xor(dot, m, 64);
@@ -383,6 +447,13 @@ unsigned blocks_of(int64_t items, int L) {
     return (unsigned)std::min<int64_t>((items * L + kThreads - 1) / kThreads, (int64_t)1 << 20);
 }
 
+// f(whether a wave takes an item, whether its rows' `bytes` go past the caches).
+template <class F> void by_wave(int L, int64_t bytes, F f) {
+    if (L < 64) f(std::false_type(), std::false_type());
+    else if (bytes < kPast) f(std::true_type(), std::false_type());
+    else f(std::true_type(), std::true_type());
+}
+
 int size_of(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
 bool row_type(int dtype) { return dtype == NAIWA_F32 || dtype == NAIWA_BF16 || dtype == NAIWA_F16; }
 
@@ -395,7 +466,7 @@ int64_t span(int64_t rows, int64_t ld, int H, int size) { return rows ? ((rows -
 
 int sizes_ok(int64_t T, int k, int H) {
     if (T < 0 || k <= 0 || H <= 0) return NAIWA_E_INVALID;
-    return T > INT32_MAX / k ? NAIWA_E_UNSUPPORTED : NAIWA_OK;
+    return T > INT32_MAX / k || H > kMaxH ? NAIWA_E_UNSUPPORTED : NAIWA_OK;
 }
 
 // f(types of y and out) for rows of dtype and out of out_dtype.
@@ -456,10 +527,11 @@ extern "C" int naiwa_tokens_to_experts(const void* x, int dtype, int64_t ld, con
     if (overlap(x, span(T, ld, H, s), rows, span(T * k, rows_ld, H, s))) return NAIWA_E_INVALID;
     const int L = lanes_of(H, 16 / s);
     hipStream_t st = (hipStream_t)stream;
-    if (s == 4)
-        to_experts_kernel<<<blocks_of(T, L), kThreads, 0, st>>>((const uint32_t*)x, ld, inv, T, k, H, (uint32_t*)rows, rows_ld, L);
-    else
-        to_experts_kernel<<<blocks_of(T, L), kThreads, 0, st>>>((const uint16_t*)x, ld, inv, T, k, H, (uint16_t*)rows, rows_ld, L);
+    auto go = [&](auto u, auto wave, auto past) {
+        typedef decltype(u) U;
+        to_experts_kernel<U, decltype(wave)::value, decltype(past)::value><<<blocks_of(T, L), kThreads, 0, st>>>((const U*)x, ld, inv, T, k, H, (U*)rows, rows_ld, L);
+    };
+    by_wave(L, T * k * H * s, [&](auto wave, auto past) { s == 4 ? go(uint32_t(), wave, past) : go(uint16_t(), wave, past); });
     return naiwa_hip_rc(hipGetLastError());
 }
 
@@ -475,12 +547,15 @@ extern "C" int naiwa_tokens_from_experts(const void* y, int dtype, int64_t ld, c
     if (!y || !inv || !out) return NAIWA_E_INVALID;
     ld = ld ? ld : H, out_ld = out_ld ? out_ld : H, w_ld = w_ld ? w_ld : k;
     if (overlap(y, span(T * k, ld, H, size_of(dtype)), out, span(T, out_ld, H, size_of(out_dtype)))) return NAIWA_E_INVALID;
-    const int L = lanes_of(H, 16 / size_of(dtype));
+    const int N = 16 / size_of(dtype), L = lanes_of(H, N);
+    const uint32_t parts = L == 64 ? (H + 64 * N - 1) / (64 * N) : 1;
     return by_types(dtype, out_dtype, [&](auto ty, auto to) {
         typedef decltype(ty) Y;
         typedef decltype(to) O;
-        from_experts_kernel<Y, O><<<blocks_of(T, L), kThreads, 0, (hipStream_t)stream>>>(
-            (const typename Y::T*)y, ld, inv, w, w_ld, T, k, H, (typename O::T*)out, out_ld, flags & NAIWA_TOKENS_ACCUMULATE, L);
+        by_wave(L, T * k * H * size_of(dtype), [&](auto wave, auto past) {
+            from_experts_kernel<Y, O, decltype(wave)::value, decltype(past)::value><<<blocks_of(T * parts, L), kThreads, 0, (hipStream_t)stream>>>(
+                (const typename Y::T*)y, ld, inv, w, w_ld, T, k, H, (typename O::T*)out, out_ld, flags & NAIWA_TOKENS_ACCUMULATE, L, parts);
+        });
     });
 }
 
@@ -508,8 +583,10 @@ extern "C" int naiwa_tokens_from_experts_backward(const void* dout, int dout_dty
     return by_types(dtype, dout_dtype, [&](auto ty, auto to) {
         typedef decltype(ty) Y;
         typedef decltype(to) O;
-        from_experts_backward_kernel<Y, O><<<blocks_of(T * k, L), kThreads, 0, (hipStream_t)stream>>>(
-            (const typename O::T*)dout, dout_ld, (const typename Y::T*)y, ld, inv, w, w_ld, T, k, H, (typename Y::T*)dy, dy_ld, dw,
-            dw_ld, L);
+        by_wave(L, T * k * H * s, [&](auto wave, auto past) {
+            from_experts_backward_kernel<Y, O, decltype(wave)::value, decltype(past)::value><<<blocks_of(T * k, L), kThreads, 0, (hipStream_t)stream>>>(
+                (const typename O::T*)dout, dout_ld, (const typename Y::T*)y, ld, inv, w, w_ld, T, k, H, (typename Y::T*)dy, dy_ld,
+                dw, dw_ld, L);
+        });
     });
 }
