@@ -218,7 +218,7 @@ template <bool F16, bool PAIR, int FJ> int launch_few(const ForwardArgs& a, hipS
 }
 
 // Which kernel a call takes (experts 0: dense).
-enum { kFew16, kFew32, kFew64, kMid, kBig };
+enum { kFew16 = kKinds, kFew32, kFew64 };
 int lin_forward_kind(int64_t rows, int experts, int64_t n, int64_t k, bool pair) {
     const bool grouped = experts > 0;
     const int64_t avg = grouped ? rows / experts : rows, bytes = 2 * std::max(experts, 1) * n * k * (pair ? 2 : 1);
@@ -231,7 +231,8 @@ int lin_forward_kind(int64_t rows, int experts, int64_t n, int64_t k, bool pair)
         return kFew16;
     }
     const int64_t tiles = (n * (pair ? 2 : 1) + 255) / 256 * lin_j_alike(rows, experts, grouped, 256);
-    return lin_big(tiles, (k + 63) / 64, avg) ? kBig : kMid;
+    if (lin_big(tiles, (k + 63) / 64, avg)) return kBig;
+    return lin_small_kind(avg, k);
 }
 
 template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hipStream_t st) {
@@ -239,9 +240,13 @@ template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hi
     if (kind == kFew16) return launch_few<F16, PAIR, 1>(a, st);
     if (kind == kFew32) return launch_few<F16, PAIR, 2>(a, st);
     if (kind == kFew64) return launch_few<F16, PAIR, 4>(a, st);
-    if (!direct) return launch<Shape<128, 128, 2, 2, kRows, kRows, F16, false, PAIR>>(a, st);
-    return kind == kBig ? launch<Shape<256, 256, 2, 4, kRows, kRows, F16, true, PAIR>>(a, st)
-                     : launch<Shape<128, 128, 2, 2, kRows, kRows, F16, true, PAIR>>(a, st);
+    if (!direct) return launch<Shape<128, 128, 2, 2, 32, 4, kRows, kRows, F16, false, PAIR>>(a, st);
+    switch (kind) {
+    case kThin: return launch<Shape<128, 32, 4, 1, 64, 4, kRows, kRows, F16, true, PAIR>>(a, st);
+    case kShort: return launch<Shape<128, 128, 2, 2, 32, 2, kRows, kRows, F16, true, PAIR>>(a, st);
+    case kMid: return launch<Shape<128, 128, 2, 2, 32, 4, kRows, kRows, F16, true, PAIR>>(a, st);
+    default: return launch<Shape<256, 256, 2, 4, 64, 2, kRows, kRows, F16, true, PAIR>>(a, st);
+    }
 }
 
 // ---- the activation's gradient alone
@@ -375,4 +380,10 @@ extern "C" int naiwa_act_backward(const void* dout, const void* pre, const void*
     else if (dtype == NAIWA_BF16) go(Act16<false>());
     else go(Act16<true>());
     return naiwa_hip_rc(hipGetLastError());
+}
+
+// Which kernel a call with aligned rows takes (experts 0: one matrix for all rows), for tests: kThin ... kBig of linear_tiles.h,
+// behind them those that read rows straight from memory, 16, 32 or 64 at a time.
+extern "C" int naiwa_linear_kind(int64_t rows, int experts, int n, int k, int pair) {
+    return lin_forward_kind(rows, experts, n, k, pair != 0);
 }

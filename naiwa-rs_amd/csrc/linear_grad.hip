@@ -220,12 +220,19 @@ template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
     }
     return naiwa_hip_rc(hipGetLastError());
 }
+int lin_input_kind(int64_t rows, int experts, int64_t n, int64_t k, bool dual) {
+    const int64_t avg = rows / std::max(experts, 1);
+    const int64_t tiles = (k + 255) / 256 * lin_j_alike(rows, experts, experts > 0, 256);
+    return lin_big(tiles, (n + 63) / 64 * (dual ? 2 : 1), avg) ? kBig : lin_small_kind(avg, n);
+}
 template <bool F16> int input_grad(const InputArgs& a, bool direct, hipStream_t st) {
-    const int64_t tiles = (int64_t)((a.k + 255) / 256) * lin_j_alike(a.rows, a.experts, a.offsets, 256);
-    const bool big = lin_big(tiles, (int64_t)(a.n + 63) / 64 * (a.u ? 2 : 1), a.rows / (a.offsets ? a.experts : 1));
-    if (!direct) return launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, false>>(a, st);
-    return big ? launch_input<Shape<256, 256, 2, 4, kCols, kRows, F16, true>>(a, st)
-                     : launch_input<Shape<128, 128, 2, 2, kCols, kRows, F16, true>>(a, st);
+    if (!direct) return launch_input<Shape<128, 128, 2, 2, 32, 4, kCols, kRows, F16, false>>(a, st);
+    switch (lin_input_kind(a.rows, a.offsets ? a.experts : 0, a.n, a.k, a.u != nullptr)) {
+    case kThin: return launch_input<Shape<128, 32, 4, 1, 64, 4, kCols, kRows, F16, true>>(a, st);
+    case kShort: return launch_input<Shape<128, 128, 2, 2, 32, 2, kCols, kRows, F16, true>>(a, st);
+    case kMid: return launch_input<Shape<128, 128, 2, 2, 32, 4, kCols, kRows, F16, true>>(a, st);
+    default: return launch_input<Shape<256, 256, 2, 4, 64, 2, kCols, kRows, F16, true>>(a, st);
+    }
 }
 
 template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream_t st) {
@@ -245,12 +252,20 @@ template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream
     }
     return naiwa_hip_rc(hipGetLastError());
 }
+int lin_weight_kind(int64_t rows, int experts, int64_t n, int64_t k) {
+    // With one step of 64 or none the ring of 2 wins even where tiles are many (it and 256 x 256, us: 64 experts of 1408 x 2048
+    // with 16 rows each 157 and 169, 8 of 14336 x 4096 328 and 363; 128 of 768 x 2048 184 and 175).
+    if (rows <= 64 * (int64_t)experts) return kShort;
+    const int64_t tiles = experts * ((k + 255) / 256) * ((n + 255) / 256);
+    return lin_big(tiles, rows / experts / 64 + 1, 64) ? kBig : kMid;
+}
 template <bool F16> int weight_grad(const WeightArgs& a, int experts, bool direct, hipStream_t st) {
-    const int64_t tiles = (int64_t)experts * ((a.k + 255) / 256) * ((a.n + 255) / 256);
-    const bool big = lin_big(tiles, a.rows / experts / 64 + 1, 64);
-    if (!direct) return launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, false>>(a, experts, st);
-    return big ? launch_weight<Shape<256, 256, 2, 4, kCols, kCols, F16, true>>(a, experts, st)
-                     : launch_weight<Shape<128, 128, 2, 2, kCols, kCols, F16, true>>(a, experts, st);
+    if (!direct) return launch_weight<Shape<128, 128, 2, 2, 32, 4, kCols, kCols, F16, false>>(a, experts, st);
+    switch (lin_weight_kind(a.rows, experts, a.n, a.k)) {
+    case kShort: return launch_weight<Shape<128, 128, 2, 2, 32, 2, kCols, kCols, F16, true>>(a, experts, st);
+    case kMid: return launch_weight<Shape<128, 128, 2, 2, 32, 4, kCols, kCols, F16, true>>(a, experts, st);
+    default: return launch_weight<Shape<256, 256, 2, 4, 64, 2, kCols, kCols, F16, true>>(a, experts, st);
+    }
 }
 
 } // namespace
@@ -310,4 +325,12 @@ extern "C" int naiwa_linear_weight_grad(const void* dy, int64_t dy_ld, const voi
     const bool direct = !((n | k) & 7) && lin_aligned(dy, dy_ld, 0) && lin_aligned(x, x_ld, 0);
     hipStream_t st = (hipStream_t)stream;
     return dtype == NAIWA_BF16 ? weight_grad<false>(a, experts, direct, st) : weight_grad<true>(a, experts, direct, st);
+}
+
+// Which kernel a call with aligned rows takes (experts 0: one matrix for all rows), for tests.
+extern "C" int naiwa_linear_input_grad_kind(int64_t rows, int experts, int n, int k, int dual) {
+    return lin_input_kind(rows, experts, n, k, dual != 0);
+}
+extern "C" int naiwa_linear_weight_grad_kind(int64_t rows, int experts, int n, int k) {
+    return lin_weight_kind(rows, experts, n, k);
 }

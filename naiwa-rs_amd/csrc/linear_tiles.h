@@ -47,8 +47,6 @@ typedef short lin_s16x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kFar = 1u << 31; // an offset past every range
 
-constexpr int kRing = 4; // steps in LDS of the 4-wave shapes
-
 enum { kRows = 0, kCols = 1 }; // the contraction index is contiguous, or the row index
 
 // An operand's tile: what a block reads of it.
@@ -256,11 +254,12 @@ template <bool F16> __device__ __forceinline__ lin_f32x4 lin_mfma(lin_s16x8 a, l
 
 // A block's shape: 8 waves and a tile that fills a CU's LDS, or 4 waves and half as much.  PAIR: the I tile's halves are two matrices' rows of the same features (a gate
 // and its up), and a wave's first and second half of fragments belong to them.
-template <int TI_, int TJ_, int NWI_, int NWJ_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false> struct Shape {
+template <int TI_, int TJ_, int NWI_, int NWJ_, int STEP_, int RING_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false>
+struct Shape {
     static constexpr int TI = TI_, TJ = TJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, TH = NW * 64;
     static constexpr int FI = TI / NWI / 16, FJ = TJ / NWJ / 16;
     static constexpr bool F16 = F16_, DIRECT = DIRECT_, PAIR = PAIR_;
-    static constexpr int kStep = NW == 8 ? 64 : 32; // contraction values of a step
+    static constexpr int kStep = STEP_, kRing = RING_; // contraction values of a step, steps in LDS
     typedef Tile<TI, LI_, NW, PAIR_, kStep> I;
     typedef Tile<TJ, LJ_, NW, false, kStep> J;
     static constexpr int kBuf = I::kBytes + J::kBytes;
@@ -389,7 +388,8 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
         if (!second) asm volatile("s_barrier" ::: "memory");
         return;
     }
-    lin_s16x8 a[2][S::FI], b[2][S::FJ];
+    constexpr int kRing = S::kRing, kHalves = kStep / 32;
+    lin_s16x8 a[2][kHalves][S::FI], b[2][kHalves][S::FJ];
     if constexpr (S::DIRECT) {
 #pragma unroll
         for (int i = 0; i < kRing; ++i) {
@@ -399,15 +399,19 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
         }
         copies_landed<(kRing - 1) * kCopies>();
     } else {
+        static_assert(S::DIRECT || kRing == 4, "what is loaded two steps ahead of its place");
         load(s0, 0), load(s0 + 1, 1);
         store(0, 0), store(S::kBuf, 1);
         load(s0 + 2, 0), load(s0 + 3, 1);
         __syncthreads();
     }
 #pragma unroll
-    for (int f = 0; f < S::FI; ++f) a[0][f] = read_i(0, f);
+    for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
-    for (int f = 0; f < S::FJ; ++f) b[0][f] = read_j(0, f);
+        for (int f = 0; f < S::FI; ++f) a[0][h][f] = read_i(0, f, h);
+#pragma unroll
+        for (int f = 0; f < S::FJ; ++f) b[0][h][f] = read_j(0, f, h);
+    }
     uint32_t mine = 0; // the buffer of step t
     auto step = [&](int t, auto parity) {
         constexpr int p = decltype(parity)::value;
@@ -421,24 +425,27 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
             store(then, p);
             load(t + kRing, p);
         }
-        each(b[p]);
         // Parts of the step in order: some reads of the next, some copies, a row of products.
         constexpr int kReads = S::FI + S::FJ, kParts = S::FI;
 #pragma unroll
-        for (int fi = 0; fi < kParts; ++fi) {
+        for (int h = 0; h < kHalves; ++h) {
+            each(b[p][h]);
 #pragma unroll
-            for (int r = 0; r < kReads; ++r)
-                if (r * kParts / kReads == fi) {
-                    if (r < S::FI) a[p ^ 1][r] = read_i(next, r);
-                    else b[p ^ 1][r - S::FI] = read_j(next, r - S::FI);
-                }
-            if constexpr (S::DIRECT)
+            for (int fi = 0; fi < kParts; ++fi) {
 #pragma unroll
-                for (int c = 0; c < kCopies; ++c)
-                    if (c * kParts / kCopies == fi) copy(c, mine);
+                for (int r = 0; r < kReads; ++r)
+                    if (r * kParts / kReads == fi) {
+                        if (r < S::FI) a[p ^ 1][h][r] = read_i(next, r, h);
+                        else b[p ^ 1][h][r - S::FI] = read_j(next, r - S::FI, h);
+                    }
+                if constexpr (S::DIRECT)
 #pragma unroll
-            for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[p][fi], b[p][fj], acc[fi][fj]);
-            __builtin_amdgcn_sched_barrier(0);
+                    for (int c = 0; c < kCopies; ++c)
+                        if (c * kParts * kHalves / kCopies == h * kParts + fi) copy(c, mine);
+#pragma unroll
+                for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[p][h][fi], b[p][h][fj], acc[fi][fj]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         mine = next;
     };
@@ -463,7 +470,7 @@ __device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[
     static_assert(kFit > 0 && S::FJ % kAt == 0, "whole fragments");
     constexpr int kTake = S::PAIR ? kPieces / 2 : kPieces;               // lanes of a row
     static_assert(64 % kTake == 0, "whole rows");
-    constexpr int kRowsAt = 64 / kTake, kAhead = 4;
+    constexpr int kRowsAt = 64 / kTake, kAhead = kAt * 16 / kRowsAt < 4 ? kAt * 16 / kRowsAt : 4;
     static_assert(kAt * 16 % (kRowsAt * kAhead) == 0, "whole turns");
     uint8_t* mine = lds + wave * (kAt * 16 * S::kWaveI * 4);
     auto at = [&](int row, int piece) { return (lin_f32x4*)(mine + row * (kPieces * 16) + ((piece ^ (row & 15 & (kPieces - 1))) << 4)); };
@@ -647,20 +654,24 @@ template <bool PAIR> __device__ __forceinline__ void PartOut<PAIR>::store(int j,
     if (PAIR) store_4<false>(q, j * width + i, ni - i, true, u);
 }
 
-__device__ __forceinline__ float lin_act(int act, float v) { return act == NAIWA_ACT_NONE ? v : naiwa_act(act, v); }
+// 1 / (1 + exp(-v)): SiLU is v times it, GELU's tanh form v times that of twice tanh's argument (1 + tanh x = 2 / (1 + exp(-2 x))).
+__device__ __forceinline__ float lin_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+__device__ __forceinline__ float gelu_twice(float v) { return 1.5957691216057308f * (v + 0.044715f * v * v * v); }
+
+__device__ __forceinline__ float lin_act(int act, float v) {
+    if (act == NAIWA_ACT_NONE) return v;
+    return v * lin_sigmoid(act == NAIWA_ACT_SILU ? v : gelu_twice(v));
+}
 // act and its slope.
 __device__ __forceinline__ void lin_act_slope(int act, float v, float* a, float* slope) {
     if (act == NAIWA_ACT_NONE) {
         *a = v, *slope = 1.0f;
-    } else if (act == NAIWA_ACT_SILU) {
-        const float s = 1.0f / (1.0f + __expf(-v));
-        *a = v * s, *slope = s * (1.0f + v * (1.0f - s));
-    } else {
-        const float k0 = 0.7978845608028654f, k1 = 0.044715f, t = tanhf(k0 * (v + k1 * v * v * v));
-        *a = 0.5f * v * (1.0f + t);
-        const float dt = 1.0f - t * t; // (0 far out, where v * v may be infinite)
-        *slope = 0.5f * (1.0f + t) + (dt > 0.0f ? 0.5f * v * dt * (k0 * (1.0f + 3.0f * k1 * v * v)) : dt);
+        return;
     }
+    const bool silu = act == NAIWA_ACT_SILU;
+    const float s = lin_sigmoid(silu ? v : gelu_twice(v)), d = s * (1.0f - s); // (d is 0 far out, where v * v may be infinite)
+    *a = v * s;
+    *slope = s + (d > 0.0f ? v * d * (silu ? 1.0f : 1.5957691216057308f * (1.0f + 0.134145f * v * v)) : d);
 }
 
 // ---- sums in parts ----------------------------------------------------------------------
@@ -751,6 +762,16 @@ static inline unsigned lin_finish_blocks(int64_t quads, int group) {
 // 70, 2048 277 and 188; gated, 64 experts of 1408 x 2048 with 64 rows each 179 and 181, 96 201 and 189, 512 590 and 444; weight
 // gradients of 2048 x 2048 from 2048 rows 35 and 42, 4096 62 and 55.
 static inline bool lin_big(int64_t tiles, int64_t steps, int64_t rows) { return tiles * steps >= 3500 && rows >= 64; }
+// Which blocks a call takes: 4 waves on 128 x 32 (steps of 64), on 128 x 128 with a ring of 2 or of 4, 8 waves on 256 x 256.
+enum { kThin, kShort, kMid, kBig, kKinds };
+// Of the blocks of 4 waves: with 32 rows a segment or fewer, thin ones hold less of nothing and more blocks a CU ask for weights
+// (thin and 128 x 128, us: gated, 64 experts of 1408 x 2048 with 16 rows each 136 and 150, 8 of 14336 x 4096 329 and 363, one of
+// 14336 x 4096 22 and 26; 48 rows 180 and 173, 458 and 413; input gradients of 60 experts of 1000 x 1000 with 16 rows 24 and 29).
+// A contraction of 64 or less never goes round a ring of 4, and a ring of 2 leaves room for twice the blocks, whose
+// epilogues overlap (2 and 4, us: 16384 rows x 4096 x 64 62 and 87; gated, 128 experts of 576 x 64 with 8 rows 128 and 175).
+static inline int lin_small_kind(int64_t rows, int64_t contraction) {
+    return rows <= 32 && contraction >= 256 ? kThin : contraction <= 64 ? kShort : kMid;
+}
 // J tiles of `tile` rows that segments of `rows` rows have in all, if they are alike.
 static inline int64_t lin_j_alike(int64_t rows, int experts, bool grouped, int tile) {
     return grouped ? std::max<int64_t>(std::min<int64_t>(experts, rows), rows / tile) : (rows + tile - 1) / tile;
