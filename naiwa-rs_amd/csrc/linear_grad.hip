@@ -220,10 +220,15 @@ template <class S> int launch_input(const InputArgs& a, hipStream_t st) {
     }
     return naiwa_hip_rc(hipGetLastError());
 }
+// Whether 256 x 256 tiles have at most `most` times the places that 128 x 128 ones have.
+bool lin_packed(int64_t i, int64_t j256, int64_t j128, double most) {
+    return (double)((i + 255) / 256 * j256 * 4) <= most * (double)((i + 127) / 128 * j128);
+}
 int lin_input_kind(int64_t rows, int experts, int64_t n, int64_t k, bool dual) {
-    const int64_t avg = rows / std::max(experts, 1);
-    const int64_t tiles = (k + 255) / 256 * lin_j_alike(rows, experts, experts > 0, 256);
-    return lin_big(tiles, (n + 63) / 64 * (dual ? 2 : 1), avg) ? kBig : lin_small_kind(avg, n);
+    const bool grouped = experts > 0;
+    const int64_t j256 = lin_j_alike(rows, experts, grouped, 256), j128 = lin_j_alike(rows, experts, grouped, 128);
+    // (64 experts of 1240 x 88 with 918 rows, two matrices: 139 us in 256 x 256 tiles, 60 in 128 x 128; of 2248 x 176: 257 and 385.)
+    return lin_kind(n * (dual ? 2 : 1), rows / std::max(experts, 1), (k + 255) / 256 * j256, lin_packed(k, j256, j128, 1.5));
 }
 template <bool F16> int input_grad(const InputArgs& a, bool direct, hipStream_t st) {
     if (!direct) return launch_input<Shape<128, 128, 2, 2, 32, 4, kCols, kRows, F16, false>>(a, st);
@@ -253,11 +258,14 @@ template <class S> int launch_weight(const WeightArgs& a, int experts, hipStream
     return naiwa_hip_rc(hipGetLastError());
 }
 int lin_weight_kind(int64_t rows, int experts, int64_t n, int64_t k) {
-    // With one step of 64 or none the ring of 2 wins even where tiles are many (it and 256 x 256, us: 64 experts of 1408 x 2048
-    // with 16 rows each 157 and 169, 8 of 14336 x 4096 328 and 363; 128 of 768 x 2048 184 and 175).
-    if (rows <= 64 * (int64_t)experts) return kShort;
-    const int64_t tiles = experts * ((k + 255) / 256) * ((n + 255) / 256);
-    return lin_big(tiles, rows / experts / 64 + 1, 64) ? kBig : kMid;
+    const int64_t j256 = (n + 255) / 256, tiles = experts * ((k + 255) / 256) * j256, avg = rows / experts;
+    // Sums are as long as a segment is, and all of dw is written, so empty places count, and few tiles are split more ways by the
+    // smaller ones (ring of 2, of 4 and 256 x 256, us: 64 experts of 1408 x 2048 with 16 rows each 157, 202 and 169; 128 of
+    // 768 x 2800 with 209 450, 484 and 432; 64 of 184 x 8112 with 602 357, 350 and 257; of 56 x 2384 with 720 79, 78 and 134; of
+    // 184 x 912 with 1166 114, 104 and 142; 9335 rows, 208 x 6952 63, 56 and 87; 10085, 3200 x 2288 220, 188 and 148).
+    const bool many = tiles >= 384 || std::min(n, k) >= 1024;
+    if (avg > 64 && many && tiles * (avg / 64 + 1) >= kManySteps && lin_packed(k, j256, (n + 127) / 128, 1.25)) return kBig;
+    return avg <= 384 ? kShort : kMid;
 }
 template <bool F16> int weight_grad(const WeightArgs& a, int experts, bool direct, hipStream_t st) {
     if (!direct) return launch_weight<Shape<128, 128, 2, 2, 32, 4, kCols, kCols, F16, false>>(a, experts, st);

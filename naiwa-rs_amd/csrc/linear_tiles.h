@@ -757,20 +757,25 @@ static inline int lin_parts(int splits, int planes, int64_t plane, hipStream_t s
 static inline unsigned lin_finish_blocks(int64_t quads, int group) {
     return (unsigned)std::min<int64_t>((quads * group + 255) / 256, 1 << 16);
 }
-// Whether a call takes 256 x 256 tiles: `tiles` of them of `steps` 64-value steps, `rows` a segment on average (few leave
-// most of a tile empty).  128 and 256 wide, us: 1024 rows x 2048 x 2048 25 and 31, 4096 48 and 52, 512 rows x 4096 x 14336 91 and
-// 70, 2048 277 and 188; gated, 64 experts of 1408 x 2048 with 64 rows each 179 and 181, 96 201 and 189, 512 590 and 444; weight
-// gradients of 2048 x 2048 from 2048 rows 35 and 42, 4096 62 and 55.
-static inline bool lin_big(int64_t tiles, int64_t steps, int64_t rows) { return tiles * steps >= 3500 && rows >= 64; }
+constexpr int64_t kManySteps = 2500; // steps of 64 of 256 x 256 tiles, 10 a CU
 // Which blocks a call takes: 4 waves on 128 x 32 (steps of 64), on 128 x 128 with a ring of 2 or of 4, 8 waves on 256 x 256.
 enum { kThin, kShort, kMid, kBig, kKinds };
-// Of the blocks of 4 waves: with 32 rows a segment or fewer, thin ones hold less of nothing and more blocks a CU ask for weights
-// (thin and 128 x 128, us: gated, 64 experts of 1408 x 2048 with 16 rows each 136 and 150, 8 of 14336 x 4096 329 and 363, one of
-// 14336 x 4096 22 and 26; 48 rows 180 and 173, 458 and 413; input gradients of 60 experts of 1000 x 1000 with 16 rows 24 and 29).
-// A contraction of 64 or less never goes round a ring of 4, and a ring of 2 leaves room for twice the blocks, whose
-// epilogues overlap (2 and 4, us: 16384 rows x 4096 x 64 62 and 87; gated, 128 experts of 576 x 64 with 8 rows 128 and 175).
-static inline int lin_small_kind(int64_t rows, int64_t contraction) {
-    return rows <= 32 && contraction >= 256 ? kThin : contraction <= 64 ? kShort : kMid;
+// For a contraction of so many values, segments of `rows` rows on average and `tiles` 256 x 256 tiles; `packed`: few enough of
+// the tiles' places are empty.  All times in us.
+// - 32 rows or fewer: thin blocks hold less of nothing, and more of them a CU ask for weights (thin and 128 x 128: gated, 64
+//   experts of 1408 x 2048 with 16 rows each 136 and 150, 8 of 14336 x 4096 329 and 363, one of 14336 x 4096 22 and 26; 48 rows 180
+//   and 173, 458 and 413; input gradients of 60 experts of 1000 x 1000 with 16 rows 24 and 29).
+// - A short sum hardly goes round a ring of 4, and a ring of 2 leaves room for twice the blocks, whose epilogues overlap (ring of 2,
+//   of 4, and 256 x 256: 16384 rows x 4096 x 64 62, 87 and 89, 7827 x 1392 x 392 28, 34 and 30, 16 experts of 576 x 1704 with 850 rows
+//   67, 75 and 55, input gradients of 64 experts of 368 x 608 with 1946 rows 134, 145 and 153, 1551 x 672 x 2520 20, 21 and 28).
+// - 256 x 256 where tiles are many or their sums long (128 and 256 wide: 1043 rows x 2920 x 584 gated 23 and 27, 555 rows of 16
+//   experts of 96 x 5488 60 and 46, 1024 rows x 2048 x 2048 25 and 31, 4096 48 and 52, 512 rows x 4096 x 14336 91 and 70, 2048
+//   277 and 188; gated, 64 experts of 1408 x 2048 with 96 rows 201 and 189, 512 590 and 444).
+static inline int lin_kind(int64_t contraction, int64_t rows, int64_t tiles, bool packed) {
+    const int64_t steps = (contraction + 63) / 64;
+    if (rows <= 32 && contraction >= 256) return kThin;
+    if (steps <= 9) return kShort;
+    return packed && tiles * steps >= kManySteps ? kBig : kMid;
 }
 // J tiles of `tile` rows that segments of `rows` rows have in all, if they are alike.
 static inline int64_t lin_j_alike(int64_t rows, int experts, bool grouped, int tile) {

@@ -26,7 +26,7 @@ ADDED = ("f16", "gelu", False, True, True, False, True, True)
     (600, 1000, 264, 60, "some", GATED, rules.THIN),
     (4500, 1032, 64, 1, "dense", WHOLE, rules.SHORT), (5000, 520, 40, 1, "dense", ADDED, rules.SHORT),
     (700, 1000, 16, 9, "all", GATED, rules.SHORT), (33, 700, 56, 200, "all", PLAIN, rules.SHORT),
-    (600, 2056, 1048, 1, "dense", ADDED, rules.MID), (700, 1000, 264, 7, "all", WHOLE, rules.MID),
+    (600, 2056, 1048, 1, "dense", ADDED, rules.MID), (700, 1000, 264, 7, "all", WHOLE, rules.SHORT), (700, 1000, 584, 7, "all", WHOLE, rules.MID),
     (100, 264, 33000, 1, "dense", GATED, rules.MID), (70, 2056, 4104, 1, "dense", PLAIN, rules.MID),     # parts of sums
     (100, 2056, 4104, 2, "all", WHOLE, rules.MID),
     (90, 136, 80, 1, "dense", WHOLE, rules.FEW16), (100, 2040, 1048, 1, "dense", PLAIN, rules.FEW32),
@@ -69,14 +69,14 @@ def test_input_grad(gpu, rows, n, k, experts, kind, how, takes):
 
 # dt, f32, accumulate, bias, tight
 @pytest.mark.parametrize("rows,n,k,experts,kind,how,takes", [
-    (5003, 1304, 2056, 1, "dense", ("bf16", True, False, True, True), rules.BIG),
+    (5003, 1544, 2056, 1, "dense", ("bf16", True, False, True, True), rules.BIG),
     (3000, 2056, 2600, 3, "all", ("f16", True, True, True, False), rules.BIG),
     (3000, 2056, 2600, 3, "some", ("bf16", False, True, True, True), rules.BIG),
     (30000, 520, 264, 2, "one", ("f16", False, False, True, False), rules.MID),
     (60, 1032, 1000, 1, "dense", ("bf16", True, True, True, False), rules.SHORT),
     (500, 520, 264, 9, "all", ("f16", False, False, True, True), rules.SHORT),
     (0, 520, 264, 3, "all", ("bf16", True, False, True, True), rules.SHORT),
-    (1000, 520, 264, 9, "past", ("bf16", True, True, False, False), rules.MID),
+    (4000, 520, 264, 9, "past", ("bf16", True, True, False, False), rules.MID),
 ])
 def test_weight_grad(gpu, rows, n, k, experts, kind, how, takes):
     assert rules.weight_grad(rows, experts, n, k) == takes
@@ -104,7 +104,7 @@ class Far:
                                 for i in range(self.shape[0])]), self.dt)
 
 
-@pytest.mark.parametrize("n,k,takes", [(72, 136, rules.FEW16), (2000, 136, rules.MID), (2000, 5640, rules.BIG), (2000, 64, rules.SHORT),
+@pytest.mark.parametrize("n,k,takes", [(72, 136, rules.FEW16), (2000, 1032, rules.MID), (2000, 5640, rules.BIG), (2000, 64, rules.SHORT),
                                        (1003, 263, None)])
 def test_rows_far_apart(gpu, n, k, takes):
     nm = gpu
