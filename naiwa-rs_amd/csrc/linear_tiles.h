@@ -337,46 +337,47 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
     if constexpr (S::NW == 8) {
         static_assert(S::DIRECT, "");
         // Two groups of 4 waves, one wave of each on a SIMD, a phase apart: while one reads half a step, the other
-        // multiplies one.  A step's copies begin when both groups have read what lies there: J's a step ahead (three
-        // phases to land), I's two steps ahead, as far as LDS reaches.
+        // multiplies one.  J's fragments of both halves are read with the first, so that the copies of J's step t + 2 can
+        // begin in the second half of step t and have six phases to land; I's begin in the first, with a third buffer.
         const bool second = wave >= 4;
-        begin_i(s0), begin_j(s0);
-#pragma unroll
-        for (int c = 0; c < J::kCopies; ++c) cj.one(c, 0);
+        begin(s0);
 #pragma unroll
         for (int c = 0; c < I::kCopies; ++c) ci.one(c, 0);
-        begin_i(s0 + 1);
+#pragma unroll
+        for (int c = 0; c < J::kCopies; ++c) cj.one(c, 0);
+        begin(s0 + 1);
 #pragma unroll
         for (int c = 0; c < I::kCopies; ++c) ci.one(c, I::kBytes);
-        copies_landed<I::kCopies>();
+#pragma unroll
+        for (int c = 0; c < J::kCopies; ++c) cj.one(c, J::kBytes);
+        copies_landed<kCopies>();
         if (second) asm volatile("s_barrier" ::: "memory");
         uint32_t mi = 0, mj = 0, then = 2 * I::kBytes;
-        lin_s16x8 a[S::FI], b[S::FJ];
+        lin_s16x8 a[S::FI], b[2][S::FJ];
         for (int t = s0; t < s1; ++t) {
-            begin_j(t + 1);
-            begin_i(t + 2);
+            begin(t + 2);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int f = 0; f < S::FJ; ++f) b[f] = rj.get(at + 3 * I::kBytes + mj, f, h);
 #pragma unroll
                 for (int f = 0; f < S::FI; ++f) a[f] = read_i(mi, f, h);
                 if (h == 0) {
 #pragma unroll
-                    for (int c = 0; c < J::kCopies; ++c) cj.one(c, J::kBytes - mj);
+                    for (int f = 0; f < 2 * S::FJ; ++f) b[f / S::FJ][f % S::FJ] = rj.get(at + 3 * I::kBytes + mj, f % S::FJ, f / S::FJ);
+#pragma unroll
+                    for (int c = 0; c < I::kCopies; ++c) ci.one(c, then);
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 } else {
 #pragma unroll
-                    for (int c = 0; c < I::kCopies; ++c) ci.one(c, then);
-                    copies_landed<I::kCopies>(); // (of the next step)
+                    for (int c = 0; c < J::kCopies; ++c) cj.one(c, mj);
+                    copies_landed<kCopies>(); // (of the next step)
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
-                each(b);
+                each(b[h]);
 #pragma unroll
                 for (int fi = 0; fi < S::FI; ++fi)
 #pragma unroll
-                    for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[fi], b[fj], acc[fi][fj]);
+                    for (int fj = 0; fj < S::FJ; ++fj) acc[fi][fj] = lin_mfma<S::F16>(a[fi], b[h][fj], acc[fi][fj]);
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
                 asm volatile("s_barrier" ::: "memory");
