@@ -18,13 +18,14 @@ struct ForwardArgs {
     void* out;
     uint16_t *pre, *pre_up;
     int64_t residual_ld, out_ld, pre_ld;
-    bool out_f32;
+    bool out_f32, past;
 };
 
 // What follows the product, for features n0 + i .. n0 + i + 3 of row m0 + j.
 template <bool F16> struct ForwardOut {
     struct More {
-        lin_f32x4 residual;
+        lin_u32x4 residual;
+        __device__ __forceinline__ void here() { in_registers(residual); }
     };
     const ForwardArgs& a;
     int e, n0;
@@ -37,23 +38,23 @@ template <bool F16> struct ForwardOut {
     }
     __device__ __forceinline__ More more(int j, int i) const {
         const int n = n0 + i;
-        return {a.residual ? load_4<F16>(a.residual, (m0 + j) * a.residual_ld + n, a.n - n, a.out_f32) : lin_f32x4{}};
+        return {a.residual ? raw_4(a.residual, (m0 + j) * a.residual_ld + n, a.n - n, a.out_f32) : lin_u32x4{}};
     }
     __device__ __forceinline__ void store(int j, int i, lin_f32x4 p, lin_f32x4 q, const More& more) const {
         const int n = n0 + i, left = a.n - n;
         const int64_t m = m0 + j;
         p += b;
-        if (a.pre) store_4<F16>(a.pre, m * a.pre_ld + n, left, false, p);
+        if (a.pre) store_4<F16>(a.pre, m * a.pre_ld + n, left, false, p, a.past);
         lin_f32x4 v;
 #pragma unroll
         for (int x = 0; x < 4; ++x) v[x] = lin_act(a.act, p[x]);
         if (a.u) {
             q += c;
-            if (a.pre_up) store_4<F16>(a.pre_up, m * a.pre_ld + n, left, false, q);
+            if (a.pre_up) store_4<F16>(a.pre_up, m * a.pre_ld + n, left, false, q, a.past);
             v *= q;
         }
-        if (a.residual) v += more.residual;
-        store_4<F16>(a.out, m * a.out_ld + n, left, a.out_f32, v);
+        if (a.residual) v += wide_4<F16>(more.residual, a.out_f32);
+        store_4<F16>(a.out, m * a.out_ld + n, left, a.out_f32, v, a.past);
     }
     // One piece alone.
     __device__ __forceinline__ void one(int j, int i, lin_f32x4 p, lin_f32x4 q) {
@@ -324,7 +325,8 @@ extern "C" int naiwa_linear(const naiwa_weights* w, const naiwa_weights* up, con
     const ForwardArgs a{(const uint16_t*)w->w, up ? (const uint16_t*)up->w : nullptr, (const uint16_t*)x,
                         lin_ld(w), lin_stride(w), up ? lin_ld(up) : 0, up ? lin_stride(up) : 0, x_ld,
                         w->bias, up ? up->bias : nullptr, offsets, (uint32_t)rows, w->experts, n, k, act,
-                        residual, out, (uint16_t*)pre, (uint16_t*)pre_up, residual_ld, out_ld, pre_ld, out_dtype == NAIWA_F32};
+                        residual, out, (uint16_t*)pre, (uint16_t*)pre_up, residual_ld, out_ld, pre_ld, out_dtype == NAIWA_F32,
+                        rows * n * lin_size(out_dtype) >= kLinPast};
     // an output is written where nothing else is read or written
     const int64_t w_bytes = lin_bytes(w), u_bytes = up ? lin_bytes(up) : 0;
     const int64_t b_bytes = (int64_t)w->experts * n * 4;

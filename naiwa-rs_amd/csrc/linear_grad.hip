@@ -19,13 +19,14 @@ struct InputArgs {
     const uint16_t *pre, *pre_up;
     void *dx, *dx_up;
     int64_t pre_ld, dx_ld;
-    bool dx_f32, accumulate;
+    bool dx_f32, accumulate, past;
 };
 
 // What follows the product, for values k0 + i .. k0 + i + 3 of row m0 + j.
 template <bool F16> struct InputOut {
     struct More {
-        lin_f32x4 p, q; // pre and pre_up, or dx's old values in p
+        lin_u32x4 p, q; // pre and pre_up, or dx's old values in p
+        __device__ __forceinline__ void here() { in_registers(p), in_registers(q); }
     };
     const InputArgs& a;
     int k0;
@@ -33,12 +34,12 @@ template <bool F16> struct InputOut {
     __device__ __forceinline__ void column(int) {}
     __device__ __forceinline__ More more(int j, int i) const {
         const int k = k0 + i, left = a.k - k;
-        More m = {{}, {1.0f, 1.0f, 1.0f, 1.0f}};
+        More m = {};
         if (a.pre) {
-            m.p = load_4<F16>(a.pre, (m0 + j) * a.pre_ld + k, left, false);
-            if (a.pre_up) m.q = load_4<F16>(a.pre_up, (m0 + j) * a.pre_ld + k, left, false);
+            m.p = raw_4(a.pre, (m0 + j) * a.pre_ld + k, left, false);
+            if (a.pre_up) m.q = raw_4(a.pre_up, (m0 + j) * a.pre_ld + k, left, false);
         } else if (a.accumulate) {
-            m.p = load_4<F16>(a.dx, (m0 + j) * a.dx_ld + k, left, a.dx_f32);
+            m.p = raw_4(a.dx, (m0 + j) * a.dx_ld + k, left, a.dx_f32);
         }
         return m;
     }
@@ -46,19 +47,20 @@ template <bool F16> struct InputOut {
         const int k = k0 + i, left = a.k - k;
         const int64_t at = (m0 + j) * a.dx_ld + k;
         if (a.pre) {
+            const lin_f32x4 p = wide_4<F16>(m.p, false), q = a.pre_up ? wide_4<F16>(m.q, false) : lin_f32x4{1.0f, 1.0f, 1.0f, 1.0f};
             lin_f32x4 up;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 float v, slope;
-                lin_act_slope(a.act, m.p[x], &v, &slope);
+                lin_act_slope(a.act, p[x], &v, &slope);
                 up[x] = g[x] * v;
-                g[x] = g[x] * slope * m.q[x];
+                g[x] = g[x] * slope * q[x];
             }
-            if (a.pre_up) store_4<F16>(a.dx_up, at, left, a.dx_f32, up);
+            if (a.pre_up) store_4<F16>(a.dx_up, at, left, a.dx_f32, up, a.past);
         } else if (a.accumulate) {
-            g += m.p;
+            g += wide_4<F16>(m.p, a.dx_f32);
         }
-        store_4<F16>(a.dx, at, left, a.dx_f32, g);
+        store_4<F16>(a.dx, at, left, a.dx_f32, g, a.past);
     }
 };
 
@@ -105,24 +107,25 @@ struct WeightArgs {
     void* dw;
     int64_t ld, stride;
     float* dbias;
-    bool dw_f32, accumulate;
+    bool dw_f32, accumulate, past;
 };
 
 // What follows the sum, for values k0 + i .. k0 + i + 3 of weight row n0 + j.
 template <bool F16> struct WeightOut {
     struct More {
-        lin_f32x4 old;
+        lin_u32x4 old;
+        __device__ __forceinline__ void here() { in_registers(old); }
     };
     const WeightArgs& a;
     int e, n0, k0;
     __device__ __forceinline__ int64_t at(int j, int i) const { return e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i; }
     __device__ __forceinline__ void column(int) {}
     __device__ __forceinline__ More more(int j, int i) const {
-        return {a.accumulate ? load_4<F16>(a.dw, at(j, i), a.k - k0 - i, a.dw_f32) : lin_f32x4{}};
+        return {a.accumulate ? raw_4(a.dw, at(j, i), a.k - k0 - i, a.dw_f32) : lin_u32x4{}};
     }
     __device__ __forceinline__ void store(int j, int i, lin_f32x4 v, lin_f32x4, const More& m) const {
-        if (a.accumulate) v += m.old;
-        store_4<F16>(a.dw, at(j, i), a.k - k0 - i, a.dw_f32, v);
+        if (a.accumulate) v += wide_4<F16>(m.old, a.dw_f32);
+        store_4<F16>(a.dw, at(j, i), a.k - k0 - i, a.dw_f32, v, a.past);
     }
 };
 __device__ __forceinline__ void bias_store(const WeightArgs& a, int e, int n, float v) {
@@ -297,7 +300,8 @@ extern "C" int naiwa_linear_input_grad(const naiwa_weights* w, const naiwa_weigh
     const InputArgs a{(const uint16_t*)w->w, up ? (const uint16_t*)up->w : nullptr, (const uint16_t*)dy, (const uint16_t*)dy_up,
                       lin_ld(w), lin_stride(w), up ? lin_ld(up) : 0, up ? lin_stride(up) : 0, dy_ld, offsets, (uint32_t)rows,
                       w->experts, n, k, act, (const uint16_t*)pre, (const uint16_t*)pre_up, dx, dx_up, pre_ld, dx_ld,
-                      dx_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0};
+                      dx_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0,
+                      !flags && rows * k * lin_size(dx_dtype) >= kLinPast};
     const int64_t w_bytes = lin_bytes(w), u_bytes = up ? lin_bytes(up) : 0;
     const int64_t o_bytes = lin_span(rows, dx_ld, k, lin_size(dx_dtype)), p_bytes = lin_span(rows, pre_ld, k, 2);
     for (const void* o : {(const void*)dx, (const void*)dx_up})
@@ -324,7 +328,8 @@ extern "C" int naiwa_linear_weight_grad(const void* dy, int64_t dy_ld, const voi
     if (rows > INT32_MAX || dy_ld > kMaxLd || x_ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (rows && (!dy || !x)) return NAIWA_E_INVALID;
     const WeightArgs a{(const uint16_t*)dy, (const uint16_t*)x, dy_ld, x_ld, offsets, (uint32_t)rows, n, k, dw, ld, stride, dbias,
-                       dw_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0};
+                       dw_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0,
+                       !flags && (int64_t)experts * n * k * lin_size(dw_dtype) >= kLinPast};
     const int64_t dy_bytes = lin_span(rows, dy_ld, n, 2), x_bytes = lin_span(rows, x_ld, k, 2);
     const int64_t w_bytes = ((experts - 1) * stride + (n - 1) * ld + k) * lin_size(dw_dtype), b_bytes = (int64_t)experts * n * 4;
     if (lin_overlap(dw, w_bytes, dy, dy_bytes) || lin_overlap(dw, w_bytes, x, x_bytes) || lin_overlap(dbias, b_bytes, dy, dy_bytes) ||

@@ -459,7 +459,7 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
 // What follows the product, for 4 values at a time: i .. i + 3 of row j of the tile (of a PAIR i runs over one matrix's).  An
 // Out has
 //   column(i): what is the same for all rows of a lane;
-//   More, more(j, i): what is read for 4 values of a row;
+//   More, more(j, i): what is read for 4 values of a row; its here() waits for it;
 //   store(j, i, v, q, more): v, and of a PAIR the second matrix's q.
 // Several rows' reads go out before the first is stored: their latency passes once.  Every wave of the block calls it.
 template <class S, class Out>
@@ -471,7 +471,7 @@ __device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[
     static_assert(kFit > 0 && S::FJ % kAt == 0, "whole fragments");
     constexpr int kTake = S::PAIR ? kPieces / 2 : kPieces;               // lanes of a row
     static_assert(64 % kTake == 0, "whole rows");
-    constexpr int kRowsAt = 64 / kTake, kAhead = kAt * 16 / kRowsAt < 4 ? kAt * 16 / kRowsAt : 4;
+    constexpr int kRowsAt = 64 / kTake, kMost = S::NW == 8 ? 8 : 4, kAhead = kAt * 16 / kRowsAt < kMost ? kAt * 16 / kRowsAt : kMost;
     static_assert(kAt * 16 % (kRowsAt * kAhead) == 0, "whole turns");
     uint8_t* mine = lds + wave * (kAt * 16 * S::kWaveI * 4);
     auto at = [&](int row, int piece) { return (lin_f32x4*)(mine + row * (kPieces * 16) + ((piece ^ (row & 15 & (kPieces - 1))) << 4)); };
@@ -490,12 +490,14 @@ __device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[
         for (int r = 0; r < kAt * 16; r += kRowsAt * kAhead) {
             const int row = r + lane / kTake, j = S::j_first(wave) + 16 * h + row;
             lin_f32x4 v[kAhead], q[kAhead];
-            typename Out::More m[kAhead];
+            typename Out::More m[kAhead] = {};
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 v[u] = *at(row + u * kRowsAt, piece), q[u] = S::PAIR ? *at(row + u * kRowsAt, piece + kTake) : v[u];
                 if (j + u * kRowsAt < nj && i < ni) m[u] = out.more(j + u * kRowsAt, i);
             }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) m[u].here(); // (one wait for all: behind the first store it would wait for that as well)
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
                 if (j + u * kRowsAt < nj && i < ni) out.store(j + u * kRowsAt, i, v[u], q[u], m[u]);
@@ -503,7 +505,10 @@ __device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[
         __builtin_amdgcn_wave_barrier();
     }
 }
-struct NoMore {};
+struct NoMore {
+    __device__ __forceinline__ void here() {}
+};
+__device__ __forceinline__ void in_registers(lin_u32x4& v) { asm volatile("" : "+v"(v)); }
 // f32 sums of a tile, to a part.
 template <bool PAIR> struct PartOut {
     typedef NoMore More;
@@ -598,11 +603,12 @@ template <bool F16> __device__ __forceinline__ float lin_get(uint16_t v) { retur
 template <bool F16> __device__ __forceinline__ uint16_t lin_put(float v) {
     return F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : __builtin_bit_cast(uint16_t, (__bf16)v);
 }
-// Up to 4 values from p (n of them), f32 or 16 bits, from any address of their type.
-template <bool F16> __device__ __forceinline__ lin_f32x4 load_4(const void* p, int64_t at, int n, bool f32) {
-    lin_f32x4 o = {};
+// Up to 4 values from p (n of them), f32 or 16 bits, from any address of their type, as they lie in memory: what is waited for is
+// the first use.
+__device__ __forceinline__ lin_u32x4 raw_4(const void* p, int64_t at, int n, bool f32) {
+    lin_u32x4 o = {};
     if (f32) {
-        const float* s = (const float*)p + at;
+        const uint32_t* s = (const uint32_t*)p + at;
         if (n >= 4) {
             __builtin_memcpy(&o, s, 16);
         } else {
@@ -612,24 +618,42 @@ template <bool F16> __device__ __forceinline__ lin_f32x4 load_4(const void* p, i
         }
     } else {
         const uint16_t* s = (const uint16_t*)p + at;
-        uint16_t v[4] = {};
         if (n >= 4) {
-            __builtin_memcpy(v, s, 8);
+            __builtin_memcpy(&o, s, 8);
         } else {
 #pragma unroll
             for (int i = 0; i < 3; ++i)
-                if (i < n) v[i] = s[i];
+                if (i < n) o[i / 2] |= (uint32_t)s[i] << 16 * (i % 2);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = lin_get<F16>(v[i]);
     }
     return o;
 }
-template <bool F16> __device__ __forceinline__ void store_4(void* p, int64_t at, int n, bool f32, lin_f32x4 o) {
+template <bool F16> __device__ __forceinline__ lin_f32x4 wide_4(lin_u32x4 v, bool f32) {
+    if (f32) return __builtin_bit_cast(lin_f32x4, v);
+    lin_f32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = lin_get<F16>((uint16_t)(v[i / 2] >> 16 * (i % 2)));
+    return o;
+}
+template <bool F16> __device__ __forceinline__ lin_f32x4 load_4(const void* p, int64_t at, int n, bool f32) {
+    return wide_4<F16>(raw_4(p, at, n, f32), f32);
+}
+// (The empty statements keep the two stores from becoming one.)
+template <class V> __device__ __forceinline__ void put(bool past, V* to, V v) {
+    if (past) {
+        asm volatile("");
+        __builtin_nontemporal_store(v, to);
+        asm volatile("");
+    } else {
+        *to = v;
+    }
+}
+template <bool F16> __device__ __forceinline__ void store_4(void* p, int64_t at, int n, bool f32, lin_f32x4 o, bool past = false) {
     if (f32) {
         float* s = (float*)p + at;
         if (n >= 4) {
-            __builtin_memcpy(s, &o, 16);
+            typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+            put(past, (V*)s, (V)o);
         } else {
 #pragma unroll
             for (int i = 0; i < 3; ++i)
@@ -641,7 +665,9 @@ template <bool F16> __device__ __forceinline__ void store_4(void* p, int64_t at,
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = lin_put<F16>(o[i]);
         if (n >= 4) {
-            __builtin_memcpy(s, v, 8);
+            typedef uint16_t V __attribute__((ext_vector_type(4), aligned(2)));
+            const V w = {v[0], v[1], v[2], v[3]};
+            put(past, (V*)s, w);
         } else {
 #pragma unroll
             for (int i = 0; i < 3; ++i)
@@ -726,6 +752,7 @@ __device__ __forceinline__ int expert_of_row(const uint32_t* offsets, int expert
 // ---- host -------------------------------------------------------------------------------
 
 constexpr int64_t kMaxLd = 1 << 21;
+constexpr int64_t kLinPast = 256 << 20; // results of so many bytes are written past the caches, which cannot hold them
 constexpr int kMaxExperts = 4096;
 
 static inline bool lin_aligned(const void* p, int64_t ld, int64_t stride) {
