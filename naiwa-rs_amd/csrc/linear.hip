@@ -36,6 +36,7 @@ template <bool F16> struct ForwardOut {
         b = a.b ? load_4<F16>(a.b, (int64_t)e * a.n + n, left, true) : lin_f32x4{};
         c = a.u && a.c ? load_4<F16>(a.c, (int64_t)e * a.n + n, left, true) : lin_f32x4{};
     }
+    __device__ __forceinline__ bool reads() const { return a.residual; }
     __device__ __forceinline__ More more(int j, int i) const {
         const int n = n0 + i;
         return {a.residual ? raw_4(a.residual, (m0 + j) * a.residual_ld + n, a.n - n, a.out_f32) : lin_u32x4{}};

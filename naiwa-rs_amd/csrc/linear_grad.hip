@@ -32,6 +32,7 @@ template <bool F16> struct InputOut {
     int k0;
     int64_t m0;
     __device__ __forceinline__ void column(int) {}
+    __device__ __forceinline__ bool reads() const { return a.pre || a.accumulate; }
     __device__ __forceinline__ More more(int j, int i) const {
         const int k = k0 + i, left = a.k - k;
         More m = {};
@@ -120,6 +121,7 @@ template <bool F16> struct WeightOut {
     int e, n0, k0;
     __device__ __forceinline__ int64_t at(int j, int i) const { return e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i; }
     __device__ __forceinline__ void column(int) {}
+    __device__ __forceinline__ bool reads() const { return a.accumulate; }
     __device__ __forceinline__ More more(int j, int i) const {
         return {a.accumulate ? raw_4(a.dw, at(j, i), a.k - k0 - i, a.dw_f32) : lin_u32x4{}};
     }

@@ -459,7 +459,7 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
 // What follows the product, for 4 values at a time: i .. i + 3 of row j of the tile (of a PAIR i runs over one matrix's).  An
 // Out has
 //   column(i): what is the same for all rows of a lane;
-//   More, more(j, i): what is read for 4 values of a row; its here() waits for it;
+//   More, more(j, i): what is read for 4 values of a row, if reads(); its here() waits for it;
 //   store(j, i, v, q, more): v, and of a PAIR the second matrix's q.
 // Several rows' reads go out before the first is stored: their latency passes once.  Every wave of the block calls it.
 template <class S, class Out>
@@ -478,14 +478,9 @@ __device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[
     const int piece = lane % kTake, i = S::i_first(wave) + 4 * piece;
     if (i < ni) out.column(i);
     copies_landed<0>(); // of steps behind the last too
-#pragma unroll
-    for (int h = 0; h < S::FJ; h += kAt) {
-        if (S::j_first(wave) + 16 * h >= nj) break; // (the wave's other rows lie behind)
-#pragma unroll
-        for (int fj = 0; fj < kAt; ++fj)
-#pragma unroll
-            for (int fi = 0; fi < S::FI; ++fi) *at(16 * fj + (lane & 15), 4 * fi + (lane >> 4)) = acc[fi][h + fj];
-        __builtin_amdgcn_wave_barrier();
+    // Without reads apart: a wait for reads in a loop is one for the stores of the turn before, and would be made in both.
+    auto rows = [&](int h, auto reads) {
+        constexpr bool kReads = decltype(reads)::value;
 #pragma unroll 1
         for (int r = 0; r < kAt * 16; r += kRowsAt * kAhead) {
             const int row = r + lane / kTake, j = S::j_first(wave) + 16 * h + row;
@@ -494,14 +489,26 @@ __device__ __forceinline__ void each_piece(uint8_t* lds, const lin_f32x4 (&acc)[
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 v[u] = *at(row + u * kRowsAt, piece), q[u] = S::PAIR ? *at(row + u * kRowsAt, piece + kTake) : v[u];
-                if (j + u * kRowsAt < nj && i < ni) m[u] = out.more(j + u * kRowsAt, i);
+                if (kReads && j + u * kRowsAt < nj && i < ni) m[u] = out.more(j + u * kRowsAt, i);
             }
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) m[u].here(); // (one wait for all: behind the first store it would wait for that as well)
+            for (int u = 0; u < kAhead; ++u)
+                if (kReads) m[u].here(); // (one wait for all: behind the first store it would wait for that as well)
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
                 if (j + u * kRowsAt < nj && i < ni) out.store(j + u * kRowsAt, i, v[u], q[u], m[u]);
         }
+    };
+#pragma unroll
+    for (int h = 0; h < S::FJ; h += kAt) {
+        if (S::j_first(wave) + 16 * h >= nj) break; // (the wave's other rows lie behind)
+#pragma unroll
+        for (int fj = 0; fj < kAt; ++fj)
+#pragma unroll
+            for (int fi = 0; fi < S::FI; ++fi) *at(16 * fj + (lane & 15), 4 * fi + (lane >> 4)) = acc[fi][h + fj];
+        __builtin_amdgcn_wave_barrier();
+        if (out.reads()) rows(h, std::true_type());
+        else rows(h, std::false_type());
         __builtin_amdgcn_wave_barrier();
     }
 }
@@ -516,6 +523,7 @@ template <bool PAIR> struct PartOut {
     int64_t width;  // of a row
     int ni;
     __device__ __forceinline__ void column(int) {}
+    static constexpr bool reads() { return false; }
     __device__ __forceinline__ More more(int, int) const { return {}; }
     __device__ __forceinline__ void store(int j, int i, lin_f32x4 v, lin_f32x4 u, More) const;
 };
