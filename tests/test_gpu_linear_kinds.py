@@ -184,3 +184,52 @@ def test_token_rows_far_apart(gpu, dt):
     close(dy.get(), rows, 2.0 ** -24 * np.abs(rows), dt)
     want = np.repeat((o * x.v).sum(1)[:, None], k, 1)
     close(dw.download(np.float32).reshape(T, k), want, H * 2.0 ** -24 * np.repeat(np.abs(o * x.v).sum(1)[:, None], k, 1), "f32")
+
+
+# ---- results too large for the caches
+
+def some(rng, n):
+    """The first and last 200 of n, and 600 between."""
+    return np.unique(np.concatenate([np.arange(200), np.arange(n - 200, n), rng.integers(0, n, 600)]))
+
+
+@pytest.mark.parametrize("rows,n,k,dt", [(70000, 1000, 24, "f32"), (70001, 2003, 17, "bf16"), (40000, 3600, 1096, "bf16")])
+def test_large_results(gpu, rows, n, k, dt):
+    """Forward and input gradient of 256 MB and more, where stores go past the caches; rows behind them stay."""
+    nm = gpu
+    rng = np.random.default_rng(rows)
+    W = Stack(nm, rng, 1, n, k, "bf16")
+    (xr, xv), d = raw_of(rng.standard_normal((rows, k)).astype(np.float32), "bf16"), dtype_of(nm, dt)
+    x, size = nm.DeviceBuffer.from_array(xr), np.dtype(np_of(dt)).itemsize
+    assert rows * n * size >= 1 << 28
+    out = nm.DeviceBuffer((rows + 1) * n * size)
+    mark = raw_of(np.full(n, 1.25, np.float32), dt)[0]
+    out.upload(mark, offset=rows * n * size)
+    nm.linear(W.w, x, rows, out, out_dtype=d)
+    for m in some(rng, rows):
+        got = values(out.download(np_of(dt), n, offset=int(m) * n * size), dt)
+        close(got, xv[m] @ W.v[0].T + W.b[0], (k + 4) * ULP * (np.abs(xv[m]) @ np.abs(W.v[0].T) + np.abs(W.b[0])), dt)
+    assert np.array_equal(out.download(np_of(dt), n, offset=rows * n * size), mark)
+    # as an input gradient: the weights' transposes, [k, n] here
+    T = nm.DeviceBuffer.from_array(np.ascontiguousarray(raw_of(W.v[0], "bf16")[0].T))
+    nm.linear_input_grad(nm.Weights(T, nm.BF16, 1, k, n), x, rows, out, dx_dtype=d)
+    for m in some(rng, rows):
+        got = values(out.download(np_of(dt), n, offset=int(m) * n * size), dt)
+        close(got, xv[m] @ W.v[0].T, (k + 4) * ULP * (np.abs(xv[m]) @ np.abs(W.v[0].T)), dt)
+    assert np.array_equal(out.download(np_of(dt), n, offset=rows * n * size), mark)
+
+
+@pytest.mark.parametrize("rows,n,k,dt", [(600, 1408, 2048, "f32"), (5000, 1408, 1504, "f32"), (90, 2003, 2051, "bf16")])
+def test_large_weight_gradients(gpu, rows, n, k, dt):
+    nm = gpu
+    rng = np.random.default_rng(rows)
+    experts, size = 34, np.dtype(np_of(dt)).itemsize
+    assert experts * n * k * size >= 1 << 28
+    o = segments(rng, rows, experts, "all")
+    (gr, gv), (xr, xv) = (raw_of(rng.standard_normal((rows, m)).astype(np.float32), "bf16") for m in (n, k))
+    g, x, dw = nm.DeviceBuffer.from_array(gr), nm.DeviceBuffer.from_array(xr), nm.DeviceBuffer(experts * n * k * size)
+    nm.linear_weight_grad(g, x, nm.BF16, rows, n, k, dw, experts=experts, offsets=off(nm, o), dw_dtype=dtype_of(nm, dt))
+    for e, s in spans(o, rows, experts):
+        got = values(dw.download(np_of(dt), n * k, offset=e * n * k * size).reshape(n, k), dt)
+        m = max(s.stop - s.start, 0)
+        close(got, gv[s].T @ xv[s], (m + 4) * ULP * (np.abs(gv[s]).T @ np.abs(xv[s])), dt)
