@@ -236,7 +236,8 @@ int lin_input_kind(int64_t rows, int experts, int64_t n, int64_t k, bool dual) {
     return lin_kind(n * (dual ? 2 : 1), rows / std::max(experts, 1), (k + 255) / 256 * j256, lin_packed(k, j256, j128, 1.5));
 }
 template <bool F16> int input_grad(const InputArgs& a, bool direct, hipStream_t st) {
-    if (!direct) return launch_input<Shape<128, 128, 2, 2, 32, 4, kCols, kRows, F16, false>>(a, st);
+    if (!direct && lin_narrow(a.rows / (a.offsets ? a.experts : 1))) return launch_input<Shape<128, 64, 2, 2, 32, 2, kCols, kRows, F16, false>>(a, st);
+    if (!direct) return launch_input<Shape<128, 128, 2, 2, 32, 2, kCols, kRows, F16, false>>(a, st);
     switch (lin_input_kind(a.rows, a.offsets ? a.experts : 0, a.n, a.k, a.u != nullptr)) {
     case kThin: return launch_input<Shape<128, 32, 4, 1, 64, 4, kCols, kRows, F16, true>>(a, st);
     case kShort: return launch_input<Shape<128, 128, 2, 2, 32, 2, kCols, kRows, F16, true>>(a, st);
@@ -273,7 +274,9 @@ int lin_weight_kind(int64_t rows, int experts, int64_t n, int64_t k) {
     return avg <= 384 ? kShort : kMid;
 }
 template <bool F16> int weight_grad(const WeightArgs& a, int experts, bool direct, hipStream_t st) {
-    if (!direct) return launch_weight<Shape<128, 128, 2, 2, 32, 4, kCols, kCols, F16, false>>(a, experts, st);
+    // (128 x 64 and 128 x 128, us: 2048 rows, 2049 x 2047 64 and 72, 4097, 4099 x 4101 296 and 300, 64 experts of 1407 x 2049 with 64 rows
+    // 207 and 264, with 384 406 and 376; 60 rows, 153 x 1088 with its input gradient 37 and 46.)
+    if (!direct) return launch_weight<Shape<128, 64, 2, 2, 32, 2, kCols, kCols, F16, false>>(a, experts, st);
     switch (lin_weight_kind(a.rows, experts, a.n, a.k)) {
     case kShort: return launch_weight<Shape<128, 128, 2, 2, 32, 2, kCols, kCols, F16, true>>(a, experts, st);
     case kMid: return launch_weight<Shape<128, 128, 2, 2, 32, 4, kCols, kCols, F16, true>>(a, experts, st);

@@ -400,7 +400,7 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
         }
         copies_landed<(kRing - 1) * kCopies>();
     } else {
-        static_assert(S::DIRECT || kRing == 4, "what is loaded two steps ahead of its place");
+        static_assert(S::DIRECT || kRing == 2, "two steps in LDS, two more in registers");
         load(s0, 0), load(s0 + 1, 1);
         store(0, 0), store(S::kBuf, 1);
         load(s0 + 2, 0), load(s0 + 3, 1);
@@ -422,9 +422,8 @@ __device__ __forceinline__ void tile_product(const TileView* iv, const TileView*
             begin(t + kRing);
         } else {
             __syncthreads();
-            const uint32_t then = mine + 2 * S::kBuf >= S::kLds ? mine + 2 * S::kBuf - S::kLds : mine + 2 * S::kBuf;
-            store(then, p);
-            load(t + kRing, p);
+            store(mine, p); // (every wave has read step t)
+            load(t + 4, p);
         }
         // Parts of the step in order: some reads of the next, some copies, a row of products.
         constexpr int kReads = S::FI + S::FJ, kParts = S::FI;
@@ -813,6 +812,10 @@ static inline int lin_kind(int64_t contraction, int64_t rows, int64_t tiles, boo
     if (steps <= 9) return kShort;
     return packed && tiles * steps >= kManySteps ? kBig : kMid;
 }
+// Rows that are not aligned pass registers, which leave a CU two blocks of 128 x 128, three of 128 x 64: the narrow ones with 64
+// rows a segment or fewer (narrow and wide, us: 64 experts of 1407 x 2049 with 64 rows each 131 and 150, 128 203 and 168, input
+// gradients 113 and 148, 169 and 164).
+static inline bool lin_narrow(int64_t rows) { return rows <= 64; }
 // J tiles of `tile` rows that segments of `rows` rows have in all, if they are alike.
 static inline int64_t lin_j_alike(int64_t rows, int experts, bool grouped, int tile) {
     return grouped ? std::max<int64_t>(std::min<int64_t>(experts, rows), rows / tile) : (rows + tile - 1) / tile;
