@@ -3,8 +3,6 @@
 // a tile of each matrix), J the rows, so that a lane ends with 4 consecutive features of a row.
 #include "linear_tiles.h"
 
-
-
 namespace {
 
 struct ForwardArgs {
@@ -242,7 +240,8 @@ template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hi
     if (kind == kFew16) return launch_few<F16, PAIR, 1>(a, st);
     if (kind == kFew32) return launch_few<F16, PAIR, 2>(a, st);
     if (kind == kFew64) return launch_few<F16, PAIR, 4>(a, st);
-    if (!direct && lin_narrow(a.rows / (a.offsets ? a.experts : 1))) return launch<Shape<128, 64, 2, 2, 32, 2, kRows, kRows, F16, false, PAIR>>(a, st);
+    if (!direct && lin_narrow(a.rows / (a.offsets ? a.experts : 1)))
+        return launch<Shape<128, 64, 2, 2, 32, 2, kRows, kRows, F16, false, PAIR>>(a, st);
     if (!direct) return launch<Shape<128, 128, 2, 2, 32, 2, kRows, kRows, F16, false, PAIR>>(a, st);
     switch (kind) {
     case kThin: return launch<Shape<128, 32, 4, 1, 64, 4, kRows, kRows, F16, true, PAIR>>(a, st);

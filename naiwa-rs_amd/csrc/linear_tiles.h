@@ -9,13 +9,15 @@
 // Steps of the contraction lie in LDS several times over: while one is read, others land, copied from memory
 // without passing registers (16 bytes a lane).  Buffer ranges make what lies behind a segment's last row zero, lanes
 // behind the last of c ask for an address out of range, and so do steps behind the last (the counted
-// waits stay the same to the end).  Two kinds of block:
+// waits stay the same to the end).  The kinds of block:
 //   8 waves, 256 x 256, steps of 64, all of a CU's LDS.  The waves are two groups, one wave of each on a SIMD, that
-//     take turns in reading and multiplying (setprio and a barrier a phase).  What bounds it is how fast rows come out of
-//     L2 (with the copies left out 4096 x 4096 x 14336 takes 233 us, without the products 377): hence whole 128-byte
-//     lines, three buffers of I and two of J, and copies spread over the phases.
-//   4 waves, 128 x 128, steps of 32 in a ring of 4, two blocks a CU: in step t a wave multiplies what it read of
-//     step t, reads step t + 1 and starts the copies of step t + 4, interleaved; one barrier a step.
+//     take turns in reading and multiplying (setprio and a barrier a phase).  4096 x 4096 x 14336 takes 345 to 375 us,
+//     1.3 to 1.4 PFLOP/s.  What bounds it is how fast rows come out of L2 (with the copies left out it took 233 us, without the
+//     products as long as with them): hence whole 128-byte lines, three buffers of I and two of J, and copies spread
+//     over the phases.  Leaving out the products and copies of a tile's empty rows gained nothing.
+//   4 waves, 128 x 128, steps of 32 in a ring of 4 or 2, two or three blocks a CU: in step t a wave multiplies what it read
+//     of step t, reads step t + 1 and starts the copies of step t + 4 (t + 2), interleaved; one barrier a step.
+//     Or 128 x 32, steps of 64, for few rows.
 // The XCDs begin at different steps and go round (turn_of_block): reading the same columns at a time they meet at
 // the same memory channels (4096 x 4096 x 14336 403 -> 389 us, the weights' gradient of 64 experts 332 -> 286).
 // Both layouts keep 16-byte pieces whole and permute them so that no two lanes of a read share a bank (the LDS takes
@@ -24,7 +26,7 @@
 //     rows in fours;
 //   row index: row c of T values, the pair of pieces f (16 values) at 32 (f ^ s(c)), s(c) = c & 3 | (c >> 3 & 1)
 //     << 2, read by the transposing LDS read (4 rows x 16 values a group of 16 lanes).
-// Operands that are not multiples of 16 bytes pass through registers two steps ahead, value by value at their ends.
+// Operands that are not multiples of 16 bytes pass through registers two steps ahead, whole pieces moved back into their row at its end.
 // At the end the accumulators go through LDS once more, so that what follows the product works on rows:
 // whole lines of memory, and code that is there once.
 #pragma once
@@ -252,8 +254,8 @@ template <bool F16> __device__ __forceinline__ lin_f32x4 lin_mfma(lin_s16x8 a, l
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf16x8, a), __builtin_bit_cast(lin_bf16x8, b), c, 0, 0, 0);
 }
 
-// A block's shape: 8 waves and a tile that fills a CU's LDS, or 4 waves and half as much.  PAIR: the I tile's halves are two matrices' rows of the same features (a gate
-// and its up), and a wave's first and second half of fragments belong to them.
+// A block's shape.  PAIR: the I tile's halves are two matrices' rows of the same features (a gate and its up), and a wave's
+// first and second half of fragments belong to them.
 template <int TI_, int TJ_, int NWI_, int NWJ_, int STEP_, int RING_, int LI_, int LJ_, bool F16_, bool DIRECT_, bool PAIR_ = false>
 struct Shape {
     static constexpr int TI = TI_, TJ = TJ_, NWI = NWI_, NWJ = NWJ_, NW = NWI * NWJ, TH = NW * 64;
@@ -271,8 +273,8 @@ struct Shape {
 };
 
 // acc[fi][fj] += the tile's product over steps s0 .. s1 - 1 of one contraction range of C, or two (DUAL): iv[0] and jv[0],
-// then iv[1] and jv[1], beginning `turn` steps behind s0 and going round.  (A PAIR has one range, and iv[0], iv[1] are the matrices of its halves.)  each(b) is
-// called with every step's J fragments.
+// then iv[1] and jv[1], beginning `turn` steps behind s0 and going round.  (A PAIR has one range, and iv[0], iv[1] are the
+// matrices of its halves.)  each(b) is called with every step's J fragments.
 template <class S, bool DUAL, class Each>
 __device__ __forceinline__ void tile_product(const TileView* iv, const TileView* jv, int64_t C, int s0, int s1, int turn, uint8_t* lds,
                                              lin_f32x4 (&acc)[S::FI][S::FJ], Each each) {
@@ -759,7 +761,10 @@ __device__ __forceinline__ int expert_of_row(const uint32_t* offsets, int expert
 // ---- host -------------------------------------------------------------------------------
 
 constexpr int64_t kMaxLd = 1 << 21;
-constexpr int64_t kLinPast = 256 << 20; // results of so many bytes are written past the caches, which cannot hold them
+// Results of so many bytes are written past the caches, which cannot hold them (past and through, us: weight gradients in f32 of 64
+// experts of 1408 x 2048 286 and 317, 128 of 768 x 1408 113 and 147; 524288 rows x 576 x 64 in bf16 352 and 378), unless they are added
+// to what was there and so read first (474 and 467).
+constexpr int64_t kLinPast = 256 << 20;
 constexpr int kMaxExperts = 4096;
 
 static inline bool lin_aligned(const void* p, int64_t ld, int64_t stride) {
