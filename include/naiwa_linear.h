@@ -23,7 +23,7 @@
  * 0: tightly packed.  Sizes of any kind: rows, n and k need not be multiples of anything;
  * rows, weights and row lengths that are multiples of 16 bytes are faster.  Outputs may not overlap
  * inputs, unless stated.  rows = 0 returns at once (naiwa_linear_weight_grad: with zeros
- * written).  rows, n, k <= 2^31 - 1 and row lengths <= 2^21 (NAIWA_E_UNSUPPORTED),
+ * written).  rows <= 2^31 - 1 and row lengths (n and k with them) <= 2^21 (NAIWA_E_UNSUPPORTED),
  * experts <= 4096.  No counterpart in the reference, whose expert weights are quantised.
  */
 #ifndef NAIWA_LINEAR_H

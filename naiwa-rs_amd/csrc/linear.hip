@@ -320,7 +320,7 @@ extern "C" int naiwa_linear(const naiwa_weights* w, const naiwa_weights* up, con
         return NAIWA_E_INVALID;
     x_ld = x_ld ? x_ld : k, residual_ld = residual_ld ? residual_ld : n, out_ld = out_ld ? out_ld : n, pre_ld = pre_ld ? pre_ld : n;
     if (!lin_act_ok(act) || (out_dtype != NAIWA_F32 && out_dtype != w->dtype)) return NAIWA_E_UNSUPPORTED;
-    if (rows > INT32_MAX || x_ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
+    if (rows > INT32_MAX || std::max({x_ld, residual_ld, out_ld, pre_ld}) > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (rows == 0) return NAIWA_OK;
     if (!x || !out) return NAIWA_E_INVALID;
     const ForwardArgs a{(const uint16_t*)w->w, up ? (const uint16_t*)up->w : nullptr, (const uint16_t*)x,

@@ -304,7 +304,7 @@ extern "C" int naiwa_linear_input_grad(const naiwa_weights* w, const naiwa_weigh
     dy_ld = dy_ld ? dy_ld : n, pre_ld = pre_ld ? pre_ld : k, dx_ld = dx_ld ? dx_ld : k;
     if (!lin_act_ok(act)) return NAIWA_E_UNSUPPORTED;
     if (dx_dtype != NAIWA_F32 && dx_dtype != w->dtype) return NAIWA_E_UNSUPPORTED;
-    if (rows > INT32_MAX || dy_ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
+    if (rows > INT32_MAX || std::max({dy_ld, pre_ld, dx_ld}) > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (rows == 0) return NAIWA_OK;
     if (!dy || !dx) return NAIWA_E_INVALID;
     const InputArgs a{(const uint16_t*)w->w, up ? (const uint16_t*)up->w : nullptr, (const uint16_t*)dy, (const uint16_t*)dy_up,

@@ -252,6 +252,7 @@ struct F16 {
 // hold (kPast): 16384 tokens of top-8, 2048 bf16 each, 537 MB, take 107 and 95 us to the experts, 140 and 126 back, 214 and
 // 200 for the gradient; 2048 tokens, 67 MB, 18 and 27 us back, 23 and 29 for the gradient.
 constexpr int64_t kPast = (int64_t)256 << 20;
+constexpr int64_t kMaxLd = 1 << 28; // row lengths: all offsets fit 63 bits
 typedef uint32_t piece16 __attribute__((ext_vector_type(4), aligned(2)));
 template <bool PAST> __device__ __forceinline__ void put16(void* p, uint4 v) {
     const piece16 w = __builtin_bit_cast(piece16, v);
@@ -519,7 +520,7 @@ extern "C" int naiwa_tokens_to_experts(const void* x, int dtype, int64_t ld, con
                                        void* rows, int64_t rows_ld, int64_t stream) {
     if (int rc = sizes_ok(T, k, H)) return rc;
     if (ld < 0 || rows_ld < 0 || (ld && ld < H) || (rows_ld && rows_ld < H)) return NAIWA_E_INVALID;
-    if (!row_type(dtype)) return NAIWA_E_UNSUPPORTED;
+    if (!row_type(dtype) || std::max(ld, rows_ld) > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (T == 0) return NAIWA_OK;
     if (!x || !inv || !rows) return NAIWA_E_INVALID;
     const int s = size_of(dtype);
@@ -542,7 +543,7 @@ extern "C" int naiwa_tokens_from_experts(const void* y, int dtype, int64_t ld, c
     if (ld < 0 || out_ld < 0 || w_ld < 0 || (ld && ld < H) || (out_ld && out_ld < H) || (w_ld && w_ld < k) ||
         (flags & ~NAIWA_TOKENS_ACCUMULATE))
         return NAIWA_E_INVALID;
-    if (!row_type(dtype) || (out_dtype != NAIWA_F32 && out_dtype != dtype)) return NAIWA_E_UNSUPPORTED;
+    if (!row_type(dtype) || (out_dtype != NAIWA_F32 && out_dtype != dtype) || std::max(ld, out_ld) > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (T == 0) return NAIWA_OK;
     if (!y || !inv || !out) return NAIWA_E_INVALID;
     ld = ld ? ld : H, out_ld = out_ld ? out_ld : H, w_ld = w_ld ? w_ld : k;
@@ -567,7 +568,8 @@ extern "C" int naiwa_tokens_from_experts_backward(const void* dout, int dout_dty
     if (dout_ld < 0 || ld < 0 || dy_ld < 0 || w_ld < 0 || dw_ld < 0 || (dout_ld && dout_ld < H) || (ld && ld < H) ||
         (dy_ld && dy_ld < H) || (w_ld && w_ld < k) || (dw_ld && dw_ld < k))
         return NAIWA_E_INVALID;
-    if (!row_type(dtype) || (dout_dtype != NAIWA_F32 && dout_dtype != dtype)) return NAIWA_E_UNSUPPORTED;
+    if (!row_type(dtype) || (dout_dtype != NAIWA_F32 && dout_dtype != dtype) || std::max({dout_ld, ld, dy_ld}) > kMaxLd)
+        return NAIWA_E_UNSUPPORTED;
     if (T == 0 || (!dy && !dw)) return NAIWA_OK;
     if (!dout || !inv || (dw && !y)) return NAIWA_E_INVALID;
     const int s = size_of(dtype);
