@@ -31,29 +31,27 @@ template <bool F16> struct ForwardOut {
     lin_f32x4 b, c;
     __device__ __forceinline__ void column(int i) {
         const int n = n0 + i, left = a.n - n;
-        b = a.b ? load_4<F16>(a.b, (int64_t)e * a.n + n, left, true) : lin_f32x4{};
-        c = a.u && a.c ? load_4<F16>(a.c, (int64_t)e * a.n + n, left, true) : lin_f32x4{};
+        b = a.b ? load_4(a.b + (int64_t)e * a.n + n, left) : lin_f32x4{};
+        c = a.u && a.c ? load_4(a.c + (int64_t)e * a.n + n, left) : lin_f32x4{};
     }
     __device__ __forceinline__ bool reads() const { return a.residual; }
     __device__ __forceinline__ More more(int j, int i) const {
-        const int n = n0 + i;
-        return {a.residual ? raw_4(a.residual, (m0 + j) * a.residual_ld + n, a.n - n, a.out_f32) : lin_u32x4{}};
+        return {a.residual ? raw_4(cell(a.residual, m0, a.residual_ld, n0, j, i, a.out_f32), a.n - n0 - i, a.out_f32) : lin_u32x4{}};
     }
     __device__ __forceinline__ void store(int j, int i, lin_f32x4 p, lin_f32x4 q, const More& more) const {
-        const int n = n0 + i, left = a.n - n;
-        const int64_t m = m0 + j;
+        const int left = a.n - n0 - i;
         p += b;
-        if (a.pre) store_4<F16>(a.pre, m * a.pre_ld + n, left, false, p, a.past);
+        if (a.pre) store_4<F16>(cell(a.pre, m0, a.pre_ld, n0, j, i, false), left, false, p, a.past);
         lin_f32x4 v;
 #pragma unroll
         for (int x = 0; x < 4; ++x) v[x] = lin_act(a.act, p[x]);
         if (a.u) {
             q += c;
-            if (a.pre_up) store_4<F16>(a.pre_up, m * a.pre_ld + n, left, false, q, a.past);
+            if (a.pre_up) store_4<F16>(cell(a.pre_up, m0, a.pre_ld, n0, j, i, false), left, false, q, a.past);
             v *= q;
         }
         if (a.residual) v += wide_4<F16>(more.residual, a.out_f32);
-        store_4<F16>(a.out, m * a.out_ld + n, left, a.out_f32, v, a.past);
+        store_4<F16>(cell(a.out, m0, a.out_ld, n0, j, i, a.out_f32), left, a.out_f32, v, a.past);
     }
     // One piece alone.
     __device__ __forceinline__ void one(int j, int i, lin_f32x4 p, lin_f32x4 q) {

@@ -32,19 +32,18 @@ template <bool F16> struct InputOut {
     __device__ __forceinline__ void column(int) {}
     __device__ __forceinline__ bool reads() const { return a.pre || a.accumulate; }
     __device__ __forceinline__ More more(int j, int i) const {
-        const int k = k0 + i, left = a.k - k;
+        const int left = a.k - k0 - i;
         More m = {};
         if (a.pre) {
-            m.p = raw_4(a.pre, (m0 + j) * a.pre_ld + k, left, false);
-            if (a.pre_up) m.q = raw_4(a.pre_up, (m0 + j) * a.pre_ld + k, left, false);
+            m.p = raw_4(cell(a.pre, m0, a.pre_ld, k0, j, i, false), left, false);
+            if (a.pre_up) m.q = raw_4(cell(a.pre_up, m0, a.pre_ld, k0, j, i, false), left, false);
         } else if (a.accumulate) {
-            m.p = raw_4(a.dx, (m0 + j) * a.dx_ld + k, left, a.dx_f32);
+            m.p = raw_4(cell(a.dx, m0, a.dx_ld, k0, j, i, a.dx_f32), left, a.dx_f32);
         }
         return m;
     }
     __device__ __forceinline__ void store(int j, int i, lin_f32x4 g, lin_f32x4, const More& m) const {
-        const int k = k0 + i, left = a.k - k;
-        const int64_t at = (m0 + j) * a.dx_ld + k;
+        const int left = a.k - k0 - i;
         if (a.pre) {
             const lin_f32x4 p = wide_4<F16>(m.p, false), q = a.pre_up ? wide_4<F16>(m.q, false) : lin_f32x4{1.0f, 1.0f, 1.0f, 1.0f};
             lin_f32x4 up;
@@ -55,11 +54,11 @@ template <bool F16> struct InputOut {
                 up[x] = g[x] * v;
                 g[x] = g[x] * slope * q[x];
             }
-            if (a.pre_up) store_4<F16>(a.dx_up, at, left, a.dx_f32, up, a.past);
+            if (a.pre_up) store_4<F16>(cell(a.dx_up, m0, a.dx_ld, k0, j, i, a.dx_f32), left, a.dx_f32, up, a.past);
         } else if (a.accumulate) {
             g += wide_4<F16>(m.p, a.dx_f32);
         }
-        store_4<F16>(a.dx, at, left, a.dx_f32, g, a.past);
+        store_4<F16>(cell(a.dx, m0, a.dx_ld, k0, j, i, a.dx_f32), left, a.dx_f32, g, a.past);
     }
 };
 
@@ -120,15 +119,15 @@ template <bool F16> struct WeightOut {
     };
     const WeightArgs& a;
     int e, n0, k0;
-    __device__ __forceinline__ int64_t at(int j, int i) const { return e * a.stride + (int64_t)(n0 + j) * a.ld + k0 + i; }
+    __device__ __forceinline__ char* at(int j, int i) const { return cell(a.dw, n0, a.ld, e * a.stride + k0, j, i, a.dw_f32); }
     __device__ __forceinline__ void column(int) {}
     __device__ __forceinline__ bool reads() const { return a.accumulate; }
     __device__ __forceinline__ More more(int j, int i) const {
-        return {a.accumulate ? raw_4(a.dw, at(j, i), a.k - k0 - i, a.dw_f32) : lin_u32x4{}};
+        return {a.accumulate ? raw_4(at(j, i), a.k - k0 - i, a.dw_f32) : lin_u32x4{}};
     }
     __device__ __forceinline__ void store(int j, int i, lin_f32x4 v, lin_f32x4, const More& m) const {
         if (a.accumulate) v += wide_4<F16>(m.old, a.dw_f32);
-        store_4<F16>(a.dw, at(j, i), a.k - k0 - i, a.dw_f32, v, a.past);
+        store_4<F16>(at(j, i), a.k - k0 - i, a.dw_f32, v, a.past);
     }
 };
 __device__ __forceinline__ void bias_store(const WeightArgs& a, int e, int n, float v) {

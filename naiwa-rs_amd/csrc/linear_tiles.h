@@ -42,6 +42,7 @@ namespace {
 
 typedef uint32_t lin_u32x4 __attribute__((ext_vector_type(4)));
 typedef float lin_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t lin_u16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 lin_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 lin_f16x8 __attribute__((ext_vector_type(8)));
 typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
@@ -612,12 +613,17 @@ template <bool F16> __device__ __forceinline__ float lin_get(uint16_t v) { retur
 template <bool F16> __device__ __forceinline__ uint16_t lin_put(float v) {
     return F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : __builtin_bit_cast(uint16_t, (__bf16)v);
 }
+// Where value (row + j, col + i) of p lies, rows ld values apart, j < 256: one 32-bit product a lane where row and col are the block's.
+__device__ __forceinline__ char* cell(const void* p, int64_t row, int64_t ld, int64_t col, int j, int i, bool f32) {
+    const int shift = f32 ? 2 : 1;
+    return (char*)p + ((row * ld + col) << shift) + (((uint32_t)j * (uint32_t)ld + (uint32_t)i) << shift);
+}
 // Up to 4 values from p (n of them), f32 or 16 bits, from any address of their type, as they lie in memory: what is waited for is
 // the first use.
-__device__ __forceinline__ lin_u32x4 raw_4(const void* p, int64_t at, int n, bool f32) {
+__device__ __forceinline__ lin_u32x4 raw_4(const void* p, int n, bool f32) {
     lin_u32x4 o = {};
     if (f32) {
-        const uint32_t* s = (const uint32_t*)p + at;
+        const uint32_t* s = (const uint32_t*)p;
         if (n >= 4) {
             __builtin_memcpy(&o, s, 16);
         } else {
@@ -626,7 +632,7 @@ __device__ __forceinline__ lin_u32x4 raw_4(const void* p, int64_t at, int n, boo
                 if (i < n) o[i] = s[i];
         }
     } else {
-        const uint16_t* s = (const uint16_t*)p + at;
+        const uint16_t* s = (const uint16_t*)p;
         if (n >= 4) {
             __builtin_memcpy(&o, s, 8);
         } else {
@@ -644,39 +650,36 @@ template <bool F16> __device__ __forceinline__ lin_f32x4 wide_4(lin_u32x4 v, boo
     for (int i = 0; i < 4; ++i) o[i] = lin_get<F16>((uint16_t)(v[i / 2] >> 16 * (i % 2)));
     return o;
 }
-template <bool F16> __device__ __forceinline__ lin_f32x4 load_4(const void* p, int64_t at, int n, bool f32) {
-    return wide_4<F16>(raw_4(p, at, n, f32), f32);
-}
-// (The empty statements keep the two stores from becoming one.)
-template <class V> __device__ __forceinline__ void put(bool past, V* to, V v) {
+__device__ __forceinline__ lin_f32x4 load_4(const float* p, int n) { return __builtin_bit_cast(lin_f32x4, raw_4(p, n, true)); }
+// To an address that is a multiple of ALIGN bytes.  (The empty statements keep the two stores from becoming one.)
+template <int ALIGN, class V> __device__ __forceinline__ void put(bool past, void* to, V v) {
+    typedef V U __attribute__((aligned(ALIGN)));
     if (past) {
         asm volatile("");
-        __builtin_nontemporal_store(v, to);
+        __builtin_nontemporal_store(v, (U*)to);
         asm volatile("");
     } else {
-        *to = v;
+        *(U*)to = v;
     }
 }
-template <bool F16> __device__ __forceinline__ void store_4(void* p, int64_t at, int n, bool f32, lin_f32x4 o, bool past = false) {
+template <bool F16> __device__ __forceinline__ void store_4(void* p, int n, bool f32, lin_f32x4 o, bool past = false) {
     if (f32) {
-        float* s = (float*)p + at;
+        float* s = (float*)p;
         if (n >= 4) {
-            typedef float V __attribute__((ext_vector_type(4), aligned(4)));
-            put(past, (V*)s, (V)o);
+            put<4>(past, s, o);
         } else {
 #pragma unroll
             for (int i = 0; i < 3; ++i)
                 if (i < n) s[i] = o[i];
         }
     } else {
-        uint16_t* s = (uint16_t*)p + at;
-        uint16_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = lin_put<F16>(o[i]);
+        typedef __bf16 B __attribute__((ext_vector_type(4)));
+        typedef _Float16 H __attribute__((ext_vector_type(4)));
+        uint16_t* s = (uint16_t*)p;
+        const lin_u16x4 v = F16 ? __builtin_bit_cast(lin_u16x4, __builtin_convertvector(o, H))
+                                : __builtin_bit_cast(lin_u16x4, __builtin_convertvector(o, B));
         if (n >= 4) {
-            typedef uint16_t V __attribute__((ext_vector_type(4), aligned(2)));
-            const V w = {v[0], v[1], v[2], v[3]};
-            put(past, (V*)s, w);
+            put<2>(past, s, v);
         } else {
 #pragma unroll
             for (int i = 0; i < 3; ++i)
@@ -686,8 +689,8 @@ template <bool F16> __device__ __forceinline__ void store_4(void* p, int64_t at,
 }
 
 template <bool PAIR> __device__ __forceinline__ void PartOut<PAIR>::store(int j, int i, lin_f32x4 v, lin_f32x4 u, More) const {
-    store_4<false>(p, j * width + i, ni - i, true, v);
-    if (PAIR) store_4<false>(q, j * width + i, ni - i, true, u);
+    store_4<false>(cell(p, 0, width, 0, j, i, true), ni - i, true, v);
+    if (PAIR) store_4<false>(cell(q, 0, width, 0, j, i, true), ni - i, true, u);
 }
 
 // 1 / (1 + exp(-v)): SiLU is v times it, GELU's tanh form v times that of twice tanh's argument (1 + tanh x = 2 / (1 + exp(-2 x))).
@@ -732,7 +735,7 @@ template <int G, class F> __device__ __forceinline__ void each_sum(const Parts& 
         f(b + t, b + t < all, g == 0, [&](int q, int64_t i, int n, bool in) {
             lin_f32x4 v = {};
             if (in)
-                for (int z = g; z < parts.splits; z += G) v += load_4<false>(parts.at(z, q), i, n, true);
+                for (int z = g; z < parts.splits; z += G) v += load_4(parts.at(z, q) + i, n);
             if constexpr (G > 1) {
                 __syncthreads();
                 sums[g][t] = v;
