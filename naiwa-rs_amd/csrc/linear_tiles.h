@@ -69,10 +69,13 @@ __device__ __forceinline__ uint32_t lds_at(const void* p) {
 
 // Lane i of the wave copies 16 bytes from the range's offset `off` to lds + 16 i; zeros past the range.
 // As inline assembly, so that the compiler's wait counts leave copies in flight alone.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // (that m0 is reserved: nothing else here uses it)
 __device__ __forceinline__ void copy16(lin_u32x4 range, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(range), "s"(lds)
                  : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ lin_u32x4 range_of(const void* p, int64_t bytes) {
     const uint64_t a = (uint64_t)p;
     const int n = bytes < 0 ? 0 : bytes < 0x7fffffff ? (int)bytes : 0x7fffffff;
