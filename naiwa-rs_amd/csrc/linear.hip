@@ -60,6 +60,9 @@ template <bool F16> struct ForwardOut {
     }
 };
 
+// A tile of out, or a part of its sums.  Streams of weights bound it up to some 48 rows an expert (8 gated experts of 14336 x 4096,
+// 4 rows each: 1.88 GB in 310 to 322 us, 6 TB/s), the tiles' rows out of L2 beyond (4096 x 4096 x 14336 345 to 375 us; 128 gated
+// experts of 768 x 2048 with 243 rows 333 to 350, their 256-row tiles 0.7 filled and 4.2 rounds taking as long as 5).
 template <class S>
 __global__ void __launch_bounds__(S::TH, 2)
 linear_kernel(ForwardArgs a, uint32_t nI, Parts parts) {
