@@ -360,10 +360,10 @@ extern "C" int naiwa_act_backward(const void* dout, const void* pre, const void*
                                   int64_t ld, int act, void* dpre, void* dpre_up, int64_t stream) {
     if (rows < 0 || n <= 0 || ld < 0 || (ld && ld < n)) return NAIWA_E_INVALID;
     if (!lin_act_ok(act) || (dtype != NAIWA_F32 && dtype != NAIWA_BF16 && dtype != NAIWA_F16)) return NAIWA_E_UNSUPPORTED;
+    ld = ld ? ld : n;
     if (rows > INT32_MAX || ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (rows == 0) return NAIWA_OK;
     if (!dout || !pre || !dpre || (!pre_up) != (!dpre_up)) return NAIWA_E_INVALID;
-    ld = ld ? ld : n;
     const int64_t bytes = lin_span(rows, ld, n, lin_size(dtype));
     // in place element by element, or apart
     const void* ins[3] = {dout, pre, pre_up};
