@@ -22,7 +22,8 @@
  * Rows that are no expert's are left as they were and not read.  Row lengths are in values,
  * 0: tightly packed.  Sizes of any kind: rows, n and k need not be multiples of anything;
  * rows, weights and row lengths that are multiples of 16 bytes are faster.  Outputs may not overlap
- * inputs, unless stated.  rows = 0 returns at once (naiwa_linear_weight_grad: with zeros
+ * inputs or each other, unless stated (NAIWA_E_INVALID); columns side by side in rows of one length in bytes (the
+ * halves of a gate-and-up buffer) do not.  rows = 0 returns at once (naiwa_linear_weight_grad: with zeros
  * written).  rows <= 2^31 - 1 and row lengths (n and k with them) <= 2^21 (NAIWA_E_UNSUPPORTED),
  * experts <= 4096.  No counterpart in the reference, whose expert weights are quantised.
  */

@@ -18,7 +18,7 @@
  * Row values are f32, bf16 or f16; products and sums are f32, each result rounded once.
  * Results do not depend on the run.  Row lengths (ld) are in values, 0: tightly packed.
  * T * k <= 2^31 - 1, H <= 2^24, row lengths <= 2^28.  Inputs and outputs may not overlap
- * unless stated.  Calls of no tokens return at once (naiwa_expert_sort then sets its offsets to 0).  Sizes and pointers are checked
+ * unless stated (NAIWA_E_INVALID); columns side by side in rows of one length in bytes do not.  Calls of no tokens return at once (naiwa_expert_sort then sets its offsets to 0).  Sizes and pointers are checked
  * (NAIWA_E_INVALID; NAIWA_E_UNSUPPORTED past a limit or for another type); entries of
  * inv and offsets that lie outside the T * k rows count as NAIWA_NO_ROW.
  */

@@ -330,24 +330,17 @@ extern "C" int naiwa_linear(const naiwa_weights* w, const naiwa_weights* up, con
                         residual, out, (uint16_t*)pre, (uint16_t*)pre_up, residual_ld, out_ld, pre_ld, out_dtype == NAIWA_F32,
                         rows * n * lin_size(out_dtype) >= kLinPast};
     // an output is written where nothing else is read or written
-    const int64_t w_bytes = lin_bytes(w), u_bytes = up ? lin_bytes(up) : 0;
-    const int64_t b_bytes = (int64_t)w->experts * n * 4;
     const int so = lin_size(out_dtype);
-    struct Out {
-        const void* p;
-        int64_t bytes;
-    } outs[3] = {{out, lin_span(rows, out_ld, n, so)}, {pre, lin_span(rows, pre_ld, n, 2)}, {pre_up, lin_span(rows, pre_ld, n, 2)}};
+    const int64_t b_bytes = (int64_t)w->experts * n * 4;
+    const Span ins[] = {span_of(x, rows, x_ld, k, 2), lin_span(w), lin_span(up), span_of(a.b, b_bytes), span_of(a.c, b_bytes)};
+    const Span outs[] = {span_of(out, rows, out_ld, n, so), span_of(pre, rows, pre_ld, n, 2), span_of(pre_up, rows, pre_ld, n, 2)};
+    const Span added = span_of(residual, rows, residual_ld, n, so);
     for (int i = 0; i < 3; ++i) {
-        const Out& o = outs[i];
-        if (lin_overlap(o.p, o.bytes, x, lin_span(rows, x_ld, k, 2)) || lin_overlap(o.p, o.bytes, a.w, w_bytes) ||
-            lin_overlap(o.p, o.bytes, a.u, u_bytes) || lin_overlap(o.p, o.bytes, a.b, b_bytes) ||
-            lin_overlap(o.p, o.bytes, a.c, b_bytes))
-            return NAIWA_E_INVALID;
-        if (!(i == 0 && residual == out && residual_ld == out_ld) &&
-            lin_overlap(o.p, o.bytes, residual, lin_span(rows, residual_ld, n, so)))
-            return NAIWA_E_INVALID;
+        for (const Span& in : ins)
+            if (overlap(outs[i], in)) return NAIWA_E_INVALID;
+        if (!(i == 0 && residual == out && residual_ld == out_ld) && overlap(outs[i], added)) return NAIWA_E_INVALID;
         for (int j = 0; j < i; ++j)
-            if (lin_overlap(o.p, o.bytes, outs[j].p, outs[j].bytes)) return NAIWA_E_INVALID;
+            if (overlap(outs[i], outs[j])) return NAIWA_E_INVALID;
     }
     const bool direct = !(k & 7) && lin_aligned(a.w, a.w_ld, a.w_stride) && lin_aligned(a.x, x_ld, 0) &&
                         (!up || lin_aligned(a.u, a.u_ld, a.u_stride));
@@ -364,13 +357,12 @@ extern "C" int naiwa_act_backward(const void* dout, const void* pre, const void*
     if (rows > INT32_MAX || ld > kMaxLd) return NAIWA_E_UNSUPPORTED;
     if (rows == 0) return NAIWA_OK;
     if (!dout || !pre || !dpre || (!pre_up) != (!dpre_up)) return NAIWA_E_INVALID;
-    const int64_t bytes = lin_span(rows, ld, n, lin_size(dtype));
     // in place element by element, or apart
-    const void* ins[3] = {dout, pre, pre_up};
+    auto span = [&](const void* p) { return span_of(p, rows, ld, n, lin_size(dtype)); };
     for (const void* o : {(const void*)dpre, (const void*)dpre_up})
-        for (const void* i : ins)
-            if (o != i && lin_overlap(o, bytes, i, bytes)) return NAIWA_E_INVALID;
-    if (lin_overlap(dpre, bytes, dpre_up, bytes)) return NAIWA_E_INVALID;
+        for (const void* i : {dout, pre, pre_up})
+            if (o != i && overlap(span(o), span(i))) return NAIWA_E_INVALID;
+    if (overlap(span(dpre), span(dpre_up))) return NAIWA_E_INVALID;
     const int pieces = dtype == NAIWA_F32 ? (n + 3) / 4 : (n + 7) / 8;
     const unsigned blocks = (unsigned)std::min<int64_t>((rows * pieces + 255) / 256, 1 << 16);
     hipStream_t st = (hipStream_t)stream;

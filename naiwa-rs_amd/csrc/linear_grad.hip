@@ -311,14 +311,13 @@ extern "C" int naiwa_linear_input_grad(const naiwa_weights* w, const naiwa_weigh
                       w->experts, n, k, act, (const uint16_t*)pre, (const uint16_t*)pre_up, dx, dx_up, pre_ld, dx_ld,
                       dx_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0,
                       !flags && rows * k * lin_size(dx_dtype) >= kLinPast};
-    const int64_t w_bytes = lin_bytes(w), u_bytes = up ? lin_bytes(up) : 0;
-    const int64_t o_bytes = lin_span(rows, dx_ld, k, lin_size(dx_dtype)), p_bytes = lin_span(rows, pre_ld, k, 2);
-    for (const void* o : {(const void*)dx, (const void*)dx_up})
-        if (lin_overlap(o, o_bytes, dy, lin_span(rows, dy_ld, n, 2)) || lin_overlap(o, o_bytes, dy_up, lin_span(rows, dy_ld, n, 2)) ||
-            lin_overlap(o, o_bytes, a.w, w_bytes) || lin_overlap(o, o_bytes, a.u, u_bytes) ||
-            lin_overlap(o, o_bytes, pre, p_bytes) || lin_overlap(o, o_bytes, pre_up, p_bytes))
-            return NAIWA_E_INVALID;
-    if (lin_overlap(dx, o_bytes, dx_up, o_bytes)) return NAIWA_E_INVALID;
+    const Span ins[] = {span_of(dy, rows, dy_ld, n, 2),   span_of(dy_up, rows, dy_ld, n, 2),   lin_span(w), lin_span(up),
+                        span_of(pre, rows, pre_ld, k, 2), span_of(pre_up, rows, pre_ld, k, 2)};
+    const Span outs[] = {span_of(dx, rows, dx_ld, k, lin_size(dx_dtype)), span_of(dx_up, rows, dx_ld, k, lin_size(dx_dtype))};
+    for (const Span& o : outs)
+        for (const Span& in : ins)
+            if (overlap(o, in)) return NAIWA_E_INVALID;
+    if (overlap(outs[0], outs[1])) return NAIWA_E_INVALID;
     const bool direct = !((n | k) & 7) && lin_aligned(a.w, a.w_ld, a.w_stride) && lin_aligned(dy, dy_ld, 0) &&
                         (!up || (lin_aligned(a.u, a.u_ld, a.u_stride) && lin_aligned(dy_up, dy_ld, 0)));
     hipStream_t st = (hipStream_t)stream;
@@ -339,11 +338,12 @@ extern "C" int naiwa_linear_weight_grad(const void* dy, int64_t dy_ld, const voi
     const WeightArgs a{(const uint16_t*)dy, (const uint16_t*)x, dy_ld, x_ld, offsets, (uint32_t)rows, n, k, dw, ld, stride, dbias,
                        dw_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0,
                        !flags && (int64_t)experts * n * k * lin_size(dw_dtype) >= kLinPast};
-    const int64_t dy_bytes = lin_span(rows, dy_ld, n, 2), x_bytes = lin_span(rows, x_ld, k, 2);
-    const int64_t w_bytes = ((experts - 1) * stride + (n - 1) * ld + k) * lin_size(dw_dtype), b_bytes = (int64_t)experts * n * 4;
-    if (lin_overlap(dw, w_bytes, dy, dy_bytes) || lin_overlap(dw, w_bytes, x, x_bytes) || lin_overlap(dbias, b_bytes, dy, dy_bytes) ||
-        lin_overlap(dbias, b_bytes, x, x_bytes) || lin_overlap(dw, w_bytes, dbias, b_bytes))
-        return NAIWA_E_INVALID;
+    const Span ins[] = {span_of(dy, rows, dy_ld, n, 2), span_of(x, rows, x_ld, k, 2)};
+    const Span to = span_of(dw, ((experts - 1) * stride + (n - 1) * ld + k) * lin_size(dw_dtype));
+    const Span bias = span_of(dbias, (int64_t)experts * n * 4);
+    for (const Span& in : ins)
+        if (overlap(to, in) || overlap(bias, in)) return NAIWA_E_INVALID;
+    if (overlap(to, bias)) return NAIWA_E_INVALID;
     const bool direct = !((n | k) & 7) && lin_aligned(dy, dy_ld, 0) && lin_aligned(x, x_ld, 0);
     hipStream_t st = (hipStream_t)stream;
     return dtype == NAIWA_BF16 ? weight_grad<false>(a, experts, direct, st) : weight_grad<true>(a, experts, direct, st);

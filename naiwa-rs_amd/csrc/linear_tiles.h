@@ -33,6 +33,7 @@
 
 #include "../../include/naiwa_linear.h"
 #include "common.h"
+#include "spans.h"
 #include "workspace.h"
 
 #include <algorithm>
@@ -776,11 +777,6 @@ constexpr int kMaxExperts = 4096;
 static inline bool lin_aligned(const void* p, int64_t ld, int64_t stride) {
     return !(((uintptr_t)p & 15) | (ld & 7) | (stride & 7));
 }
-static inline bool lin_overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && a_bytes > 0 && b_bytes > 0 && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
-}
-static inline int64_t lin_span(int64_t rows, int64_t ld, int64_t n, int size) { return rows > 0 ? ((rows - 1) * ld + n) * size : 0; }
 static inline int lin_size(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
 // How many blocks take a tile of `steps` steps in a call of `tiles` tiles whose sums are `values` f32 values: a block a CU, of 8
 // steps at least, or of long sums two, and at most 64 MB of parts.  (One block a tile, 16 rows x 88 x 728 and 1 x 128 x 3424
@@ -859,8 +855,9 @@ static inline int lin_pair_ok(const naiwa_weights* w, const naiwa_weights* up) {
 }
 static inline int64_t lin_ld(const naiwa_weights* w) { return w->ld ? w->ld : w->k; }
 static inline int64_t lin_stride(const naiwa_weights* w) { return w->stride ? w->stride : w->n * lin_ld(w); }
-static inline int64_t lin_bytes(const naiwa_weights* w) {
-    return ((w->experts - 1) * lin_stride(w) + (w->n - 1) * lin_ld(w) + w->k) * 2;
+// From the first weight to the last.
+static inline Span lin_span(const naiwa_weights* w) {
+    return w ? span_of(w->w, ((w->experts - 1) * lin_stride(w) + (w->n - 1) * lin_ld(w) + w->k) * 2) : Span{};
 }
 
 } // namespace

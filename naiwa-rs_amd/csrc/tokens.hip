@@ -11,6 +11,7 @@
 // takes unaligned ones) with single values behind the last whole piece.
 #include "../../include/naiwa_tokens.h"
 #include "common.h"
+#include "spans.h"
 #include "workspace.h"
 
 #include <algorithm>
@@ -458,13 +459,6 @@ template <class F> void by_wave(int L, int64_t bytes, F f) {
 int size_of(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
 bool row_type(int dtype) { return dtype == NAIWA_F32 || dtype == NAIWA_BF16 || dtype == NAIWA_F16; }
 
-// Whether [a, a + bytes of T rows) and the same of b share memory.
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
-}
-int64_t span(int64_t rows, int64_t ld, int H, int size) { return rows ? ((rows - 1) * ld + H) * size : 0; }
-
 int sizes_ok(int64_t T, int k, int H) {
     if (T < 0 || k <= 0 || H <= 0) return NAIWA_E_INVALID;
     return T > INT32_MAX / k || H > kMaxH ? NAIWA_E_UNSUPPORTED : NAIWA_OK;
@@ -525,7 +519,7 @@ extern "C" int naiwa_tokens_to_experts(const void* x, int dtype, int64_t ld, con
     if (!x || !inv || !rows) return NAIWA_E_INVALID;
     const int s = size_of(dtype);
     ld = ld ? ld : H, rows_ld = rows_ld ? rows_ld : H;
-    if (overlap(x, span(T, ld, H, s), rows, span(T * k, rows_ld, H, s))) return NAIWA_E_INVALID;
+    if (overlap(span_of(x, T, ld, H, s), span_of(rows, T * k, rows_ld, H, s))) return NAIWA_E_INVALID;
     const int L = lanes_of(H, 16 / s);
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto u, auto wave, auto past) {
@@ -547,7 +541,7 @@ extern "C" int naiwa_tokens_from_experts(const void* y, int dtype, int64_t ld, c
     if (T == 0) return NAIWA_OK;
     if (!y || !inv || !out) return NAIWA_E_INVALID;
     ld = ld ? ld : H, out_ld = out_ld ? out_ld : H, w_ld = w_ld ? w_ld : k;
-    if (overlap(y, span(T * k, ld, H, size_of(dtype)), out, span(T, out_ld, H, size_of(out_dtype)))) return NAIWA_E_INVALID;
+    if (overlap(span_of(y, T * k, ld, H, size_of(dtype)), span_of(out, T, out_ld, H, size_of(out_dtype)))) return NAIWA_E_INVALID;
     const int N = 16 / size_of(dtype), L = lanes_of(H, N);
     const uint32_t parts = L == 64 ? (H + 64 * N - 1) / (64 * N) : 1;
     return by_types(dtype, out_dtype, [&](auto ty, auto to) {
@@ -576,10 +570,10 @@ extern "C" int naiwa_tokens_from_experts_backward(const void* dout, int dout_dty
     dout_ld = dout_ld ? dout_ld : H, ld = ld ? ld : H, dy_ld = dy_ld ? dy_ld : H;
     w_ld = w_ld ? w_ld : k, dw_ld = dw_ld ? dw_ld : k;
     if (dy) {
-        if (overlap(dout, span(T, dout_ld, H, size_of(dout_dtype)), dy, span(T * k, dy_ld, H, s))) return NAIWA_E_INVALID;
+        const Span to = span_of(dy, T * k, dy_ld, H, s);
+        if (overlap(span_of(dout, T, dout_ld, H, size_of(dout_dtype)), to)) return NAIWA_E_INVALID;
         // in y's place row by row, or nowhere near it
-        if (dw && !(dy == y && dy_ld == ld) && overlap(y, span(T * k, ld, H, s), dy, span(T * k, dy_ld, H, s)))
-            return NAIWA_E_INVALID;
+        if (dw && !(dy == y && dy_ld == ld) && overlap(span_of(y, T * k, ld, H, s), to)) return NAIWA_E_INVALID;
     }
     const int L = lanes_of(H, 16 / s);
     return by_types(dtype, dout_dtype, [&](auto ty, auto to) {
