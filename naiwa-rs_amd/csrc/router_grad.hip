@@ -8,6 +8,7 @@
 #include "../../include/naiwa_tokens.h"
 #include "common.h"
 #include "router_rows.h"
+#include "spans.h"
 
 #include <algorithm>
 
@@ -148,8 +149,13 @@ extern "C" int naiwa_router_topk_backward(const void* logits, int dtype, int ld,
     if (E > kMaxE || k > 32 || T > INT32_MAX / k) return NAIWA_E_UNSUPPORTED;
     if (T == 0) return NAIWA_OK;
     if (!logits || !ids || !dw || !dlogits) return NAIWA_E_INVALID;
-    if (dlogits == logits && (dld ? dld : E) != (ld ? ld : E)) return NAIWA_E_INVALID; // rows over other rows
     ld = ld ? ld : E, dld = dld ? dld : E, ids_ld = ids_ld ? ids_ld : k, dw_ld = dw_ld ? dw_ld : k;
+    // in the logits' place row by row, or apart from all that is read
+    const int size = dtype == NAIWA_BF16 ? 2 : 4;
+    const Span to = span_of(dlogits, T, dld, E, size);
+    if (!(dlogits == logits && dld == ld) && overlap(to, span_of(logits, T, ld, E, size))) return NAIWA_E_INVALID;
+    if (overlap(to, span_of(ids, T, ids_ld, k, 4)) || overlap(to, span_of(dw, T, dw_ld, k, 4)) || overlap(to, span_of(mask, T)))
+        return NAIWA_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
     const int accumulate = flags & NAIWA_TOKENS_ACCUMULATE;
     auto blocks = [&](int L) { return (unsigned)std::min<int64_t>((T * L + kThreads - 1) / kThreads, 4096); };
