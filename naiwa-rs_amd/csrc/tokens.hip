@@ -485,6 +485,14 @@ extern "C" int naiwa_expert_sort(const uint32_t* ids, int ids_ld, int64_t T, int
     }
     if (!ids || !perm || !inv) return NAIWA_E_INVALID;
     const Pairs a{ids, ids_ld ? ids_ld : k, T * k, k, E, mask};
+    const Span ins[] = {span_of(ids, T, a.ids_ld, k, 4), span_of(mask, T)};
+    const Span outs[] = {span_of(perm, a.n * 4), span_of(inv, a.n * 4), span_of(offsets, (E + 1) * 4), span_of(bad, 4)};
+    for (int i = 0; i < 4; ++i) {
+        for (const Span& in : ins)
+            if (overlap(outs[i], in)) return NAIWA_E_INVALID;
+        for (int j = 0; j < i; ++j)
+            if (overlap(outs[i], outs[j])) return NAIWA_E_INVALID;
+    }
     if (a.n <= kOne) {
         if (E <= 512)
             sort_one_kernel<16><<<1, 1024, 17 * 4 * E, st>>>(a, perm, inv, offsets, bad);
@@ -519,7 +527,8 @@ extern "C" int naiwa_tokens_to_experts(const void* x, int dtype, int64_t ld, con
     if (!x || !inv || !rows) return NAIWA_E_INVALID;
     const int s = size_of(dtype);
     ld = ld ? ld : H, rows_ld = rows_ld ? rows_ld : H;
-    if (overlap(span_of(x, T, ld, H, s), span_of(rows, T * k, rows_ld, H, s))) return NAIWA_E_INVALID;
+    const Span to = span_of(rows, T * k, rows_ld, H, s);
+    if (overlap(to, span_of(x, T, ld, H, s)) || overlap(to, span_of(inv, T * k * 4))) return NAIWA_E_INVALID;
     const int L = lanes_of(H, 16 / s);
     hipStream_t st = (hipStream_t)stream;
     auto go = [&](auto u, auto wave, auto past) {
@@ -541,7 +550,10 @@ extern "C" int naiwa_tokens_from_experts(const void* y, int dtype, int64_t ld, c
     if (T == 0) return NAIWA_OK;
     if (!y || !inv || !out) return NAIWA_E_INVALID;
     ld = ld ? ld : H, out_ld = out_ld ? out_ld : H, w_ld = w_ld ? w_ld : k;
-    if (overlap(span_of(y, T * k, ld, H, size_of(dtype)), span_of(out, T, out_ld, H, size_of(out_dtype)))) return NAIWA_E_INVALID;
+    const Span sums = span_of(out, T, out_ld, H, size_of(out_dtype));
+    if (overlap(sums, span_of(y, T * k, ld, H, size_of(dtype))) || overlap(sums, span_of(inv, T * k * 4)) ||
+        overlap(sums, span_of(w, T, w_ld, k, 4)))
+        return NAIWA_E_INVALID;
     const int N = 16 / size_of(dtype), L = lanes_of(H, N);
     const uint32_t parts = L == 64 ? (H + 64 * N - 1) / (64 * N) : 1;
     return by_types(dtype, out_dtype, [&](auto ty, auto to) {
@@ -569,12 +581,14 @@ extern "C" int naiwa_tokens_from_experts_backward(const void* dout, int dout_dty
     const int s = size_of(dtype);
     dout_ld = dout_ld ? dout_ld : H, ld = ld ? ld : H, dy_ld = dy_ld ? dy_ld : H;
     w_ld = w_ld ? w_ld : k, dw_ld = dw_ld ? dw_ld : k;
-    if (dy) {
-        const Span to = span_of(dy, T * k, dy_ld, H, s);
-        if (overlap(span_of(dout, T, dout_ld, H, size_of(dout_dtype)), to)) return NAIWA_E_INVALID;
-        // in y's place row by row, or nowhere near it
-        if (dw && !(dy == y && dy_ld == ld) && overlap(span_of(y, T * k, ld, H, s), to)) return NAIWA_E_INVALID;
-    }
+    const Span rows = span_of(dw ? y : nullptr, T * k, ld, H, s), drows = span_of(dy, T * k, dy_ld, H, s);
+    const Span sums = span_of(dout, T, dout_ld, H, size_of(dout_dtype)), dots = span_of(dw, T, dw_ld, k, 4);
+    for (const Span& out : {drows, dots})
+        for (const Span& in : {sums, span_of(inv, T * k * 4), span_of(w, T, w_ld, k, 4)})
+            if (overlap(out, in)) return NAIWA_E_INVALID;
+    if (overlap(dots, rows) || overlap(dots, drows)) return NAIWA_E_INVALID;
+    // in y's place row by row, or nowhere near it
+    if (!(dy == y && dy_ld == ld) && overlap(drows, rows)) return NAIWA_E_INVALID;
     const int L = lanes_of(H, 16 / s);
     return by_types(dtype, dout_dtype, [&](auto ty, auto to) {
         typedef decltype(ty) Y;
