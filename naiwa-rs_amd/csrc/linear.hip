@@ -332,7 +332,8 @@ extern "C" int naiwa_linear(const naiwa_weights* w, const naiwa_weights* up, con
     // an output is written where nothing else is read or written
     const int so = lin_size(out_dtype);
     const int64_t b_bytes = (int64_t)w->experts * n * 4;
-    const Span ins[] = {span_of(x, rows, x_ld, k, 2), lin_span(w), lin_span(up), span_of(a.b, b_bytes), span_of(a.c, b_bytes)};
+    const Span ins[] = {span_of(x, rows, x_ld, k, 2), lin_span(w), lin_span(up), span_of(a.b, b_bytes), span_of(a.c, b_bytes),
+                        lin_span(offsets, w->experts)};
     const Span outs[] = {span_of(out, rows, out_ld, n, so), span_of(pre, rows, pre_ld, n, 2), span_of(pre_up, rows, pre_ld, n, 2)};
     const Span added = span_of(residual, rows, residual_ld, n, so);
     for (int i = 0; i < 3; ++i) {

@@ -311,8 +311,8 @@ extern "C" int naiwa_linear_input_grad(const naiwa_weights* w, const naiwa_weigh
                       w->experts, n, k, act, (const uint16_t*)pre, (const uint16_t*)pre_up, dx, dx_up, pre_ld, dx_ld,
                       dx_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0,
                       !flags && rows * k * lin_size(dx_dtype) >= kLinPast};
-    const Span ins[] = {span_of(dy, rows, dy_ld, n, 2),   span_of(dy_up, rows, dy_ld, n, 2),   lin_span(w), lin_span(up),
-                        span_of(pre, rows, pre_ld, k, 2), span_of(pre_up, rows, pre_ld, k, 2)};
+    const Span ins[] = {span_of(dy, rows, dy_ld, n, 2), span_of(dy_up, rows, dy_ld, n, 2), lin_span(w), lin_span(up),
+                        span_of(pre, rows, pre_ld, k, 2), span_of(pre_up, rows, pre_ld, k, 2), lin_span(offsets, w->experts)};
     const Span outs[] = {span_of(dx, rows, dx_ld, k, lin_size(dx_dtype)), span_of(dx_up, rows, dx_ld, k, lin_size(dx_dtype))};
     for (const Span& o : outs)
         for (const Span& in : ins)
@@ -338,7 +338,7 @@ extern "C" int naiwa_linear_weight_grad(const void* dy, int64_t dy_ld, const voi
     const WeightArgs a{(const uint16_t*)dy, (const uint16_t*)x, dy_ld, x_ld, offsets, (uint32_t)rows, n, k, dw, ld, stride, dbias,
                        dw_dtype == NAIWA_F32, (flags & NAIWA_LINEAR_ACCUMULATE) != 0,
                        !flags && (int64_t)experts * n * k * lin_size(dw_dtype) >= kLinPast};
-    const Span ins[] = {span_of(dy, rows, dy_ld, n, 2), span_of(x, rows, x_ld, k, 2)};
+    const Span ins[] = {span_of(dy, rows, dy_ld, n, 2), span_of(x, rows, x_ld, k, 2), lin_span(offsets, experts)};
     const Span to = span_of(dw, ((experts - 1) * stride + (n - 1) * ld + k) * lin_size(dw_dtype));
     const Span bias = span_of(dbias, (int64_t)experts * n * 4);
     for (const Span& in : ins)

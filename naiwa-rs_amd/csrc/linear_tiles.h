@@ -855,6 +855,7 @@ static inline int lin_pair_ok(const naiwa_weights* w, const naiwa_weights* up) {
 }
 static inline int64_t lin_ld(const naiwa_weights* w) { return w->ld ? w->ld : w->k; }
 static inline int64_t lin_stride(const naiwa_weights* w) { return w->stride ? w->stride : w->n * lin_ld(w); }
+static inline Span lin_span(const uint32_t* offsets, int experts) { return span_of(offsets, ((int64_t)experts + 1) * 4); }
 // From the first weight to the last.
 static inline Span lin_span(const naiwa_weights* w) {
     return w ? span_of(w->w, ((w->experts - 1) * lin_stride(w) + (w->n - 1) * lin_ld(w) + w->k) * 2) : Span{};
