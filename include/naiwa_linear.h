@@ -25,7 +25,13 @@
  * inputs or each other, unless stated (NAIWA_E_INVALID); columns side by side in rows of one length in bytes (the
  * halves of a gate-and-up buffer) do not.  rows = 0 returns at once (naiwa_linear_weight_grad: with zeros
  * written).  rows <= 2^31 - 1 and row lengths (n and k with them) <= 2^21 (NAIWA_E_UNSUPPORTED),
- * experts <= 4096.  No counterpart in the reference, whose expert weights are quantised.
+ * experts <= 4096.
+ *
+ * All three products leave parts of long sums in scratch where a call has few tiles: a buffer of the
+ * stream's own, which only grows (to 64 MB; the first call that needs more allocates, with a device
+ * sync), so that calls on different streams need no order.  Captured calls have another, which is kept
+ * until the process ends and which all graphs captured on the stream share: their replays have to be
+ * ordered.  A stream is destroyed behind its calls.  No counterpart in the reference, whose expert weights are quantised.
  */
 #ifndef NAIWA_LINEAR_H
 #define NAIWA_LINEAR_H
@@ -72,9 +78,7 @@ int naiwa_linear_input_grad(const naiwa_weights* w, const naiwa_weights* up, con
 /* dw [experts, n, k] (f32 or dtype: dw_dtype; ld and stride as in naiwa_weights) and dbias
  * f32 [experts, n] (NULL: not wanted) from dy [rows, n] and x [rows, k] of dtype.  Experts
  * without rows get zeros.  flags NAIWA_LINEAR_ACCUMULATE: dw += and dbias +=, in f32,
- * rounded once.  Calls of few and long sums share one grow-only scratch buffer per device (as
- * naiwa_linear and naiwa_linear_input_grad of few outputs do): on different streams they have to be ordered, and a
- * graph's replays too.  Captured calls keep the buffer that they were given. */
+ * rounded once. */
 int naiwa_linear_weight_grad(const void* dy, int64_t dy_ld, const void* x, int64_t x_ld, int dtype,
                              const uint32_t* offsets, int experts, int64_t rows, int n, int k, void* dw, int dw_dtype,
                              int64_t ld, int64_t stride, float* dbias, int flags, int64_t stream);

@@ -36,9 +36,9 @@ extern "C" {
 /* ids u32 [T, k] (rows ids_ld entries apart, 0: k), mask u8 [T] or NULL ->
  * perm u32 [T * k] (the first offsets[E] entries are written), inv u32 [T, k], offsets
  * u32 [E + 1].  *bad (NULL: not reported) = ids >= E among the valid tokens.  E <= 4096,
- * T * k <= 2^31 - 1.  Calls of more than 4096 pairs share one grow-only scratch buffer
- * per device: on different streams they have to be ordered, and a graph's replays too.
- * Captured calls keep the buffer that they were given. */
+ * T * k <= 2^31 - 1.  Calls of more than 4096 pairs use a scratch buffer of the stream's
+ * own, which only grows; captured ones have another, which all graphs captured on the
+ * stream share: their replays have to be ordered.  A stream is destroyed behind its calls. */
 int naiwa_expert_sort(const uint32_t* ids, int ids_ld, int64_t T, int k, int E, const uint8_t* mask, uint32_t* perm,
                       uint32_t* inv, uint32_t* offsets, uint32_t* bad, int64_t stream);
 

@@ -792,7 +792,7 @@ static inline int lin_parts(int splits, int planes, int64_t plane, hipStream_t s
     *p = Parts{nullptr, splits, planes, plane};
     if (splits == 1) return NAIWA_OK;
     int rc = 0;
-    p->p = (float*)naiwa_scratch(NAIWA_SCRATCH_LINEAR, (size_t)splits * planes * plane * 4, &rc, st);
+    p->p = (float*)naiwa_scratch_of_stream(NAIWA_SCRATCH_LINEAR, (size_t)splits * planes * plane * 4, &rc, st);
     return p->p ? NAIWA_OK : rc;
 }
 // Blocks of 256 threads that finish so many quads of sums, `group` threads each.

@@ -5,6 +5,7 @@
 
 #include <mutex>
 #include <string.h>
+#include <vector>
 
 #include "common.h"
 #include "mxfp4.h"
@@ -12,11 +13,23 @@
 
 namespace {
 constexpr int kMaxDevices = 64;
+struct StreamScratch { // of the calls on one stream, those under capture apart
+    hipStream_t stream;
+    bool capturing;
+    NaiwaScratch s;
+};
 std::mutex g_scratch_mu;
 NaiwaScratch g_scratch[kMaxDevices][NAIWA_SCRATCH_TAGS];
-} // namespace
+std::vector<StreamScratch> g_of_streams[kMaxDevices][NAIWA_SCRATCH_TAGS];
 
-static void* scratch(int tag, size_t bytes, int* rc, bool* fresh, bool capturing) {
+bool is_capturing(hipStream_t stream) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone; // (the null stream cannot be captured)
+    if (stream && hipStreamIsCapturing(stream, &st) != hipSuccess) st = hipStreamCaptureStatusNone;
+    return st != hipStreamCaptureStatusNone;
+}
+
+// find(device): the buffer that the call takes, which grows where it is too small.
+template <class Find> void* scratch(Find find, int tag, size_t bytes, int* rc, bool* fresh, bool capturing) {
     if (fresh) *fresh = false;
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -25,7 +38,7 @@ static void* scratch(int tag, size_t bytes, int* rc, bool* fresh, bool capturing
         return nullptr;
     }
     std::lock_guard<std::mutex> lock(g_scratch_mu);
-    NaiwaScratch& s = g_scratch[dev][tag];
+    NaiwaScratch& s = find(dev);
     if (s.bytes < bytes) {
         size_t want = bytes < 4096 ? 4096 : bytes;
         want = (want + 255) & ~size_t(255);
@@ -39,7 +52,12 @@ static void* scratch(int tag, size_t bytes, int* rc, bool* fresh, bool capturing
             (void)hipFree(s.ptr);
             s = NaiwaScratch{};
         }
-        if (hipMalloc(&p, want) != hipSuccess) {
+        // (an allocation is no part of a graph, but a capture that is not relaxed refuses it)
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        if (capturing) (void)hipThreadExchangeStreamCaptureMode(&mode);
+        e = hipMalloc(&p, want);
+        if (capturing) (void)hipThreadExchangeStreamCaptureMode(&mode);
+        if (e != hipSuccess) {
             *rc = NAIWA_E_NOMEM;
             return nullptr;
         }
@@ -50,13 +68,26 @@ static void* scratch(int tag, size_t bytes, int* rc, bool* fresh, bool capturing
     *rc = NAIWA_OK;
     return s.ptr;
 }
+} // namespace
 
-void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh) { return scratch(tag, bytes, rc, fresh, false); }
+void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh) {
+    return scratch([&](int dev) -> NaiwaScratch& { return g_scratch[dev][tag]; }, tag, bytes, rc, fresh, false);
+}
 
 void* naiwa_scratch(int tag, size_t bytes, int* rc, hipStream_t stream) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone; // (the null stream cannot be captured)
-    if (stream && hipStreamIsCapturing(stream, &st) != hipSuccess) st = hipStreamCaptureStatusNone;
-    return scratch(tag, bytes, rc, nullptr, st != hipStreamCaptureStatusNone);
+    return scratch([&](int dev) -> NaiwaScratch& { return g_scratch[dev][tag]; }, tag, bytes, rc, nullptr, is_capturing(stream));
+}
+
+void* naiwa_scratch_of_stream(int tag, size_t bytes, int* rc, hipStream_t stream) {
+    const bool capturing = is_capturing(stream);
+    auto find = [&](int dev) -> NaiwaScratch& {
+        std::vector<StreamScratch>& all = g_of_streams[dev][tag];
+        for (StreamScratch& x : all)
+            if (x.stream == stream && x.capturing == capturing) return x.s;
+        all.push_back({stream, capturing, {}});
+        return all.back().s;
+    };
+    return scratch(find, tag, bytes, rc, nullptr, capturing);
 }
 
 extern "C" {

@@ -505,7 +505,7 @@ extern "C" int naiwa_expert_sort(const uint32_t* ids, int ids_ld, int64_t T, int
     const int64_t run = std::max<int64_t>(kRunLeast, (least + unit - 1) / unit * unit);
     const int blocks = (int)((a.n + run - 1) / run);
     int rc = 0;
-    uint32_t* ws = (uint32_t*)naiwa_scratch(NAIWA_SCRATCH_SORT, ((size_t)blocks * E + E + blocks) * 4, &rc, st);
+    uint32_t* ws = (uint32_t*)naiwa_scratch_of_stream(NAIWA_SCRATCH_SORT, ((size_t)blocks * E + E + blocks) * 4, &rc, st);
     if (!ws) return rc;
     uint32_t *totals = ws + (size_t)blocks * E, *badof = totals + E;
     auto go = [&](auto waves) { // fewer waves where their counts would pass 64 KB of LDS
