@@ -218,26 +218,32 @@ template <bool F16, bool PAIR, int FJ> int launch_few(const ForwardArgs& a, hipS
     return naiwa_hip_rc(hipGetLastError());
 }
 
-// Which kernel a call takes (experts 0: dense).
+// Which kernel a call takes (experts 0: dense; odd: rows at addresses that are no multiples of 4 bytes, which 16-byte reads are slow at).
 enum { kFew16 = kKinds, kFew32, kFew64 };
-int lin_forward_kind(int64_t rows, int experts, int64_t n, int64_t k, bool pair) {
+int lin_forward_kind(int64_t rows, int experts, int64_t n, int64_t k, bool pair, bool odd) {
     const bool grouped = experts > 0;
     const int64_t avg = grouped ? rows / experts : rows, bytes = 2 * std::max(experts, 1) * n * k * (pair ? 2 : 1);
     const int64_t strips = (n + (pair ? 15 : 31)) / (pair ? 16 : 32);
     // Straight from memory while a strip's rows are one tile's or what more read again is in the caches, and a block a CU takes it.
+    // A block reads its whole sum, so long ones are the tiles' parts.  Both take as long at 4096 values, odd rows at 1500 (straight
+    // from memory and tiles, us: 1 row x 16 x 4096 7.7 and 8.4, 8192 12.9 and 8.1, 262144 344 and 44; 16 rows x 1003 x 4096 13.2 and
+    // 13.3, 8192 23.6 and 9.9; 1 row x 200 x 1001 7.9 and 10.0, 2501 16.6 and 10.1, 4097 28.4 and 10.3).
+    const int64_t longest = odd ? 1536 : 4096;
     if (bytes <= (16 << 20)) {
         for (int f = 0; f < 3; ++f)
-            if (strips * lin_j_alike(rows, experts, grouped, 16 << f) <= 256) return kFew16 + f;
+            if (k <= longest && strips * lin_j_alike(rows, experts, grouped, 16 << f) <= 256) return kFew16 + f;
     } else if (avg <= 2 && strips * std::min<int64_t>(std::max(experts, 1), rows) >= 256) {
-        return kFew16;
+        // Every CU has blocks, so long sums do not matter here, but odd rows do where there are many (8192 x 1001 gated 12.9 and
+        // 14.7, 14336 x 1001 gated 22.9 and 19.1, 64 experts of 1000 x 1001 42 and 26, 14336 x 4097 53 and 27; 4096 21 and 22).
+        if (!odd || (k <= longest && bytes <= (32 << 20))) return kFew16;
     }
     // (Empty places cost little here, where a tile's rows are read whole: 16 experts of 7600 x 1568 with 73 rows take 213 us in
     // 256 x 256 tiles, 239 in 128 x 128.)
     return lin_kind(k, avg, (n * (pair ? 2 : 1) + 255) / 256 * lin_j_alike(rows, experts, grouped, 256), true);
 }
 
-template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, hipStream_t st) {
-    const int kind = lin_forward_kind(a.rows, a.offsets ? a.experts : 0, a.n, a.k, PAIR);
+template <bool F16, bool PAIR> int forward(const ForwardArgs& a, bool direct, bool odd, hipStream_t st) {
+    const int kind = lin_forward_kind(a.rows, a.offsets ? a.experts : 0, a.n, a.k, PAIR, odd);
     if (kind == kFew16) return launch_few<F16, PAIR, 1>(a, st);
     if (kind == kFew32) return launch_few<F16, PAIR, 2>(a, st);
     if (kind == kFew64) return launch_few<F16, PAIR, 4>(a, st);
@@ -345,9 +351,10 @@ extern "C" int naiwa_linear(const naiwa_weights* w, const naiwa_weights* up, con
     }
     const bool direct = !(k & 7) && lin_aligned(a.w, a.w_ld, a.w_stride) && lin_aligned(a.x, x_ld, 0) &&
                         (!up || lin_aligned(a.u, a.u_ld, a.u_stride));
+    const bool odd = lin_odd(a.w, a.w_ld, a.w_stride) || lin_odd(a.x, x_ld, 0) || (up && lin_odd(a.u, a.u_ld, a.u_stride));
     hipStream_t st = (hipStream_t)stream;
-    if (w->dtype == NAIWA_BF16) return up ? forward<false, true>(a, direct, st) : forward<false, false>(a, direct, st);
-    return up ? forward<true, true>(a, direct, st) : forward<true, false>(a, direct, st);
+    if (w->dtype == NAIWA_BF16) return up ? forward<false, true>(a, direct, odd, st) : forward<false, false>(a, direct, odd, st);
+    return up ? forward<true, true>(a, direct, odd, st) : forward<true, false>(a, direct, odd, st);
 }
 
 extern "C" int naiwa_act_backward(const void* dout, const void* pre, const void* pre_up, int dtype, int64_t rows, int n,
@@ -380,7 +387,8 @@ extern "C" int naiwa_act_backward(const void* dout, const void* pre, const void*
 }
 
 // Which kernel a call with aligned rows takes (experts 0: one matrix for all rows), for tests: kThin ... kBig of linear_tiles.h,
-// behind them those that read rows straight from memory, 16, 32 or 64 at a time.
-extern "C" int naiwa_linear_kind(int64_t rows, int experts, int n, int k, int pair) {
-    return lin_forward_kind(rows, experts, n, k, pair != 0);
+// behind them those that read rows straight from memory, 16, 32 or 64 at a time.  how: 1 a gated product, 2 odd rows (of which only
+// the latter kinds are told apart), or both.
+extern "C" int naiwa_linear_kind(int64_t rows, int experts, int n, int k, int how) {
+    return lin_forward_kind(rows, experts, n, k, how & 1, how & 2);
 }

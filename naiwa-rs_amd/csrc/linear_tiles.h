@@ -777,6 +777,8 @@ constexpr int kMaxExperts = 4096;
 static inline bool lin_aligned(const void* p, int64_t ld, int64_t stride) {
     return !(((uintptr_t)p & 15) | (ld & 7) | (stride & 7));
 }
+// Rows at addresses that are no multiples of 4 bytes.
+static inline bool lin_odd(const void* p, int64_t ld, int64_t stride) { return ((uintptr_t)p & 3) | (ld & 1) | (stride & 1); }
 static inline int lin_size(int dtype) { return dtype == NAIWA_F32 ? 4 : 2; }
 // How many blocks take a tile of `steps` steps in a call of `tiles` tiles whose sums are `values` f32 values: a block a CU, of 8
 // steps at least, or of long sums two, and at most 64 MB of parts.  (One block a tile, 16 rows x 88 x 728 and 1 x 128 x 3424
