@@ -15,7 +15,9 @@
  * Values are bf16 or f16 (x, the weights and the gradients the same), bias f32, out f32 or
  * the values' type.  Products are exact, sums f32 on the matrix cores, everything behind
  * them f32, each result rounded once.  A NaN or an infinity stays in the results that its
- * row and its weights have a part in.  Results do not depend on the run.
+ * row and its weights have a part in.  Results do not depend on the run.  SiLU(v) is right to
+ * (1.3 |v| + 6) 2^-24 of itself, GELU(v), with u = 1.6 (v + 0.045 v^3), to (8.3 |u| + 6) 2^-24 of itself:
+ * as far as a few half steps of v move them; values below 2^-119 may be 0.
  *
  * offsets u32 [experts + 1] (device; NULL: one expert, all rows): rows offsets[e] ..
  * offsets[e + 1] - 1 are expert e's, at most `rows`; entries past `rows` count as `rows`.

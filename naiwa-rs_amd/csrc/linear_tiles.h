@@ -698,6 +698,8 @@ template <bool PAIR> __device__ __forceinline__ void PartOut<PAIR>::store(int j,
 }
 
 // 1 / (1 + exp(-v)): SiLU is v times it, GELU's tanh form v times that of twice tanh's argument (1 + tanh x = 2 / (1 + exp(-2 x))).
+// exp as a power of 2 errs by 1.22 |v| + 2 units of 2^-24, the sum by 1, the reciprocal by 2 (and is 0 below 2^-126): in
+// the negative tail too, where 1 + tanh x in f32 would have no digits left.
 __device__ __forceinline__ float lin_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 __device__ __forceinline__ float gelu_twice(float v) { return 1.5957691216057308f * (v + 0.044715f * v * v * v); }
 
