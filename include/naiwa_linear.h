@@ -27,7 +27,8 @@
  * inputs or each other, unless stated (NAIWA_E_INVALID); columns side by side in rows of one length in bytes (the
  * halves of a gate-and-up buffer) do not.  rows = 0 returns at once (naiwa_linear_weight_grad: with zeros
  * written).  rows <= 2^31 - 1 and row lengths (n and k with them) <= 2^21 (NAIWA_E_UNSUPPORTED),
- * experts <= 4096.
+ * experts <= 4096; and the tiles of a call have to fit one launch's 2^32 threads (NAIWA_E_UNSUPPORTED otherwise):
+ * those of 2^29 rows of n <= 128 do, or 512 experts' weight gradients of n <= 128 and k <= 2^20.
  *
  * All three products leave parts of long sums in scratch where a call has few tiles: a buffer of the
  * stream's own, which only grows (to 64 MB; the first call that needs more allocates, with a device
