@@ -62,9 +62,11 @@ template <bool F16> struct InputOut {
     }
 };
 
-// dx = dy W (+ dy_up U, the sum going on through both).  64 experts of 1408 x 2048 x 2 with 384 rows each take 337 to 355 us, the
+// dx = dy W (+ dy_up U, the sum going on through both).  64 experts of 1408 x 2048 x 2 with 384 rows each take 325 to 355 us, the
 // products alone at a large library product's rate 210: the rows fill three quarters of the 256-row tiles, 4.06 rounds of blocks
 // take as long as 5, and a step takes 1.6 us as in the forward (the tiles' rows coming out of L2).
+// One matrix of 4096 x 14336 and 4096 rows takes 381 (1.26 PFLOP/s), 14336 x 4096 339.  What follows the product, 64 experts of
+// 2048 x 1408 with 384 rows: 193 alone, 242 with pre, 276 with pre and pre_up (208 MB more to read and write, 40 at a copy's rate).
 template <class S, bool DUAL>
 __global__ void __launch_bounds__(S::TH, 2)
 input_grad_kernel(InputArgs a, uint32_t nI, Parts parts) {

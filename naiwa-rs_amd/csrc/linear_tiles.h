@@ -11,13 +11,14 @@
 // behind the last of c ask for an address out of range, and so do steps behind the last (the counted
 // waits stay the same to the end).  The kinds of block:
 //   8 waves, 256 x 256, steps of 64, all of a CU's LDS.  The waves are two groups, one wave of each on a SIMD, that
-//     take turns in reading and multiplying (setprio and a barrier a phase).  4096 x 4096 x 14336 takes 345 to 375 us,
+//     take turns in reading and multiplying (setprio and a barrier a phase).  4096 x 4096 x 14336 takes 340 to 375 us,
 //     1.3 to 1.4 PFLOP/s.  What bounds it is how fast rows come out of L2 (with the copies left out it took 233 us, without the
 //     products as long as with them): hence whole 128-byte lines, three buffers of I and two of J, and copies spread
 //     over the phases.  Leaving out the products and copies of a tile's empty rows gained nothing.
-//   4 waves, 128 x 128, steps of 32 in a ring of 4 or 2, two or three blocks a CU: in step t a wave multiplies what it read
-//     of step t, reads step t + 1 and starts the copies of step t + 4 (t + 2), interleaved; one barrier a step.
-//     Or 128 x 32, steps of 64, for few rows.
+//   4 waves, 128 x 128, steps of 32 in a ring of 4 (64 KB, two blocks a CU) or 2 (three, by registers): in step t a wave multiplies
+//     what it read of step t, reads step t + 1 and starts the copies of step t + 4 (t + 2), interleaved; one barrier a step.
+//     Or 128 x 32, steps of 64 in a ring of 4 (80 KB, two blocks a CU), for few rows.
+//   4 waves, 128 x 128 or 128 x 64, steps of 32 in a ring of 2, for rows that are not aligned (two or three blocks a CU).
 // The XCDs begin at different steps and go round (turn_of_block): reading the same columns at a time they meet at
 // the same memory channels (4096 x 4096 x 14336 403 -> 389 us, the weights' gradient of 64 experts 332 -> 286).
 // Both layouts keep 16-byte pieces whole and permute them so that no two lanes of a read share a bank (the LDS takes
@@ -807,11 +808,14 @@ constexpr int64_t kManySteps = 2500; // steps of 64 of 256 x 256 tiles, 10 a CU
 // Which blocks a call takes: 4 waves on 128 x 32 (steps of 64), on 128 x 128 with a ring of 2 or of 4, 8 waves on 256 x 256.
 enum { kThin, kShort, kMid, kBig, kKinds };
 // For a contraction of so many values, segments of `rows` rows on average and `tiles` 256 x 256 tiles; `packed`: few enough of
-// the tiles' places are empty.  All times in us.
-// - 32 rows or fewer: thin blocks hold less of nothing, and more of them a CU ask for weights (thin and 128 x 128: gated, 64
+// the tiles' places are empty.  Segments lie on the device, so their average speaks for all of them: the figures here are of
+// segments of unequal popularity (logits N(0, 0.5) apart).  With all 2048 rows of 64 experts of 1408 x 2048 one expert's, their
+// forward and input gradient take 34 and 32 in thin tiles, one matrix's 32 in 128 x 128.  All times in us.
+// - 32 rows or fewer: thin blocks hold less of nothing, so that a step copies and multiplies 160 rows and not 256, and have 64
+//   values of a weight's row a step in flight and not 32, two a CU like 128 x 128 (thin and 128 x 128: gated, 64
 //   experts of 1408 x 2048 with 16 rows each 136 and 150, 8 of 14336 x 4096 329 and 363, one of 14336 x 4096 22 and 26; 48 rows 180
 //   and 173, 458 and 413; input gradients of 60 experts of 1000 x 1000 with 16 rows 24 and 29).
-// - A short sum hardly goes round a ring of 4, and a ring of 2 leaves room for twice the blocks, whose epilogues overlap (ring of 2,
+// - A short sum hardly goes round a ring of 4, and a ring of 2 leaves room for three blocks and not two, whose epilogues overlap (ring of 2,
 //   of 4, and 256 x 256: 16384 rows x 4096 x 64 62, 87 and 89, 7827 x 1392 x 392 28, 34 and 30, 16 experts of 576 x 1704 with 850 rows
 //   67, 75 and 55, input gradients of 64 experts of 368 x 608 with 1946 rows 134, 145 and 153, 1551 x 672 x 2520 20, 21 and 28).
 // - 256 x 256 where tiles are many or their sums long (128 and 256 wide: 1043 rows x 2920 x 584 gated 23 and 27, 555 rows of 16

@@ -5,6 +5,8 @@
 //
 // 16 lanes take a row of up to 128 experts and 16 chosen (64 lanes a longer one): its values stay in registers.
 // Calls that add to a gradient where only chosen experts have one touch those alone.
+// 32768 rows of 128, us (f32 and bf16): over the chosen 9.0 and 8.2, added 7.3 and 5.1; over all experts 10.7 and 9.8, added 11.2
+// and 10.0, of 6.9 and 3.7 (added 10.2 and 5.3) at a copy's rate; a launch takes 3.
 #include "../../include/naiwa_tokens.h"
 #include "common.h"
 #include "router_rows.h"

@@ -5,7 +5,8 @@
 - ``Weights``, ``linear``, ``linear_input_grad``, ``linear_weight_grad``, ``act_backward``
   (include/naiwa_linear.h).
 
-Arguments that name memory are device pointers or ``DeviceBuffer``s.  A training step of a
+Arguments that name memory are device pointers or ``DeviceBuffer``s.  Calls on different streams need no order (long sorts and
+products with parts of sums have scratch of the stream's own), replays of graphs that were captured on one stream do.  A training step of a
 MoE layer over them: router_topk, expert_sort, tokens_to_experts, linear (gate and up),
 linear (down), tokens_from_experts; then the backwards in the opposite order.
 """
