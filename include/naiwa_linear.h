@@ -33,8 +33,10 @@
  * All three products leave parts of long sums in scratch where a call has few tiles: a buffer of the
  * stream's own, which only grows (to 64 MB; the first call that needs more allocates, with a device
  * sync), so that calls on different streams need no order.  Captured calls have another, which is kept
- * until the process ends and which all graphs captured on the stream share: their replays have to be
- * ordered.  A stream is destroyed behind its calls.  No counterpart in the reference, whose expert weights are quantised.
+ * until the process ends and which all graphs captured on the stream (or on one made after its
+ * destruction) share: their replays have to be ordered.  A stream is destroyed behind its calls.
+ *
+ * No counterpart in the reference, whose expert weights are quantised.
  */
 #ifndef NAIWA_LINEAR_H
 #define NAIWA_LINEAR_H

@@ -18,9 +18,11 @@
  * Row values are f32, bf16 or f16; products and sums are f32, each result rounded once.
  * Results do not depend on the run.  Row lengths (ld) are in values, 0: tightly packed.
  * T * k <= 2^31 - 1, H <= 2^24, row lengths <= 2^28.  Inputs and outputs may not overlap
- * unless stated (NAIWA_E_INVALID); columns side by side in rows of one length in bytes do not.  Calls of no tokens return at once (naiwa_expert_sort then sets its offsets to 0).  Sizes and pointers are checked
- * (NAIWA_E_INVALID; NAIWA_E_UNSUPPORTED past a limit or for another type); entries of
- * inv and offsets that lie outside the T * k rows count as NAIWA_NO_ROW.
+ * unless stated (NAIWA_E_INVALID); columns side by side in rows of one length in bytes do
+ * not.  Calls of no tokens return at once (naiwa_expert_sort then sets its offsets to 0).
+ * Sizes and pointers are checked (NAIWA_E_INVALID; NAIWA_E_UNSUPPORTED past a limit or for
+ * another type); entries of inv and offsets that lie outside the T * k rows count as
+ * NAIWA_NO_ROW.
  */
 #ifndef NAIWA_TOKENS_H
 #define NAIWA_TOKENS_H
@@ -38,7 +40,8 @@ extern "C" {
  * u32 [E + 1].  *bad (NULL: not reported) = ids >= E among the valid tokens.  E <= 4096,
  * T * k <= 2^31 - 1.  Calls of more than 4096 pairs use a scratch buffer of the stream's
  * own, which only grows; captured ones have another, which all graphs captured on the
- * stream share: their replays have to be ordered.  A stream is destroyed behind its calls. */
+ * stream (or on one made after its destruction) share: their replays have to be ordered.
+ * A stream is destroyed behind its calls. */
 int naiwa_expert_sort(const uint32_t* ids, int ids_ld, int64_t T, int k, int E, const uint8_t* mask, uint32_t* perm,
                       uint32_t* inv, uint32_t* offsets, uint32_t* bad, int64_t stream);
 

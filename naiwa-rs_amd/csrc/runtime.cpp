@@ -4,8 +4,8 @@
 #include <hip/hip_runtime.h>
 
 #include <mutex>
+#include <new>
 #include <string.h>
-#include <vector>
 
 #include "common.h"
 #include "mxfp4.h"
@@ -17,10 +17,11 @@ struct StreamScratch { // of the calls on one stream, those under capture apart
     hipStream_t stream;
     bool capturing;
     NaiwaScratch s;
+    StreamScratch* next;
 };
 std::mutex g_scratch_mu;
 NaiwaScratch g_scratch[kMaxDevices][NAIWA_SCRATCH_TAGS];
-std::vector<StreamScratch> g_of_streams[kMaxDevices][NAIWA_SCRATCH_TAGS];
+StreamScratch* g_of_streams[kMaxDevices][NAIWA_SCRATCH_TAGS];
 
 bool is_capturing(hipStream_t stream) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone; // (the null stream cannot be captured)
@@ -28,7 +29,7 @@ bool is_capturing(hipStream_t stream) {
     return st != hipStreamCaptureStatusNone;
 }
 
-// find(device): the buffer that the call takes, which grows where it is too small.
+// find(device): the buffer that the call takes (NULL: no memory for one), which grows where it is too small.
 template <class Find> void* scratch(Find find, int tag, size_t bytes, int* rc, bool* fresh, bool capturing) {
     if (fresh) *fresh = false;
     int dev = 0;
@@ -38,7 +39,12 @@ template <class Find> void* scratch(Find find, int tag, size_t bytes, int* rc, b
         return nullptr;
     }
     std::lock_guard<std::mutex> lock(g_scratch_mu);
-    NaiwaScratch& s = find(dev);
+    NaiwaScratch* found = find(dev);
+    if (!found) {
+        *rc = NAIWA_E_NOMEM;
+        return nullptr;
+    }
+    NaiwaScratch& s = *found;
     if (s.bytes < bytes) {
         size_t want = bytes < 4096 ? 4096 : bytes;
         want = (want + 255) & ~size_t(255);
@@ -71,21 +77,23 @@ template <class Find> void* scratch(Find find, int tag, size_t bytes, int* rc, b
 } // namespace
 
 void* naiwa_scratch(int tag, size_t bytes, int* rc, bool* fresh) {
-    return scratch([&](int dev) -> NaiwaScratch& { return g_scratch[dev][tag]; }, tag, bytes, rc, fresh, false);
+    return scratch([&](int dev) { return &g_scratch[dev][tag]; }, tag, bytes, rc, fresh, false);
 }
 
 void* naiwa_scratch(int tag, size_t bytes, int* rc, hipStream_t stream) {
-    return scratch([&](int dev) -> NaiwaScratch& { return g_scratch[dev][tag]; }, tag, bytes, rc, nullptr, is_capturing(stream));
+    return scratch([&](int dev) { return &g_scratch[dev][tag]; }, tag, bytes, rc, nullptr, is_capturing(stream));
 }
 
 void* naiwa_scratch_of_stream(int tag, size_t bytes, int* rc, hipStream_t stream) {
     const bool capturing = is_capturing(stream);
-    auto find = [&](int dev) -> NaiwaScratch& {
-        std::vector<StreamScratch>& all = g_of_streams[dev][tag];
-        for (StreamScratch& x : all)
-            if (x.stream == stream && x.capturing == capturing) return x.s;
-        all.push_back({stream, capturing, {}});
-        return all.back().s;
+    auto find = [&](int dev) -> NaiwaScratch* {
+        StreamScratch*& first = g_of_streams[dev][tag];
+        for (StreamScratch* x = first; x; x = x->next)
+            if (x->stream == stream && x->capturing == capturing) return &x->s;
+        StreamScratch* x = new (std::nothrow) StreamScratch{stream, capturing, {}, first};
+        if (!x) return nullptr;
+        first = x;
+        return &x->s;
     };
     return scratch(find, tag, bytes, rc, nullptr, capturing);
 }

@@ -24,7 +24,7 @@ struct NaiwaScratch {
 // its address: a larger call leaves it and allocates another.
 void* naiwa_scratch(int tag, size_t bytes, int* rc, hipStream_t stream);
 // A buffer of the stream's own for (device, tag, stream), so that calls on different streams need no order; captured
-// calls have another, which the graphs that were captured on the stream share.
+// calls have another, which the graphs that were captured on the stream share (and on a later stream of its handle).
 void* naiwa_scratch_of_stream(int tag, size_t bytes, int* rc, hipStream_t stream);
 // For calls that are not captured; *fresh tells whether this call (re)allocated the
 // buffer, whose contents are then undefined.
