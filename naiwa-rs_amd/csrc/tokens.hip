@@ -356,7 +356,7 @@ from_experts_kernel(const typename Y::T* y, int64_t ld, const uint32_t* inv, con
                             __builtin_memcpy(v[u], &z, 16);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < N; ++i) v[u][i] = 0;
+                            for (int i = 0; i < N; ++i) v[u][i] = Y::put(-0.0f); // 0 times it changes no sum, -0 neither
                         }
                     }
 #pragma unroll
